@@ -196,9 +196,10 @@ def _to_codes(x, keep):
 
     The largest magnitude of a group (at least 2^-100) becomes the format's largest value; the codes are rounded to
     nearest, ties to even."""
-    top = 127.0 if keep == "int8" else 448.0
     r, c = x.shape
     groups = -(-c // GROUP)
+    # a tensor: by a number torch would multiply with the reciprocal, which rounds twice
+    top = torch.full((r, groups), 127.0 if keep == "int8" else 448.0, device=x.device)
     x = torch.nn.functional.pad(x, (0, groups * GROUP - c)).view(r, groups, GROUP)
     most = x.abs().amax(dim=2).clamp(min=2.0 ** -100)
     q = x * (top / most).unsqueeze(2)
