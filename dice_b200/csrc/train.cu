@@ -1,0 +1,101 @@
+// Entry points of the expert FFN's training step: the gradients of the products grouped by expert, and the whole
+// forward and backward pass over expert-sorted rows (arguments are checked here, the kernels are in train_simt.cu
+// and train_rows.cu; the forward products are those of the eval path).
+#include "train.cuh"
+
+namespace {
+
+constexpr int kMaxSegTrain = 256;
+
+// what every grouped product asks of its sizes
+int check_product(int64_t n_rows, int n_dim, int k_dim, int n_slabs, int n_seg, int dtype) {
+  DICE_CHECK_ARG(n_rows >= 0 && n_dim > 0 && k_dim > 0 && n_slabs > 0 && n_seg >= 0, DICE_ERR_ARG);
+  DICE_CHECK_ARG(dice_dtype_size(dtype) != 0, DICE_ERR_DTYPE);
+  DICE_CHECK_ARG(n_dim % 8 == 0 && k_dim % 8 == 0, DICE_ERR_SHAPE);
+  DICE_CHECK_ARG(n_seg <= kMaxSegTrain && n_rows < 0x7fffff00LL && n_dim <= (1 << 24) && k_dim <= (1 << 22) &&
+                     static_cast<int64_t>(n_slabs) * n_dim < 0x7fffff00LL && static_cast<int64_t>(n_slabs) * k_dim < 0x7fffff00LL,
+                 DICE_ERR_LIMIT);
+  return DICE_OK;
+}
+
+}  // namespace
+
+extern "C" int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, const void* w, int n_slabs, int k_dim,
+                                  const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, int dtype, void* dx,
+                                  uint32_t* status, void* stream) {
+  const int rc = check_product(n_rows, n_dim, k_dim, n_slabs, n_seg, dtype);
+  if (rc != DICE_OK) return rc;
+  DICE_CHECK_ARG(seg_slab != nullptr || n_seg <= n_slabs, DICE_ERR_ARG);
+  if (n_rows == 0 || n_seg == 0) return DICE_OK;
+  DICE_CHECK_ARG(dy && w && seg_offsets && dx, DICE_ERR_ARG);
+  DICE_CHECK_ARG(dice_aligned16(dy) && dice_aligned16(w) && dice_aligned16(dx), DICE_ERR_ALIGN);
+  return dice_internal_simt_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dtype, dx, status,
+                                  static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int dice_grouped_wgrad(const void* dy, const void* x, int64_t n_rows, int n_dim, int k_dim,
+                                  const int32_t* seg_offsets, int n_slabs, int gate_up, int dtype, void* dw, void* dw_up,
+                                  uint32_t* status, void* stream) {
+  const int rc = check_product(n_rows, n_dim, k_dim, n_slabs, n_slabs, dtype);
+  if (rc != DICE_OK) return rc;
+  DICE_CHECK_ARG(gate_up >= 0, DICE_ERR_ARG);
+  DICE_CHECK_ARG(gate_up == 0 || (gate_up % 8 == 0 && static_cast<int64_t>(n_dim) == dice_w13_rows(gate_up)), DICE_ERR_SHAPE);
+  DICE_CHECK_ARG(seg_offsets && dw && (gate_up == 0 || dw_up) && (n_rows == 0 || (dy && x)), DICE_ERR_ARG);
+  DICE_CHECK_ARG(dice_aligned16(dy) && dice_aligned16(x) && dice_aligned16(dw) && dice_aligned16(dw_up), DICE_ERR_ALIGN);
+  return dice_internal_simt_wgrad(dy, x, n_rows, n_dim, k_dim, seg_offsets, n_slabs, gate_up, dtype, dw, dw_up, status,
+                                  static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int dice_grouped_ffn_train(const void* rows_in, int64_t n_rows, int hidden, int ffn, int act, int keep, int dtype,
+                                      const void* w1, const void* w2, int n_slabs, const int32_t* seg_offsets, int n_seg,
+                                      void* pre, void* a, void* codes, float* scales, void* rows_out, uint32_t* status,
+                                      void* stream) {
+  DICE_CHECK_ARG(act == DICE_ACT_SWIGLU || act == DICE_ACT_GELU_TANH, DICE_ERR_ARG);
+  DICE_CHECK_ARG(ffn > 0 && n_seg <= n_slabs, DICE_ERR_ARG);
+  const int64_t cols = act == DICE_ACT_SWIGLU ? dice_w13_rows(ffn) : ffn;
+  DICE_CHECK_ARG(cols <= (1 << 22), DICE_ERR_LIMIT);
+  int rc = check_product(n_rows, static_cast<int>(cols), hidden, n_slabs, n_seg, dtype);
+  if (rc == DICE_OK) rc = check_product(n_rows, hidden, ffn, n_slabs, n_seg, dtype);
+  if (rc != DICE_OK) return rc;
+  if (n_rows == 0 || n_seg == 0) return DICE_OK;
+  DICE_CHECK_ARG(rows_in && w1 && w2 && seg_offsets && pre && a && rows_out, DICE_ERR_ARG);
+  DICE_CHECK_ARG(dice_aligned16(rows_in) && dice_aligned16(w1) && dice_aligned16(w2) && dice_aligned16(pre) &&
+                     dice_aligned16(a) && dice_aligned16(rows_out),
+                 DICE_ERR_ALIGN);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == DICE_BF16)
+    rc = dice_grouped_gemm(rows_in, n_rows, hidden, w1, n_slabs, cols, seg_offsets, nullptr, n_seg, DICE_EPI_STORE, pre,
+                           cols, static_cast<int>(cols), 0, status, stream);
+  else
+    rc = dice_internal_simt_linear(rows_in, n_rows, hidden, w1, n_slabs, static_cast<int>(cols), seg_offsets, nullptr, n_seg,
+                                   dtype, pre, status, s);
+  if (rc != DICE_OK) return rc;
+  rc = dice_act_keep(pre, n_rows, ffn, act, keep, dtype, a, codes, scales, stream);
+  if (rc != DICE_OK) return rc;
+  if (dtype == DICE_BF16)
+    return dice_grouped_gemm(a, n_rows, ffn, w2, n_slabs, hidden, seg_offsets, nullptr, n_seg, DICE_EPI_STORE, rows_out,
+                             hidden, hidden, 0, status, stream);
+  return dice_internal_simt_linear(a, n_rows, ffn, w2, n_slabs, hidden, seg_offsets, nullptr, n_seg, dtype, rows_out, status, s);
+}
+
+extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in, const void* kept, const float* scales,
+                                         int64_t n_rows, int hidden, int ffn, int act, int keep, int dtype, const void* w1,
+                                         const void* w2, int n_slabs, const int32_t* seg_offsets, void* da, void* d_pre,
+                                         void* a, void* d_rows, void* dw1, void* dw1_up, void* dw2, uint32_t* status,
+                                         void* stream) {
+  DICE_CHECK_ARG(act == DICE_ACT_SWIGLU || act == DICE_ACT_GELU_TANH, DICE_ERR_ARG);
+  DICE_CHECK_ARG(ffn > 0, DICE_ERR_ARG);
+  const bool glu = act == DICE_ACT_SWIGLU;
+  const int64_t cols = glu ? dice_w13_rows(ffn) : ffn;
+  DICE_CHECK_ARG(cols <= (1 << 22), DICE_ERR_LIMIT);
+  int rc = check_product(n_rows, hidden, ffn, n_slabs, n_slabs, dtype);
+  if (rc == DICE_OK) rc = check_product(n_rows, static_cast<int>(cols), hidden, n_slabs, n_slabs, dtype);
+  if (rc != DICE_OK) return rc;
+  DICE_CHECK_ARG(seg_offsets && dw1 && dw2 && (!glu || dw1_up), DICE_ERR_ARG);
+  DICE_CHECK_ARG(n_rows == 0 || (d_out && rows_in && kept && w1 && w2 && da && d_pre && a && d_rows), DICE_ERR_ARG);
+  if ((rc = dice_grouped_dgrad(d_out, n_rows, hidden, w2, n_slabs, ffn, seg_offsets, nullptr, n_slabs, dtype, da, status, stream)) != DICE_OK) return rc;
+  if ((rc = dice_act_backward(da, kept, scales, n_rows, ffn, act, keep, dtype, d_pre, a, stream)) != DICE_OK) return rc;
+  if ((rc = dice_grouped_wgrad(d_out, a, n_rows, hidden, ffn, seg_offsets, n_slabs, 0, dtype, dw2, nullptr, status, stream)) != DICE_OK) return rc;
+  if ((rc = dice_grouped_dgrad(d_pre, n_rows, static_cast<int>(cols), w1, n_slabs, hidden, seg_offsets, nullptr, n_slabs, dtype, d_rows, status, stream)) != DICE_OK) return rc;
+  return dice_grouped_wgrad(d_pre, rows_in, n_rows, static_cast<int>(cols), hidden, seg_offsets, n_slabs, glu ? ffn : 0, dtype, dw1, dw1_up, status, stream);
+}

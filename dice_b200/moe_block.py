@@ -7,9 +7,10 @@ reference's, so checkpoints load unchanged and ``models.py`` / ``sample_ddp.py``
 can use this class in place of their own.  In eval mode on a CUDA device the
 forward runs the hand-written kernels (fused router, permute, grouped expert
 FFN on the tensor cores, un-permute + weighted combine); there is no CPU or
-PyTorch fallback for that path.  Training (``self.training``) is outside the
-accelerated path and is expressed with ordinary differentiable torch
-operations, as the reference does (``models.py:313-320``).
+PyTorch fallback for that path.  Training (``self.training``) is expressed
+with ordinary differentiable torch operations, as the reference does
+(``models.py:313-320``); a block built with ``train_kernels=True`` runs its
+experts' forward and backward pass on kernels too (``expert_train.py``).
 """
 from __future__ import annotations
 
@@ -390,14 +391,24 @@ class SparseMoeBlock(nn.Module):
     synthetic benchmark variant: ``expert_act="gelu_tanh"`` builds two-matrix
     GELU-tanh experts, ``shared_expert=False`` drops the shared expert;
     ``self.gate.norm_topk_prob = True`` renormalises the top-2 weights
-    (the reference's switch, models.py:170)."""
+    (the reference's switch, models.py:170).  ``train_kernels=True`` trains
+    the experts on the kernels (CUDA tensors, one device, two experts per
+    token; the gate stays with torch), in bf16 wherever the eval path would
+    compute in bf16; ``train_keep`` says what they keep of the activation's
+    argument for the backward pass: "int8" or "e4m3" (8 bits, one scale per
+    128 values) or None (all of it)."""
 
     def __init__(self, embed_dim, mlp_ratio=4, num_experts=16, num_experts_per_tok=2, pretraining_tp=2,
                  layer_idx=None, total_layers=None, para_mode: ParaMode = None, *, expert_act="swiglu",
-                 shared_expert=True):
+                 shared_expert=True, train_kernels=False, train_keep: Optional[str] = "int8"):
         super().__init__()
         assert para_mode is not None
         assert expert_act in ("swiglu", "gelu_tanh")
+        if train_keep not in ops.KEEP_CODES:
+            raise ValueError(f"train_keep is None, 'int8' or 'e4m3', got {train_keep!r}")
+        if train_kernels and (para_mode.ep or num_experts_per_tok != 2):
+            raise ValueError("train_kernels takes two experts per token and no expert parallelism")
+        self.train_kernels, self.train_keep = train_kernels, train_keep
         self.num_experts_per_tok = num_experts_per_tok
         self.expert_act = expert_act
         inter = mlp_ratio * embed_dim
@@ -594,6 +605,8 @@ class SparseMoeBlock(nn.Module):
         """models.py:313-320 with differentiable torch operations."""
         identity, orig_shape = hidden_states, hidden_states.shape
         topk_idx, topk_weight, aux_loss = self.gate(hidden_states)
+        if self.train_kernels:
+            return self._experts_train(hidden_states, topk_idx, topk_weight, aux_loss)
         x = hidden_states.view(-1, orig_shape[-1]).repeat_interleave(self.num_experts_per_tok, dim=0)
         flat = topk_idx.view(-1)
         y = torch.empty_like(x)
@@ -606,4 +619,26 @@ class SparseMoeBlock(nn.Module):
             y = AddAuxiliaryLoss.apply(y, aux_loss)
         if self.n_shared_experts is not None:
             y = y + self.shared_experts(identity)
+        return y
+
+    def _experts_train(self, hidden_states, topk_idx, topk_weight, aux_loss):
+        """The experts' part of the training forward on the kernels."""
+        from .expert_train import DenseExpert, RoutedExperts
+
+        if not hidden_states.is_cuda:
+            raise RuntimeError("a SparseMoeBlock with train_kernels trains on CUDA tensors only (no CPU fallback)")
+        if not self.layer_idx:
+            ops.poll_status(hidden_states.device)
+        h = hidden_states.shape[-1]
+        x = hidden_states.reshape(-1, h).to(_compute_dtype(hidden_states))
+        act, ffn = self.expert_act, self.experts[0].intermediate_size
+        params = [p for e in self.experts for p in ExpertPack._params(e)[1]]
+        y = RoutedExperts.apply(x, topk_idx, topk_weight.float(), act, ffn, self.train_keep, *params)
+        y = y.view(hidden_states.shape).to(hidden_states.dtype)
+        if aux_loss is not None:
+            y = AddAuxiliaryLoss.apply(y, aux_loss)
+        if self.n_shared_experts is not None:
+            shared = self.shared_experts
+            s = DenseExpert.apply(x, act, shared.intermediate_size, self.train_keep, *ExpertPack._params(shared)[1])
+            y = y + s.view(hidden_states.shape).to(hidden_states.dtype)
         return y

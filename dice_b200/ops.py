@@ -8,7 +8,8 @@ of expert-sorted rows.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+import contextlib
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -554,3 +555,255 @@ def shared_expert_can_ride() -> bool:
     import os
 
     return os.environ.get("DICE_GEMM_PAIR", "1") != "0"
+
+
+# --------------------------------------------------------------------------- #
+# the training step: gradients of the grouped products, 8-bit kept activations
+# --------------------------------------------------------------------------- #
+
+KEEP_CODES = {None: 0, "int8": 1, "e4m3": 2}
+KEEP_DTYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+KEEP_GROUP = 128  # columns that share a scale
+
+
+class KeptAct(NamedTuple):
+    """What the forward pass keeps of an activation's argument: ``codes`` int8 or float8_e4m3fn ``[R, C]`` with fp32
+    ``scales [R, ceil(C / 128)]`` (the value is ``code * scale``), or the argument itself with ``scales`` None."""
+
+    codes: torch.Tensor
+    scales: Optional[torch.Tensor]
+
+    @property
+    def keep(self) -> Optional[str]:
+        return None if self.scales is None else {v: k for k, v in KEEP_DTYPES.items()}[self.codes.dtype]
+
+
+def _on(*tensors: Optional[torch.Tensor]):
+    """The context in which kernels for these tensors are launched: their device (all have the same one), with that
+    device's current stream."""
+    _require_cuda(*tensors)
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise RuntimeError(f"all tensors of a call must be on one device, got {device} and {t.device}")
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _status_or_default(status: Optional[torch.Tensor], device: torch.device) -> torch.Tensor:
+    if status is None:
+        if device not in _status_words and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("call dice_b200.ops.device_status(device) once before capturing a graph")
+        return device_status(device)
+    assert status.dtype == torch.int32 and status.numel() >= 1
+    return status
+
+
+def _check_segments(seg_offsets: torch.Tensor) -> int:
+    assert seg_offsets.dtype == torch.int32 and seg_offsets.dim() == 1 and seg_offsets.is_contiguous()
+    assert seg_offsets.numel() >= 1, "seg_offsets holds one offset more than there are segments"
+    return seg_offsets.numel() - 1
+
+
+def act_columns(act: str, ffn: int) -> int:
+    """Columns of an activation's argument: ``ffn``, or the packed gate / up width of SwiGLU."""
+    if act not in ACT_CODES:
+        raise ValueError(f"unknown activation {act!r}")
+    return w13_rows(ffn) if act == "swiglu" else ffn
+
+
+def grouped_dgrad(dy: torch.Tensor, w: torch.Tensor, seg_offsets: torch.Tensor, status: Optional[torch.Tensor] = None,
+                  seg_slab: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Input gradient of :func:`grouped_gemm`: ``dx[r] = dy[r] @ w[slab(seg(r))]`` with ``dy [R, N]``,
+    ``w [S, N, K]`` (bf16 or fp32).  Rows of no segment are left as they are in ``out`` (uninitialised without it)."""
+    with _on(dy, w, seg_offsets, status, seg_slab, out):
+        assert dy.dim() == 2 and w.dim() == 3 and w.shape[1] == dy.shape[1] and w.dtype == dy.dtype
+        n_seg = _check_segments(seg_offsets)
+        assert seg_slab is None or (seg_slab.dtype == torch.int32 and seg_slab.is_contiguous() and seg_slab.numel() == n_seg)
+        code = _dtype_code(dy)
+        dy, w = dy.contiguous(), w.contiguous()
+        n_rows, n_dim = dy.shape
+        n_slabs, _, k_dim = w.shape
+        if out is None:
+            out = torch.empty((n_rows, k_dim), dtype=dy.dtype, device=dy.device)
+        assert out.is_contiguous() and out.shape == (n_rows, k_dim) and out.dtype == dy.dtype
+        _lib.check(
+            _lib.load().dice_grouped_dgrad(_ptr(dy), n_rows, n_dim, _ptr(w), n_slabs, k_dim, _ptr(seg_offsets), _ptr(seg_slab),
+                                           n_seg, code, _ptr(out), _ptr(_status_or_default(status, dy.device)), _stream()),
+            "dice_grouped_dgrad",
+        )
+    return out
+
+
+def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, seg_offsets: torch.Tensor, status: Optional[torch.Tensor] = None,
+                  gate_up: Optional[int] = None):
+    """Weight gradient of :func:`grouped_gemm`: ``dw[s] = dy[seg s].T @ x[seg s]`` ``[S, N, K]`` in the rows' type, zero
+    for a segment without rows.  ``gate_up=ffn``: ``dy`` has the packed gate / up columns of :func:`pack_w13`, and the
+    result is the pair of gradients ``[S, ffn, K]`` of the gate and the up projections."""
+    with _on(dy, x, seg_offsets, status):
+        assert dy.dim() == 2 and x.dim() == 2 and x.shape[0] == dy.shape[0] and x.dtype == dy.dtype
+        n_slabs = _check_segments(seg_offsets)
+        assert n_slabs >= 1
+        code = _dtype_code(dy)
+        dy, x = dy.contiguous(), x.contiguous()
+        n_rows, n_dim = dy.shape
+        k_dim = x.shape[1]
+        rows = gate_up if gate_up else n_dim
+        dw = torch.empty((n_slabs, rows, k_dim), dtype=dy.dtype, device=dy.device)
+        dw_up = torch.empty_like(dw) if gate_up else None
+        _lib.check(
+            _lib.load().dice_grouped_wgrad(_ptr(dy), _ptr(x), n_rows, n_dim, k_dim, _ptr(seg_offsets), n_slabs, gate_up or 0,
+                                           code, _ptr(dw), _ptr(dw_up), _ptr(_status_or_default(status, dy.device)), _stream()),
+            "dice_grouped_wgrad",
+        )
+    return (dw, dw_up) if gate_up else dw
+
+
+def _empty_kept(n_rows: int, cols: int, keep: str, device) -> KeptAct:
+    return KeptAct(torch.empty((n_rows, cols), dtype=KEEP_DTYPES[keep], device=device),
+                   torch.empty((n_rows, (cols + KEEP_GROUP - 1) // KEEP_GROUP), dtype=torch.float32, device=device))
+
+
+def _check_kept(kept: KeptAct, n_rows: int, cols: int, dtype: torch.dtype) -> None:
+    assert kept.codes.shape == (n_rows, cols) and kept.codes.is_contiguous()
+    if kept.scales is None:
+        assert kept.codes.dtype == dtype
+        return
+    if kept.codes.dtype not in KEEP_DTYPES.values():
+        raise TypeError(f"codes are int8 or float8_e4m3fn, got {kept.codes.dtype}")
+    assert kept.scales.dtype == torch.float32 and kept.scales.is_contiguous()
+    assert kept.scales.shape == (n_rows, (cols + KEEP_GROUP - 1) // KEEP_GROUP)
+
+
+def _check_keep(keep: Optional[str]) -> None:
+    if keep not in KEEP_CODES:
+        raise ValueError(f"keep is None, 'int8' or 'e4m3', got {keep!r}")
+
+
+def act_keep(pre: torch.Tensor, act: str, ffn: int, keep: Optional[str] = "int8") -> Tuple[torch.Tensor, KeptAct]:
+    """The activation ``a [R, ffn]`` of ``pre`` (SwiGLU: packed gate / up columns ``[R, w13_rows(ffn)]``; GELU:
+    ``[R, ffn]``) and, in the same pass, ``pre`` in 8 bits for :func:`act_backward`: every row's 128 columns share a
+    scale.  ``keep=None`` keeps ``pre`` itself."""
+    _check_keep(keep)
+    with _on(pre):
+        assert pre.dim() == 2 and pre.shape[1] == act_columns(act, ffn)
+        code = _dtype_code(pre)
+        pre = pre.contiguous()
+        n_rows, cols = pre.shape
+        a = torch.empty((n_rows, ffn), dtype=pre.dtype, device=pre.device)
+        kept = KeptAct(pre, None) if keep is None else _empty_kept(n_rows, cols, keep, pre.device)
+        _lib.check(
+            _lib.load().dice_act_keep(_ptr(pre), n_rows, ffn, ACT_CODES[act], KEEP_CODES[keep], code, _ptr(a),
+                                      None if keep is None else _ptr(kept.codes), _ptr(kept.scales), _stream()),
+            "dice_act_keep",
+        )
+    return a, kept
+
+
+def act_backward(da: torch.Tensor, kept: KeptAct, act: str, ffn: int, want_act: bool = True):
+    """Backward pass of :func:`act_keep`: ``(d_pre, a)`` from the activation's gradient ``da [R, ffn]`` and what was
+    kept; ``a`` is the activation of the kept argument (None without ``want_act``), which the second product's weight
+    gradient needs."""
+    codes, scales = kept
+    with _on(da, codes, scales):
+        cols = act_columns(act, ffn)
+        assert da.dim() == 2 and da.shape[1] == ffn
+        code = _dtype_code(da)
+        n_rows = da.shape[0]
+        _check_kept(kept, n_rows, cols, da.dtype)
+        da = da.contiguous()
+        d_pre = torch.empty((n_rows, cols), dtype=da.dtype, device=da.device)
+        a = torch.empty_like(da) if want_act else None
+        _lib.check(
+            _lib.load().dice_act_backward(_ptr(da), _ptr(codes), _ptr(scales), n_rows, ffn, ACT_CODES[act],
+                                          KEEP_CODES[kept.keep], code, _ptr(d_pre), _ptr(a), _stream()),
+            "dice_act_backward",
+        )
+    return d_pre, a
+
+
+def combine_backward(dout: torch.Tensor, rows_out: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor):
+    """Gradient of the gate-weighted sum of a token's two rows (:func:`unpermute_combine`): ``d_rows [R, h]`` with
+    ``d_rows[pos[t, s]] = weights[t, s] * dout[t]`` and ``d_weights [N, 2]`` fp32 ``= <dout[t], rows_out[pos[t, s]]>``.
+    ``pos`` int32 ``[N, 2]`` names no row twice (a plan's); rows that it does not name are left uninitialised, a
+    position outside ``rows_out`` has gradient 0."""
+    with _on(dout, rows_out, pos, weights):
+        assert dout.dim() == 2 and rows_out.dim() == 2 and dout.shape[1] == rows_out.shape[1] and rows_out.dtype == dout.dtype
+        n_tokens, h = dout.shape
+        assert pos.dtype == torch.int32 and pos.shape == (n_tokens, 2)
+        assert weights.dtype == torch.float32 and weights.shape == (n_tokens, 2)
+        code = _dtype_code(dout)
+        dout, rows_out, pos, weights = dout.contiguous(), rows_out.contiguous(), pos.contiguous(), weights.contiguous()
+        d_rows = torch.empty_like(rows_out)
+        d_weights = torch.empty((n_tokens, 2), dtype=torch.float32, device=dout.device)
+        _lib.check(
+            _lib.load().dice_combine_backward(_ptr(dout), _ptr(rows_out), _ptr(pos), _ptr(weights), n_tokens,
+                                              rows_out.shape[0], h, code, _ptr(d_rows), _ptr(d_weights), _stream()),
+            "dice_combine_backward",
+        )
+    return d_rows, d_weights
+
+
+def _check_ffn(rows, w1, w2, seg_offsets, act, ffn):
+    cols = act_columns(act, ffn)
+    assert rows.dim() == 2 and w1.dim() == 3 and w2.dim() == 3
+    n_slabs, h = w1.shape[0], rows.shape[1]
+    assert w1.shape == (n_slabs, cols, h) and w2.shape == (n_slabs, h, ffn)
+    assert w1.dtype == rows.dtype and w2.dtype == rows.dtype and w1.is_contiguous() and w2.is_contiguous()
+    assert _check_segments(seg_offsets) == n_slabs, "one segment per expert"
+    return n_slabs, h, cols
+
+
+def grouped_ffn_train(rows: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, seg_offsets: torch.Tensor, act: str, ffn: int,
+                      status: Optional[torch.Tensor] = None, keep: Optional[str] = "int8"):
+    """:func:`grouped_ffn` for training: ``(rows_out, kept)``, where ``kept`` is the activation's argument in 8 bits
+    (``keep`` "int8" or "e4m3") or as it is (None), for :func:`grouped_ffn_backward`.  The first product is rounded to
+    the rows' type before the activation.  bf16, or fp32 on the CUDA cores."""
+    _check_keep(keep)
+    with _on(rows, w1, w2, seg_offsets, status):
+        code = _dtype_code(rows)
+        n_slabs, h, cols = _check_ffn(rows, w1, w2, seg_offsets, act, ffn)
+        rows = rows.contiguous()
+        n_rows, dev = rows.shape[0], rows.device
+        pre = torch.empty((n_rows, cols), dtype=rows.dtype, device=dev)
+        a = torch.empty((n_rows, ffn), dtype=rows.dtype, device=dev)
+        rows_out = torch.empty_like(rows)
+        kept = KeptAct(pre, None) if keep is None else _empty_kept(n_rows, cols, keep, dev)
+        _lib.check(
+            _lib.load().dice_grouped_ffn_train(
+                _ptr(rows), n_rows, h, ffn, ACT_CODES[act], KEEP_CODES[keep], code, _ptr(w1), _ptr(w2), n_slabs,
+                _ptr(seg_offsets), n_slabs, _ptr(pre), _ptr(a), None if keep is None else _ptr(kept.codes), _ptr(kept.scales),
+                _ptr(rows_out), _ptr(_status_or_default(status, dev)), _stream(),
+            ),
+            "dice_grouped_ffn_train",
+        )
+    return rows_out, kept
+
+
+def grouped_ffn_backward(d_out: torch.Tensor, rows: torch.Tensor, kept: KeptAct, w1: torch.Tensor, w2: torch.Tensor,
+                         seg_offsets: torch.Tensor, act: str, ffn: int, status: Optional[torch.Tensor] = None):
+    """Backward pass of :func:`grouped_ffn_train` from what it kept: ``(d_rows, dw1, dw2)``; for SwiGLU ``dw1`` is the
+    pair of the gate and the up projections' gradients ``[S, ffn, h]``."""
+    codes, scales = kept
+    with _on(d_out, rows, codes, scales, w1, w2, seg_offsets, status):
+        code = _dtype_code(rows)
+        n_slabs, h, cols = _check_ffn(rows, w1, w2, seg_offsets, act, ffn)
+        n_rows, dev = rows.shape[0], rows.device
+        assert d_out.shape == rows.shape and d_out.dtype == rows.dtype
+        _check_kept(kept, n_rows, cols, rows.dtype)
+        d_out, rows = d_out.contiguous(), rows.contiguous()
+        new = lambda *shape: torch.empty(shape, dtype=rows.dtype, device=dev)  # noqa: E731
+        da, d_pre, a, d_rows = new(n_rows, ffn), new(n_rows, cols), new(n_rows, ffn), new(n_rows, h)
+        dw2 = new(n_slabs, h, ffn)
+        dw1 = new(n_slabs, ffn, h)
+        dw1_up = new(n_slabs, ffn, h) if act == "swiglu" else None
+        _lib.check(
+            _lib.load().dice_grouped_ffn_backward(
+                _ptr(d_out), _ptr(rows), _ptr(codes), _ptr(scales), n_rows, h, ffn, ACT_CODES[act], KEEP_CODES[kept.keep], code,
+                _ptr(w1), _ptr(w2), n_slabs, _ptr(seg_offsets), _ptr(da), _ptr(d_pre), _ptr(a), _ptr(d_rows), _ptr(dw1),
+                _ptr(dw1_up), _ptr(dw2), _ptr(_status_or_default(status, dev)), _stream(),
+            ),
+            "dice_grouped_ffn_backward",
+        )
+    return d_rows, (dw1 if dw1_up is None else (dw1, dw1_up)), dw2

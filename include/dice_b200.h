@@ -315,6 +315,93 @@ DICE_API int dice_grouped_ffn_f32(const void* rows_in, int64_t n_rows, int hidde
                          void* stream);
 
 /* ---------------------------------------------------------------------------
+ * The training step of the expert FFN (the reference trains through autograd
+ * over a Python loop of experts, models.py:313-320).  Rows are expert-sorted as
+ * above; both element types are taken everywhere: bf16, and fp32 on the CUDA
+ * cores (no tensor-core rounding).  Sums are fp32; outputs are rounded once.
+ *
+ * Input gradient of a product grouped by expert (out = a * w^T):
+ *   dx[r, :] = dy[r, :] * w[slab(seg(r))]
+ *   dy [n_rows, n_dim], w [n_slabs, n_dim, k_dim], dx [n_rows, k_dim]
+ *   seg_offsets [n_seg + 1], seg_slab as in dice_grouped_gemm
+ * Rows outside every segment (and rows of a segment with slab -1) are left as
+ * they are.  n_dim and k_dim multiples of 8, n_seg <= 256.  `status` (may be
+ * NULL) receives a code when the segments are not monotone or reach beyond
+ * n_rows, or a slab does not exist: such segments are not computed. */
+DICE_API int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, const void* w, int n_slabs, int k_dim,
+                       const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, int dtype, void* dx,
+                       uint32_t* status, void* stream);
+
+/* Weight gradient of the same product, one segment per slab:
+ *   dw[s] = dy[seg s]^T * x[seg s]     (zero for a segment without rows)
+ *   dy [n_rows, n_dim], x [n_rows, k_dim], dw [n_slabs, n_dim, k_dim]
+ * Rows outside every segment are not read.  gate_up = ffn > 0: dy has the
+ * packed order of dice_pack_w13 (n_dim == dice_w13_rows(ffn)) and the gradient
+ * is written apart: dw [n_slabs, ffn, k_dim] for the gate rows, dw_up for the up
+ * rows (else dw_up is NULL).  n_slabs <= 256. */
+DICE_API int dice_grouped_wgrad(const void* dy, const void* x, int64_t n_rows, int n_dim, int k_dim,
+                       const int32_t* seg_offsets, int n_slabs, int gate_up, int dtype, void* dw, void* dw_up,
+                       uint32_t* status, void* stream);
+
+/* what the forward pass keeps of the activation's argument */
+#define DICE_KEEP_NONE 0 /* the argument itself                                   */
+#define DICE_KEEP_INT8 1 /* 8-bit integers, one fp32 scale per row and 128 columns */
+#define DICE_KEEP_E4M3 2 /* 8-bit floats (e4m3), the same scales                  */
+
+/* The activation, and its argument in 8 bits:
+ *   SWIGLU     pre [n_rows, dice_w13_rows(ffn)] in the packed order (gate and up
+ *              columns in turns of 128), a = silu(gate) * up
+ *   GELU_TANH  pre [n_rows, ffn], a = gelu_tanh(pre)
+ *   codes  [n_rows, columns of pre], one byte each:
+ *          rn(pre * (top / most)), ties to even, top = 127 (int8) or 448 (e4m3)
+ *   scales [n_rows, ceil(columns of pre / 128)] fp32: most / top, where `most` is
+ *          the largest magnitude of the row's 128 columns, at least 2^-100
+ * A group that holds an infinity or a NaN gets the scale NaN.  The packed
+ * order's filling columns are not read; their codes are zero.  ffn a multiple of
+ * 8.  keep == NONE writes a alone (codes and scales may be NULL). */
+DICE_API int dice_act_keep(const void* pre, int64_t n_rows, int ffn, int act, int keep, int dtype, void* a, void* codes,
+                  float* scales, void* stream);
+
+/* Its backward pass.  p = codes * scale (keep == NONE: `kept` is pre itself):
+ *   d_pre = da * act'(p)  [n_rows, columns of pre] (filling columns: zero)
+ *   a     = act(p)        [n_rows, ffn], what the second product's weight
+ *           gradient is made from (NULL to skip) */
+DICE_API int dice_act_backward(const void* da, const void* kept, const float* scales, int64_t n_rows, int ffn, int act,
+                      int keep, int dtype, void* d_pre, void* a, void* stream);
+
+/* Gradient of out[t] = weights[t,0] * rows_out[pos[t,0]] + weights[t,1] * rows_out[pos[t,1]]
+ * (dice_unpermute_combine; models.py:377-381):
+ *   d_rows[pos[t,s]] = weights[t,s] * dout[t],  d_weights[t,s] = <dout[t], rows_out[pos[t,s]]>
+ * The positions are a plan's: no row is named twice.  A position outside
+ * [0, n_rows) writes no row and has gradient 0; rows that no position names are
+ * left as they are.  hidden a multiple of 8. */
+DICE_API int dice_combine_backward(const void* dout, const void* rows_out, const int32_t* pos, const float* weights,
+                          int64_t n_tokens, int64_t n_rows, int hidden, int dtype, void* d_rows,
+                          float* d_weights, void* stream);
+
+/* The expert FFN's forward pass for training (operands as in dice_grouped_ffn,
+ * one segment per slab): the first product rounded to dtype, the activation and
+ * what is kept of its argument, the second product.
+ *   pre   [n_rows, columns of the first product]: what is kept with keep ==
+ *         NONE, else scratch
+ *   a     [n_rows, ffn] scratch */
+DICE_API int dice_grouped_ffn_train(const void* rows_in, int64_t n_rows, int hidden, int ffn, int act, int keep, int dtype,
+                           const void* w1, const void* w2, int n_slabs, const int32_t* seg_offsets, int n_seg,
+                           void* pre, void* a, void* codes, float* scales, void* rows_out, uint32_t* status,
+                           void* stream);
+
+/* and its backward pass from what was kept:
+ *   d_out [n_rows, hidden] -> d_rows [n_rows, hidden], dw1 (and dw1_up: SWIGLU's
+ *   gate and up gradients [n_slabs, ffn, hidden] apart), dw2 [n_slabs, hidden, ffn]
+ *   da [n_rows, ffn], d_pre [n_rows, columns of the first product] and
+ *   a [n_rows, ffn] are scratch. */
+DICE_API int dice_grouped_ffn_backward(const void* d_out, const void* rows_in, const void* kept, const float* scales,
+                              int64_t n_rows, int hidden, int ffn, int act, int keep, int dtype, const void* w1,
+                              const void* w2, int n_slabs, const int32_t* seg_offsets, void* da, void* d_pre,
+                              void* a, void* d_rows, void* dw1, void* dw1_up, void* dw2, uint32_t* status,
+                              void* stream);
+
+/* ---------------------------------------------------------------------------
  * Expert-parallel exchange over NVLink peer memory (one process per GPU, one
  * box).  Replaces, for the synchronous exchange, exchange_token_counts
  * (ep_fwd.py:214-245), global_dispatch (:247-293) and global_combine (:295-342)
