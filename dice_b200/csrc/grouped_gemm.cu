@@ -350,6 +350,19 @@ int encode_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
   return r == CUDA_SUCCESS ? DICE_OK : DICE_ERR_CUDA;
 }
 
+int encode_map3(CUtensorMap* map, const void* base, uint64_t slabs, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (fn == nullptr) return DICE_ERR_CUDA;
+  const cuuint64_t dims[3] = {cols, rows, slabs};
+  const cuuint64_t strides[2] = {cols * 2, rows * cols * 2};
+  const cuuint32_t box[3] = {BK, box_rows, 1};
+  const cuuint32_t elem_strides[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+                        elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? DICE_OK : DICE_ERR_CUDA;
+}
+
 int sm_count_cached() {
   static int cached[64] = {0};
   int dev = 0;

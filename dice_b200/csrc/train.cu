@@ -29,6 +29,9 @@ extern "C" int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, con
   if (n_rows == 0 || n_seg == 0) return DICE_OK;
   DICE_CHECK_ARG(dy && w && seg_offsets && dx, DICE_ERR_ARG);
   DICE_CHECK_ARG(dice_aligned16(dy) && dice_aligned16(w) && dice_aligned16(dx), DICE_ERR_ALIGN);
+  if (dtype == DICE_BF16)
+    return dice_internal_tc_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dx, status,
+                                  static_cast<cudaStream_t>(stream));
   return dice_internal_simt_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dtype, dx, status,
                                   static_cast<cudaStream_t>(stream));
 }
@@ -42,6 +45,9 @@ extern "C" int dice_grouped_wgrad(const void* dy, const void* x, int64_t n_rows,
   DICE_CHECK_ARG(gate_up == 0 || (gate_up % 8 == 0 && static_cast<int64_t>(n_dim) == dice_w13_rows(gate_up)), DICE_ERR_SHAPE);
   DICE_CHECK_ARG(seg_offsets && dw && (gate_up == 0 || dw_up) && (n_rows == 0 || (dy && x)), DICE_ERR_ARG);
   DICE_CHECK_ARG(dice_aligned16(dy) && dice_aligned16(x) && dice_aligned16(dw) && dice_aligned16(dw_up), DICE_ERR_ALIGN);
+  if (dtype == DICE_BF16)
+    return dice_internal_tc_wgrad(dy, x, n_rows, n_dim, k_dim, seg_offsets, n_slabs, gate_up, dw, dw_up, status,
+                                  static_cast<cudaStream_t>(stream));
   return dice_internal_simt_wgrad(dy, x, n_rows, n_dim, k_dim, seg_offsets, n_slabs, gate_up, dtype, dw, dw_up, status,
                                   static_cast<cudaStream_t>(stream));
 }

@@ -14,6 +14,13 @@ int dice_internal_simt_wgrad(const void* dy, const void* x, int64_t n_rows, int 
                              const int32_t* seg_offsets, int n_slabs, int gate_up, int dtype, void* dw, void* dw_up,
                              uint32_t* status, cudaStream_t s);
 
+// bf16 on the tensor cores (train_gemm.cu)
+int dice_internal_tc_dgrad(const void* dy, int64_t n_rows, int n_dim, const void* w, int n_slabs, int k_dim,
+                           const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, void* dx, uint32_t* status,
+                           cudaStream_t s);
+int dice_internal_tc_wgrad(const void* dy, const void* x, int64_t n_rows, int n_dim, int k_dim, const int32_t* seg_offsets,
+                           int n_slabs, int gate_up, void* dw, void* dw_up, uint32_t* status, cudaStream_t s);
+
 constexpr int kKeepGroup = 128;               // columns of a kept argument that share a scale
 constexpr float kKeepFloor = 7.888609e-31f;   // 2^-100: the smallest group maximum a scale is made from
 

@@ -239,6 +239,8 @@ __device__ __forceinline__ void store_row_chunk(__nv_bfloat16* dst, const float 
 
 // ---- host side, shared ------------------------------------------------------------
 int encode_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows);
+// [slabs][rows][cols]; a box never reaches from one slab into the next (zeros are read there)
+int encode_map3(CUtensorMap* map, const void* base, uint64_t slabs, uint64_t rows, uint64_t cols, uint32_t box_rows);
 int sm_count_cached();
 
 }  // namespace dice_umma
