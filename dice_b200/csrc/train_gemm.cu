@@ -13,8 +13,9 @@
 // into rows that hold anything): the instructions stop at the last 16 rows that the segment touches, and the up to
 // 15 rows of those that are not the segment's are zeroed in shared memory, in both operands, since a zero in one
 // would not silence a NaN in the other.  For such a block each CTA's copies complete on a barrier of its own; a warp
-// waits there, zeroes, makes the zeros visible to the asynchronous proxy and arrives at the leader's "full" barrier.
-// All other blocks go from the copies to the tensor cores directly.
+// waits there, zeroes, makes the zeros visible to the asynchronous proxy and completes the copies' bytes on the leader's
+// "full" barrier in their place.  All other blocks go from the copies to the tensor cores directly.  (The leader expects
+// both CTAs' bytes; a peer that announced its own with a cluster-scope arrival cost twice the time of a block.)
 //
 // Few tiles and a long reduction: the pairs that would idle take a share of the reduction each (split).  Every epilogue
 // warp files its part of the sum in fp32; the last one to arrive at a part adds them up in the order of the shares, so
@@ -76,15 +77,12 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
       "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void mbar_expect_tx_cluster(uint32_t cluster_addr, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_addr), "r"(bytes)
-               : "memory");
+// bytes of a ragged end accounted for on the leader's barrier, in the place of the copies (whose bytes the leader expects)
+__device__ __forceinline__ void mbar_complete_tx_cluster(uint32_t cluster_addr, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cluster.b64 [%0], %1;" ::"r"(cluster_addr), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-// the issuing warp's acquire of what the other CTA zeroed
-__device__ __forceinline__ void fence_acquire_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+// orders the zeroing before that (release), and after it in the issuing warp (acquire)
+__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 template <int MODE>
@@ -115,8 +113,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   pdl_trigger();
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStagesT; ++s) {
-      // TN: both CTAs announce their own bytes (or, at a ragged end, that they have zeroed); NN: the leader both's
-      mbar_init(full_bar + 8 * s, MODE == MODE_TN ? 2 : 1);
+      mbar_init(full_bar + 8 * s, 1);
       mbar_init(empty_bar + 8 * s, 1);
       mbar_init(tail_bar + 8 * s, 1);
     }
@@ -213,7 +210,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     if (ti.kb1 < blocks) ti.last_rows = BK;
     int n_valid = p.n_cols - ti.nb * BN;
     if (n_valid > BN) n_valid = BN;
-    ti.n_mma = (n_valid + 31) & ~31;
+    ti.n_mma = (n_valid + 31) & ~31;  // half of the columns come from each CTA
     return ti;
   };
 
@@ -237,8 +234,8 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         const uint32_t a_dst = tiles_smem + stage * kStageBytesT, b_dst = a_dst + kOperandBytes;
         const uint32_t leader_full = map_to_cta(full_bar + 8 * stage, 0);
         if (elect_one()) {
+          if (leader) mbar_expect_tx(full_bar + 8 * stage, 2 * bytes);
           if (MODE == MODE_NN) {
-            if (leader) mbar_expect_tx(full_bar + 8 * stage, 2 * bytes);
             tma_load_2d_pair(a_dst, &tm_a, kb * BK, ti.row0, leader_full);
             for (int j = 0; j < b_boxes; ++j)
               tma_load_3d_pair(b_dst + j * kBoxBytes, &tm_b, col0 + 64 * j, kb * BK, ti.slab, leader_full);
@@ -249,8 +246,6 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
               bar = tail_bar + 8 * stage;
               mbar_expect_tx(bar, bytes);
               bar = map_to_cta(bar, cta_rank);
-            } else {
-              mbar_expect_tx_cluster(leader_full, bytes);
             }
             for (int j = 0; j < 2; ++j) tma_load_2d_pair(a_dst + j * kBoxBytes, &tm_a, ti.row0 + 64 * j, row, bar);
             for (int j = 0; j < b_boxes; ++j) tma_load_2d_pair(b_dst + j * kBoxBytes, &tm_b, col0 + 64 * j, row, bar);
@@ -282,7 +277,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           int steps = BK / UMMA_K;
           if (MODE == MODE_TN && kb == ti.kb1 - 1) {
             steps = (ti.last_rows + UMMA_K - 1) / UMMA_K;
-            if (ti.last_rows & 15) fence_acquire_cluster();
+            if (ti.last_rows & 15) fence_cluster();
           }
           tc_fence_after_sync();
           const uint32_t a_addr = tiles_smem + stage * kStageBytesT;
@@ -328,8 +323,10 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
 #pragma unroll
             for (int b = 0; b < 4; ++b) *reinterpret_cast<uint4*>(base + b * kBoxBytes + i * 16) = make_uint4(0, 0, 0, 0);
           fence_async_smem();
+          fence_cluster();
           __syncwarp();
-          if (lane == 0) mbar_arrive_release_cluster(map_to_cta(full_bar + 8 * stage, 0));
+          if (lane == 0)
+            mbar_complete_tx_cluster(map_to_cta(full_bar + 8 * stage, 0), kOperandBytes + (ti.n_mma > 128 ? 2 : 1) * kBoxBytes);
         }
         slot = (slot + blocks) % kStagesT;
       }
