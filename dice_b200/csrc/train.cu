@@ -32,7 +32,7 @@ extern "C" int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, con
   if (dtype == DICE_BF16)
     return dice_internal_tc_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dx, status,
                                   static_cast<cudaStream_t>(stream));
-  return dice_internal_simt_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dtype, dx, status,
+  return dice_internal_simt_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dx, status,
                                   static_cast<cudaStream_t>(stream));
 }
 
@@ -48,7 +48,7 @@ extern "C" int dice_grouped_wgrad(const void* dy, const void* x, int64_t n_rows,
   if (dtype == DICE_BF16)
     return dice_internal_tc_wgrad(dy, x, n_rows, n_dim, k_dim, seg_offsets, n_slabs, gate_up, dw, dw_up, status,
                                   static_cast<cudaStream_t>(stream));
-  return dice_internal_simt_wgrad(dy, x, n_rows, n_dim, k_dim, seg_offsets, n_slabs, gate_up, dtype, dw, dw_up, status,
+  return dice_internal_simt_wgrad(dy, x, n_rows, n_dim, k_dim, seg_offsets, n_slabs, gate_up, dw, dw_up, status,
                                   static_cast<cudaStream_t>(stream));
 }
 
@@ -74,14 +74,14 @@ extern "C" int dice_grouped_ffn_train(const void* rows_in, int64_t n_rows, int h
                            cols, static_cast<int>(cols), 0, status, stream);
   else
     rc = dice_internal_simt_linear(rows_in, n_rows, hidden, w1, n_slabs, static_cast<int>(cols), seg_offsets, nullptr, n_seg,
-                                   dtype, pre, status, s);
+                                   pre, status, s);
   if (rc != DICE_OK) return rc;
   rc = dice_act_keep(pre, n_rows, ffn, act, keep, dtype, a, codes, scales, stream);
   if (rc != DICE_OK) return rc;
   if (dtype == DICE_BF16)
     return dice_grouped_gemm(a, n_rows, ffn, w2, n_slabs, hidden, seg_offsets, nullptr, n_seg, DICE_EPI_STORE, rows_out,
                              hidden, hidden, 0, status, stream);
-  return dice_internal_simt_linear(a, n_rows, ffn, w2, n_slabs, hidden, seg_offsets, nullptr, n_seg, dtype, rows_out, status, s);
+  return dice_internal_simt_linear(a, n_rows, ffn, w2, n_slabs, hidden, seg_offsets, nullptr, n_seg, rows_out, status, s);
 }
 
 extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in, const void* kept, const float* scales,

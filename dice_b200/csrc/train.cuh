@@ -4,14 +4,15 @@
 
 #include "common.cuh"
 
+// fp32 on the CUDA cores (train_simt.cu)
 int dice_internal_simt_linear(const void* a, int64_t n_rows, int k_dim, const void* w, int n_slabs, int n_dim,
-                              const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, int dtype, void* out,
+                              const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, void* out,
                               uint32_t* status, cudaStream_t s);
 int dice_internal_simt_dgrad(const void* dy, int64_t n_rows, int n_dim, const void* w, int n_slabs, int k_dim,
-                             const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, int dtype, void* dx,
+                             const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, void* dx,
                              uint32_t* status, cudaStream_t s);
 int dice_internal_simt_wgrad(const void* dy, const void* x, int64_t n_rows, int n_dim, int k_dim,
-                             const int32_t* seg_offsets, int n_slabs, int gate_up, int dtype, void* dw, void* dw_up,
+                             const int32_t* seg_offsets, int n_slabs, int gate_up, void* dw, void* dw_up,
                              uint32_t* status, cudaStream_t s);
 
 // bf16 on the tensor cores (train_gemm.cu)

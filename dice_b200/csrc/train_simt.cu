@@ -5,62 +5,105 @@
 //   NN  dx[r, k]  = sum_n dy[r, n] w[seg(r)][n, k]       its input gradient
 //   TN  dw[s][n, k] = sum_{r in seg s} dy[r, n] x[r, k]  its weight gradient
 //
-// 128 x 128 output tile per CTA, 16-deep shared-memory slices in two buffers (the next slice is loaded into
-// registers while the present one is multiplied), 8 x 8 fp32 accumulators per thread.  Segments are ragged: each
-// CTA finds its own on the device.
+// Bound: the fp32 pipe (74 TFLOP/s nominal).  Every thread holds 8 x 8 sums and multiplies with two-wide fused
+// multiply-adds, which leaves issue slots to the shared-memory reads; the next two slices of the operands are copied
+// into shared memory asynchronously while the present one is multiplied (staging one slice in registers instead left
+// the pipe idle a third of the time).  An operand whose reduction index is contiguous is transposed on its way, four
+// bytes a copy.  Segments are ragged, and each CTA finds its own on the device.
+//
+// NT and NN have few rows in a segment and a long reduction: 64 x 64 tiles (an expert with 130 rows fills 3 of them
+// to 68 %, but 2 tiles of 128 rows to 51 %), and a CTA's four groups of 64 threads each sum every fourth slice of the
+// reduction, added up in shared memory at the end (1024 rows through 8 experts, 4608 -> 1152: 180 tiles alone would
+// leave most of the GPU's warp slots empty).  TN has many tiles and a short reduction: 128 x 128 tiles, one group.
 #include "common.cuh"
 #include "train.cuh"
 
 namespace {
 
-constexpr int TM = 128, TN = 128, TK = 16;
-constexpr int kMaxSegSimt = 256;
-enum { MODE_NT = 0, MODE_NN = 1, MODE_TN = 2 };
+constexpr int WM = 128, WN = 128, WK = 16;           // TN: tile and slice
+constexpr int TM = 64, TN = 64, TK = 8, GROUPS = 4;  // NT, NN: tile, slice, groups that share the reduction
+enum { MODE_NT = 0, MODE_NN = 1 };
 
-__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
-  const uint2 v = *reinterpret_cast<const uint2*>(p);
-  return make_float4(bf16lo_to_f32(v.x), bf16hi_to_f32(v.x), bf16lo_to_f32(v.y), bf16hi_to_f32(v.y));
+constexpr int kRing = 3;  // slices in shared memory: one being multiplied, two on their way
+
+// asynchronous copy of BYTES (4 or 16); zeros where !ok (nothing is read then)
+template <int BYTES>
+__device__ __forceinline__ void copy_async(float* dst, const float* src, bool ok) {
+  const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(ok ? 16 : 0) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(ok ? 4 : 0) : "memory");
 }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory"); }
 __device__ __forceinline__ void store4(float* p, const float* v) {
   *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
 }
-__device__ __forceinline__ void store4(__nv_bfloat16* p, const float* v) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-}
 
-// One thread's share (two groups of 4) of a 128 x 16 operand slice.  KMAJOR: the reduction index is contiguous in
-// memory ([mn][k]), the thread holds 8 reduction elements of one row; else ([k][mn]) it holds columns c .. c+3 and
-// c+64 .. c+67 of one reduction row.  mn_valid / k_valid: what is left of the operand from the slice's corner.
-template <typename T, bool KMAJOR>
-__device__ __forceinline__ void load_slice(const T* base, int64_t ld, int mn_valid, int64_t k_valid, float4 (&v)[2]) {
-  v[0] = v[1] = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (KMAJOR) {
-    const int r = threadIdx.x >> 1, k = (threadIdx.x & 1) * 8;
-    if (r < mn_valid) {
-      const T* p = base + static_cast<int64_t>(r) * ld + k;
-      if (k < k_valid) v[0] = load4(p);
-      if (k + 4 < k_valid) v[1] = load4(p + 4);
-    }
-  } else {
-    const int k = threadIdx.x >> 4, c = (threadIdx.x & 15) * 4;
-    if (k < k_valid) {
-      const T* p = base + static_cast<int64_t>(k) * ld + c;
-      if (c < mn_valid) v[0] = load4(p);
-      if (c + 64 < mn_valid) v[1] = load4(p + 64);
+
+// acc (two neighbouring columns) += a * b; rounds as two fmaf do
+__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t a, uint64_t b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ uint64_t twice(float a) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(a));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+// 8 x 8 sums of one slice: rows ra .. ra+3 and ra+STEP .. of A, columns likewise of B
+template <int DEPTH, int WIDTH, int STEP>
+__device__ __forceinline__ void multiply(const float (*As)[WIDTH + 4], const float (*Bs)[WIDTH + 4], int ra, int cb,
+                                         uint64_t (&acc)[8][4]) {
+#pragma unroll
+  for (int k = 0; k < DEPTH; ++k) {
+    float ar[8];
+    uint64_t br[4];
+    *reinterpret_cast<float4*>(ar) = *reinterpret_cast<const float4*>(&As[k][ra]);
+    *reinterpret_cast<float4*>(ar + 4) = *reinterpret_cast<const float4*>(&As[k][ra + STEP]);
+    *reinterpret_cast<ulonglong2*>(br) = *reinterpret_cast<const ulonglong2*>(&Bs[k][cb]);
+    *reinterpret_cast<ulonglong2*>(br + 2) = *reinterpret_cast<const ulonglong2*>(&Bs[k][cb + STEP]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint64_t a2 = twice(ar[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fma2(acc[i][j], a2, br[j]);
     }
   }
 }
+__device__ __forceinline__ void store_tile_row(float* o, const uint64_t (&acc)[4], int c0, int step, int n_valid) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int c = c0 + h * step;
+    if (c < n_valid) {
+      const float2 lo = halves(acc[2 * h]), hi = halves(acc[2 * h + 1]);
+      const float v[4] = {lo.x, lo.y, hi.x, hi.y};
+      store4(o + c, v);
+    }
+  }
+}
+
+// One thread's share of a group's 64 x 8 operand slice.  KMAJOR: the reduction index is contiguous in memory
+// ([mn][k]); eight lanes copy a row's eight elements (one 32-byte sector), into eight banks.  Else ([k][mn]).
 template <bool KMAJOR>
-__device__ __forceinline__ void put_slice(float (*s)[TM + 4], const float4 (&v)[2]) {
+__device__ __forceinline__ void copy_slice(float (*s)[TM + 4], const float* base, int64_t ld, int mn_valid, int64_t k_valid, int t) {
   if (KMAJOR) {
-    const int r = threadIdx.x >> 1, k = (threadIdx.x & 1) * 8;
-    s[k + 0][r] = v[0].x; s[k + 1][r] = v[0].y; s[k + 2][r] = v[0].z; s[k + 3][r] = v[0].w;
-    s[k + 4][r] = v[1].x; s[k + 5][r] = v[1].y; s[k + 6][r] = v[1].z; s[k + 7][r] = v[1].w;
+    const int k = t & 7, r = t >> 3;
+#pragma unroll
+    for (int h = 0; h < 8; ++h) {
+      const bool ok = r + 8 * h < mn_valid && k < k_valid;
+      copy_async<4>(&s[k][r + 8 * h], ok ? base + static_cast<int64_t>(r + 8 * h) * ld + k : base, ok);
+    }
   } else {
-    const int k = threadIdx.x >> 4, c = (threadIdx.x & 15) * 4;
-    *reinterpret_cast<float4*>(&s[k][c]) = v[0];
-    *reinterpret_cast<float4*>(&s[k][c + 64]) = v[1];
+    const int k = t >> 4, c = (t & 15) * 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool ok = c < mn_valid && k + 4 * h < k_valid;
+      copy_async<16>(&s[k + 4 * h][c], ok ? base + static_cast<int64_t>(k + 4 * h) * ld + c : base, ok);
+    }
   }
 }
 
@@ -80,173 +123,223 @@ struct SimtParams {
   uint32_t* status;
 };
 
-template <typename T, int MODE>
-__global__ void __launch_bounds__(256) simt_grouped_kernel(const SimtParams p) {
-  __shared__ __align__(16) float As[2][TK][TM + 4];
-  __shared__ __align__(16) float Bs[2][TK][TN + 4];
-  __shared__ int s_seg, s_row0, s_rows;
+struct Slices {
+  float a[kRing][TK][TM + 4], b[kRing][TK][TN + 4];
+};
+constexpr int kRowsSmem = GROUPS * sizeof(Slices);
+static_assert(kRowsSmem >= 2 * TM * TN * sizeof(float), "the groups' sums are exchanged in place of the slices");
+
+template <int MODE>
+__global__ void __launch_bounds__(64 * GROUPS, 2) simt_rows_kernel(const SimtParams p) {
+  constexpr bool kB = MODE == MODE_NT;  // B has the reduction contiguous (A always has)
+  extern __shared__ __align__(16) uint8_t smem_rows[];
+  Slices* slices = reinterpret_cast<Slices*>(smem_rows);
+  __shared__ int s_slab, s_row0, s_rows;
   pdl_trigger();
   pdl_wait();
   if (threadIdx.x == 0) {
-    int found = -1, row0 = 0, rows = 0;
-    bool ok = true;
-    if (MODE == MODE_TN) {
-      found = blockIdx.z;
-      row0 = p.seg_offsets[found];
-      rows = p.seg_offsets[found + 1] - row0;
-      ok = row0 >= 0 && rows >= 0 && static_cast<int64_t>(row0) + rows <= p.n_rows;
-    } else {
-      int run = 0;
-      for (int s = 0; s < p.n_seg && found < 0 && ok; ++s) {
-        const int beg = p.seg_offsets[s], cnt = p.seg_offsets[s + 1] - beg;
-        ok = beg >= 0 && cnt >= 0 && static_cast<int64_t>(beg) + cnt <= p.n_rows;
-        const int nb = ok ? (cnt + TM - 1) / TM : 0;
-        if (ok && static_cast<int>(blockIdx.x) < run + nb) {
-          found = s;
-          row0 = beg + (static_cast<int>(blockIdx.x) - run) * TM;
-          rows = beg + cnt - row0;
-        }
-        run += nb;
+    int slab = -1, row0 = 0, rows = 0, run = 0;
+    bool ok = true, found = false;
+    for (int s = 0; s < p.n_seg && !found && ok; ++s) {
+      const int beg = p.seg_offsets[s], end = p.seg_offsets[s + 1];
+      ok = beg >= 0 && end >= beg && end <= p.n_rows;
+      const int nb = ok ? (end - beg + TM - 1) / TM : 0;
+      if (static_cast<int>(blockIdx.x) < run + nb) {
+        found = true;
+        slab = p.seg_slab != nullptr ? p.seg_slab[s] : s;  // -1: rows of no expert
+        row0 = beg + (static_cast<int>(blockIdx.x) - run) * TM;
+        rows = end - row0;
+        ok = slab < p.n_slabs;
       }
-      if (found >= 0 && p.seg_slab != nullptr) {
-        found = p.seg_slab[found];  // -1: rows that belong to no expert
-        ok = found < p.n_slabs;
-      }
+      run += nb;
     }
     if (!ok) {
-      found = -1;
+      slab = -1;
       if (p.status != nullptr) atomicCAS(p.status, 0u, DICE_STATUS_BAD_SEGMENTS);
     }
-    s_seg = found; s_row0 = row0; s_rows = rows;
+    s_slab = slab; s_row0 = row0; s_rows = rows;
   }
   __syncthreads();
-  if (s_seg < 0) return;
-  const int slab = s_seg, row0 = s_row0, seg_rows = s_rows;
-  const int col0 = blockIdx.y * TN;
+  if (s_slab < 0) return;
+  const int row0 = s_row0, m_valid = s_rows;
+  const int col0 = blockIdx.y * TN, n_valid = p.n_cols - col0;
+  const int group = threadIdx.x >> 6, t = threadIdx.x & 63;
+  const int ra = (t >> 3) * 4, cb = (t & 7) * 4;
 
-  const T* a = static_cast<const T*>(p.a);
-  const T* b = static_cast<const T*>(p.b);
-  int64_t lda, ldb, red;   // strides and reduction length
-  int m_valid;
-  const int n_valid = p.n_cols - col0;
-  constexpr bool kA = MODE != MODE_TN, kB = MODE == MODE_NT;  // which operands have the reduction contiguous
-  if (MODE == MODE_TN) {
-    lda = p.m_cols; ldb = p.n_cols; red = seg_rows;
-    a += static_cast<int64_t>(row0) * lda + static_cast<int64_t>(blockIdx.x) * TM;
-    b += static_cast<int64_t>(row0) * ldb + col0;
-    m_valid = p.m_cols - static_cast<int>(blockIdx.x) * TM;
-  } else {
-    lda = red = p.red;
-    a += static_cast<int64_t>(row0) * lda;
-    m_valid = seg_rows;
-    if (MODE == MODE_NT) {
-      ldb = p.red;
-      b += (static_cast<int64_t>(slab) * p.n_cols + col0) * ldb;
-    } else {
-      ldb = p.n_cols;
-      b += static_cast<int64_t>(slab) * p.red * ldb + col0;
-    }
-  }
-  const int64_t a_step = kA ? TK : static_cast<int64_t>(TK) * lda;
-  const int64_t b_step = kB ? TK : static_cast<int64_t>(TK) * ldb;
+  const int64_t lda = p.red, ldb = kB ? p.red : p.n_cols;
+  const float* a = static_cast<const float*>(p.a) + static_cast<int64_t>(row0) * lda;
+  const float* b = static_cast<const float*>(p.b) + (kB ? (static_cast<int64_t>(s_slab) * p.n_cols + col0) * ldb
+                                               : static_cast<int64_t>(s_slab) * p.red * ldb + col0);
+  const int64_t b_slice = kB ? TK : static_cast<int64_t>(TK) * ldb;
+  a += static_cast<int64_t>(group) * TK;
+  b += group * b_slice;
+  int64_t left = static_cast<int64_t>(p.red) - group * TK;  // of the reduction, from this group's slice on
 
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  float acc[8][8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
-
-  float4 av[2], bv[2];
-  load_slice<T, kA>(a, lda, m_valid, red, av);
-  load_slice<T, kB>(b, ldb, n_valid, red, bv);
-  put_slice<kA>(As[0], av);
-  put_slice<kB>(Bs[0], bv);
-  __syncthreads();
-  int buf = 0;
-  for (int64_t k0 = 0; k0 < red; k0 += TK) {
-    const bool more = k0 + TK < red;
-    if (more) {
-      a += a_step;
-      b += b_step;
-      load_slice<T, kA>(a, lda, m_valid, red - k0 - TK, av);
-      load_slice<T, kB>(b, ldb, n_valid, red - k0 - TK, bv);
+  uint64_t acc[8][4] = {};
+  Slices& mine = slices[group];
+  auto fetch = [&](int buf) {
+    if (left > 0) {
+      copy_slice<true>(mine.a[buf], a, lda, m_valid, left, t);
+      copy_slice<kB>(mine.b[buf], b, ldb, n_valid, left, t);
+      a += GROUPS * TK;
+      b += GROUPS * b_slice;
+      left -= GROUPS * TK;
     }
-#pragma unroll
-    for (int k = 0; k < TK; ++k) {
-      float ar[8], br[8];
-      *reinterpret_cast<float4*>(ar) = *reinterpret_cast<const float4*>(&As[buf][k][ty * 4]);
-      *reinterpret_cast<float4*>(ar + 4) = *reinterpret_cast<const float4*>(&As[buf][k][ty * 4 + 64]);
-      *reinterpret_cast<float4*>(br) = *reinterpret_cast<const float4*>(&Bs[buf][k][tx * 4]);
-      *reinterpret_cast<float4*>(br + 4) = *reinterpret_cast<const float4*>(&Bs[buf][k][tx * 4 + 64]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(ar[i], br[j], acc[i][j]);
-    }
-    if (more) {
-      put_slice<kA>(As[buf ^ 1], av);
-      put_slice<kB>(Bs[buf ^ 1], bv);
-      __syncthreads();
-      buf ^= 1;
-    }
+    copies_commit();
+  };
+  int todo = left > 0 ? static_cast<int>((left + GROUPS * TK - 1) / (GROUPS * TK)) : 0;
+  fetch(0);
+  fetch(1);
+  for (int buf = 0; todo > 0; --todo) {
+    copies_wait();
+    asm volatile("bar.sync %0, 64;" ::"r"(group + 1) : "memory");  // the slice is there, the one before it is done with
+    fetch(buf == 0 ? kRing - 1 : buf - 1);
+    multiply<TK, TM, 32>(mine.a[buf], mine.b[buf], ra, cb, acc);
+    buf = buf == kRing - 1 ? 0 : buf + 1;
   }
 
-  T* out = static_cast<T*>(p.out);
-  if (MODE == MODE_TN) {
-    if (p.gate_up == 0) {
-      out += (static_cast<int64_t>(slab) * p.m_cols + static_cast<int64_t>(blockIdx.x) * TM) * p.n_cols;
-    } else {
-      // a tile is one 128-row block of the packed order: even blocks are gate rows, odd ones the matching up rows
-      if (blockIdx.x & 1) out = static_cast<T*>(p.out_up);
-      const int r0 = static_cast<int>(blockIdx.x >> 1) * TM;
-      out += (static_cast<int64_t>(slab) * p.gate_up + r0) * p.n_cols;
-      m_valid = p.gate_up - r0;
+  // groups 2 and 3 hand their sums to 0 and 1, then 1 to 0
+  uint64_t* sums = reinterpret_cast<uint64_t*>(slices);
+#pragma unroll
+  for (int half = GROUPS / 2; half >= 1; half >>= 1) {
+    __syncthreads();
+    if (group >= half && group < 2 * half) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) sums[(group - half) * (TM * TN / 2) + i * 64 + t] = acc[i >> 2][i & 3];
     }
-  } else {
-    out += static_cast<int64_t>(row0) * p.n_cols;
+    __syncthreads();
+    if (group < half) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float2 x = halves(acc[i >> 2][i & 3]), y = halves(sums[group * (TM * TN / 2) + i * 64 + t]);
+        asm("mov.b64 %0, {%1, %2};" : "=l"(acc[i >> 2][i & 3]) : "f"(x.x + y.x), "f"(x.y + y.y));
+      }
+    }
   }
-  out += col0;
+  if (group != 0) return;
+  float* out = static_cast<float*>(p.out) + static_cast<int64_t>(row0) * p.n_cols + col0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int r = ty * 4 + (i & 3) + (i >> 2) * 64;
-    if (r >= m_valid) continue;
-    T* o = out + static_cast<int64_t>(r) * p.n_cols;
-    if (tx * 4 < n_valid) store4(o + tx * 4, acc[i]);
-    if (tx * 4 + 64 < n_valid) store4(o + tx * 4 + 64, acc[i] + 4);
+    const int r = ra + (i & 3) + (i >> 2) * 32;
+    if (r < m_valid) store_tile_row(out + static_cast<int64_t>(r) * p.n_cols, acc[i], cb, 32, n_valid);
   }
 }
 
+// one thread's share of a 128 x 16 slice: columns c .. c+3 and c+64 .. c+67 of one reduction row
+__device__ __forceinline__ void copy_wide(float (*s)[WM + 4], const float* base, int64_t ld, int mn_valid, int k_valid) {
+  const int k = threadIdx.x >> 4, c = (threadIdx.x & 15) * 4;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const bool ok = k < k_valid && c + 64 * h < mn_valid;
+    copy_async<16>(&s[k][c + 64 * h], ok ? base + static_cast<int64_t>(k) * ld + c + 64 * h : base, ok);
+  }
+}
+
+struct WideSlices {
+  float a[kRing][WK][WM + 4], b[kRing][WK][WN + 4];
+};
+
+__global__ void __launch_bounds__(256, 2) simt_wgrad_kernel(const SimtParams p) {
+  extern __shared__ __align__(16) uint8_t smem_wide[];
+  WideSlices& sl = *reinterpret_cast<WideSlices*>(smem_wide);
+  pdl_trigger();
+  pdl_wait();
+  const int slab = blockIdx.z;
+  const int row0 = p.seg_offsets[slab], end = p.seg_offsets[slab + 1];
+  if (row0 < 0 || end < row0 || end > p.n_rows) {
+    if (threadIdx.x == 0 && p.status != nullptr) atomicCAS(p.status, 0u, DICE_STATUS_BAD_SEGMENTS);
+    return;
+  }
+  const int m0 = static_cast<int>(blockIdx.x) * WM, col0 = blockIdx.y * WN;
+  const int n_valid = p.n_cols - col0;
+  int m_valid = p.m_cols - m0;
+  const float* a = static_cast<const float*>(p.a) + static_cast<int64_t>(row0) * p.m_cols + m0;
+  const float* b = static_cast<const float*>(p.b) + static_cast<int64_t>(row0) * p.n_cols + col0;
+  int left = end - row0;
+
+  const int ra = (threadIdx.x >> 4) * 4, cb = (threadIdx.x & 15) * 4;
+  uint64_t acc[8][4] = {};
+  auto fetch = [&](int buf) {
+    if (left > 0) {
+      copy_wide(sl.a[buf], a, p.m_cols, m_valid, left);
+      copy_wide(sl.b[buf], b, p.n_cols, n_valid, left);
+      a += static_cast<int64_t>(WK) * p.m_cols;
+      b += static_cast<int64_t>(WK) * p.n_cols;
+      left -= WK;
+    }
+    copies_commit();
+  };
+  int todo = (left + WK - 1) / WK;
+  fetch(0);
+  fetch(1);
+  for (int buf = 0; todo > 0; --todo) {
+    copies_wait();
+    __syncthreads();  // the slice is there, the one before it is done with
+    fetch(buf == 0 ? kRing - 1 : buf - 1);
+    multiply<WK, WM, 64>(sl.a[buf], sl.b[buf], ra, cb, acc);
+    buf = buf == kRing - 1 ? 0 : buf + 1;
+  }
+
+  float* out = static_cast<float*>(p.out);
+  if (p.gate_up == 0) {
+    out += (static_cast<int64_t>(slab) * p.m_cols + m0) * p.n_cols + col0;
+  } else {
+    // a tile is one 128-row block of the packed order: even blocks are gate rows, odd ones the matching up rows
+    if (blockIdx.x & 1) out = static_cast<float*>(p.out_up);
+    const int r0 = static_cast<int>(blockIdx.x >> 1) * WM;
+    out += (static_cast<int64_t>(slab) * p.gate_up + r0) * p.n_cols + col0;
+    m_valid = p.gate_up - r0;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = ra + (i & 3) + (i >> 2) * 64;
+    if (r < m_valid) store_tile_row(out + static_cast<int64_t>(r) * p.n_cols, acc[i], cb, 64, n_valid);
+  }
+}
+
+// both kernels use more shared memory than the default limit; set once per device and kernel
+template <typename K>
+bool allow_smem(K kernel, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (!done[dev]) done[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+  return done[dev];
+}
+
 template <int MODE>
-int launch_simt(const SimtParams& p, int64_t gx, int dtype, cudaStream_t s) {
-  const int64_t gy = (static_cast<int64_t>(p.n_cols) + TN - 1) / TN;
+int launch_rows(const SimtParams& p, cudaStream_t s) {
+  const int64_t gx = (p.n_rows + TM - 1) / TM + p.n_seg, gy = (static_cast<int64_t>(p.n_cols) + TN - 1) / TN;
   if (gx > 0x7fffffffLL || gy > 65535) return DICE_ERR_LIMIT;
-  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy), MODE == MODE_TN ? p.n_slabs : 1);
-  const cudaError_t err = dtype == DICE_F32
-                              ? dice_launch(simt_grouped_kernel<float, MODE>, grid, dim3(256), 0, s, p)
-                              : dice_launch(simt_grouped_kernel<__nv_bfloat16, MODE>, grid, dim3(256), 0, s, p);
-  return err == cudaSuccess ? DICE_OK : DICE_ERR_CUDA;
+  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
+  static bool done[64];
+  if (!allow_smem(simt_rows_kernel<MODE>, kRowsSmem, done)) return DICE_ERR_CUDA;
+  return dice_launch(simt_rows_kernel<MODE>, grid, dim3(64 * GROUPS), kRowsSmem, s, p) == cudaSuccess ? DICE_OK : DICE_ERR_CUDA;
 }
 
 }  // namespace
 
 int dice_internal_simt_linear(const void* a, int64_t n_rows, int k_dim, const void* w, int n_slabs, int n_dim,
-                              const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, int dtype, void* out,
+                              const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, void* out,
                               uint32_t* status, cudaStream_t s) {
   SimtParams p = {a, w, out, nullptr, seg_offsets, seg_slab, n_seg, n_slabs, n_rows, 0, n_dim, k_dim, 0, status};
-  return launch_simt<MODE_NT>(p, (n_rows + TM - 1) / TM + n_seg, dtype, s);
+  return launch_rows<MODE_NT>(p, s);
 }
 
 int dice_internal_simt_dgrad(const void* dy, int64_t n_rows, int n_dim, const void* w, int n_slabs, int k_dim,
-                             const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, int dtype, void* dx,
+                             const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, void* dx,
                              uint32_t* status, cudaStream_t s) {
   SimtParams p = {dy, w, dx, nullptr, seg_offsets, seg_slab, n_seg, n_slabs, n_rows, 0, k_dim, n_dim, 0, status};
-  return launch_simt<MODE_NN>(p, (n_rows + TM - 1) / TM + n_seg, dtype, s);
+  return launch_rows<MODE_NN>(p, s);
 }
 
 int dice_internal_simt_wgrad(const void* dy, const void* x, int64_t n_rows, int n_dim, int k_dim,
-                             const int32_t* seg_offsets, int n_slabs, int gate_up, int dtype, void* dw, void* dw_up,
+                             const int32_t* seg_offsets, int n_slabs, int gate_up, void* dw, void* dw_up,
                              uint32_t* status, cudaStream_t s) {
   SimtParams p = {dy, x, dw, dw_up, seg_offsets, nullptr, n_slabs, n_slabs, n_rows, n_dim, k_dim, 0, gate_up, status};
-  return launch_simt<MODE_TN>(p, (n_dim + TM - 1) / TM, dtype, s);
+  const int64_t gy = (static_cast<int64_t>(k_dim) + WN - 1) / WN;
+  if (gy > 65535) return DICE_ERR_LIMIT;
+  const dim3 grid(static_cast<unsigned>((n_dim + WM - 1) / WM), static_cast<unsigned>(gy), static_cast<unsigned>(n_slabs));
+  static bool done[64];
+  if (!allow_smem(simt_wgrad_kernel, static_cast<int>(sizeof(WideSlices)), done)) return DICE_ERR_CUDA;
+  return dice_launch(simt_wgrad_kernel, grid, dim3(256), sizeof(WideSlices), s, p) == cudaSuccess ? DICE_OK : DICE_ERR_CUDA;
 }
