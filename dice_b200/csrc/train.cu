@@ -64,23 +64,28 @@ extern "C" int dice_grouped_ffn_train(const void* rows_in, int64_t n_rows, int h
   if (rc == DICE_OK) rc = check_product(n_rows, hidden, ffn, n_slabs, n_seg, dtype);
   if (rc != DICE_OK) return rc;
   if (n_rows == 0 || n_seg == 0) return DICE_OK;
-  DICE_CHECK_ARG(rows_in && w1 && w2 && seg_offsets && pre && a && rows_out, DICE_ERR_ARG);
+  DICE_CHECK_ARG(rows_in && w1 && w2 && seg_offsets && a && rows_out, DICE_ERR_ARG);
+  // bf16 keeps the first product in its epilogue: `pre` is written only when it is what is kept
+  DICE_CHECK_ARG(pre || (dtype == DICE_BF16 && keep != DICE_KEEP_NONE), DICE_ERR_ARG);
   DICE_CHECK_ARG(dice_aligned16(rows_in) && dice_aligned16(w1) && dice_aligned16(w2) && dice_aligned16(pre) &&
                      dice_aligned16(a) && dice_aligned16(rows_out),
                  DICE_ERR_ALIGN);
+  DICE_CHECK_ARG(keep == DICE_KEEP_NONE || keep == DICE_KEEP_INT8 || keep == DICE_KEEP_E4M3, DICE_ERR_ARG);
+  DICE_CHECK_ARG(keep == DICE_KEEP_NONE || (codes && scales), DICE_ERR_ARG);
+  DICE_CHECK_ARG(dice_aligned16(codes), DICE_ERR_ALIGN);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == DICE_BF16)
-    rc = dice_grouped_gemm(rows_in, n_rows, hidden, w1, n_slabs, cols, seg_offsets, nullptr, n_seg, DICE_EPI_STORE, pre,
-                           cols, static_cast<int>(cols), 0, status, stream);
-  else
-    rc = dice_internal_simt_linear(rows_in, n_rows, hidden, w1, n_slabs, static_cast<int>(cols), seg_offsets, nullptr, n_seg,
-                                   pre, status, s);
+  if (dtype == DICE_BF16) {
+    rc = dice_internal_tc_keep(rows_in, n_rows, hidden, ffn, act, keep, w1, n_slabs, seg_offsets, n_seg, pre, a, codes, scales,
+                               status, s);
+    if (rc != DICE_OK) return rc;
+    return dice_grouped_gemm(a, n_rows, ffn, w2, n_slabs, hidden, seg_offsets, nullptr, n_seg, DICE_EPI_STORE, rows_out,
+                             hidden, hidden, 0, status, stream);
+  }
+  rc = dice_internal_simt_linear(rows_in, n_rows, hidden, w1, n_slabs, static_cast<int>(cols), seg_offsets, nullptr, n_seg,
+                                 pre, status, s);
   if (rc != DICE_OK) return rc;
   rc = dice_act_keep(pre, n_rows, ffn, act, keep, dtype, a, codes, scales, stream);
   if (rc != DICE_OK) return rc;
-  if (dtype == DICE_BF16)
-    return dice_grouped_gemm(a, n_rows, ffn, w2, n_slabs, hidden, seg_offsets, nullptr, n_seg, DICE_EPI_STORE, rows_out,
-                             hidden, hidden, 0, status, stream);
   return dice_internal_simt_linear(a, n_rows, ffn, w2, n_slabs, hidden, seg_offsets, nullptr, n_seg, rows_out, status, s);
 }
 
@@ -98,9 +103,21 @@ extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in,
   if (rc == DICE_OK) rc = check_product(n_rows, static_cast<int>(cols), hidden, n_slabs, n_slabs, dtype);
   if (rc != DICE_OK) return rc;
   DICE_CHECK_ARG(seg_offsets && dw1 && dw2 && (!glu || dw1_up), DICE_ERR_ARG);
-  DICE_CHECK_ARG(n_rows == 0 || (d_out && rows_in && kept && w1 && w2 && da && d_pre && a && d_rows), DICE_ERR_ARG);
-  if ((rc = dice_grouped_dgrad(d_out, n_rows, hidden, w2, n_slabs, ffn, seg_offsets, nullptr, n_slabs, dtype, da, status, stream)) != DICE_OK) return rc;
-  if ((rc = dice_act_backward(da, kept, scales, n_rows, ffn, act, keep, dtype, d_pre, a, stream)) != DICE_OK) return rc;
+  DICE_CHECK_ARG(keep == DICE_KEEP_NONE || keep == DICE_KEEP_INT8 || keep == DICE_KEEP_E4M3, DICE_ERR_ARG);
+  if (n_rows > 0) {
+    DICE_CHECK_ARG(d_out && rows_in && kept && w1 && w2 && d_pre && a && d_rows && (keep == DICE_KEEP_NONE || scales), DICE_ERR_ARG);
+    DICE_CHECK_ARG(da || dtype == DICE_BF16, DICE_ERR_ARG);  // bf16: the activation's gradient stays in the epilogue
+    DICE_CHECK_ARG(dice_aligned16(d_out) && dice_aligned16(kept) && dice_aligned16(w2) && dice_aligned16(d_pre) && dice_aligned16(a),
+                   DICE_ERR_ALIGN);
+    if (dtype == DICE_BF16) {
+      rc = dice_internal_tc_back(d_out, n_rows, hidden, ffn, act, keep, w2, n_slabs, seg_offsets, kept, scales, d_pre, a, status,
+                                 static_cast<cudaStream_t>(stream));
+      if (rc != DICE_OK) return rc;
+    } else {
+      if ((rc = dice_grouped_dgrad(d_out, n_rows, hidden, w2, n_slabs, ffn, seg_offsets, nullptr, n_slabs, dtype, da, status, stream)) != DICE_OK) return rc;
+      if ((rc = dice_act_backward(da, kept, scales, n_rows, ffn, act, keep, dtype, d_pre, a, stream)) != DICE_OK) return rc;
+    }
+  }
   if ((rc = dice_grouped_wgrad(d_out, a, n_rows, hidden, ffn, seg_offsets, n_slabs, 0, dtype, dw2, nullptr, status, stream)) != DICE_OK) return rc;
   if ((rc = dice_grouped_dgrad(d_pre, n_rows, static_cast<int>(cols), w1, n_slabs, hidden, seg_offsets, nullptr, n_slabs, dtype, d_rows, status, stream)) != DICE_OK) return rc;
   return dice_grouped_wgrad(d_pre, rows_in, n_rows, static_cast<int>(cols), hidden, seg_offsets, n_slabs, glu ? ffn : 0, dtype, dw1, dw1_up, status, stream);

@@ -22,6 +22,15 @@ int dice_internal_tc_dgrad(const void* dy, int64_t n_rows, int n_dim, const void
 int dice_internal_tc_wgrad(const void* dy, const void* x, int64_t n_rows, int n_dim, int k_dim, const int32_t* seg_offsets,
                            int n_slabs, int gate_up, void* dw, void* dw_up, uint32_t* status, cudaStream_t s);
 
+// the forward product with the activation and what is kept in its epilogue, and the second product's input gradient with
+// the activation's backward pass in its epilogue (see train_gemm.cu); pointers as in the public entry points
+int dice_internal_tc_keep(const void* rows, int64_t n_rows, int hidden, int ffn, int act, int keep, const void* w1, int n_slabs,
+                          const int32_t* seg_offsets, int n_seg, void* pre, void* a, void* codes, float* scales,
+                          uint32_t* status, cudaStream_t s);
+int dice_internal_tc_back(const void* d_out, int64_t n_rows, int hidden, int ffn, int act, int keep, const void* w2, int n_slabs,
+                          const int32_t* seg_offsets, const void* kept, const float* scales, void* d_pre, void* a,
+                          uint32_t* status, cudaStream_t s);
+
 constexpr int kKeepGroup = 128;               // columns of a kept argument that share a scale
 constexpr float kKeepFloor = 7.888609e-31f;   // 2^-100: the smallest group maximum a scale is made from
 
@@ -73,9 +82,13 @@ __device__ __forceinline__ void keep_scale(float most, float top, float& scale, 
 template <int KEEP>
 __device__ __forceinline__ uint32_t keep_codes4(float a, float b, float c, float d) {
   if (KEEP == DICE_KEEP_INT8) {
-    // rounded to nearest even; what a NaN gives is never read (its scale is NaN)
-    const uint32_t ia = __float2int_rn(a), ib = __float2int_rn(b), ic = __float2int_rn(c), id = __float2int_rn(d);
-    return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
+    // adding 1.5 * 2^23 rounds to an integer (ties to even) and leaves it in the low byte; the conversion instruction
+    // would take the pipe of exp and reciprocal, which the activation needs.  What a NaN gives is never read (its
+    // scale is NaN).
+    // (__fadd_rn: fused with the caller's multiplication the sum would round once, and ties elsewhere.)
+    const float kRound = 12582912.0f;
+    return __byte_perm(__byte_perm(__float_as_uint(__fadd_rn(a, kRound)), __float_as_uint(__fadd_rn(b, kRound)), 0x0040),
+                       __byte_perm(__float_as_uint(__fadd_rn(c, kRound)), __float_as_uint(__fadd_rn(d, kRound)), 0x0040), 0x5410);
   }
   uint16_t lo, hi;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
@@ -85,8 +98,13 @@ __device__ __forceinline__ uint32_t keep_codes4(float a, float b, float c, float
 template <int KEEP>
 __device__ __forceinline__ void keep_read4(uint32_t w, float scale, float* v) {
   if (KEEP == DICE_KEEP_INT8) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i))) * scale;
+    // the byte plus 128 becomes the low mantissa bits of 2^23: exact, and again without the conversion instruction
+    const uint32_t biased = w ^ 0x80808080u;
+    const uint32_t kBase = 0x4b000000u;
+    v[0] = (__uint_as_float(__byte_perm(biased, kBase, 0x7540)) - 8388736.0f) * scale;
+    v[1] = (__uint_as_float(__byte_perm(biased, kBase, 0x7541)) - 8388736.0f) * scale;
+    v[2] = (__uint_as_float(__byte_perm(biased, kBase, 0x7542)) - 8388736.0f) * scale;
+    v[3] = (__uint_as_float(__byte_perm(biased, kBase, 0x7543)) - 8388736.0f) * scale;
   } else {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {

@@ -17,6 +17,14 @@
 // "full" barrier in their place.  All other blocks go from the copies to the tensor cores directly.  (The leader expects
 // both CTAs' bytes; a peer that announced its own with a cluster-scope arrival cost twice the time of a block.)
 //
+// Two products have the activation in their epilogue, so that neither its argument nor its gradient passes through
+// memory in 16 bits between two kernels:
+//   NT + EPI_KEEP  the first forward product (rows and weights as they lie): a warp pair holds a row's 128 columns of a
+//                  group in registers, rounds them to bf16, makes the group's scale, and writes the activation and the
+//                  8-bit codes.  SwiGLU's packed order makes a 256-column tile one group of gate and one of up columns.
+//   NN + EPI_BACK  the second product's input gradient: every column's gradient meets the codes of its argument in fp32
+//                  and leaves as the argument's gradient, beside the activation for the weight gradient behind it.
+//
 // Few tiles and a long reduction: the pairs that would idle take a share of the reduction each (split).  Every epilogue
 // warp files its part of the sum in fp32; the last one to arrive at a part adds them up in the order of the shares, so
 // the result does not depend on who was last.
@@ -29,16 +37,19 @@ using namespace dice_umma;
 
 namespace {
 
-enum { MODE_NN = 1, MODE_TN = 2 };
+enum { MODE_NT = 0, MODE_NN = 1, MODE_TN = 2 };
+enum { EPI_PLAIN = 0, EPI_KEEP = 1, EPI_BACK = 2 };
 
 constexpr int PM = 256;
 constexpr int kStagesT = 6;
 constexpr int kStageBytesT = 32768;  // 128 rows (or columns) x 64 of each operand
 constexpr int kOperandBytes = 16384;
 constexpr int kBoxBytes = 8192;      // 64 reduction rows x 128 bytes
-constexpr int kThreadsT = 352;       // warp 0 loader, 1 tensor-core issue, 2..9 epilogue, 10 ragged ends
+// warp 0 loader, 1 tensor-core issue, 2..9 epilogue, TN: 10 ragged ends
+constexpr int threads_of(int mode) { return mode == MODE_TN ? 352 : 320; }
 constexpr int kStageStore = 2048;    // per epilogue warp, as in grouped_gemm_pair.cu
-constexpr int kSmemT = kStagesT * kStageBytesT + kAuxBytes + kEpilogueWarps * kStageStore + 1024;
+constexpr int kExchangeBytes = 4096;  // EPI_KEEP, SwiGLU: group maxima, [2 tiles][2 halves][gate, up][128 rows]
+constexpr int kSmemT = kStagesT * kStageBytesT + kAuxBytes + kEpilogueWarps * kStageStore + kExchangeBytes + 1024;
 constexpr int kSplitFloats = 4 * 32 * 32;  // an epilogue warp's part of a tile: 4 chunks of 32 rows x 32 columns
 constexpr int kMinSplitBlocks = 4;         // k-blocks of a share, at least
 
@@ -58,6 +69,13 @@ struct TrainGemm {
   float* split_ws;  // NULL: no split.  [pair][cta][epilogue warp][kSplitFloats]
   unsigned int* split_count;  // zero on entry: [tile][cta][epilogue warp]
   uint32_t* status;
+  // EPI_KEEP and EPI_BACK: `out` is d_pre (EPI_BACK) or pre (EPI_KEEP that keeps it), its rows are arg_cols wide
+  int ffn, arg_cols, groups;
+  __nv_bfloat16* act_out;
+  const void* kept;             // EPI_BACK: codes or pre
+  const float* kept_scales;
+  uint8_t* codes;               // EPI_KEEP
+  float* scales;
 };
 
 // Shared-memory operand descriptor of an MN-major tile: boxes of 64 reduction rows x 128 bytes with the 128-byte
@@ -85,8 +103,253 @@ __device__ __forceinline__ void mbar_complete_tx_cluster(uint32_t cluster_addr, 
 __device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-template <int MODE>
-__global__ void __launch_bounds__(kThreadsT, 1)
+// 32 rows of 64 bytes that a warp holds one row per lane, stored so that an instruction covers whole 64-byte pieces:
+// through shared memory, where lane l then takes piece (l & 3) of rows (l >> 2) + 8 i.  `put(i, piece, v)` stores one.
+template <typename F>
+__device__ __forceinline__ void store_transposed(uint4* buf, int lane, const uint4 (&mine)[4], F put) {
+  const int swz = (lane >> 1) & 3;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) buf[lane * 4 + (j ^ swz)] = mine[j];
+  __syncwarp();
+  const int piece = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int rr = i * 8 + (lane >> 2);
+    put(i, piece, buf[rr * 4 + (piece ^ ((rr >> 1) & 3))]);
+  }
+  __syncwarp();
+}
+__device__ __forceinline__ uint4 pack8(const float* v) {
+  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+
+// EPI_KEEP: one tile of the first product, by one of the two warps that share 32 rows.  SwiGLU: the tile's columns are
+// 128 gate and 128 up columns of the same 128 activations, a warp takes 64 of them, and the two warps exchange their parts
+// of the groups' maxima; GELU: the tile is two groups, a warp takes one.  Columns behind ffn count as zeros.
+template <int ACT, int KEEP, typename Fetch, typename Store>
+__device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, int half, int lane, int row, bool row_ok,
+                                          const int64_t (&dst_row)[4], uint4* stage_buf, float* exchange, uint32_t bar,
+                                          uint32_t phase, volatile uint32_t* abort_flag, Fetch fetch, Store store_bf16) {
+  constexpr bool GLU = ACT == DICE_ACT_SWIGLU;
+  // this warp's first activation column, and how many of its 64 (GELU: 128) exist
+  const int act0 = GLU ? nb * 128 + half * 64 : nb * 256 + half * 128;
+  int valid = p.ffn - act0;
+  valid = valid < 0 ? 0 : (valid > (GLU ? 64 : 128) ? (GLU ? 64 : 128) : valid);
+  // four chunks of 32 columns of the argument, rounded to bf16: SwiGLU gate, gate, up, up; GELU four in a row
+  uint32_t w[4][16];
+  float most[2] = {0.f, 0.f};  // gate and up (GELU: the first)
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int left = valid - (GLU ? (q & 1) : q) * 32;
+    if (left > 0) {
+      float v[32];
+      fetch(GLU ? (q >> 1) * 128 + half * 64 + (q & 1) * 32 : half * 128 + q * 32, v);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        w[q][j] = 2 * j < left ? pack_bf16x2(v[2 * j], v[2 * j + 1]) : 0u;  // (valid is a multiple of 8)
+        if (KEEP != DICE_KEEP_NONE) {
+          float& m = most[GLU ? q >> 1 : 0];
+          m = max_nan(m, max_nan(fabsf(bf16lo_to_f32(w[q][j])), fabsf(bf16hi_to_f32(w[q][j]))));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) w[q][j] = 0u;
+    }
+  }
+  float scale[2], factor[2];
+  if (KEEP != DICE_KEEP_NONE) {
+    if (GLU) {
+      // two buffers in turn: a warp writes the next tile's only after the other has read this one's predecessor
+      float* buf = exchange + phase * 512;
+      const int r = quad * 32 + lane;
+      buf[half * 256 + r] = most[0];
+      buf[half * 256 + 128 + r] = most[1];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+      // (should the other warp have given up, the values below are of no use, but nothing waits for them)
+      mbar_wait(bar, phase, abort_flag, p.status, DICE_STATUS_WAIT_ACC_FULL);
+      most[0] = max_nan(most[0], buf[(half ^ 1) * 256 + r]);
+      most[1] = max_nan(most[1], buf[(half ^ 1) * 256 + 128 + r]);
+    }
+#pragma unroll
+    for (int g = 0; g < (GLU ? 2 : 1); ++g) keep_scale(most[g], keep_top(KEEP), scale[g], factor[g]);
+    if (row_ok && (GLU || valid > 0))
+      p.scales[static_cast<int64_t>(row) * p.groups + nb * 2 + half] = GLU && half ? scale[1] : scale[0];
+  }
+  // the activation
+#pragma unroll
+  for (int q = 0; q < (GLU ? 2 : 4); ++q) {
+    if (valid > q * 32) {
+      uint4 o[4];
+      uint32_t* ow = reinterpret_cast<uint32_t*>(o);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float x0 = bf16lo_to_f32(w[q][j]), x1 = bf16hi_to_f32(w[q][j]);
+        if (GLU)
+          ow[j] = pack_bf16x2(x0 * sigmoid_t<false>(x0) * bf16lo_to_f32(w[q + 2][j]), x1 * sigmoid_t<false>(x1) * bf16hi_to_f32(w[q + 2][j]));
+        else
+          ow[j] = pack_bf16x2(gelu_t<false>(x0), gelu_t<false>(x1));
+      }
+      store_bf16(o, p.act_out, p.ffn, act0 + q * 32, valid - q * 32);
+    }
+  }
+  // what is kept: SwiGLU all 64 gate and 64 up columns (the filling ones are zeros), GELU those that exist
+  if (KEEP == DICE_KEEP_NONE) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int left = GLU ? 32 : valid - q * 32;
+      if (left > 0) {
+        uint4 o[4];
+        uint32_t* ow = reinterpret_cast<uint32_t*>(o);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) ow[j] = w[q][j];
+        store_bf16(o, p.out, p.arg_cols, GLU ? nb * 256 + (q >> 1) * 128 + half * 64 + (q & 1) * 32 : act0 + q * 32, left);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {  // 64 codes each
+      const int left = GLU ? 64 : valid - g * 64;
+      if (left > 0) {
+        const float f = GLU ? factor[g] : factor[0];
+        uint4 o[4];
+        uint32_t* ow = reinterpret_cast<uint32_t*>(o);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const uint32_t lo = w[2 * g + (j >> 3)][(j & 7) * 2], hi = w[2 * g + (j >> 3)][(j & 7) * 2 + 1];
+          ow[j] = keep_codes4<KEEP>(bf16lo_to_f32(lo) * f, bf16hi_to_f32(lo) * f, bf16lo_to_f32(hi) * f, bf16hi_to_f32(hi) * f);
+        }
+        const int c = GLU ? nb * 256 + g * 128 + half * 64 : act0 + g * 64;
+        store_transposed(stage_buf, lane, o, [&](int i, int piece, const uint4& v) {
+          if (dst_row[i] < 0) return;
+          uint8_t* dst = p.codes + dst_row[i] * p.arg_cols + c + piece * 16;
+          // a row of GELU codes may start on 8 bytes only, and end in the middle of a piece
+          if (GLU || (piece * 16 + 16 <= left && (p.arg_cols & 15) == 0)) {
+            *reinterpret_cast<uint4*>(dst) = v;
+          } else {
+            if (piece * 16 < left) *reinterpret_cast<uint2*>(dst) = make_uint2(v.x, v.y);
+            if (piece * 16 + 8 < left) *reinterpret_cast<uint2*>(dst + 8) = make_uint2(v.z, v.w);
+          }
+        });
+      }
+    }
+  }
+}
+
+// 32 columns of a row's kept argument
+template <int KEEP>
+struct KeptChunk {
+  uint4 v[KEEP == DICE_KEEP_NONE ? 4 : 2];
+  float scale;
+  // at: element offset of the first column; n_left: columns that exist (a multiple of 8); aligned: 16-byte loads
+  __device__ __forceinline__ void load(const TrainGemm& p, int64_t at, const float* sc, int n_left, bool ok, bool aligned) {
+    constexpr int kVecs = KEEP == DICE_KEEP_NONE ? 4 : 2, kCols = 32 / kVecs;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) v[i] = make_uint4(0, 0, 0, 0);
+    scale = 0.f;
+    if (!ok) return;
+    if (KEEP != DICE_KEEP_NONE) scale = *sc;
+    const uint8_t* src = static_cast<const uint8_t*>(p.kept) + at * (KEEP == DICE_KEEP_NONE ? 2 : 1);
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      if (KEEP == DICE_KEEP_NONE || aligned) {
+        if (i * kCols + kCols <= n_left) v[i] = *reinterpret_cast<const uint4*>(src + i * 16);
+        else if (KEEP != DICE_KEEP_NONE && i * kCols < n_left) {
+          const uint2 lo = *reinterpret_cast<const uint2*>(src + i * 16);
+          v[i].x = lo.x;
+          v[i].y = lo.y;
+        }
+      } else {
+        if (i * kCols < n_left) {
+          const uint2 lo = *reinterpret_cast<const uint2*>(src + i * 16);
+          v[i].x = lo.x;
+          v[i].y = lo.y;
+        }
+        if (i * kCols + 8 < n_left) {
+          const uint2 hi = *reinterpret_cast<const uint2*>(src + i * 16 + 8);
+          v[i].z = hi.x;
+          v[i].w = hi.y;
+        }
+      }
+    }
+  }
+  // columns 8 g .. 8 g + 7
+  __device__ __forceinline__ void get8(int g, float (&f)[8]) const {
+    if (KEEP == DICE_KEEP_NONE) {
+      const uint4 x = v[KEEP == DICE_KEEP_NONE ? g : 0];
+      f[0] = bf16lo_to_f32(x.x); f[1] = bf16hi_to_f32(x.x); f[2] = bf16lo_to_f32(x.y); f[3] = bf16hi_to_f32(x.y);
+      f[4] = bf16lo_to_f32(x.z); f[5] = bf16hi_to_f32(x.z); f[6] = bf16lo_to_f32(x.w); f[7] = bf16hi_to_f32(x.w);
+    } else {
+      const uint4 x = v[g >> 1];
+      keep_read4<KEEP>(g & 1 ? x.z : x.x, scale, f);
+      keep_read4<KEEP>(g & 1 ? x.w : x.y, scale, f + 4);
+    }
+  }
+};
+
+// EPI_BACK: a warp's chunks of 32 columns of one tile of the activation's gradient, with SwiGLU up to the end of the
+// packed order's last block (whose filling columns get gradient zero)
+template <int ACT, int KEEP, typename Fetch, typename Store>
+__device__ __forceinline__ void back_tile(const TrainGemm& p, int nb, int half, int row, bool row_ok, Fetch fetch, Store store_bf16) {
+  constexpr bool GLU = ACT == DICE_ACT_SWIGLU;
+  const int end = GLU ? p.arg_cols / 2 : p.ffn;
+  const int stop = end - nb * BN < BN ? end - nb * BN : BN;
+  const bool aligned = GLU || (p.arg_cols & 15) == 0;
+  KeptChunk<KEEP> kg, ku;
+  auto load = [&](int c) {
+    const int col = nb * BN + c, b = col / kKeepGroup;
+    const int64_t at = static_cast<int64_t>(row) * p.arg_cols + (GLU ? col + b * kKeepGroup : col);
+    const float* sc = KEEP == DICE_KEEP_NONE ? nullptr : p.kept_scales + static_cast<int64_t>(row) * p.groups + (GLU ? 2 * b : b);
+    const int n_left = GLU ? 32 : p.ffn - col;
+    kg.load(p, at, sc, n_left, row_ok, aligned);
+    if (GLU) ku.load(p, at + kKeepGroup, sc + 1, n_left, row_ok, aligned);
+  };
+  if (half * 32 < stop) load(half * 32);
+  for (int c = half * 32; c < stop; c += 64) {
+    const int col = nb * BN + c, left = p.ffn - col;  // activation columns from here on (none: only filling)
+    float v[32];
+    if (left > 0) {
+      fetch(c, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = 0.f;
+    }
+    uint4 og[4], ou[4], oa[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float x[8], u[8], a[8];
+      kg.get8(g, x);
+      if (GLU) ku.get8(g, u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        // columns behind ffn: whatever the product left there, the gradient is zero
+        const float da = g * 8 < left ? v[g * 8 + i] : 0.f;
+        float act, slope;
+        if (GLU) {
+          silu_grad_t<false>(x[i], act, slope);
+          a[i] = act * u[i];
+          x[i] = da * u[i] * slope;
+          u[i] = da * act;
+        } else {
+          gelu_grad_t<false>(x[i], a[i], slope);
+          x[i] = da * slope;
+        }
+      }
+      og[g] = pack8(x);
+      if (GLU) ou[g] = pack8(u);
+      oa[g] = pack8(a);
+    }
+    if (c + 64 < stop) load(c + 64);  // on its way while this chunk is stored
+    const int at = GLU ? col + col / kKeepGroup * kKeepGroup : col;
+    store_bf16(og, p.out, p.arg_cols, at, GLU ? 32 : left);
+    if (GLU) store_bf16(ou, p.out, p.arg_cols, at + kKeepGroup, 32);
+    if (left > 0) store_bf16(oa, p.act_out, p.ffn, col, left);
+  }
+}
+
+template <int MODE, int EPI, int ACT, int KEEP>
+__global__ void __launch_bounds__(threads_of(MODE), 1)
 train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const TrainGemm p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -97,11 +360,12 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   const uint32_t tail_bar = smem_u32(bars + 2 * kStagesT);                  // [kStagesT] in both CTAs (TN)
   const uint32_t acc_full_bar = smem_u32(bars + 3 * kStagesT);              // [kAccStages] in both CTAs
   const uint32_t acc_empty_bar = smem_u32(bars + 3 * kStagesT + kAccStages);  // used in the leader
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * kStagesT + 2 * kAccStages);
+  const uint32_t xchg_bar = smem_u32(bars + 3 * kStagesT + 2 * kAccStages);  // [4] EPI_KEEP: a quadrant's two warps
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * kStagesT + 2 * kAccStages + 4);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   int* s_split = reinterpret_cast<int*>(tmem_slot + 2);
   int* s_seg_off = reinterpret_cast<int*>(tmem_slot + 4);
-  int* s_mprefix = s_seg_off + (kMaxSeg + 1);  // NN: first row tile of every segment
+  int* s_mprefix = s_seg_off + (kMaxSeg + 1);  // NT, NN: first row tile of every segment
   const uint32_t tiles_smem = smem_u32(smem);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -121,13 +385,14 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       mbar_init(acc_full_bar + 8 * a, 1);
       mbar_init(acc_empty_bar + 8 * a, 2 * kEpilogueWarps);
     }
+    for (int q = 0; q < 4; ++q) mbar_init(xchg_bar + 8 * q, 2);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc_pair(smem_u32(tmem_slot), kTmemCols);
   pdl_wait();
 
-  for (int i = threadIdx.x; i <= p.n_seg; i += kThreadsT) s_seg_off[i] = p.seg_offsets[i];
+  for (int i = threadIdx.x; i <= p.n_seg; i += threads_of(MODE)) s_seg_off[i] = p.seg_offsets[i];
   __syncthreads();
   if (threadIdx.x == 0) {
     int run = 0, most = 0;
@@ -158,7 +423,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     int split = 1;
     if (p.split_ws != nullptr && run > 0) {
       const int64_t per_tile = n_pairs / (static_cast<int64_t>(run) * p.n_nblk);
-      const int blocks = MODE == MODE_NN ? p.red_blocks : (most + BK - 1) / BK;
+      const int blocks = MODE != MODE_TN ? p.red_blocks : (most + BK - 1) / BK;
       split = static_cast<int>(per_tile < blocks / kMinSplitBlocks ? per_tile : blocks / kMinSplitBlocks);
       if (split < 1) split = 1;
     }
@@ -186,7 +451,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     const int m = static_cast<int>(ti.tile / p.n_nblk);
     ti.nb = static_cast<int>(ti.tile - static_cast<int64_t>(m) * p.n_nblk);
     int blocks;
-    if (MODE == MODE_NN) {
+    if (MODE != MODE_TN) {
       while (m >= s_mprefix[seg + 1]) ++seg;
       ti.mb = m - s_mprefix[seg];
       ti.row0 = s_seg_off[seg] + ti.mb * PM + static_cast<int>(cta_rank) * BM;
@@ -235,7 +500,11 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         const uint32_t leader_full = map_to_cta(full_bar + 8 * stage, 0);
         if (elect_one()) {
           if (leader) mbar_expect_tx(full_bar + 8 * stage, 2 * bytes);
-          if (MODE == MODE_NN) {
+          if (MODE == MODE_NT) {
+            tma_load_2d_pair(a_dst, &tm_a, kb * BK, ti.row0, leader_full);
+            for (int j = 0; j < b_boxes; ++j)
+              tma_load_2d_pair(b_dst + j * kBoxBytes, &tm_b, kb * BK, ti.slab * p.arg_cols + col0 + 64 * j, leader_full);
+          } else if (MODE == MODE_NN) {
             tma_load_2d_pair(a_dst, &tm_a, kb * BK, ti.row0, leader_full);
             for (int j = 0; j < b_boxes; ++j)
               tma_load_3d_pair(b_dst + j * kBoxBytes, &tm_b, col0 + 64 * j, kb * BK, ti.slab, leader_full);
@@ -264,8 +533,8 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       for (int64_t t = pair_id; alive && t < total; t += n_pairs) {
         const Tile ti = decode(t, seg);
         if (ti.kb0 == ti.kb1) continue;
-        // both operands' majors: A is K-major in NN, MN-major in TN; B is MN-major
-        const uint32_t idesc = make_instr_desc(PM, ti.n_mma) | (MODE == MODE_TN ? 1u << 15 : 0u) | (1u << 16);
+        // both operands' majors: A is MN-major in TN, B in NN and TN
+        const uint32_t idesc = make_instr_desc(PM, ti.n_mma) | (MODE == MODE_TN ? 1u << 15 : 0u) | (MODE != MODE_NT ? 1u << 16 : 0u);
         if (!mbar_wait(acc_empty_bar + 8 * acc, acc_phase ^ 1u, abort_flag, p.status, DICE_STATUS_WAIT_ACC_EMPTY)) break;
         tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
@@ -281,10 +550,10 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           }
           tc_fence_after_sync();
           const uint32_t a_addr = tiles_smem + stage * kStageBytesT;
-          const uint64_t a_desc = MODE == MODE_NN ? make_operand_desc(a_addr) : make_mn_desc(a_addr);
-          const uint64_t b_desc = make_mn_desc(a_addr + kOperandBytes);
+          const uint64_t a_desc = MODE != MODE_TN ? make_operand_desc(a_addr) : make_mn_desc(a_addr);
+          const uint64_t b_desc = MODE == MODE_NT ? make_operand_desc(a_addr + kOperandBytes) : make_mn_desc(a_addr + kOperandBytes);
           // 16 reduction elements further: 32 bytes along a K-major row, 16 rows of 128 bytes in an MN-major box
-          constexpr uint64_t kStepA = MODE == MODE_NN ? 2 : 128, kStepB = 128;
+          constexpr uint64_t kStepA = MODE != MODE_TN ? 2 : 128, kStepB = MODE == MODE_NT ? 2 : 128;
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < BK / UMMA_K; ++kk)
@@ -336,7 +605,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     const int quad = warp & 3;
     const int half = (warp - 2) >> 2;
     int acc = 0, seg = 0;
-    uint32_t acc_phase = 0;
+    uint32_t acc_phase = 0, xchg_phase = 0;
     for (int64_t t = pair_id; t < total; t += n_pairs) {
       const Tile ti = decode(t, seg);
       if (ti.zero && ti.share != 0) continue;
@@ -350,43 +619,32 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       int n_valid = p.n_cols - col0;
       if (n_valid > BN) n_valid = BN;
 
-      // rows of the output this lane stores pieces of (see store_chunk): NULL beyond the segment or the gradient
-      __nv_bfloat16* dst_rows[4];
+      // the rows of the output that this lane stores pieces of (store_transposed): -1 beyond the segment or the gradient
+      int64_t dst_row[4];
+      bool up_rows = false;  // TN with gate_up: the peer's rows are the up projection's
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int rr = quad * 32 + i * 8 + (lane >> 2);
-        dst_rows[i] = nullptr;
+        dst_row[i] = -1;
         if (rr < ti.rows_valid) {
-          if (MODE == MODE_NN) {
-            dst_rows[i] = p.out + static_cast<int64_t>(ti.row0 + rr) * p.n_cols + col0;
+          if (MODE != MODE_TN) {
+            dst_row[i] = ti.row0 + rr;
           } else if (p.gate_up == 0) {
-            dst_rows[i] = p.out + (static_cast<int64_t>(ti.slab) * p.m_rows + ti.row0 + rr) * p.n_cols + col0;
+            dst_row[i] = static_cast<int64_t>(ti.slab) * p.m_rows + ti.row0 + rr;
           } else {
             // a pair's tile is a 128-row block of gate rows (leader) and its block of up rows (peer)
             const int r = ti.mb * BM + rr;
-            if (r < p.gate_up)
-              dst_rows[i] = (leader ? p.out : p.out_up) + (static_cast<int64_t>(ti.slab) * p.gate_up + r) * p.n_cols + col0;
+            up_rows = !leader;
+            if (r < p.gate_up) dst_row[i] = static_cast<int64_t>(ti.slab) * p.gate_up + r;
           }
         }
       }
       uint4* stage_buf = reinterpret_cast<uint4*>(aux + kAuxBytes + (warp - 2) * kStageStore);
-      // 32 columns of 32 rows: a lane holds a row, the stores cover 64-byte pieces of rows
-      auto store_chunk = [&](const float (&v)[32], int c) {
-        const int swz = (lane >> 1) & 3;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          stage_buf[lane * 4 + (j ^ swz)] =
-              make_uint4(pack_bf16x2(v[8 * j + 0], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
-                         pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
-        __syncwarp();
-        const int piece = lane & 3;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int rr = i * 8 + (lane >> 2);
-          const uint4 val = stage_buf[rr * 4 + (piece ^ ((rr >> 1) & 3))];
-          if (dst_rows[i] != nullptr && piece * 8 < n_valid - c) *reinterpret_cast<uint4*>(dst_rows[i] + c + piece * 8) = val;
-        }
-        __syncwarp();
+      // 32 bf16 columns (eight words of eight) from column c of a tensor with ld columns, of which n_left exist
+      auto store_bf16 = [&](const uint4 (&w)[4], __nv_bfloat16* base, int64_t ld, int c, int n_left) {
+        store_transposed(stage_buf, lane, w, [&](int i, int piece, const uint4& v) {
+          if (dst_row[i] >= 0 && piece * 8 < n_left) *reinterpret_cast<uint4*>(base + dst_row[i] * ld + c + piece * 8) = v;
+        });
       };
 
       bool store = true;
@@ -412,30 +670,43 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         store = __shfl_sync(0xffffffffu, before, 0) == static_cast<unsigned int>(split - 1);
         __threadfence();
       }
-      if (store) {
-        const float* parts = shared_tile ? p.split_ws + ti.tile * split * kPairFloats + part + lane : nullptr;
-        for (int c = half * 32; c < n_valid; c += 64) {
-          float v[32];
-          if (shared_tile) {
+      const float* parts = shared_tile ? p.split_ws + ti.tile * split * kPairFloats + part + lane : nullptr;
+      // 32 columns of the tile from column c on, of this lane's row
+      auto fetch = [&](int c, float (&v)[32]) {
+        if (shared_tile) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0.f;
-            const float* src = parts + (c >> 6) * 1024;
-            for (int s = 0; s < split; ++s, src += kPairFloats) {
+          for (int j = 0; j < 32; ++j) v[j] = 0.f;
+          const float* src = parts + (c >> 6) * 1024;
+          for (int s = 0; s < split; ++s, src += kPairFloats) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] += __ldcg(src + j * 32);
-            }
-          } else if (summed) {
-            uint32_t a[32];
-            tmem_ld32(taddr + c, a);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(a[j]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0.f;
+            for (int j = 0; j < 32; ++j) v[j] += __ldcg(src + j * 32);
           }
-          store_chunk(v, c);
+        } else if (summed) {
+          uint32_t a[32];
+          tmem_ld32(taddr + c, a);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(a[j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = 0.f;
         }
+      };
+
+      if (EPI == EPI_PLAIN) {
+        for (int c = half * 32; store && c < n_valid; c += 64) {
+          float v[32];
+          fetch(c, v);
+          const uint4 w[4] = {pack8(v), pack8(v + 8), pack8(v + 16), pack8(v + 24)};
+          store_bf16(w, up_rows ? p.out_up : p.out, p.n_cols, col0 + c, n_valid - c);
+        }
+      } else if (EPI == EPI_KEEP) {
+        keep_tile<ACT, KEEP>(p, ti.nb, quad, half, lane, ti.row0 + quad * 32 + lane, quad * 32 + lane < ti.rows_valid, dst_row,
+                             stage_buf, reinterpret_cast<float*>(aux + kAuxBytes + kEpilogueWarps * kStageStore),
+                             xchg_bar + 8 * quad, xchg_phase, abort_flag, fetch, store_bf16);
+        xchg_phase ^= 1u;
+      } else {
+        if (store) back_tile<ACT, KEEP>(p, ti.nb, half, ti.row0 + quad * 32 + lane, quad * 32 + lane < ti.rows_valid, fetch, store_bf16);
       }
       if (summed) {
         tc_fence_before_sync();
@@ -463,18 +734,18 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
 }
 
 // CTA pairs of this kernel that can be resident at once (cached per device); 0 on error
-template <int MODE>
+template <int MODE, int EPI = EPI_PLAIN, int ACT = 0, int KEEP = 0>
 int resident_pairs_train() {
   static int cached[64] = {0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   if (cached[dev] == 0) {
-    if (cudaFuncSetAttribute(train_gemm_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemT) != cudaSuccess) return 0;
+    if (cudaFuncSetAttribute(train_gemm_kernel<MODE, EPI, ACT, KEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemT) != cudaSuccess) return 0;
     const int sms = sm_count_cached();
     if (sms <= 0) return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(sms & ~1), 1, 1);
-    cfg.blockDim = dim3(kThreadsT, 1, 1);
+    cfg.blockDim = dim3(threads_of(MODE), 1, 1);
     cfg.dynamicSmemBytes = kSmemT;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -484,19 +755,19 @@ int resident_pairs_train() {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, train_gemm_kernel<MODE>, &cfg) != cudaSuccess || n <= 0) return 0;
+    if (cudaOccupancyMaxActiveClusters(&n, train_gemm_kernel<MODE, EPI, ACT, KEEP>, &cfg) != cudaSuccess || n <= 0) return 0;
     cached[dev] = n < sms / 2 ? n : sms / 2;
   }
   return cached[dev];
 }
 
-template <int MODE>
+template <int MODE, int EPI = EPI_PLAIN, int ACT = 0, int KEEP = 0>
 int launch_train(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const TrainGemm& p, int64_t most_tiles, int pairs,
                  cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   const int64_t use = most_tiles < pairs && p.split_ws == nullptr ? most_tiles : pairs;
   cfg.gridDim = dim3(static_cast<unsigned>(2 * use), 1, 1);
-  cfg.blockDim = dim3(kThreadsT, 1, 1);
+  cfg.blockDim = dim3(threads_of(MODE), 1, 1);
   cfg.dynamicSmemBytes = kSmemT;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -509,7 +780,7 @@ int launch_train(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const TrainGe
   cfg.attrs = attr;
   cfg.numAttrs = dice_pdl_enabled() ? 2 : 1;
   dice_count_launch();
-  return cudaLaunchKernelEx(&cfg, train_gemm_kernel<MODE>, tm_a, tm_b, p) == cudaSuccess ? DICE_OK : DICE_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, train_gemm_kernel<MODE, EPI, ACT, KEEP>, tm_a, tm_b, p) == cudaSuccess ? DICE_OK : DICE_ERR_CUDA;
 }
 
 }  // namespace
@@ -562,4 +833,88 @@ int dice_internal_tc_wgrad(const void* dy, const void* x, int64_t n_rows, int n_
   p.out_up = static_cast<__nv_bfloat16*>(dw_up);
   p.status = status;
   return launch_train<MODE_TN>(tm_a, tm_b, p, static_cast<int64_t>(n_slabs) * p.n_mblk * p.n_nblk, pairs, s);
+}
+
+namespace {
+
+template <int ACT, int KEEP>
+int run_keep(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const TrainGemm& p, cudaStream_t s) {
+  const int pairs = resident_pairs_train<MODE_NT, EPI_KEEP, ACT, KEEP>();
+  if (pairs <= 0) return DICE_ERR_CUDA;
+  return launch_train<MODE_NT, EPI_KEEP, ACT, KEEP>(tm_a, tm_b, p, ((p.n_rows + PM - 1ll) / PM + p.n_seg) * p.n_nblk, pairs, s);
+}
+template <int ACT, int KEEP>
+int run_back(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const TrainGemm& p, cudaStream_t s) {
+  const int pairs = resident_pairs_train<MODE_NN, EPI_BACK, ACT, KEEP>();
+  if (pairs <= 0) return DICE_ERR_CUDA;
+  return launch_train<MODE_NN, EPI_BACK, ACT, KEEP>(tm_a, tm_b, p, ((p.n_rows + PM - 1ll) / PM + p.n_seg) * p.n_nblk, pairs, s);
+}
+template <int ACT>
+int run_epilogue(bool back, int keep, const CUtensorMap& tm_a, const CUtensorMap& tm_b, const TrainGemm& p, cudaStream_t s) {
+  switch (keep) {
+    case DICE_KEEP_INT8: return back ? run_back<ACT, DICE_KEEP_INT8>(tm_a, tm_b, p, s) : run_keep<ACT, DICE_KEEP_INT8>(tm_a, tm_b, p, s);
+    case DICE_KEEP_E4M3: return back ? run_back<ACT, DICE_KEEP_E4M3>(tm_a, tm_b, p, s) : run_keep<ACT, DICE_KEEP_E4M3>(tm_a, tm_b, p, s);
+    default: return back ? run_back<ACT, DICE_KEEP_NONE>(tm_a, tm_b, p, s) : run_keep<ACT, DICE_KEEP_NONE>(tm_a, tm_b, p, s);
+  }
+}
+
+void set_argument(TrainGemm& p, int ffn, int act) {
+  const int blocks = (ffn + kKeepGroup - 1) / kKeepGroup;
+  p.ffn = ffn;
+  p.arg_cols = act == DICE_ACT_SWIGLU ? 2 * blocks * kKeepGroup : ffn;
+  p.groups = act == DICE_ACT_SWIGLU ? 2 * blocks : blocks;
+}
+
+}  // namespace
+
+int dice_internal_tc_keep(const void* rows, int64_t n_rows, int hidden, int ffn, int act, int keep, const void* w1, int n_slabs,
+                          const int32_t* seg_offsets, int n_seg, void* pre, void* a, void* codes, float* scales,
+                          uint32_t* status, cudaStream_t s) {
+  TrainGemm p = {};
+  set_argument(p, ffn, act);
+  CUtensorMap tm_a, tm_b;
+  int rc = encode_map(&tm_a, rows, static_cast<uint64_t>(n_rows), static_cast<uint64_t>(hidden), BM);
+  if (rc == DICE_OK)
+    rc = encode_map(&tm_b, w1, static_cast<uint64_t>(n_slabs) * static_cast<uint64_t>(p.arg_cols), static_cast<uint64_t>(hidden), BK);
+  if (rc != DICE_OK) return rc;
+  p.seg_offsets = seg_offsets;
+  p.n_seg = n_seg;
+  p.n_slabs = n_slabs;
+  p.n_rows = static_cast<int>(n_rows);
+  p.red_blocks = (hidden + BK - 1) / BK;
+  p.n_nblk = (p.arg_cols + BN - 1) / BN;
+  p.n_cols = p.arg_cols;
+  p.out = static_cast<__nv_bfloat16*>(pre);
+  p.act_out = static_cast<__nv_bfloat16*>(a);
+  p.codes = static_cast<uint8_t*>(codes);
+  p.scales = scales;
+  p.status = status;
+  return act == DICE_ACT_SWIGLU ? run_epilogue<DICE_ACT_SWIGLU>(false, keep, tm_a, tm_b, p, s)
+                                : run_epilogue<DICE_ACT_GELU_TANH>(false, keep, tm_a, tm_b, p, s);
+}
+
+int dice_internal_tc_back(const void* d_out, int64_t n_rows, int hidden, int ffn, int act, int keep, const void* w2, int n_slabs,
+                          const int32_t* seg_offsets, const void* kept, const float* scales, void* d_pre, void* a,
+                          uint32_t* status, cudaStream_t s) {
+  TrainGemm p = {};
+  set_argument(p, ffn, act);
+  CUtensorMap tm_a, tm_b;
+  int rc = encode_map(&tm_a, d_out, static_cast<uint64_t>(n_rows), static_cast<uint64_t>(hidden), BM);
+  if (rc == DICE_OK)
+    rc = encode_map3(&tm_b, w2, static_cast<uint64_t>(n_slabs), static_cast<uint64_t>(hidden), static_cast<uint64_t>(ffn), BK);
+  if (rc != DICE_OK) return rc;
+  p.seg_offsets = seg_offsets;
+  p.n_seg = n_slabs;
+  p.n_slabs = n_slabs;
+  p.n_rows = static_cast<int>(n_rows);
+  p.red_blocks = (hidden + BK - 1) / BK;
+  p.n_nblk = (ffn + BN - 1) / BN;
+  p.n_cols = ffn;
+  p.out = static_cast<__nv_bfloat16*>(d_pre);
+  p.act_out = static_cast<__nv_bfloat16*>(a);
+  p.kept = kept;
+  p.kept_scales = scales;
+  p.status = status;
+  return act == DICE_ACT_SWIGLU ? run_epilogue<DICE_ACT_SWIGLU>(true, keep, tm_a, tm_b, p, s)
+                                : run_epilogue<DICE_ACT_GELU_TANH>(true, keep, tm_a, tm_b, p, s);
 }

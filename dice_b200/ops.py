@@ -766,7 +766,8 @@ def grouped_ffn_train(rows: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, se
         n_slabs, h, cols = _check_ffn(rows, w1, w2, seg_offsets, act, ffn)
         rows = rows.contiguous()
         n_rows, dev = rows.shape[0], rows.device
-        pre = torch.empty((n_rows, cols), dtype=rows.dtype, device=dev)
+        # bf16 makes the activation and the 8-bit codes in the first product's epilogue
+        pre = torch.empty((n_rows, cols), dtype=rows.dtype, device=dev) if keep is None or code == DICE_F32 else None
         a = torch.empty((n_rows, ffn), dtype=rows.dtype, device=dev)
         rows_out = torch.empty_like(rows)
         kept = KeptAct(pre, None) if keep is None else _empty_kept(n_rows, cols, keep, dev)
@@ -794,7 +795,8 @@ def grouped_ffn_backward(d_out: torch.Tensor, rows: torch.Tensor, kept: KeptAct,
         _check_kept(kept, n_rows, cols, rows.dtype)
         d_out, rows = d_out.contiguous(), rows.contiguous()
         new = lambda *shape: torch.empty(shape, dtype=rows.dtype, device=dev)  # noqa: E731
-        da, d_pre, a, d_rows = new(n_rows, ffn), new(n_rows, cols), new(n_rows, ffn), new(n_rows, h)
+        da = new(n_rows, ffn) if code == DICE_F32 else None  # bf16: stays in the product's epilogue
+        d_pre, a, d_rows = new(n_rows, cols), new(n_rows, ffn), new(n_rows, h)
         dw2 = new(n_slabs, h, ffn)
         dw1 = new(n_slabs, ffn, h)
         dw1_up = new(n_slabs, ffn, h) if act == "swiglu" else None

@@ -383,7 +383,7 @@ DICE_API int dice_combine_backward(const void* dout, const void* rows_out, const
  * one segment per slab): the first product rounded to dtype, the activation and
  * what is kept of its argument, the second product.
  *   pre   [n_rows, columns of the first product]: what is kept with keep ==
- *         NONE, else scratch
+ *         NONE, else scratch in fp32 and not used in bf16 (may be NULL)
  *   a     [n_rows, ffn] scratch */
 DICE_API int dice_grouped_ffn_train(const void* rows_in, int64_t n_rows, int hidden, int ffn, int act, int keep, int dtype,
                            const void* w1, const void* w2, int n_slabs, const int32_t* seg_offsets, int n_seg,
@@ -393,8 +393,8 @@ DICE_API int dice_grouped_ffn_train(const void* rows_in, int64_t n_rows, int hid
 /* and its backward pass from what was kept:
  *   d_out [n_rows, hidden] -> d_rows [n_rows, hidden], dw1 (and dw1_up: SWIGLU's
  *   gate and up gradients [n_slabs, ffn, hidden] apart), dw2 [n_slabs, hidden, ffn]
- *   da [n_rows, ffn], d_pre [n_rows, columns of the first product] and
- *   a [n_rows, ffn] are scratch. */
+ *   d_pre [n_rows, columns of the first product], a [n_rows, ffn] and, in fp32,
+ *   da [n_rows, ffn] are scratch (bf16: da may be NULL). */
 DICE_API int dice_grouped_ffn_backward(const void* d_out, const void* rows_in, const void* kept, const float* scales,
                               int64_t n_rows, int hidden, int ffn, int act, int keep, int dtype, const void* w1,
                               const void* w2, int n_slabs, const int32_t* seg_offsets, void* da, void* d_pre,

@@ -33,7 +33,8 @@ def test_c_abi_refuses_on_the_host():
     train = lambda act=0, h=64, ffn=64, segs=2, kp=1: lib.dice_grouped_ffn_train(  # noqa: E731
         P, 4, h, ffn, act, kp, 0, P, P, 2, P, segs, None, P, P, P, P, None, None)
     assert train(act=7) == -1 and train(h=60) == -2 and train(ffn=12) == -2 and train(segs=3) == -1
-    assert train() == -1  # no buffer for the first product
+    assert train(kp=0) == -1  # no buffer for the first product, which is what would be kept
+    assert train(kp=5) == -1
     backward = lambda act=0, up=P, dw2=P, h=64: lib.dice_grouped_ffn_backward(  # noqa: E731
         P, P, P, P, 4, h, 64, act, 1, 0, P, P, 2, P, P, P, P, P, P, up, dw2, None, None)
     assert backward(act=9) == -1 and backward(up=None) == -1 and backward(dw2=None) == -1 and backward(h=20) == -2
