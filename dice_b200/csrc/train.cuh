@@ -34,32 +34,100 @@ int dice_internal_tc_back(const void* d_out, int64_t n_rows, int hidden, int ffn
 constexpr int kKeepGroup = 128;               // columns of a kept argument that share a scale
 constexpr float kKeepFloor = 7.888609e-31f;   // 2^-100: the smallest group maximum a scale is made from
 
+// ---- two fp32 values in a register pair --------------------------------------------
+// Blackwell multiplies and adds two at a time (each rounded as the plain operation): the activation's epilogues and the
+// row-wise kernels are bounded by the instructions they issue, and these are half as many.
+typedef uint64_t f32x2;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 both(float v) { return pair(v, v); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 bf16_pair(uint32_t w) { return pair(bf16lo_to_f32(w), bf16hi_to_f32(w)); }
+__device__ __forceinline__ uint32_t to_bf16(f32x2 v) {
+  const float2 f = halves(v);
+  return pack_bf16x2(f.x, f.y);
+}
+
 // ---- activation functions and their derivatives, fp32 ------------------------------
 // gelu_tanh(p) = p/2 (1 + tanh(u)) = p sigmoid(2u), u = sqrt(2/pi) (p + 0.044715 p^3): the sigmoid form has no
 // cancellation for negative p.  EXACT (fp32 tensors) uses the correctly rounded division and expf; the other form
-// (16-bit tensors, whose rounding is 2^-9) the fast ones, good to about 2^-21.
+// (16-bit tensors, whose rounding is 2^-9) the hardware's exp2 and reciprocal, good to about 2^-21.
 template <bool EXACT>
-__device__ __forceinline__ float sigmoid_t(float x) {
-  if (EXACT) return 1.0f / (1.0f + expf(-x));
-  return __fdividef(1.0f, 1.0f + __expf(-x));
+__device__ __forceinline__ f32x2 sigmoid2(f32x2 x) {
+  if (EXACT) {
+    const float2 v = halves(x);
+    return pair(1.0f / (1.0f + expf(-v.x)), 1.0f / (1.0f + expf(-v.y)));
+  }
+  float2 t = halves(mul2(x, both(-1.4426950408889634f)));  // -log2(e) x
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t.y));
+  t = halves(add2(pair(t.x, t.y), both(1.0f)));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(t.x));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(t.y));
+  return pair(t.x, t.y);
 }
 constexpr float kGeluTwoC = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 template <bool EXACT>
-__device__ __forceinline__ float gelu_t(float p) {
-  return p * sigmoid_t<EXACT>(kGeluTwoC * fmaf(0.044715f * p * p, p, p));
-}
-// value and derivative
-template <bool EXACT>
-__device__ __forceinline__ void gelu_grad_t(float p, float& a, float& da) {
-  const float s = sigmoid_t<EXACT>(kGeluTwoC * fmaf(0.044715f * p * p, p, p));
-  a = p * s;
-  da = fmaf(a * (1.0f - s), kGeluTwoC * fmaf(3.0f * 0.044715f * p, p, 1.0f), s);
+__device__ __forceinline__ f32x2 gelu_sigmoid2(f32x2 p) {
+  return sigmoid2<EXACT>(mul2(both(kGeluTwoC), fma2(mul2(mul2(both(0.044715f), p), p), p, p)));
 }
 template <bool EXACT>
-__device__ __forceinline__ void silu_grad_t(float g, float& a, float& da) {
-  const float s = sigmoid_t<EXACT>(g);
-  a = g * s;
-  da = s * fmaf(g, 1.0f - s, 1.0f);
+__device__ __forceinline__ f32x2 gelu2(f32x2 p) {
+  return mul2(p, gelu_sigmoid2<EXACT>(p));
+}
+template <bool EXACT>
+__device__ __forceinline__ f32x2 swiglu2(f32x2 g, f32x2 u) {
+  return mul2(mul2(g, sigmoid2<EXACT>(g)), u);
+}
+// value a and derivative
+template <bool EXACT>
+__device__ __forceinline__ f32x2 gelu_grad2(f32x2 p, f32x2& a) {
+  const f32x2 s = gelu_sigmoid2<EXACT>(p), one = both(1.0f);
+  a = mul2(p, s);
+  const f32x2 inner = mul2(both(kGeluTwoC), fma2(mul2(both(3.0f * 0.044715f), p), p, one));
+  return fma2(mul2(a, fma2(s, both(-1.0f), one)), inner, s);
+}
+template <bool EXACT>
+__device__ __forceinline__ f32x2 silu_grad2(f32x2 g, f32x2& a) {
+  const f32x2 s = sigmoid2<EXACT>(g), one = both(1.0f);
+  a = mul2(g, s);
+  return mul2(s, fma2(g, fma2(s, both(-1.0f), one), one));
+}
+// the argument's gradient from the activation's (da): SwiGLU g, u -> their gradients, GELU g -> its; and the activation
+template <bool EXACT, int ACT>
+__device__ __forceinline__ f32x2 act_backward2(f32x2 da, f32x2& g, f32x2& u) {
+  f32x2 a;
+  if (ACT == DICE_ACT_SWIGLU) {
+    const f32x2 slope = silu_grad2<EXACT>(g, a), act = a;
+    g = mul2(mul2(da, u), slope);
+    a = mul2(act, u);
+    u = mul2(da, act);
+  } else {
+    g = mul2(da, gelu_grad2<EXACT>(g, a));
+  }
+  return a;
 }
 
 // ---- 8-bit codes ---------------------------------------------------------------------
@@ -78,41 +146,40 @@ __device__ __forceinline__ void keep_scale(float most, float top, float& scale, 
   factor = __fdiv_rn(top, most);
   scale = most <= 3.402823466e+38f ? __fdiv_rn(most, top) : __int_as_float(0x7fc00000);
 }
-// four codes in a word
+// four values (already times the factor) as codes in a word
 template <int KEEP>
-__device__ __forceinline__ uint32_t keep_codes4(float a, float b, float c, float d) {
+__device__ __forceinline__ uint32_t keep_codes4(f32x2 ab, f32x2 cd) {
   if (KEEP == DICE_KEEP_INT8) {
     // adding 1.5 * 2^23 rounds to an integer (ties to even) and leaves it in the low byte; the conversion instruction
     // would take the pipe of exp and reciprocal, which the activation needs.  What a NaN gives is never read (its
     // scale is NaN).
-    // (__fadd_rn: fused with the caller's multiplication the sum would round once, and ties elsewhere.)
+    // (Scalar additions: the compiler joins a two-wide one with the caller's multiplication, and the sum would round once.)
     const float kRound = 12582912.0f;
-    return __byte_perm(__byte_perm(__float_as_uint(__fadd_rn(a, kRound)), __float_as_uint(__fadd_rn(b, kRound)), 0x0040),
-                       __byte_perm(__float_as_uint(__fadd_rn(c, kRound)), __float_as_uint(__fadd_rn(d, kRound)), 0x0040), 0x5410);
+    const float2 x = halves(ab), y = halves(cd);
+    return __byte_perm(__byte_perm(__float_as_uint(__fadd_rn(x.x, kRound)), __float_as_uint(__fadd_rn(x.y, kRound)), 0x0040),
+                       __byte_perm(__float_as_uint(__fadd_rn(y.x, kRound)), __float_as_uint(__fadd_rn(y.y, kRound)), 0x0040), 0x5410);
   }
+  const float2 x = halves(ab), y = halves(cd);
   uint16_t lo, hi;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x.y), "f"(x.x));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y.y), "f"(y.x));
   return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
 }
+// and back, times the scale
 template <int KEEP>
-__device__ __forceinline__ void keep_read4(uint32_t w, float scale, float* v) {
+__device__ __forceinline__ void keep_read4(uint32_t w, f32x2 scale, f32x2& ab, f32x2& cd) {
   if (KEEP == DICE_KEEP_INT8) {
     // the byte plus 128 becomes the low mantissa bits of 2^23: exact, and again without the conversion instruction
-    const uint32_t biased = w ^ 0x80808080u;
-    const uint32_t kBase = 0x4b000000u;
-    v[0] = (__uint_as_float(__byte_perm(biased, kBase, 0x7540)) - 8388736.0f) * scale;
-    v[1] = (__uint_as_float(__byte_perm(biased, kBase, 0x7541)) - 8388736.0f) * scale;
-    v[2] = (__uint_as_float(__byte_perm(biased, kBase, 0x7542)) - 8388736.0f) * scale;
-    v[3] = (__uint_as_float(__byte_perm(biased, kBase, 0x7543)) - 8388736.0f) * scale;
+    const uint32_t biased = w ^ 0x80808080u, base = 0x4b000000u;
+    const f32x2 off = both(-8388736.0f);
+    ab = mul2(add2(pair(__uint_as_float(__byte_perm(biased, base, 0x7540)), __uint_as_float(__byte_perm(biased, base, 0x7541))), off), scale);
+    cd = mul2(add2(pair(__uint_as_float(__byte_perm(biased, base, 0x7542)), __uint_as_float(__byte_perm(biased, base, 0x7543))), off), scale);
   } else {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t h2;
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(w >> (16 * i))));
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-      v[2 * i] = f.x * scale;
-      v[2 * i + 1] = f.y * scale;
-    }
+    uint32_t lo, hi;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"(static_cast<uint16_t>(w)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"(static_cast<uint16_t>(w >> 16)));
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo)), y = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    ab = mul2(pair(x.x, x.y), scale);
+    cd = mul2(pair(y.x, y.y), scale);
   }
 }

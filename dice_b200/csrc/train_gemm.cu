@@ -46,7 +46,7 @@ constexpr int kStageBytesT = 32768;  // 128 rows (or columns) x 64 of each opera
 constexpr int kOperandBytes = 16384;
 constexpr int kBoxBytes = 8192;      // 64 reduction rows x 128 bytes
 // warp 0 loader, 1 tensor-core issue, 2..9 epilogue, TN: 10 ragged ends
-constexpr int threads_of(int mode) { return mode == MODE_TN ? 352 : 320; }
+constexpr int threads_of(int mode) { return 32 * (2 + kEpilogueWarps + (mode == MODE_TN ? 1 : 0)); }
 constexpr int kStageStore = 2048;    // per epilogue warp, as in grouped_gemm_pair.cu
 constexpr int kExchangeBytes = 4096;  // EPI_KEEP, SwiGLU: group maxima, [2 tiles][2 halves][gate, up][128 rows]
 constexpr int kSmemT = kStagesT * kStageBytesT + kAuxBytes + kEpilogueWarps * kStageStore + kExchangeBytes + 1024;
@@ -74,6 +74,7 @@ struct TrainGemm {
   __nv_bfloat16* act_out;
   const void* kept;             // EPI_BACK: codes or pre
   const float* kept_scales;
+  int kept_wide;                // its rows are whole pieces of 32 bytes
   uint8_t* codes;               // EPI_KEEP
   float* scales;
 };
@@ -137,7 +138,7 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
   valid = valid < 0 ? 0 : (valid > (GLU ? 64 : 128) ? (GLU ? 64 : 128) : valid);
   // four chunks of 32 columns of the argument, rounded to bf16: SwiGLU gate, gate, up, up; GELU four in a row
   uint32_t w[4][16];
-  float most[2] = {0.f, 0.f};  // gate and up (GELU: the first)
+  uint32_t most2[2] = {0u, 0u};  // largest magnitudes, two bf16 each: gate and up (GELU: the first)
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int left = valid - (GLU ? (q & 1) : q) * 32;
@@ -148,8 +149,8 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
       for (int j = 0; j < 16; ++j) {
         w[q][j] = 2 * j < left ? pack_bf16x2(v[2 * j], v[2 * j + 1]) : 0u;  // (valid is a multiple of 8)
         if (KEEP != DICE_KEEP_NONE) {
-          float& m = most[GLU ? q >> 1 : 0];
-          m = max_nan(m, max_nan(fabsf(bf16lo_to_f32(w[q][j])), fabsf(bf16hi_to_f32(w[q][j]))));
+          uint32_t& m = most2[GLU ? q >> 1 : 0];
+          asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[q][j] & 0x7fff7fffu));
         }
       }
     } else {
@@ -159,6 +160,9 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
   }
   float scale[2], factor[2];
   if (KEEP != DICE_KEEP_NONE) {
+    float most[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) most[g] = max_nan(bf16lo_to_f32(most2[g]), bf16hi_to_f32(most2[g]));
     if (GLU) {
       // two buffers in turn: a warp writes the next tile's only after the other has read this one's predecessor
       float* buf = exchange + phase * 512;
@@ -185,11 +189,8 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
       uint32_t* ow = reinterpret_cast<uint32_t*>(o);
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const float x0 = bf16lo_to_f32(w[q][j]), x1 = bf16hi_to_f32(w[q][j]);
-        if (GLU)
-          ow[j] = pack_bf16x2(x0 * sigmoid_t<false>(x0) * bf16lo_to_f32(w[q + 2][j]), x1 * sigmoid_t<false>(x1) * bf16hi_to_f32(w[q + 2][j]));
-        else
-          ow[j] = pack_bf16x2(gelu_t<false>(x0), gelu_t<false>(x1));
+        const f32x2 x = bf16_pair(w[q][j]);
+        ow[j] = to_bf16(GLU ? swiglu2<false>(x, bf16_pair(w[q + 2][j])) : gelu2<false>(x));
       }
       store_bf16(o, p.act_out, p.ffn, act0 + q * 32, valid - q * 32);
     }
@@ -212,13 +213,13 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
     for (int g = 0; g < 2; ++g) {  // 64 codes each
       const int left = GLU ? 64 : valid - g * 64;
       if (left > 0) {
-        const float f = GLU ? factor[g] : factor[0];
+        const f32x2 f = both(GLU ? factor[g] : factor[0]);
         uint4 o[4];
         uint32_t* ow = reinterpret_cast<uint32_t*>(o);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const uint32_t lo = w[2 * g + (j >> 3)][(j & 7) * 2], hi = w[2 * g + (j >> 3)][(j & 7) * 2 + 1];
-          ow[j] = keep_codes4<KEEP>(bf16lo_to_f32(lo) * f, bf16hi_to_f32(lo) * f, bf16lo_to_f32(hi) * f, bf16hi_to_f32(hi) * f);
+          ow[j] = keep_codes4<KEEP>(mul2(bf16_pair(lo), f), mul2(bf16_pair(hi), f));
         }
         const int c = GLU ? nb * 256 + g * 128 + half * 64 : act0 + g * 64;
         store_transposed(stage_buf, lane, o, [&](int i, int piece, const uint4& v) {
@@ -237,110 +238,111 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
   }
 }
 
+// 32 bytes in one load.  A lane holds a row of its own, so a load touches 32 lines whatever its width, and those lines
+// are what the memory path of an SM has too few of beside the operands' copies and the matrix instructions' reads (the
+// product of 32768 x 1152 x 4608 took 564 us with 16-byte loads and a scale for every 32 columns, 535 us like this; 16
+// epilogue warps in the place of 8, with stores of 32 bytes a lane, took 588).
+__device__ __forceinline__ void ld_32bytes(const void* p, uint4& a, uint4& b) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+               : "l"(p));
+}
+
 // 32 columns of a row's kept argument
 template <int KEEP>
 struct KeptChunk {
-  uint4 v[KEEP == DICE_KEEP_NONE ? 4 : 2];
-  float scale;
-  // at: element offset of the first column; n_left: columns that exist (a multiple of 8); aligned: 16-byte loads
-  __device__ __forceinline__ void load(const TrainGemm& p, int64_t at, const float* sc, int n_left, bool ok, bool aligned) {
-    constexpr int kVecs = KEEP == DICE_KEEP_NONE ? 4 : 2, kCols = 32 / kVecs;
+  static constexpr int kVecs = KEEP == DICE_KEEP_NONE ? 4 : 2, kCols = 32 / kVecs;
+  uint4 v[kVecs];
+  // at: element offset of the first column; n_left: columns that exist (a multiple of 8); wide: rows of whole 32 bytes
+  __device__ __forceinline__ void load(const TrainGemm& p, int64_t at, int n_left, bool ok) {
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) v[i] = make_uint4(0, 0, 0, 0);
-    scale = 0.f;
     if (!ok) return;
-    if (KEEP != DICE_KEEP_NONE) scale = *sc;
     const uint8_t* src = static_cast<const uint8_t*>(p.kept) + at * (KEEP == DICE_KEEP_NONE ? 2 : 1);
+    if (p.kept_wide && n_left >= 32) {
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      if (KEEP == DICE_KEEP_NONE || aligned) {
-        if (i * kCols + kCols <= n_left) v[i] = *reinterpret_cast<const uint4*>(src + i * 16);
-        else if (KEEP != DICE_KEEP_NONE && i * kCols < n_left) {
-          const uint2 lo = *reinterpret_cast<const uint2*>(src + i * 16);
-          v[i].x = lo.x;
-          v[i].y = lo.y;
-        }
-      } else {
-        if (i * kCols < n_left) {
-          const uint2 lo = *reinterpret_cast<const uint2*>(src + i * 16);
-          v[i].x = lo.x;
-          v[i].y = lo.y;
-        }
-        if (i * kCols + 8 < n_left) {
-          const uint2 hi = *reinterpret_cast<const uint2*>(src + i * 16 + 8);
-          v[i].z = hi.x;
-          v[i].w = hi.y;
+      for (int i = 0; i < kVecs; i += 2) ld_32bytes(src + i * 16, v[i], v[i + 1]);
+    } else {  // the ragged end of a row, or rows that start on 8 bytes
+#pragma unroll
+      for (int i = 0; i < 2 * kVecs; ++i) {
+        if (i * kCols / 2 < n_left) {
+          const uint2 w = *reinterpret_cast<const uint2*>(src + i * 8);
+          uint4& x = v[i >> 1];
+          if (i & 1) { x.z = w.x; x.w = w.y; }
+          else { x.x = w.x; x.y = w.y; }
         }
       }
     }
   }
   // columns 8 g .. 8 g + 7
-  __device__ __forceinline__ void get8(int g, float (&f)[8]) const {
+  __device__ __forceinline__ void get8(int g, f32x2 scale, f32x2 (&f)[4]) const {
     if (KEEP == DICE_KEEP_NONE) {
       const uint4 x = v[KEEP == DICE_KEEP_NONE ? g : 0];
-      f[0] = bf16lo_to_f32(x.x); f[1] = bf16hi_to_f32(x.x); f[2] = bf16lo_to_f32(x.y); f[3] = bf16hi_to_f32(x.y);
-      f[4] = bf16lo_to_f32(x.z); f[5] = bf16hi_to_f32(x.z); f[6] = bf16lo_to_f32(x.w); f[7] = bf16hi_to_f32(x.w);
+      f[0] = bf16_pair(x.x); f[1] = bf16_pair(x.y); f[2] = bf16_pair(x.z); f[3] = bf16_pair(x.w);
     } else {
       const uint4 x = v[g >> 1];
-      keep_read4<KEEP>(g & 1 ? x.z : x.x, scale, f);
-      keep_read4<KEEP>(g & 1 ? x.w : x.y, scale, f + 4);
+      keep_read4<KEEP>(g & 1 ? x.z : x.x, scale, f[0], f[1]);
+      keep_read4<KEEP>(g & 1 ? x.w : x.y, scale, f[2], f[3]);
     }
   }
 };
 
-// EPI_BACK: a warp's chunks of 32 columns of one tile of the activation's gradient, with SwiGLU up to the end of the
+// What an EPI_BACK warp holds of a row's kept argument: 32 columns, and the scales of their group.  A warp's share of a
+// tile is 128 columns of the activation's gradient, a group.
+template <int ACT, int KEEP>
+struct BackChunk {
+  static constexpr bool GLU = ACT == DICE_ACT_SWIGLU;
+  KeptChunk<KEEP> g, u;
+  float scale_g, scale_u;
+  __device__ __forceinline__ void load(const TrainGemm& p, int col, int row, bool ok) {
+    const int64_t at = static_cast<int64_t>(row) * p.arg_cols + (GLU ? col + col / kKeepGroup * kKeepGroup : col);
+    const int n_left = GLU ? 32 : p.ffn - col;
+    g.load(p, at, n_left, ok);
+    if (GLU) u.load(p, at + kKeepGroup, n_left, ok);
+  }
+  __device__ __forceinline__ void load_first(const TrainGemm& p, int nb, int half, int row, bool ok) {
+    const int col = nb * BN + half * 128;
+    ok = ok && col < (GLU ? p.arg_cols / 2 : p.ffn);
+    scale_g = scale_u = 0.f;
+    if (KEEP != DICE_KEEP_NONE && ok) {
+      const float* sc = p.kept_scales + static_cast<int64_t>(row) * p.groups + col / kKeepGroup * (GLU ? 2 : 1);
+      scale_g = sc[0];
+      if (GLU) scale_u = sc[1];
+    }
+    load(p, col, row, ok);
+  }
+};
+
+// EPI_BACK: a warp's 128 columns of one tile of the activation's gradient, 32 at a time, with SwiGLU up to the end of the
 // packed order's last block (whose filling columns get gradient zero)
 template <int ACT, int KEEP, typename Fetch, typename Store>
-__device__ __forceinline__ void back_tile(const TrainGemm& p, int nb, int half, int row, bool row_ok, Fetch fetch, Store store_bf16) {
+__device__ __forceinline__ void back_tile(const TrainGemm& p, int nb, int half, int row, bool row_ok, BackChunk<ACT, KEEP>& kept,
+                                          Fetch fetch, Store store_bf16) {
   constexpr bool GLU = ACT == DICE_ACT_SWIGLU;
   const int end = GLU ? p.arg_cols / 2 : p.ffn;
-  const int stop = end - nb * BN < BN ? end - nb * BN : BN;
-  const bool aligned = GLU || (p.arg_cols & 15) == 0;
-  KeptChunk<KEEP> kg, ku;
-  auto load = [&](int c) {
-    const int col = nb * BN + c, b = col / kKeepGroup;
-    const int64_t at = static_cast<int64_t>(row) * p.arg_cols + (GLU ? col + b * kKeepGroup : col);
-    const float* sc = KEEP == DICE_KEEP_NONE ? nullptr : p.kept_scales + static_cast<int64_t>(row) * p.groups + (GLU ? 2 * b : b);
-    const int n_left = GLU ? 32 : p.ffn - col;
-    kg.load(p, at, sc, n_left, row_ok, aligned);
-    if (GLU) ku.load(p, at + kKeepGroup, sc + 1, n_left, row_ok, aligned);
-  };
-  if (half * 32 < stop) load(half * 32);
-  for (int c = half * 32; c < stop; c += 64) {
-    const int col = nb * BN + c, left = p.ffn - col;  // activation columns from here on (none: only filling)
+  for (int h = 0; h < 128; h += 32) {
+    const int c = half * 128 + h, col = nb * BN + c, left = p.ffn - col;  // activation columns from here on (none: only filling)
+    if (col >= end) break;
     float v[32];
-    if (left > 0) {
-      fetch(c, v);
-    } else {
+    if (left > 0) fetch(c, v);
+    if (left < 32) {
+      // columns behind ffn: whatever the product left there, the gradient is zero
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = 0.f;
+      for (int j = 0; j < 32; ++j) v[j] = j < left ? v[j] : 0.f;
     }
     uint4 og[4], ou[4], oa[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      float x[8], u[8], a[8];
-      kg.get8(g, x);
-      if (GLU) ku.get8(g, u);
+      f32x2 x[4], u[4], a[4];
+      kept.g.get8(g, both(kept.scale_g), x);
+      if (GLU) kept.u.get8(g, both(kept.scale_u), u);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        // columns behind ffn: whatever the product left there, the gradient is zero
-        const float da = g * 8 < left ? v[g * 8 + i] : 0.f;
-        float act, slope;
-        if (GLU) {
-          silu_grad_t<false>(x[i], act, slope);
-          a[i] = act * u[i];
-          x[i] = da * u[i] * slope;
-          u[i] = da * act;
-        } else {
-          gelu_grad_t<false>(x[i], a[i], slope);
-          x[i] = da * slope;
-        }
-      }
-      og[g] = pack8(x);
-      if (GLU) ou[g] = pack8(u);
-      oa[g] = pack8(a);
+      for (int i = 0; i < 4; ++i) a[i] = act_backward2<false, ACT>(pair(v[g * 8 + 2 * i], v[g * 8 + 2 * i + 1]), x[i], u[i]);
+      og[g] = make_uint4(to_bf16(x[0]), to_bf16(x[1]), to_bf16(x[2]), to_bf16(x[3]));
+      if (GLU) ou[g] = make_uint4(to_bf16(u[0]), to_bf16(u[1]), to_bf16(u[2]), to_bf16(u[3]));
+      oa[g] = make_uint4(to_bf16(a[0]), to_bf16(a[1]), to_bf16(a[2]), to_bf16(a[3]));
     }
-    if (c + 64 < stop) load(c + 64);  // on its way while this chunk is stored
+    if (h + 32 < 128 && col + 32 < end) kept.load(p, col + 32, row, row_ok);  // on its way while this chunk is stored
     const int at = GLU ? col + col / kKeepGroup * kKeepGroup : col;
     store_bf16(og, p.out, p.arg_cols, at, GLU ? 32 : left);
     if (GLU) store_bf16(ou, p.out, p.arg_cols, at + kKeepGroup, 32);
@@ -571,7 +573,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         if (++acc == kAccStages) { acc = 0; acc_phase ^= 1u; }
       }
     }
-  } else if (warp == 10) {
+  } else if (warp == 2 + kEpilogueWarps) {
     // ---------------- ragged ends of a weight gradient's reduction (both CTAs) ----------------
     if (MODE == MODE_TN) {
       int seg = 0;
@@ -603,13 +605,15 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   } else {
     // ---------------- epilogue (both CTAs, each over its own 128 rows) ----------------
     const int quad = warp & 3;
-    const int half = (warp - 2) >> 2;
+    const int half = (warp - 2) >> 2;  // which of the quadrant's warps: its share of the columns
     int acc = 0, seg = 0;
     uint32_t acc_phase = 0, xchg_phase = 0;
     for (int64_t t = pair_id; t < total; t += n_pairs) {
       const Tile ti = decode(t, seg);
       if (ti.zero && ti.share != 0) continue;
       const bool summed = ti.kb0 != ti.kb1;  // this share has something in tensor memory
+      BackChunk<ACT, KEEP> kept;
+      if (EPI == EPI_BACK) kept.load_first(p, ti.nb, half, ti.row0 + quad * 32 + lane, quad * 32 + lane < ti.rows_valid);
       if (summed) {
         if (!mbar_wait(acc_full_bar + 8 * acc, acc_phase, abort_flag, p.status, DICE_STATUS_WAIT_ACC_FULL)) break;
         tc_fence_after_sync();
@@ -706,7 +710,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
                              xchg_bar + 8 * quad, xchg_phase, abort_flag, fetch, store_bf16);
         xchg_phase ^= 1u;
       } else {
-        if (store) back_tile<ACT, KEEP>(p, ti.nb, half, ti.row0 + quad * 32 + lane, quad * 32 + lane < ti.rows_valid, fetch, store_bf16);
+        back_tile<ACT, KEEP>(p, ti.nb, half, ti.row0 + quad * 32 + lane, quad * 32 + lane < ti.rows_valid, kept, fetch, store_bf16);
       }
       if (summed) {
         tc_fence_before_sync();
@@ -914,6 +918,7 @@ int dice_internal_tc_back(const void* d_out, int64_t n_rows, int hidden, int ffn
   p.act_out = static_cast<__nv_bfloat16*>(a);
   p.kept = kept;
   p.kept_scales = scales;
+  p.kept_wide = (reinterpret_cast<uintptr_t>(kept) & 31) == 0 && static_cast<int64_t>(p.arg_cols) * (keep == DICE_KEEP_NONE ? 2 : 1) % 32 == 0;
   p.status = status;
   return act == DICE_ACT_SWIGLU ? run_epilogue<DICE_ACT_SWIGLU>(true, keep, tm_a, tm_b, p, s)
                                 : run_epilogue<DICE_ACT_GELU_TANH>(true, keep, tm_a, tm_b, p, s);

@@ -14,6 +14,7 @@ namespace {
 constexpr int kThreadsRows = 256;
 constexpr int kHalfWarps = kThreadsRows / 16;
 
+// eight neighbouring values in their storage type, and as four pairs of fp32
 template <typename T>
 struct Vec8;
 template <>
@@ -21,9 +22,16 @@ struct Vec8<__nv_bfloat16> {
   uint4 v;
   __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = ldg_stream16(p); }
-  __device__ __forceinline__ void get(float* f) const {
-    f[0] = bf16lo_to_f32(v.x); f[1] = bf16hi_to_f32(v.x); f[2] = bf16lo_to_f32(v.y); f[3] = bf16hi_to_f32(v.y);
-    f[4] = bf16lo_to_f32(v.z); f[5] = bf16hi_to_f32(v.z); f[6] = bf16lo_to_f32(v.w); f[7] = bf16hi_to_f32(v.w);
+  __device__ __forceinline__ void get(f32x2 (&f)[4]) const {
+    f[0] = bf16_pair(v.x); f[1] = bf16_pair(v.y); f[2] = bf16_pair(v.z); f[3] = bf16_pair(v.w);
+  }
+  // largest magnitude (NaN if there is one)
+  __device__ __forceinline__ float most() const {
+    uint32_t m = v.x & 0x7fff7fffu;
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(v.y & 0x7fff7fffu));
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(v.z & 0x7fff7fffu));
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(v.w & 0x7fff7fffu));
+    return max_nan(bf16lo_to_f32(m), bf16hi_to_f32(m));
   }
 };
 template <>
@@ -34,37 +42,43 @@ struct Vec8<float> {
     v[0] = ldg_stream16(p);
     v[1] = ldg_stream16(p + 4);
   }
-  __device__ __forceinline__ void get(float* f) const {
-    f[0] = __uint_as_float(v[0].x); f[1] = __uint_as_float(v[0].y); f[2] = __uint_as_float(v[0].z); f[3] = __uint_as_float(v[0].w);
-    f[4] = __uint_as_float(v[1].x); f[5] = __uint_as_float(v[1].y); f[6] = __uint_as_float(v[1].z); f[7] = __uint_as_float(v[1].w);
+  __device__ __forceinline__ void get(f32x2 (&f)[4]) const {
+    f[0] = pair(__uint_as_float(v[0].x), __uint_as_float(v[0].y));
+    f[1] = pair(__uint_as_float(v[0].z), __uint_as_float(v[0].w));
+    f[2] = pair(__uint_as_float(v[1].x), __uint_as_float(v[1].y));
+    f[3] = pair(__uint_as_float(v[1].z), __uint_as_float(v[1].w));
+  }
+  __device__ __forceinline__ float most() const {
+    const float* f = reinterpret_cast<const float*>(v);
+    float m = fabsf(f[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(f[i]));
+    return m;
   }
 };
-__device__ __forceinline__ void put8(__nv_bfloat16* p, const float* f) {
-  stg_stream16(p, make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])));
+__device__ __forceinline__ void put8(__nv_bfloat16* p, const f32x2 (&f)[4]) {
+  stg_stream16(p, make_uint4(to_bf16(f[0]), to_bf16(f[1]), to_bf16(f[2]), to_bf16(f[3])));
 }
-__device__ __forceinline__ void put8(float* p, const float* f) {
-  stg_stream16(p, make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])));
-  stg_stream16(p + 4, make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])));
-}
-
-__device__ __forceinline__ float group_max(const float* f) {
-  float m = fabsf(f[0]);
+__device__ __forceinline__ void put8(float* p, const f32x2 (&f)[4]) {
 #pragma unroll
-  for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(f[i]));
-  const unsigned mask = 0xffffu << (threadIdx.x & 16);
-#pragma unroll
-  for (int off = 8; off > 0; off >>= 1) m = max_nan(m, __shfl_xor_sync(mask, m, off));
-  return m;
+  for (int i = 0; i < 2; ++i) {
+    const float2 x = halves(f[2 * i]), y = halves(f[2 * i + 1]);
+    stg_stream16(p + 4 * i, make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y)));
+  }
 }
 
 // eight values to their codes; the group's first lane stores the scale
-template <int KEEP>
-__device__ __forceinline__ void keep8(const float* f, uint8_t* codes, float* scale_out, bool ok) {
-  float scale, factor, q[8];
-  keep_scale(group_max(f), keep_top(KEEP), scale, factor);
+template <int KEEP, typename T>
+__device__ __forceinline__ void keep8(const Vec8<T>& v, const f32x2 (&f)[4], uint8_t* codes, float* scale_out, bool ok) {
+  float m = v.most(), scale, factor;
+  const unsigned mask = 0xffffu << (threadIdx.x & 16);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) q[i] = f[i] * factor;
-  if (ok) *reinterpret_cast<uint2*>(codes) = make_uint2(keep_codes4<KEEP>(q[0], q[1], q[2], q[3]), keep_codes4<KEEP>(q[4], q[5], q[6], q[7]));
+  for (int off = 8; off > 0; off >>= 1) m = max_nan(m, __shfl_xor_sync(mask, m, off));
+  keep_scale(m, keep_top(KEEP), scale, factor);
+  const f32x2 k = both(factor);
+  if (ok)
+    *reinterpret_cast<uint2*>(codes) =
+        make_uint2(keep_codes4<KEEP>(mul2(f[0], k), mul2(f[1], k)), keep_codes4<KEEP>(mul2(f[2], k), mul2(f[3], k)));
   if ((threadIdx.x & 15) == 0) *scale_out = scale;
 }
 
@@ -103,17 +117,17 @@ __global__ void __launch_bounds__(kThreadsRows) act_keep_kernel(const ActParams 
       v.load(static_cast<const T*>(p.in) + at);
       if (GLU) u.load(static_cast<const T*>(p.in) + at + kKeepGroup);
     }
-    float g[8], h[8], a[8];
+    f32x2 g[4], h[4], a[4];
     v.get(g);
     if (GLU) u.get(h);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = GLU ? g[i] * sigmoid_t<EXACT>(g[i]) * h[i] : gelu_t<EXACT>(g[i]);
+    for (int i = 0; i < 4; ++i) a[i] = GLU ? swiglu2<EXACT>(g[i], h[i]) : gelu2<EXACT>(g[i]);
     if (ok) put8(static_cast<T*>(p.a) + row * p.ffn + col, a);
     if (KEEP != DICE_KEEP_NONE) {
       // the packed order's filling columns get codes too (of zero)
       float* sc = p.scales + row * p.groups_in + (GLU ? 2 * b : b);
-      keep8<KEEP>(g, p.codes + at, sc, GLU || ok);
-      if (GLU) keep8<KEEP>(h, p.codes + at + kKeepGroup, sc + 1, true);
+      keep8<KEEP>(v, g, p.codes + at, sc, GLU || ok);
+      if (GLU) keep8<KEEP>(u, h, p.codes + at + kKeepGroup, sc + 1, true);
     }
   }
 }
@@ -125,7 +139,7 @@ template <typename T>
 struct Kept8<T, DICE_KEEP_NONE> {
   Vec8<T> v;
   __device__ __forceinline__ void load(const void* base, int64_t at, const float*) { v.load(static_cast<const T*>(base) + at); }
-  __device__ __forceinline__ void get(float* f) const { v.get(f); }
+  __device__ __forceinline__ void get(f32x2 (&f)[4]) const { v.get(f); }
 };
 template <typename T, int KEEP>
 struct Kept8 {
@@ -135,9 +149,9 @@ struct Kept8 {
     w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(base) + at);
     scale = *sc;
   }
-  __device__ __forceinline__ void get(float* f) const {
-    keep_read4<KEEP>(w.x, scale, f);
-    keep_read4<KEEP>(w.y, scale, f + 4);
+  __device__ __forceinline__ void get(f32x2 (&f)[4]) const {
+    keep_read4<KEEP>(w.x, both(scale), f[0], f[1]);
+    keep_read4<KEEP>(w.y, both(scale), f[2], f[3]);
   }
 };
 
@@ -158,7 +172,7 @@ __global__ void __launch_bounds__(kThreadsRows) act_backward_kernel(const ActPar
     T* d_pre = static_cast<T*>(p.d_pre) + at;
     if (col >= p.ffn) {
       if (GLU) {  // the packed order's filling columns: their gradient is zero
-        const float z[8] = {};
+        const f32x2 z[4] = {};
         put8(d_pre, z);
         put8(d_pre + kKeepGroup, z);
       }
@@ -170,24 +184,13 @@ __global__ void __launch_bounds__(kThreadsRows) act_backward_kernel(const ActPar
     d.load(static_cast<const T*>(p.in) + row * p.ffn + col);
     kg.load(p.kept, at, sc);
     if (GLU) ku.load(p.kept, at + kKeepGroup, sc + 1);
-    float da[8], g[8], u[8], a[8], dg[8];
+    f32x2 da[4], g[4], u[4], a[4];
     d.get(da);
     kg.get(g);
     if (GLU) ku.get(u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float act, slope;
-      if (GLU) {
-        silu_grad_t<EXACT>(g[i], act, slope);
-        dg[i] = da[i] * u[i] * slope;
-        a[i] = act * u[i];
-        u[i] = da[i] * act;  // the up column's gradient
-      } else {
-        gelu_grad_t<EXACT>(g[i], a[i], slope);
-        dg[i] = da[i] * slope;
-      }
-    }
-    put8(d_pre, dg);
+    for (int i = 0; i < 4; ++i) a[i] = act_backward2<EXACT, ACT>(da[i], g[i], u[i]);
+    put8(d_pre, g);
     if (GLU) put8(d_pre + kKeepGroup, u);
     if (p.a != nullptr) put8(static_cast<T*>(p.a) + row * p.ffn + col, a);
   }
@@ -242,7 +245,8 @@ combine_backward_kernel(const T* dout, const T* rows_out, const int32_t* pos, co
   const bool ok0 = pp.x >= 0 && pp.x < n_rows, ok1 = pp.y >= 0 && pp.y < n_rows;
   const T* src = dout + t * hidden;
   const int64_t o0 = static_cast<int64_t>(pp.x) * hidden, o1 = static_cast<int64_t>(pp.y) * hidden;
-  float s0 = 0.f, s1 = 0.f;
+  f32x2 d0 = 0, d1 = 0;
+  const f32x2 w0 = both(w.x), w1 = both(w.y);
   for (int c = lane * 8; c < hidden; c += 256) {
     Vec8<T> d, y0, y1;
     y0.zero();
@@ -250,27 +254,28 @@ combine_backward_kernel(const T* dout, const T* rows_out, const int32_t* pos, co
     d.load(src + c);
     if (ok0) y0.load(rows_out + o0 + c);
     if (ok1) y1.load(rows_out + o1 + c);
-    float f[8], y[8], r[8];
+    f32x2 f[4], y[4], r[4];
     d.get(f);
     if (ok0) {
       y0.get(y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        s0 = fmaf(f[i], y[i], s0);
-        r[i] = w.x * f[i];
+      for (int i = 0; i < 4; ++i) {
+        d0 = fma2(f[i], y[i], d0);
+        r[i] = mul2(w0, f[i]);
       }
       put8(d_rows + o0 + c, r);
     }
     if (ok1) {
       y1.get(y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        s1 = fmaf(f[i], y[i], s1);
-        r[i] = w.y * f[i];
+      for (int i = 0; i < 4; ++i) {
+        d1 = fma2(f[i], y[i], d1);
+        r[i] = mul2(w1, f[i]);
       }
       put8(d_rows + o1 + c, r);
     }
   }
+  float s0 = halves(d0).x + halves(d0).y, s1 = halves(d1).x + halves(d1).y;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
     s0 += __shfl_xor_sync(0xffffffffu, s0, off);

@@ -42,41 +42,27 @@ __device__ __forceinline__ void store4(float* p, const float* v) {
 }
 
 
-// acc (two neighbouring columns) += a * b; rounds as two fmaf do
-__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t a, uint64_t b) {
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
-}
-__device__ __forceinline__ uint64_t twice(float a) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(a));
-  return r;
-}
-__device__ __forceinline__ float2 halves(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
 // 8 x 8 sums of one slice: rows ra .. ra+3 and ra+STEP .. of A, columns likewise of B
 template <int DEPTH, int WIDTH, int STEP>
 __device__ __forceinline__ void multiply(const float (*As)[WIDTH + 4], const float (*Bs)[WIDTH + 4], int ra, int cb,
-                                         uint64_t (&acc)[8][4]) {
+                                         f32x2 (&acc)[8][4]) {
 #pragma unroll
   for (int k = 0; k < DEPTH; ++k) {
     float ar[8];
-    uint64_t br[4];
+    f32x2 br[4];
     *reinterpret_cast<float4*>(ar) = *reinterpret_cast<const float4*>(&As[k][ra]);
     *reinterpret_cast<float4*>(ar + 4) = *reinterpret_cast<const float4*>(&As[k][ra + STEP]);
     *reinterpret_cast<ulonglong2*>(br) = *reinterpret_cast<const ulonglong2*>(&Bs[k][cb]);
     *reinterpret_cast<ulonglong2*>(br + 2) = *reinterpret_cast<const ulonglong2*>(&Bs[k][cb + STEP]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint64_t a2 = twice(ar[i]);
+      const f32x2 a2 = both(ar[i]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) fma2(acc[i][j], a2, br[j]);
+      for (int j = 0; j < 4; ++j) acc[i][j] = fma2(a2, br[j], acc[i][j]);
     }
   }
 }
-__device__ __forceinline__ void store_tile_row(float* o, const uint64_t (&acc)[4], int c0, int step, int n_valid) {
+__device__ __forceinline__ void store_tile_row(float* o, const f32x2 (&acc)[4], int c0, int step, int n_valid) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int c = c0 + h * step;
@@ -183,7 +169,7 @@ __global__ void __launch_bounds__(64 * GROUPS, 2) simt_rows_kernel(const SimtPar
   b += share * b_slice;
   int64_t left = static_cast<int64_t>(p.red) - share * TK;  // of the reduction, from this group's slice on
 
-  uint64_t acc[8][4] = {};
+  f32x2 acc[8][4] = {};
   Slices& mine = slices[group];
   auto fetch = [&](int buf) {
     if (left > 0) {
@@ -207,7 +193,7 @@ __global__ void __launch_bounds__(64 * GROUPS, 2) simt_rows_kernel(const SimtPar
   }
 
   // groups 2 and 3 hand their sums to 0 and 1, then 1 to 0
-  uint64_t* sums = reinterpret_cast<uint64_t*>(slices);
+  f32x2* sums = reinterpret_cast<f32x2*>(slices);
 #pragma unroll
   for (int half = GROUPS / 2; half >= 1; half >>= 1) {
     __syncthreads();
@@ -219,8 +205,7 @@ __global__ void __launch_bounds__(64 * GROUPS, 2) simt_rows_kernel(const SimtPar
     if (group < half) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        const float2 x = halves(acc[i >> 2][i & 3]), y = halves(sums[group * (TM * TN / 2) + i * 64 + t]);
-        asm("mov.b64 %0, {%1, %2};" : "=l"(acc[i >> 2][i & 3]) : "f"(x.x + y.x), "f"(x.y + y.y));
+        acc[i >> 2][i & 3] = add2(acc[i >> 2][i & 3], sums[group * (TM * TN / 2) + i * 64 + t]);
       }
     }
   }
@@ -240,10 +225,9 @@ __global__ void __launch_bounds__(64 * GROUPS, 2) simt_rows_kernel(const SimtPar
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(other));
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          float y0, y1;
-          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(y0), "=f"(y1) : "r"(there + i * 512));
-          const float2 x = halves(acc[i >> 2][i & 3]);
-          asm("mov.b64 %0, {%1, %2};" : "=l"(acc[i >> 2][i & 3]) : "f"(x.x + y0), "f"(x.y + y1));
+          f32x2 y;
+          asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(y) : "r"(there + i * 512));
+          acc[i >> 2][i & 3] = add2(acc[i >> 2][i & 3], y);
         }
       }
     }
@@ -292,7 +276,7 @@ __global__ void __launch_bounds__(256, 2) simt_wgrad_kernel(const SimtParams p) 
   int left = end - row0;
 
   const int ra = (threadIdx.x >> 4) * 4, cb = (threadIdx.x & 15) * 4;
-  uint64_t acc[8][4] = {};
+  f32x2 acc[8][4] = {};
   auto fetch = [&](int buf) {
     if (left > 0) {
       copy_wide(sl.a[buf], a, p.m_cols, m_valid, left);

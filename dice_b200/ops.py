@@ -8,7 +8,6 @@ of expert-sorted rows.
 """
 from __future__ import annotations
 
-import contextlib
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -575,29 +574,55 @@ class KeptAct(NamedTuple):
 
     @property
     def keep(self) -> Optional[str]:
-        return None if self.scales is None else {v: k for k, v in KEEP_DTYPES.items()}[self.codes.dtype]
+        return None if self.scales is None else "int8" if self.codes.dtype == torch.int8 else "e4m3"
 
 
-def _on(*tensors: Optional[torch.Tensor]):
-    """The context in which kernels for these tensors are launched: their device (all have the same one), with that
-    device's current stream."""
-    _require_cuda(*tensors)
-    device = tensors[0].device
+# The small calls of a training step are bounded by the host: one token's gradients cost the GPU a few microseconds, and
+# every torch.empty with keyword arguments two, every look-up of a device half of one.  Hence one comparison per tensor
+# (_one_device), allocations through torch's own short path where it exists, and widths computed here.
+_empty_cuda = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+
+
+def _new(shape: Tuple[int, ...], dtype: torch.dtype, index: int) -> torch.Tensor:
+    """An uninitialised contiguous tensor on the current device, which is number ``index``."""
+    if _empty_cuda is not None:
+        stride = (shape[1], 1) if len(shape) == 2 else (shape[1] * shape[2], shape[2], 1)
+        return _empty_cuda(shape, stride, dtype)
+    return torch.empty(shape, dtype=dtype, device=torch.device("cuda", index))
+
+
+def _one_device(*tensors: Optional[torch.Tensor]) -> int:
+    """The number of the CUDA device that all these tensors are on."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != device:
-            raise RuntimeError(f"all tensors of a call must be on one device, got {device} and {t.device}")
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+        if t is not None and (index < 0 or t.get_device() != index):
+            _require_cuda(*tensors)
+            raise RuntimeError(f"all tensors of a call must be on one device, got {tensors[0].device} and {t.device}")
+    return index
 
 
-def _status_or_default(status: Optional[torch.Tensor], device: torch.device) -> torch.Tensor:
+def _away(index: int):
+    """Launches go to the current device's current stream: the context for tensors of another device, None for its own."""
+    return None if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def _stream_of(index: int) -> int:
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _status_ptr(status: Optional[torch.Tensor], index: int) -> int:
     if status is None:
-        if device not in _status_words and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("call dice_b200.ops.device_status(device) once before capturing a graph")
-        return device_status(device)
+        word = _status_by_index.get(index)
+        if word is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("call dice_b200.ops.device_status(device) once before capturing a graph")
+            word = _status_by_index[index] = device_status(torch.device("cuda", index)).data_ptr()
+        return word
     assert status.dtype == torch.int32 and status.numel() >= 1
-    return status
+    return status.data_ptr()
+
+
+_status_by_index = {}  # device number -> address of its status word, which lives as long as the process
 
 
 def _check_segments(seg_offsets: torch.Tensor) -> int:
@@ -607,32 +632,39 @@ def _check_segments(seg_offsets: torch.Tensor) -> int:
 
 
 def act_columns(act: str, ffn: int) -> int:
-    """Columns of an activation's argument: ``ffn``, or the packed gate / up width of SwiGLU."""
+    """Columns of an activation's argument: ``ffn``, or the packed gate / up width of SwiGLU (``w13_rows(ffn)``)."""
+    if act == "swiglu":
+        return (ffn + 127) // 128 * 256
     if act not in ACT_CODES:
         raise ValueError(f"unknown activation {act!r}")
-    return w13_rows(ffn) if act == "swiglu" else ffn
+    return ffn
 
 
 def grouped_dgrad(dy: torch.Tensor, w: torch.Tensor, seg_offsets: torch.Tensor, status: Optional[torch.Tensor] = None,
                   seg_slab: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Input gradient of :func:`grouped_gemm`: ``dx[r] = dy[r] @ w[slab(seg(r))]`` with ``dy [R, N]``,
     ``w [S, N, K]`` (bf16 or fp32).  Rows of no segment are left as they are in ``out`` (uninitialised without it)."""
-    with _on(dy, w, seg_offsets, status, seg_slab, out):
-        assert dy.dim() == 2 and w.dim() == 3 and w.shape[1] == dy.shape[1] and w.dtype == dy.dtype
-        n_seg = _check_segments(seg_offsets)
-        assert seg_slab is None or (seg_slab.dtype == torch.int32 and seg_slab.is_contiguous() and seg_slab.numel() == n_seg)
-        code = _dtype_code(dy)
-        dy, w = dy.contiguous(), w.contiguous()
-        n_rows, n_dim = dy.shape
-        n_slabs, _, k_dim = w.shape
-        if out is None:
-            out = torch.empty((n_rows, k_dim), dtype=dy.dtype, device=dy.device)
-        assert out.is_contiguous() and out.shape == (n_rows, k_dim) and out.dtype == dy.dtype
-        _lib.check(
-            _lib.load().dice_grouped_dgrad(_ptr(dy), n_rows, n_dim, _ptr(w), n_slabs, k_dim, _ptr(seg_offsets), _ptr(seg_slab),
-                                           n_seg, code, _ptr(out), _ptr(_status_or_default(status, dy.device)), _stream()),
-            "dice_grouped_dgrad",
-        )
+    index = _one_device(dy, w, seg_offsets, status, seg_slab, out)
+    away = _away(index)
+    if away is not None:
+        with away:
+            return grouped_dgrad(dy, w, seg_offsets, status, seg_slab, out)
+    assert dy.dim() == 2 and w.dim() == 3 and w.dtype == dy.dtype
+    n_seg = _check_segments(seg_offsets)
+    assert seg_slab is None or (seg_slab.dtype == torch.int32 and seg_slab.is_contiguous() and seg_slab.numel() == n_seg)
+    code = _dtype_code(dy)
+    dy, w = dy.contiguous(), w.contiguous()
+    n_rows, n_dim = dy.shape
+    n_slabs, w_rows, k_dim = w.shape
+    assert w_rows == n_dim
+    if out is None:
+        out = _new((n_rows, k_dim), dy.dtype, index)
+    assert out.is_contiguous() and out.shape == (n_rows, k_dim) and out.dtype == dy.dtype
+    _lib.check(
+        _lib.load().dice_grouped_dgrad(dy.data_ptr(), n_rows, n_dim, w.data_ptr(), n_slabs, k_dim, seg_offsets.data_ptr(),
+                                       _ptr(seg_slab), n_seg, code, out.data_ptr(), _status_ptr(status, index), _stream_of(index)),
+        "dice_grouped_dgrad",
+    )
     return out
 
 
@@ -641,39 +673,47 @@ def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, seg_offsets: torch.Tensor, 
     """Weight gradient of :func:`grouped_gemm`: ``dw[s] = dy[seg s].T @ x[seg s]`` ``[S, N, K]`` in the rows' type, zero
     for a segment without rows.  ``gate_up=ffn``: ``dy`` has the packed gate / up columns of :func:`pack_w13`, and the
     result is the pair of gradients ``[S, ffn, K]`` of the gate and the up projections."""
-    with _on(dy, x, seg_offsets, status):
-        assert dy.dim() == 2 and x.dim() == 2 and x.shape[0] == dy.shape[0] and x.dtype == dy.dtype
-        n_slabs = _check_segments(seg_offsets)
-        assert n_slabs >= 1
-        code = _dtype_code(dy)
-        dy, x = dy.contiguous(), x.contiguous()
-        n_rows, n_dim = dy.shape
-        k_dim = x.shape[1]
-        rows = gate_up if gate_up else n_dim
-        dw = torch.empty((n_slabs, rows, k_dim), dtype=dy.dtype, device=dy.device)
-        dw_up = torch.empty_like(dw) if gate_up else None
-        _lib.check(
-            _lib.load().dice_grouped_wgrad(_ptr(dy), _ptr(x), n_rows, n_dim, k_dim, _ptr(seg_offsets), n_slabs, gate_up or 0,
-                                           code, _ptr(dw), _ptr(dw_up), _ptr(_status_or_default(status, dy.device)), _stream()),
-            "dice_grouped_wgrad",
-        )
+    index = _one_device(dy, x, seg_offsets, status)
+    away = _away(index)
+    if away is not None:
+        with away:
+            return grouped_wgrad(dy, x, seg_offsets, status, gate_up)
+    assert dy.dim() == 2 and x.dim() == 2 and x.dtype == dy.dtype
+    n_slabs = _check_segments(seg_offsets)
+    assert n_slabs >= 1
+    code = _dtype_code(dy)
+    dy, x = dy.contiguous(), x.contiguous()
+    n_rows, n_dim = dy.shape
+    x_rows, k_dim = x.shape
+    assert x_rows == n_rows
+    shape = (n_slabs, gate_up or n_dim, k_dim)
+    dw = _new(shape, dy.dtype, index)
+    dw_up = _new(shape, dy.dtype, index) if gate_up else None
+    _lib.check(
+        _lib.load().dice_grouped_wgrad(dy.data_ptr(), x.data_ptr(), n_rows, n_dim, k_dim, seg_offsets.data_ptr(), n_slabs,
+                                       gate_up or 0, code, dw.data_ptr(), _ptr(dw_up), _status_ptr(status, index),
+                                       _stream_of(index)),
+        "dice_grouped_wgrad",
+    )
     return (dw, dw_up) if gate_up else dw
 
 
-def _empty_kept(n_rows: int, cols: int, keep: str, device) -> KeptAct:
-    return KeptAct(torch.empty((n_rows, cols), dtype=KEEP_DTYPES[keep], device=device),
-                   torch.empty((n_rows, (cols + KEEP_GROUP - 1) // KEEP_GROUP), dtype=torch.float32, device=device))
+def _groups(cols: int) -> int:
+    return (cols + KEEP_GROUP - 1) // KEEP_GROUP
 
 
-def _check_kept(kept: KeptAct, n_rows: int, cols: int, dtype: torch.dtype) -> None:
-    assert kept.codes.shape == (n_rows, cols) and kept.codes.is_contiguous()
-    if kept.scales is None:
-        assert kept.codes.dtype == dtype
-        return
-    if kept.codes.dtype not in KEEP_DTYPES.values():
-        raise TypeError(f"codes are int8 or float8_e4m3fn, got {kept.codes.dtype}")
-    assert kept.scales.dtype == torch.float32 and kept.scales.is_contiguous()
-    assert kept.scales.shape == (n_rows, (cols + KEEP_GROUP - 1) // KEEP_GROUP)
+def _check_kept(codes: torch.Tensor, scales: Optional[torch.Tensor], n_rows: int, cols: int, dtype: torch.dtype) -> int:
+    """The keep code of what was kept for ``n_rows`` rows of ``cols`` columns."""
+    assert codes.shape == (n_rows, cols) and codes.is_contiguous()
+    if scales is None:
+        assert codes.dtype == dtype
+        return 0
+    assert scales.dtype == torch.float32 and scales.is_contiguous() and scales.shape == (n_rows, _groups(cols))
+    if codes.dtype == torch.int8:
+        return 1
+    if codes.dtype != torch.float8_e4m3fn:
+        raise TypeError(f"codes are int8 or float8_e4m3fn, got {codes.dtype}")
+    return 2
 
 
 def _check_keep(keep: Optional[str]) -> None:
@@ -686,18 +726,28 @@ def act_keep(pre: torch.Tensor, act: str, ffn: int, keep: Optional[str] = "int8"
     ``[R, ffn]``) and, in the same pass, ``pre`` in 8 bits for :func:`act_backward`: every row's 128 columns share a
     scale.  ``keep=None`` keeps ``pre`` itself."""
     _check_keep(keep)
-    with _on(pre):
-        assert pre.dim() == 2 and pre.shape[1] == act_columns(act, ffn)
-        code = _dtype_code(pre)
-        pre = pre.contiguous()
-        n_rows, cols = pre.shape
-        a = torch.empty((n_rows, ffn), dtype=pre.dtype, device=pre.device)
-        kept = KeptAct(pre, None) if keep is None else _empty_kept(n_rows, cols, keep, pre.device)
-        _lib.check(
-            _lib.load().dice_act_keep(_ptr(pre), n_rows, ffn, ACT_CODES[act], KEEP_CODES[keep], code, _ptr(a),
-                                      None if keep is None else _ptr(kept.codes), _ptr(kept.scales), _stream()),
-            "dice_act_keep",
-        )
+    index = _one_device(pre)
+    away = _away(index)
+    if away is not None:
+        with away:
+            return act_keep(pre, act, ffn, keep)
+    cols = act_columns(act, ffn)
+    assert pre.dim() == 2
+    code = _dtype_code(pre)
+    pre = pre.contiguous()
+    n_rows, pre_cols = pre.shape
+    assert pre_cols == cols
+    a = _new((n_rows, ffn), pre.dtype, index)
+    if keep is None:
+        kept, codes_ptr, scales_ptr = KeptAct(pre, None), None, None
+    else:
+        kept = KeptAct(_new((n_rows, cols), KEEP_DTYPES[keep], index), _new((n_rows, _groups(cols)), torch.float32, index))
+        codes_ptr, scales_ptr = kept.codes.data_ptr(), kept.scales.data_ptr()
+    _lib.check(
+        _lib.load().dice_act_keep(pre.data_ptr(), n_rows, ffn, ACT_CODES[act], KEEP_CODES[keep], code, a.data_ptr(), codes_ptr,
+                                  scales_ptr, _stream_of(index)),
+        "dice_act_keep",
+    )
     return a, kept
 
 
@@ -706,20 +756,25 @@ def act_backward(da: torch.Tensor, kept: KeptAct, act: str, ffn: int, want_act: 
     kept; ``a`` is the activation of the kept argument (None without ``want_act``), which the second product's weight
     gradient needs."""
     codes, scales = kept
-    with _on(da, codes, scales):
-        cols = act_columns(act, ffn)
-        assert da.dim() == 2 and da.shape[1] == ffn
-        code = _dtype_code(da)
-        n_rows = da.shape[0]
-        _check_kept(kept, n_rows, cols, da.dtype)
-        da = da.contiguous()
-        d_pre = torch.empty((n_rows, cols), dtype=da.dtype, device=da.device)
-        a = torch.empty_like(da) if want_act else None
-        _lib.check(
-            _lib.load().dice_act_backward(_ptr(da), _ptr(codes), _ptr(scales), n_rows, ffn, ACT_CODES[act],
-                                          KEEP_CODES[kept.keep], code, _ptr(d_pre), _ptr(a), _stream()),
-            "dice_act_backward",
-        )
+    index = _one_device(da, codes, scales)
+    away = _away(index)
+    if away is not None:
+        with away:
+            return act_backward(da, kept, act, ffn, want_act)
+    cols = act_columns(act, ffn)
+    assert da.dim() == 2
+    code = _dtype_code(da)
+    n_rows, da_cols = da.shape
+    assert da_cols == ffn
+    keep = _check_kept(codes, scales, n_rows, cols, da.dtype)
+    da = da.contiguous()
+    d_pre = _new((n_rows, cols), da.dtype, index)
+    a = _new((n_rows, ffn), da.dtype, index) if want_act else None
+    _lib.check(
+        _lib.load().dice_act_backward(da.data_ptr(), codes.data_ptr(), _ptr(scales), n_rows, ffn, ACT_CODES[act], keep, code,
+                                      d_pre.data_ptr(), _ptr(a), _stream_of(index)),
+        "dice_act_backward",
+    )
     return d_pre, a
 
 
@@ -728,20 +783,26 @@ def combine_backward(dout: torch.Tensor, rows_out: torch.Tensor, pos: torch.Tens
     ``d_rows[pos[t, s]] = weights[t, s] * dout[t]`` and ``d_weights [N, 2]`` fp32 ``= <dout[t], rows_out[pos[t, s]]>``.
     ``pos`` int32 ``[N, 2]`` names no row twice (a plan's); rows that it does not name are left uninitialised, a
     position outside ``rows_out`` has gradient 0."""
-    with _on(dout, rows_out, pos, weights):
-        assert dout.dim() == 2 and rows_out.dim() == 2 and dout.shape[1] == rows_out.shape[1] and rows_out.dtype == dout.dtype
-        n_tokens, h = dout.shape
-        assert pos.dtype == torch.int32 and pos.shape == (n_tokens, 2)
-        assert weights.dtype == torch.float32 and weights.shape == (n_tokens, 2)
-        code = _dtype_code(dout)
-        dout, rows_out, pos, weights = dout.contiguous(), rows_out.contiguous(), pos.contiguous(), weights.contiguous()
-        d_rows = torch.empty_like(rows_out)
-        d_weights = torch.empty((n_tokens, 2), dtype=torch.float32, device=dout.device)
-        _lib.check(
-            _lib.load().dice_combine_backward(_ptr(dout), _ptr(rows_out), _ptr(pos), _ptr(weights), n_tokens,
-                                              rows_out.shape[0], h, code, _ptr(d_rows), _ptr(d_weights), _stream()),
-            "dice_combine_backward",
-        )
+    index = _one_device(dout, rows_out, pos, weights)
+    away = _away(index)
+    if away is not None:
+        with away:
+            return combine_backward(dout, rows_out, pos, weights)
+    assert dout.dim() == 2 and rows_out.dim() == 2 and rows_out.dtype == dout.dtype
+    n_tokens, h = dout.shape
+    n_rows, row_cols = rows_out.shape
+    assert row_cols == h
+    assert pos.dtype == torch.int32 and pos.shape == (n_tokens, 2)
+    assert weights.dtype == torch.float32 and weights.shape == (n_tokens, 2)
+    code = _dtype_code(dout)
+    dout, rows_out, pos, weights = dout.contiguous(), rows_out.contiguous(), pos.contiguous(), weights.contiguous()
+    d_rows = _new((n_rows, h), dout.dtype, index)
+    d_weights = _new((n_tokens, 2), torch.float32, index)
+    _lib.check(
+        _lib.load().dice_combine_backward(dout.data_ptr(), rows_out.data_ptr(), pos.data_ptr(), weights.data_ptr(), n_tokens,
+                                          n_rows, h, code, d_rows.data_ptr(), d_weights.data_ptr(), _stream_of(index)),
+        "dice_combine_backward",
+    )
     return d_rows, d_weights
 
 
@@ -761,24 +822,31 @@ def grouped_ffn_train(rows: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, se
     (``keep`` "int8" or "e4m3") or as it is (None), for :func:`grouped_ffn_backward`.  The first product is rounded to
     the rows' type before the activation.  bf16, or fp32 on the CUDA cores."""
     _check_keep(keep)
-    with _on(rows, w1, w2, seg_offsets, status):
-        code = _dtype_code(rows)
-        n_slabs, h, cols = _check_ffn(rows, w1, w2, seg_offsets, act, ffn)
-        rows = rows.contiguous()
-        n_rows, dev = rows.shape[0], rows.device
-        # bf16 makes the activation and the 8-bit codes in the first product's epilogue
-        pre = torch.empty((n_rows, cols), dtype=rows.dtype, device=dev) if keep is None or code == DICE_F32 else None
-        a = torch.empty((n_rows, ffn), dtype=rows.dtype, device=dev)
-        rows_out = torch.empty_like(rows)
-        kept = KeptAct(pre, None) if keep is None else _empty_kept(n_rows, cols, keep, dev)
-        _lib.check(
-            _lib.load().dice_grouped_ffn_train(
-                _ptr(rows), n_rows, h, ffn, ACT_CODES[act], KEEP_CODES[keep], code, _ptr(w1), _ptr(w2), n_slabs,
-                _ptr(seg_offsets), n_slabs, _ptr(pre), _ptr(a), None if keep is None else _ptr(kept.codes), _ptr(kept.scales),
-                _ptr(rows_out), _ptr(_status_or_default(status, dev)), _stream(),
-            ),
-            "dice_grouped_ffn_train",
-        )
+    index = _one_device(rows, w1, w2, seg_offsets, status)
+    away = _away(index)
+    if away is not None:
+        with away:
+            return grouped_ffn_train(rows, w1, w2, seg_offsets, act, ffn, status, keep)
+    code = _dtype_code(rows)
+    n_slabs, h, cols = _check_ffn(rows, w1, w2, seg_offsets, act, ffn)
+    rows = rows.contiguous()
+    n_rows, dt = rows.shape[0], rows.dtype
+    # bf16 makes the activation and the 8-bit codes in the first product's epilogue
+    pre = _new((n_rows, cols), dt, index) if keep is None or code == DICE_F32 else None
+    a = _new((n_rows, ffn), dt, index)
+    rows_out = _new((n_rows, h), dt, index)
+    if keep is None:
+        kept = KeptAct(pre, None)
+    else:
+        kept = KeptAct(_new((n_rows, cols), KEEP_DTYPES[keep], index), _new((n_rows, _groups(cols)), torch.float32, index))
+    _lib.check(
+        _lib.load().dice_grouped_ffn_train(
+            rows.data_ptr(), n_rows, h, ffn, ACT_CODES[act], KEEP_CODES[keep], code, w1.data_ptr(), w2.data_ptr(), n_slabs,
+            seg_offsets.data_ptr(), n_slabs, _ptr(pre), a.data_ptr(), None if keep is None else kept.codes.data_ptr(),
+            _ptr(kept.scales), rows_out.data_ptr(), _status_ptr(status, index), _stream_of(index),
+        ),
+        "dice_grouped_ffn_train",
+    )
     return rows_out, kept
 
 
@@ -787,25 +855,27 @@ def grouped_ffn_backward(d_out: torch.Tensor, rows: torch.Tensor, kept: KeptAct,
     """Backward pass of :func:`grouped_ffn_train` from what it kept: ``(d_rows, dw1, dw2)``; for SwiGLU ``dw1`` is the
     pair of the gate and the up projections' gradients ``[S, ffn, h]``."""
     codes, scales = kept
-    with _on(d_out, rows, codes, scales, w1, w2, seg_offsets, status):
-        code = _dtype_code(rows)
-        n_slabs, h, cols = _check_ffn(rows, w1, w2, seg_offsets, act, ffn)
-        n_rows, dev = rows.shape[0], rows.device
-        assert d_out.shape == rows.shape and d_out.dtype == rows.dtype
-        _check_kept(kept, n_rows, cols, rows.dtype)
-        d_out, rows = d_out.contiguous(), rows.contiguous()
-        new = lambda *shape: torch.empty(shape, dtype=rows.dtype, device=dev)  # noqa: E731
-        da = new(n_rows, ffn) if code == DICE_F32 else None  # bf16: stays in the product's epilogue
-        d_pre, a, d_rows = new(n_rows, cols), new(n_rows, ffn), new(n_rows, h)
-        dw2 = new(n_slabs, h, ffn)
-        dw1 = new(n_slabs, ffn, h)
-        dw1_up = new(n_slabs, ffn, h) if act == "swiglu" else None
-        _lib.check(
-            _lib.load().dice_grouped_ffn_backward(
-                _ptr(d_out), _ptr(rows), _ptr(codes), _ptr(scales), n_rows, h, ffn, ACT_CODES[act], KEEP_CODES[kept.keep], code,
-                _ptr(w1), _ptr(w2), n_slabs, _ptr(seg_offsets), _ptr(da), _ptr(d_pre), _ptr(a), _ptr(d_rows), _ptr(dw1),
-                _ptr(dw1_up), _ptr(dw2), _ptr(_status_or_default(status, dev)), _stream(),
-            ),
-            "dice_grouped_ffn_backward",
-        )
+    index = _one_device(d_out, rows, codes, scales, w1, w2, seg_offsets, status)
+    away = _away(index)
+    if away is not None:
+        with away:
+            return grouped_ffn_backward(d_out, rows, kept, w1, w2, seg_offsets, act, ffn, status)
+    code = _dtype_code(rows)
+    n_slabs, h, cols = _check_ffn(rows, w1, w2, seg_offsets, act, ffn)
+    n_rows, dt = rows.shape[0], rows.dtype
+    assert d_out.shape == rows.shape and d_out.dtype == dt
+    keep = _check_kept(codes, scales, n_rows, cols, dt)
+    d_out, rows = d_out.contiguous(), rows.contiguous()
+    da = _new((n_rows, ffn), dt, index) if code == DICE_F32 else None  # bf16: stays in the product's epilogue
+    d_pre, a, d_rows = _new((n_rows, cols), dt, index), _new((n_rows, ffn), dt, index), _new((n_rows, h), dt, index)
+    dw2, dw1 = _new((n_slabs, h, ffn), dt, index), _new((n_slabs, ffn, h), dt, index)
+    dw1_up = _new((n_slabs, ffn, h), dt, index) if act == "swiglu" else None
+    _lib.check(
+        _lib.load().dice_grouped_ffn_backward(
+            d_out.data_ptr(), rows.data_ptr(), codes.data_ptr(), _ptr(scales), n_rows, h, ffn, ACT_CODES[act], keep, code,
+            w1.data_ptr(), w2.data_ptr(), n_slabs, seg_offsets.data_ptr(), _ptr(da), d_pre.data_ptr(), a.data_ptr(),
+            d_rows.data_ptr(), dw1.data_ptr(), _ptr(dw1_up), dw2.data_ptr(), _status_ptr(status, index), _stream_of(index),
+        ),
+        "dice_grouped_ffn_backward",
+    )
     return d_rows, (dw1 if dw1_up is None else (dw1, dw1_up)), dw2
