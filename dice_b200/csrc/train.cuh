@@ -34,21 +34,33 @@ int dice_internal_tc_back(const void* d_out, int64_t n_rows, int hidden, int ffn
 constexpr int kKeepGroup = 128;               // columns of a kept argument that share a scale
 constexpr float kKeepFloor = 7.888609e-31f;   // 2^-100: the smallest group maximum a scale is made from
 
-// ---- two fp32 values in a register pair --------------------------------------------
-// Blackwell multiplies and adds two at a time (each rounded as the plain operation): the activation's epilogues and the
-// row-wise kernels are bounded by the instructions they issue, and these are half as many.
+// ---- two fp32 values --------------------------------------------------------------
+// The functions below work on two values at a time, in one of two forms that round alike: `f32x2` is a register pair for
+// Blackwell's two-wide multiplies and adds, half the instructions where those are what bounds a kernel (the products'
+// epilogues); `two` is two plain registers, which the row-wise kernels take: bounded by memory, they lose more to the
+// moves in and out of pairs than they gain (activation's backward pass at 32768 x 4608: 229 us plain, 239 two-wide).
 typedef uint64_t f32x2;
-__device__ __forceinline__ f32x2 pair(float lo, float hi) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
+struct two {
+  float x, y;
+};
+template <typename V>
+__device__ __forceinline__ V pair(float lo, float hi) {
+  if constexpr (sizeof(V) == sizeof(f32x2) && !__is_class(V)) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+  } else {
+    return V{lo, hi};
+  }
 }
-__device__ __forceinline__ float2 halves(f32x2 v) {
-  float2 r;
+template <typename V>
+__device__ __forceinline__ V both(float v) { return pair<V>(v, v); }
+__device__ __forceinline__ two halves(f32x2 v) {
+  two r;
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
   return r;
 }
-__device__ __forceinline__ f32x2 both(float v) { return pair(v, v); }
+__device__ __forceinline__ two halves(two v) { return v; }
 __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
   f32x2 r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -64,9 +76,14 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-__device__ __forceinline__ f32x2 bf16_pair(uint32_t w) { return pair(bf16lo_to_f32(w), bf16hi_to_f32(w)); }
-__device__ __forceinline__ uint32_t to_bf16(f32x2 v) {
-  const float2 f = halves(v);
+__device__ __forceinline__ two mul2(two a, two b) { return {__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y)}; }
+__device__ __forceinline__ two add2(two a, two b) { return {__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)}; }
+__device__ __forceinline__ two fma2(two a, two b, two c) { return {__fmaf_rn(a.x, b.x, c.x), __fmaf_rn(a.y, b.y, c.y)}; }
+template <typename V>
+__device__ __forceinline__ V bf16_pair(uint32_t w) { return pair<V>(bf16lo_to_f32(w), bf16hi_to_f32(w)); }
+template <typename V>
+__device__ __forceinline__ uint32_t to_bf16(V v) {
+  const two f = halves(v);
   return pack_bf16x2(f.x, f.y);
 }
 
@@ -74,53 +91,53 @@ __device__ __forceinline__ uint32_t to_bf16(f32x2 v) {
 // gelu_tanh(p) = p/2 (1 + tanh(u)) = p sigmoid(2u), u = sqrt(2/pi) (p + 0.044715 p^3): the sigmoid form has no
 // cancellation for negative p.  EXACT (fp32 tensors) uses the correctly rounded division and expf; the other form
 // (16-bit tensors, whose rounding is 2^-9) the hardware's exp2 and reciprocal, good to about 2^-21.
-template <bool EXACT>
-__device__ __forceinline__ f32x2 sigmoid2(f32x2 x) {
+template <bool EXACT, typename V>
+__device__ __forceinline__ V sigmoid2(V x) {
   if (EXACT) {
-    const float2 v = halves(x);
-    return pair(1.0f / (1.0f + expf(-v.x)), 1.0f / (1.0f + expf(-v.y)));
+    const two v = halves(x);
+    return pair<V>(1.0f / (1.0f + expf(-v.x)), 1.0f / (1.0f + expf(-v.y)));
   }
-  float2 t = halves(mul2(x, both(-1.4426950408889634f)));  // -log2(e) x
+  two t = halves(mul2(x, both<V>(-1.4426950408889634f)));  // -log2(e) x
   asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t.x));
   asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t.y));
-  t = halves(add2(pair(t.x, t.y), both(1.0f)));
+  t = halves(add2(pair<V>(t.x, t.y), both<V>(1.0f)));
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(t.x));
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(t.y));
-  return pair(t.x, t.y);
+  return pair<V>(t.x, t.y);
 }
 constexpr float kGeluTwoC = 1.5957691216057308f;  // 2 sqrt(2 / pi)
-template <bool EXACT>
-__device__ __forceinline__ f32x2 gelu_sigmoid2(f32x2 p) {
-  return sigmoid2<EXACT>(mul2(both(kGeluTwoC), fma2(mul2(mul2(both(0.044715f), p), p), p, p)));
+template <bool EXACT, typename V>
+__device__ __forceinline__ V gelu_sigmoid2(V p) {
+  return sigmoid2<EXACT>(mul2(both<V>(kGeluTwoC), fma2(mul2(mul2(both<V>(0.044715f), p), p), p, p)));
 }
-template <bool EXACT>
-__device__ __forceinline__ f32x2 gelu2(f32x2 p) {
+template <bool EXACT, typename V>
+__device__ __forceinline__ V gelu2(V p) {
   return mul2(p, gelu_sigmoid2<EXACT>(p));
 }
-template <bool EXACT>
-__device__ __forceinline__ f32x2 swiglu2(f32x2 g, f32x2 u) {
+template <bool EXACT, typename V>
+__device__ __forceinline__ V swiglu2(V g, V u) {
   return mul2(mul2(g, sigmoid2<EXACT>(g)), u);
 }
 // value a and derivative
-template <bool EXACT>
-__device__ __forceinline__ f32x2 gelu_grad2(f32x2 p, f32x2& a) {
-  const f32x2 s = gelu_sigmoid2<EXACT>(p), one = both(1.0f);
+template <bool EXACT, typename V>
+__device__ __forceinline__ V gelu_grad2(V p, V& a) {
+  const V s = gelu_sigmoid2<EXACT>(p), one = both<V>(1.0f);
   a = mul2(p, s);
-  const f32x2 inner = mul2(both(kGeluTwoC), fma2(mul2(both(3.0f * 0.044715f), p), p, one));
-  return fma2(mul2(a, fma2(s, both(-1.0f), one)), inner, s);
+  const V inner = mul2(both<V>(kGeluTwoC), fma2(mul2(both<V>(3.0f * 0.044715f), p), p, one));
+  return fma2(mul2(a, fma2(s, both<V>(-1.0f), one)), inner, s);
 }
-template <bool EXACT>
-__device__ __forceinline__ f32x2 silu_grad2(f32x2 g, f32x2& a) {
-  const f32x2 s = sigmoid2<EXACT>(g), one = both(1.0f);
+template <bool EXACT, typename V>
+__device__ __forceinline__ V silu_grad2(V g, V& a) {
+  const V s = sigmoid2<EXACT>(g), one = both<V>(1.0f);
   a = mul2(g, s);
-  return mul2(s, fma2(g, fma2(s, both(-1.0f), one), one));
+  return mul2(s, fma2(g, fma2(s, both<V>(-1.0f), one), one));
 }
 // the argument's gradient from the activation's (da): SwiGLU g, u -> their gradients, GELU g -> its; and the activation
-template <bool EXACT, int ACT>
-__device__ __forceinline__ f32x2 act_backward2(f32x2 da, f32x2& g, f32x2& u) {
-  f32x2 a;
+template <bool EXACT, int ACT, typename V>
+__device__ __forceinline__ V act_backward2(V da, V& g, V& u) {
+  V a;
   if (ACT == DICE_ACT_SWIGLU) {
-    const f32x2 slope = silu_grad2<EXACT>(g, a), act = a;
+    const V slope = silu_grad2<EXACT>(g, a), act = a;
     g = mul2(mul2(da, u), slope);
     a = mul2(act, u);
     u = mul2(da, act);
@@ -147,39 +164,39 @@ __device__ __forceinline__ void keep_scale(float most, float top, float& scale, 
   scale = most <= 3.402823466e+38f ? __fdiv_rn(most, top) : __int_as_float(0x7fc00000);
 }
 // four values (already times the factor) as codes in a word
-template <int KEEP>
-__device__ __forceinline__ uint32_t keep_codes4(f32x2 ab, f32x2 cd) {
+template <int KEEP, typename V>
+__device__ __forceinline__ uint32_t keep_codes4(V ab, V cd) {
   if (KEEP == DICE_KEEP_INT8) {
     // adding 1.5 * 2^23 rounds to an integer (ties to even) and leaves it in the low byte; the conversion instruction
     // would take the pipe of exp and reciprocal, which the activation needs.  What a NaN gives is never read (its
     // scale is NaN).
     // (Scalar additions: the compiler joins a two-wide one with the caller's multiplication, and the sum would round once.)
     const float kRound = 12582912.0f;
-    const float2 x = halves(ab), y = halves(cd);
+    const two x = halves(ab), y = halves(cd);
     return __byte_perm(__byte_perm(__float_as_uint(__fadd_rn(x.x, kRound)), __float_as_uint(__fadd_rn(x.y, kRound)), 0x0040),
                        __byte_perm(__float_as_uint(__fadd_rn(y.x, kRound)), __float_as_uint(__fadd_rn(y.y, kRound)), 0x0040), 0x5410);
   }
-  const float2 x = halves(ab), y = halves(cd);
+  const two x = halves(ab), y = halves(cd);
   uint16_t lo, hi;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x.y), "f"(x.x));
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y.y), "f"(y.x));
   return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
 }
 // and back, times the scale
-template <int KEEP>
-__device__ __forceinline__ void keep_read4(uint32_t w, f32x2 scale, f32x2& ab, f32x2& cd) {
+template <int KEEP, typename V>
+__device__ __forceinline__ void keep_read4(uint32_t w, V scale, V& ab, V& cd) {
   if (KEEP == DICE_KEEP_INT8) {
     // the byte plus 128 becomes the low mantissa bits of 2^23: exact, and again without the conversion instruction
     const uint32_t biased = w ^ 0x80808080u, base = 0x4b000000u;
-    const f32x2 off = both(-8388736.0f);
-    ab = mul2(add2(pair(__uint_as_float(__byte_perm(biased, base, 0x7540)), __uint_as_float(__byte_perm(biased, base, 0x7541))), off), scale);
-    cd = mul2(add2(pair(__uint_as_float(__byte_perm(biased, base, 0x7542)), __uint_as_float(__byte_perm(biased, base, 0x7543))), off), scale);
+    const V off = both<V>(-8388736.0f);
+    ab = mul2(add2(pair<V>(__uint_as_float(__byte_perm(biased, base, 0x7540)), __uint_as_float(__byte_perm(biased, base, 0x7541))), off), scale);
+    cd = mul2(add2(pair<V>(__uint_as_float(__byte_perm(biased, base, 0x7542)), __uint_as_float(__byte_perm(biased, base, 0x7543))), off), scale);
   } else {
     uint32_t lo, hi;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"(static_cast<uint16_t>(w)));
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"(static_cast<uint16_t>(w >> 16)));
     const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo)), y = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-    ab = mul2(pair(x.x, x.y), scale);
-    cd = mul2(pair(y.x, y.y), scale);
+    ab = mul2(pair<V>(x.x, x.y), scale);
+    cd = mul2(pair<V>(y.x, y.y), scale);
   }
 }

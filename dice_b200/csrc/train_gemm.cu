@@ -189,8 +189,8 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
       uint32_t* ow = reinterpret_cast<uint32_t*>(o);
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const f32x2 x = bf16_pair(w[q][j]);
-        ow[j] = to_bf16(GLU ? swiglu2<false>(x, bf16_pair(w[q + 2][j])) : gelu2<false>(x));
+        const f32x2 x = bf16_pair<f32x2>(w[q][j]);
+        ow[j] = to_bf16(GLU ? swiglu2<false>(x, bf16_pair<f32x2>(w[q + 2][j])) : gelu2<false>(x));
       }
       store_bf16(o, p.act_out, p.ffn, act0 + q * 32, valid - q * 32);
     }
@@ -213,13 +213,13 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
     for (int g = 0; g < 2; ++g) {  // 64 codes each
       const int left = GLU ? 64 : valid - g * 64;
       if (left > 0) {
-        const f32x2 f = both(GLU ? factor[g] : factor[0]);
+        const f32x2 f = both<f32x2>(GLU ? factor[g] : factor[0]);
         uint4 o[4];
         uint32_t* ow = reinterpret_cast<uint32_t*>(o);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const uint32_t lo = w[2 * g + (j >> 3)][(j & 7) * 2], hi = w[2 * g + (j >> 3)][(j & 7) * 2 + 1];
-          ow[j] = keep_codes4<KEEP>(mul2(bf16_pair(lo), f), mul2(bf16_pair(hi), f));
+          ow[j] = keep_codes4<KEEP>(mul2(bf16_pair<f32x2>(lo), f), mul2(bf16_pair<f32x2>(hi), f));
         }
         const int c = GLU ? nb * 256 + g * 128 + half * 64 : act0 + g * 64;
         store_transposed(stage_buf, lane, o, [&](int i, int piece, const uint4& v) {
@@ -278,7 +278,7 @@ struct KeptChunk {
   __device__ __forceinline__ void get8(int g, f32x2 scale, f32x2 (&f)[4]) const {
     if (KEEP == DICE_KEEP_NONE) {
       const uint4 x = v[KEEP == DICE_KEEP_NONE ? g : 0];
-      f[0] = bf16_pair(x.x); f[1] = bf16_pair(x.y); f[2] = bf16_pair(x.z); f[3] = bf16_pair(x.w);
+      f[0] = bf16_pair<f32x2>(x.x); f[1] = bf16_pair<f32x2>(x.y); f[2] = bf16_pair<f32x2>(x.z); f[3] = bf16_pair<f32x2>(x.w);
     } else {
       const uint4 x = v[g >> 1];
       keep_read4<KEEP>(g & 1 ? x.z : x.x, scale, f[0], f[1]);
@@ -334,10 +334,10 @@ __device__ __forceinline__ void back_tile(const TrainGemm& p, int nb, int half, 
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       f32x2 x[4], u[4], a[4];
-      kept.g.get8(g, both(kept.scale_g), x);
-      if (GLU) kept.u.get8(g, both(kept.scale_u), u);
+      kept.g.get8(g, both<f32x2>(kept.scale_g), x);
+      if (GLU) kept.u.get8(g, both<f32x2>(kept.scale_u), u);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = act_backward2<false, ACT>(pair(v[g * 8 + 2 * i], v[g * 8 + 2 * i + 1]), x[i], u[i]);
+      for (int i = 0; i < 4; ++i) a[i] = act_backward2<false, ACT>(pair<f32x2>(v[g * 8 + 2 * i], v[g * 8 + 2 * i + 1]), x[i], u[i]);
       og[g] = make_uint4(to_bf16(x[0]), to_bf16(x[1]), to_bf16(x[2]), to_bf16(x[3]));
       if (GLU) ou[g] = make_uint4(to_bf16(u[0]), to_bf16(u[1]), to_bf16(u[2]), to_bf16(u[3]));
       oa[g] = make_uint4(to_bf16(a[0]), to_bf16(a[1]), to_bf16(a[2]), to_bf16(a[3]));

@@ -14,7 +14,7 @@ namespace {
 constexpr int kThreadsRows = 256;
 constexpr int kHalfWarps = kThreadsRows / 16;
 
-// eight neighbouring values in their storage type, and as four pairs of fp32
+// eight neighbouring values in their storage type, and as four times two fp32
 template <typename T>
 struct Vec8;
 template <>
@@ -22,8 +22,8 @@ struct Vec8<__nv_bfloat16> {
   uint4 v;
   __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = ldg_stream16(p); }
-  __device__ __forceinline__ void get(f32x2 (&f)[4]) const {
-    f[0] = bf16_pair(v.x); f[1] = bf16_pair(v.y); f[2] = bf16_pair(v.z); f[3] = bf16_pair(v.w);
+  __device__ __forceinline__ void get(two (&f)[4]) const {
+    f[0] = bf16_pair<two>(v.x); f[1] = bf16_pair<two>(v.y); f[2] = bf16_pair<two>(v.z); f[3] = bf16_pair<two>(v.w);
   }
   // largest magnitude (NaN if there is one)
   __device__ __forceinline__ float most() const {
@@ -42,11 +42,11 @@ struct Vec8<float> {
     v[0] = ldg_stream16(p);
     v[1] = ldg_stream16(p + 4);
   }
-  __device__ __forceinline__ void get(f32x2 (&f)[4]) const {
-    f[0] = pair(__uint_as_float(v[0].x), __uint_as_float(v[0].y));
-    f[1] = pair(__uint_as_float(v[0].z), __uint_as_float(v[0].w));
-    f[2] = pair(__uint_as_float(v[1].x), __uint_as_float(v[1].y));
-    f[3] = pair(__uint_as_float(v[1].z), __uint_as_float(v[1].w));
+  __device__ __forceinline__ void get(two (&f)[4]) const {
+    f[0] = pair<two>(__uint_as_float(v[0].x), __uint_as_float(v[0].y));
+    f[1] = pair<two>(__uint_as_float(v[0].z), __uint_as_float(v[0].w));
+    f[2] = pair<two>(__uint_as_float(v[1].x), __uint_as_float(v[1].y));
+    f[3] = pair<two>(__uint_as_float(v[1].z), __uint_as_float(v[1].w));
   }
   __device__ __forceinline__ float most() const {
     const float* f = reinterpret_cast<const float*>(v);
@@ -56,30 +56,58 @@ struct Vec8<float> {
     return m;
   }
 };
-__device__ __forceinline__ void put8(__nv_bfloat16* p, const f32x2 (&f)[4]) {
+__device__ __forceinline__ void put8(__nv_bfloat16* p, const two (&f)[4]) {
   stg_stream16(p, make_uint4(to_bf16(f[0]), to_bf16(f[1]), to_bf16(f[2]), to_bf16(f[3])));
 }
-__device__ __forceinline__ void put8(float* p, const f32x2 (&f)[4]) {
+__device__ __forceinline__ void put8(float* p, const two (&f)[4]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float2 x = halves(f[2 * i]), y = halves(f[2 * i + 1]);
+    const two x = halves(f[2 * i]), y = halves(f[2 * i + 1]);
     stg_stream16(p + 4 * i, make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y)));
   }
 }
 
-// eight values to their codes; the group's first lane stores the scale
-template <int KEEP, typename T>
-__device__ __forceinline__ void keep8(const Vec8<T>& v, const f32x2 (&f)[4], uint8_t* codes, float* scale_out, bool ok) {
-  float m = v.most(), scale, factor;
+// The largest magnitudes of a half-warp's one or two groups of 128, from its lanes' own; of two bf16 groups, both at once.
+template <bool BOTH, typename T>
+__device__ __forceinline__ void group_most(float& g, float& u) {
   const unsigned mask = 0xffffu << (threadIdx.x & 16);
+  if constexpr (BOTH && sizeof(T) == 2) {
+    uint32_t m = (__float_as_uint(g) >> 16) | (__float_as_uint(u) & 0xffff0000u);
 #pragma unroll
-  for (int off = 8; off > 0; off >>= 1) m = max_nan(m, __shfl_xor_sync(mask, m, off));
-  keep_scale(m, keep_top(KEEP), scale, factor);
-  const f32x2 k = both(factor);
-  if (ok)
-    *reinterpret_cast<uint2*>(codes) =
-        make_uint2(keep_codes4<KEEP>(mul2(f[0], k), mul2(f[1], k)), keep_codes4<KEEP>(mul2(f[2], k), mul2(f[3], k)));
-  if ((threadIdx.x & 15) == 0) *scale_out = scale;
+    for (int off = 8; off > 0; off >>= 1) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(__shfl_xor_sync(mask, m, off)));
+    g = bf16lo_to_f32(m);
+    u = bf16hi_to_f32(m);
+  } else {
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) {
+      g = max_nan(g, __shfl_xor_sync(mask, g, off));
+      if (BOTH) u = max_nan(u, __shfl_xor_sync(mask, u, off));
+    }
+  }
+}
+
+// The factors of the groups (all 16 lanes), whose scales one lane each stores.  One division a lane makes all four
+// quotients: lanes 0-3 the first group's factor, 4-7 its scale, 8-11 and 12-15 the second group's.
+template <bool BOTH, int KEEP>
+__device__ __forceinline__ void group_factors(float g, float u, float* scales, float& factor_g, float& factor_u) {
+  const int lane = threadIdx.x & 15;
+  const unsigned mask = 0xffffu << (threadIdx.x & 16);
+  const float top = keep_top(KEEP);
+  float most = BOTH && (lane & 8) ? u : g;
+  const bool finite = most <= 3.402823466e+38f;
+  most = max_nan(most, kKeepFloor);
+  const bool scale = lane & 4;
+  const float q = __fdiv_rn(scale ? most : top, scale ? top : most);
+  factor_g = __shfl_sync(mask, q, 0, 16);
+  factor_u = BOTH ? __shfl_sync(mask, q, 8, 16) : 0.f;
+  if (lane == 4 || (BOTH && lane == 12)) scales[lane >> 3] = finite ? q : __int_as_float(0x7fc00000);
+}
+
+template <int KEEP>
+__device__ __forceinline__ void put_codes(const two (&f)[4], float factor, uint8_t* codes) {
+  const two k = both<two>(factor);
+  *reinterpret_cast<uint2*>(codes) =
+      make_uint2(keep_codes4<KEEP>(mul2(f[0], k), mul2(f[1], k)), keep_codes4<KEEP>(mul2(f[2], k), mul2(f[3], k)));
 }
 
 struct ActParams {
@@ -104,9 +132,10 @@ __global__ void __launch_bounds__(kThreadsRows) act_keep_kernel(const ActParams 
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * p.rows_per_cta;
   const int64_t left = p.n_rows - row0;
   const int items = static_cast<int>(left < p.rows_per_cta ? left : p.rows_per_cta) * p.blocks;
-  for (int it = hw; it < items; it += kHalfWarps) {
-    const int64_t row = row0 + it / p.blocks;
-    const int b = it % p.blocks;
+  int b = hw % p.blocks;
+  int64_t row = row0 + hw / p.blocks;
+  for (int it = hw; it < items; it += kHalfWarps, b += kHalfWarps) {
+    for (; b >= p.blocks; b -= p.blocks) ++row;
     const int col = b * kKeepGroup + lane * 8;  // of the activation
     const bool ok = col < p.ffn;
     const int64_t at = row * p.cols + (GLU ? b * 2 * kKeepGroup + lane * 8 : col);  // of the argument
@@ -117,18 +146,20 @@ __global__ void __launch_bounds__(kThreadsRows) act_keep_kernel(const ActParams 
       v.load(static_cast<const T*>(p.in) + at);
       if (GLU) u.load(static_cast<const T*>(p.in) + at + kKeepGroup);
     }
-    f32x2 g[4], h[4], a[4];
+    two g[4], h[4], a[4];
     v.get(g);
     if (GLU) u.get(h);
+    if (KEEP != DICE_KEEP_NONE) {
+      float mg = v.most(), mu = GLU ? u.most() : 0.f, fg, fu;
+      group_most<GLU, T>(mg, mu);
+      group_factors<GLU, KEEP>(mg, mu, p.scales + row * p.groups_in + (GLU ? 2 * b : b), fg, fu);
+      // the packed order's filling columns get codes too (of zero)
+      if (GLU || ok) put_codes<KEEP>(g, fg, p.codes + at);
+      if (GLU) put_codes<KEEP>(h, fu, p.codes + at + kKeepGroup);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = GLU ? swiglu2<EXACT>(g[i], h[i]) : gelu2<EXACT>(g[i]);
     if (ok) put8(static_cast<T*>(p.a) + row * p.ffn + col, a);
-    if (KEEP != DICE_KEEP_NONE) {
-      // the packed order's filling columns get codes too (of zero)
-      float* sc = p.scales + row * p.groups_in + (GLU ? 2 * b : b);
-      keep8<KEEP>(v, g, p.codes + at, sc, GLU || ok);
-      if (GLU) keep8<KEEP>(u, h, p.codes + at + kKeepGroup, sc + 1, true);
-    }
   }
 }
 
@@ -139,7 +170,7 @@ template <typename T>
 struct Kept8<T, DICE_KEEP_NONE> {
   Vec8<T> v;
   __device__ __forceinline__ void load(const void* base, int64_t at, const float*) { v.load(static_cast<const T*>(base) + at); }
-  __device__ __forceinline__ void get(f32x2 (&f)[4]) const { v.get(f); }
+  __device__ __forceinline__ void get(two (&f)[4]) const { v.get(f); }
 };
 template <typename T, int KEEP>
 struct Kept8 {
@@ -149,9 +180,9 @@ struct Kept8 {
     w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(base) + at);
     scale = *sc;
   }
-  __device__ __forceinline__ void get(f32x2 (&f)[4]) const {
-    keep_read4<KEEP>(w.x, both(scale), f[0], f[1]);
-    keep_read4<KEEP>(w.y, both(scale), f[2], f[3]);
+  __device__ __forceinline__ void get(two (&f)[4]) const {
+    keep_read4<KEEP>(w.x, both<two>(scale), f[0], f[1]);
+    keep_read4<KEEP>(w.y, both<two>(scale), f[2], f[3]);
   }
 };
 
@@ -164,15 +195,16 @@ __global__ void __launch_bounds__(kThreadsRows) act_backward_kernel(const ActPar
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * p.rows_per_cta;
   const int64_t left = p.n_rows - row0;
   const int items = static_cast<int>(left < p.rows_per_cta ? left : p.rows_per_cta) * p.blocks;
-  for (int it = hw; it < items; it += kHalfWarps) {
-    const int64_t row = row0 + it / p.blocks;
-    const int b = it % p.blocks;
+  int b = hw % p.blocks;
+  int64_t row = row0 + hw / p.blocks;
+  for (int it = hw; it < items; it += kHalfWarps, b += kHalfWarps) {
+    for (; b >= p.blocks; b -= p.blocks) ++row;
     const int col = b * kKeepGroup + lane * 8;
     const int64_t at = row * p.cols + (GLU ? b * 2 * kKeepGroup + lane * 8 : col);
     T* d_pre = static_cast<T*>(p.d_pre) + at;
     if (col >= p.ffn) {
       if (GLU) {  // the packed order's filling columns: their gradient is zero
-        const f32x2 z[4] = {};
+        const two z[4] = {};
         put8(d_pre, z);
         put8(d_pre + kKeepGroup, z);
       }
@@ -184,7 +216,7 @@ __global__ void __launch_bounds__(kThreadsRows) act_backward_kernel(const ActPar
     d.load(static_cast<const T*>(p.in) + row * p.ffn + col);
     kg.load(p.kept, at, sc);
     if (GLU) ku.load(p.kept, at + kKeepGroup, sc + 1);
-    f32x2 da[4], g[4], u[4], a[4];
+    two da[4], g[4], u[4], a[4];
     d.get(da);
     kg.get(g);
     if (GLU) ku.get(u);
@@ -245,8 +277,8 @@ combine_backward_kernel(const T* dout, const T* rows_out, const int32_t* pos, co
   const bool ok0 = pp.x >= 0 && pp.x < n_rows, ok1 = pp.y >= 0 && pp.y < n_rows;
   const T* src = dout + t * hidden;
   const int64_t o0 = static_cast<int64_t>(pp.x) * hidden, o1 = static_cast<int64_t>(pp.y) * hidden;
-  f32x2 d0 = 0, d1 = 0;
-  const f32x2 w0 = both(w.x), w1 = both(w.y);
+  two d0 = {0.f, 0.f}, d1 = {0.f, 0.f};
+  const two w0 = both<two>(w.x), w1 = both<two>(w.y);
   for (int c = lane * 8; c < hidden; c += 256) {
     Vec8<T> d, y0, y1;
     y0.zero();
@@ -254,7 +286,7 @@ combine_backward_kernel(const T* dout, const T* rows_out, const int32_t* pos, co
     d.load(src + c);
     if (ok0) y0.load(rows_out + o0 + c);
     if (ok1) y1.load(rows_out + o1 + c);
-    f32x2 f[4], y[4], r[4];
+    two f[4], y[4], r[4];
     d.get(f);
     if (ok0) {
       y0.get(y);

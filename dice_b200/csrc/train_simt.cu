@@ -56,7 +56,7 @@ __device__ __forceinline__ void multiply(const float (*As)[WIDTH + 4], const flo
     *reinterpret_cast<ulonglong2*>(br + 2) = *reinterpret_cast<const ulonglong2*>(&Bs[k][cb + STEP]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const f32x2 a2 = both(ar[i]);
+      const f32x2 a2 = both<f32x2>(ar[i]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = fma2(a2, br[j], acc[i][j]);
     }
@@ -67,7 +67,7 @@ __device__ __forceinline__ void store_tile_row(float* o, const f32x2 (&acc)[4], 
   for (int h = 0; h < 2; ++h) {
     const int c = c0 + h * step;
     if (c < n_valid) {
-      const float2 lo = halves(acc[2 * h]), hi = halves(acc[2 * h + 1]);
+      const two lo = halves(acc[2 * h]), hi = halves(acc[2 * h + 1]);
       const float v[4] = {lo.x, lo.y, hi.x, hi.y};
       store4(o + c, v);
     }
