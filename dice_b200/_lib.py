@@ -67,13 +67,16 @@ SIGNATURES = {
         [c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p,
          c_void_p, c_void_p],
     ),
+    "dice_grouped_scratch_bytes": (c_size_t, [c_int64, c_int, c_int, c_int, c_int, c_int]),
     "dice_grouped_dgrad": (
         c_int,
-        [c_void_p, c_int64, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p],
+        [c_void_p, c_int64, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_size_t,
+         c_void_p, c_void_p],
     ),
     "dice_grouped_wgrad": (
         c_int,
-        [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+        [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_size_t,
+         c_void_p, c_void_p],
     ),
     "dice_act_keep": (
         c_int, [c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
@@ -89,7 +92,8 @@ SIGNATURES = {
     "dice_grouped_ffn_backward": (
         c_int,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int,
-         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p,
+         c_void_p],
     ),
     "dice_ep_meta_ints": (c_int, [c_int, c_int]),
     "dice_ep_exchange_counts": (

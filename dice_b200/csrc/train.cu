@@ -20,9 +20,14 @@ int check_product(int64_t n_rows, int n_dim, int k_dim, int n_slabs, int n_seg, 
 
 }  // namespace
 
+extern "C" size_t dice_grouped_scratch_bytes(int64_t n_rows, int n_dim, int k_dim, int n_slabs, int weight_gradient, int dtype) {
+  if (dtype != DICE_BF16 || check_product(n_rows, n_dim, k_dim, n_slabs, 0, dtype) != DICE_OK) return 0;
+  return dice_internal_split_bytes(n_rows, n_dim, k_dim, n_slabs, weight_gradient != 0);
+}
+
 extern "C" int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, const void* w, int n_slabs, int k_dim,
                                   const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, int dtype, void* dx,
-                                  uint32_t* status, void* stream) {
+                                  void* scratch, size_t scratch_bytes, uint32_t* status, void* stream) {
   const int rc = check_product(n_rows, n_dim, k_dim, n_slabs, n_seg, dtype);
   if (rc != DICE_OK) return rc;
   DICE_CHECK_ARG(seg_slab != nullptr || n_seg <= n_slabs, DICE_ERR_ARG);
@@ -30,15 +35,15 @@ extern "C" int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, con
   DICE_CHECK_ARG(dy && w && seg_offsets && dx, DICE_ERR_ARG);
   DICE_CHECK_ARG(dice_aligned16(dy) && dice_aligned16(w) && dice_aligned16(dx), DICE_ERR_ALIGN);
   if (dtype == DICE_BF16)
-    return dice_internal_tc_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dx, status,
-                                  static_cast<cudaStream_t>(stream));
+    return dice_internal_tc_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dx, scratch,
+                                  scratch_bytes, status, static_cast<cudaStream_t>(stream));
   return dice_internal_simt_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dx, status,
                                   static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int dice_grouped_wgrad(const void* dy, const void* x, int64_t n_rows, int n_dim, int k_dim,
                                   const int32_t* seg_offsets, int n_slabs, int gate_up, int dtype, void* dw, void* dw_up,
-                                  uint32_t* status, void* stream) {
+                                  void* scratch, size_t scratch_bytes, uint32_t* status, void* stream) {
   const int rc = check_product(n_rows, n_dim, k_dim, n_slabs, n_slabs, dtype);
   if (rc != DICE_OK) return rc;
   DICE_CHECK_ARG(gate_up >= 0, DICE_ERR_ARG);
@@ -46,8 +51,8 @@ extern "C" int dice_grouped_wgrad(const void* dy, const void* x, int64_t n_rows,
   DICE_CHECK_ARG(seg_offsets && dw && (gate_up == 0 || dw_up) && (n_rows == 0 || (dy && x)), DICE_ERR_ARG);
   DICE_CHECK_ARG(dice_aligned16(dy) && dice_aligned16(x) && dice_aligned16(dw) && dice_aligned16(dw_up), DICE_ERR_ALIGN);
   if (dtype == DICE_BF16)
-    return dice_internal_tc_wgrad(dy, x, n_rows, n_dim, k_dim, seg_offsets, n_slabs, gate_up, dw, dw_up, status,
-                                  static_cast<cudaStream_t>(stream));
+    return dice_internal_tc_wgrad(dy, x, n_rows, n_dim, k_dim, seg_offsets, n_slabs, gate_up, dw, dw_up, scratch,
+                                  scratch_bytes, status, static_cast<cudaStream_t>(stream));
   return dice_internal_simt_wgrad(dy, x, n_rows, n_dim, k_dim, seg_offsets, n_slabs, gate_up, dw, dw_up, status,
                                   static_cast<cudaStream_t>(stream));
 }
@@ -92,8 +97,8 @@ extern "C" int dice_grouped_ffn_train(const void* rows_in, int64_t n_rows, int h
 extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in, const void* kept, const float* scales,
                                          int64_t n_rows, int hidden, int ffn, int act, int keep, int dtype, const void* w1,
                                          const void* w2, int n_slabs, const int32_t* seg_offsets, void* da, void* d_pre,
-                                         void* a, void* d_rows, void* dw1, void* dw1_up, void* dw2, uint32_t* status,
-                                         void* stream) {
+                                         void* a, void* d_rows, void* dw1, void* dw1_up, void* dw2, void* scratch,
+                                         size_t scratch_bytes, uint32_t* status, void* stream) {
   DICE_CHECK_ARG(act == DICE_ACT_SWIGLU || act == DICE_ACT_GELU_TANH, DICE_ERR_ARG);
   DICE_CHECK_ARG(ffn > 0, DICE_ERR_ARG);
   const bool glu = act == DICE_ACT_SWIGLU;
@@ -114,11 +119,21 @@ extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in,
                                  static_cast<cudaStream_t>(stream));
       if (rc != DICE_OK) return rc;
     } else {
-      if ((rc = dice_grouped_dgrad(d_out, n_rows, hidden, w2, n_slabs, ffn, seg_offsets, nullptr, n_slabs, dtype, da, status, stream)) != DICE_OK) return rc;
+      if ((rc = dice_grouped_dgrad(d_out, n_rows, hidden, w2, n_slabs, ffn, seg_offsets, nullptr, n_slabs, dtype, da, nullptr, 0, status, stream)) != DICE_OK) return rc;
       if ((rc = dice_act_backward(da, kept, scales, n_rows, ffn, act, keep, dtype, d_pre, a, stream)) != DICE_OK) return rc;
     }
   }
-  if ((rc = dice_grouped_wgrad(d_out, a, n_rows, hidden, ffn, seg_offsets, n_slabs, 0, dtype, dw2, nullptr, status, stream)) != DICE_OK) return rc;
-  if ((rc = dice_grouped_dgrad(d_pre, n_rows, static_cast<int>(cols), w1, n_slabs, hidden, seg_offsets, nullptr, n_slabs, dtype, d_rows, status, stream)) != DICE_OK) return rc;
-  return dice_grouped_wgrad(d_pre, rows_in, n_rows, static_cast<int>(cols), hidden, seg_offsets, n_slabs, glu ? ffn : 0, dtype, dw1, dw1_up, status, stream);
+  // each product takes the scratch only if it can split
+  auto part = [&](int n_dim, int k_dim, bool weight_gradient) {
+    return dice_grouped_scratch_bytes(n_rows, n_dim, k_dim, n_slabs, weight_gradient, dtype) > 0 ? scratch : nullptr;
+  };
+  const int c = static_cast<int>(cols);
+  if ((rc = dice_grouped_wgrad(d_out, a, n_rows, hidden, ffn, seg_offsets, n_slabs, 0, dtype, dw2, nullptr,
+                               part(hidden, ffn, true), scratch_bytes, status, stream)) != DICE_OK)
+    return rc;
+  if ((rc = dice_grouped_dgrad(d_pre, n_rows, c, w1, n_slabs, hidden, seg_offsets, nullptr, n_slabs, dtype, d_rows,
+                               part(c, hidden, false), scratch_bytes, status, stream)) != DICE_OK)
+    return rc;
+  return dice_grouped_wgrad(d_pre, rows_in, n_rows, c, hidden, seg_offsets, n_slabs, glu ? ffn : 0, dtype, dw1, dw1_up,
+                            part(c, hidden, true), scratch_bytes, status, stream);
 }

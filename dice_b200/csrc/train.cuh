@@ -16,11 +16,13 @@ int dice_internal_simt_wgrad(const void* dy, const void* x, int64_t n_rows, int 
                              uint32_t* status, cudaStream_t s);
 
 // bf16 on the tensor cores (train_gemm.cu)
+size_t dice_internal_split_bytes(int64_t n_rows, int n_dim, int k_dim, int n_slabs, bool weight_gradient);
 int dice_internal_tc_dgrad(const void* dy, int64_t n_rows, int n_dim, const void* w, int n_slabs, int k_dim,
-                           const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, void* dx, uint32_t* status,
-                           cudaStream_t s);
+                           const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, void* dx, void* scratch,
+                           size_t scratch_bytes, uint32_t* status, cudaStream_t s);
 int dice_internal_tc_wgrad(const void* dy, const void* x, int64_t n_rows, int n_dim, int k_dim, const int32_t* seg_offsets,
-                           int n_slabs, int gate_up, void* dw, void* dw_up, uint32_t* status, cudaStream_t s);
+                           int n_slabs, int gate_up, void* dw, void* dw_up, void* scratch, size_t scratch_bytes, uint32_t* status,
+                           cudaStream_t s);
 
 // the forward product with the activation and what is kept in its epilogue, and the second product's input gradient with
 // the activation's backward pass in its epilogue (see train_gemm.cu); pointers as in the public entry points

@@ -25,7 +25,9 @@
 //   NN + EPI_BACK  the second product's input gradient: every column's gradient meets the codes of its argument in fp32
 //                  and leaves as the argument's gradient, beside the activation for the weight gradient behind it.
 //
-// Few tiles and a long reduction: the pairs that would idle take a share of the reduction each (split).  Every epilogue
+// Few tiles: they are made half as wide if that keeps more pairs busy (one token's two rows, 1152 -> 4608: 36 tiles of
+// 256 columns, 72 of 128).  Fewer still, and a long reduction: the pairs that would idle take a share of the reduction
+// each (split).  Every epilogue
 // warp files its part of the sum in fp32; the last one to arrive at a part adds them up in the order of the shares, so
 // the result does not depend on who was last.
 #include <cuda.h>
@@ -52,6 +54,7 @@ constexpr int kExchangeBytes = 4096;  // EPI_KEEP, SwiGLU: group maxima, [2 tile
 constexpr int kSmemT = kStagesT * kStageBytesT + kAuxBytes + kEpilogueWarps * kStageStore + kExchangeBytes + 1024;
 constexpr int kSplitFloats = 4 * 32 * 32;  // an epilogue warp's part of a tile: 4 chunks of 32 rows x 32 columns
 constexpr int kMinSplitBlocks = 4;         // k-blocks of a share, at least
+constexpr int kMaxSplit = 16;              // the last warp reads the shares one after the other
 
 struct TrainGemm {
   const int* seg_offsets;
@@ -60,7 +63,6 @@ struct TrainGemm {
   int n_rows;
   int red_blocks;   // NN: k-blocks of the reduction
   int n_mblk;       // TN: row tiles of a slab's gradient
-  int n_nblk;       // column tiles
   int n_cols;       // output columns
   int m_rows;       // TN: output rows of a slab
   int gate_up;      // TN: 0, or ffn: the rows are packed gate / up blocks and go to two tensors
@@ -365,7 +367,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   const uint32_t xchg_bar = smem_u32(bars + 3 * kStagesT + 2 * kAccStages);  // [4] EPI_KEEP: a quadrant's two warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * kStagesT + 2 * kAccStages + 4);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  int* s_split = reinterpret_cast<int*>(tmem_slot + 2);
+  int* s_split = reinterpret_cast<int*>(tmem_slot + 2);  // shares of the reduction; columns of a tile
   int* s_seg_off = reinterpret_cast<int*>(tmem_slot + 4);
   int* s_mprefix = s_seg_off + (kMaxSeg + 1);  // NT, NN: first row tile of every segment
   const uint32_t tiles_smem = smem_u32(smem);
@@ -423,13 +425,16 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     s_mprefix[p.n_seg] = run;
     // shares of the reduction: as many as there are pairs for every tile, if each is long enough
     int split = 1;
-    if (p.split_ws != nullptr && run > 0) {
-      const int64_t per_tile = n_pairs / (static_cast<int64_t>(run) * p.n_nblk);
+    const int64_t wide_tiles = static_cast<int64_t>(run) * ((p.n_cols + BN - 1) / BN);
+    const int bn = EPI == EPI_PLAIN && 2 * wide_tiles <= n_pairs ? BN / 2 : BN;
+    if (EPI == EPI_PLAIN && p.split_ws != nullptr && run > 0) {
+      const int64_t per_tile = n_pairs / (static_cast<int64_t>(run) * ((p.n_cols + bn - 1) / bn));
       const int blocks = MODE != MODE_TN ? p.red_blocks : (most + BK - 1) / BK;
       split = static_cast<int>(per_tile < blocks / kMinSplitBlocks ? per_tile : blocks / kMinSplitBlocks);
-      if (split < 1) split = 1;
+      split = split < 1 ? 1 : (split > kMaxSplit ? kMaxSplit : split);
     }
-    *s_split = split;
+    s_split[0] = split;
+    s_split[1] = bn;
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -437,8 +442,9 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   tc_fence_after_sync();
 
   const uint32_t tmem_base = *tmem_slot;
-  const int split = *s_split;
-  const int64_t total = static_cast<int64_t>(s_mprefix[p.n_seg]) * p.n_nblk * split;
+  const int split = EPI == EPI_PLAIN ? s_split[0] : 1, bn = EPI == EPI_PLAIN ? s_split[1] : BN;
+  const int n_nblk = (p.n_cols + bn - 1) / bn;
+  const int64_t total = static_cast<int64_t>(s_mprefix[p.n_seg]) * n_nblk * split;
 
   // work item t -> tile, share of the reduction, this CTA's rows
   struct Tile {
@@ -450,8 +456,8 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     Tile ti;
     ti.tile = split == 1 ? t : t / split;
     ti.share = split == 1 ? 0 : static_cast<int>(t - ti.tile * split);
-    const int m = static_cast<int>(ti.tile / p.n_nblk);
-    ti.nb = static_cast<int>(ti.tile - static_cast<int64_t>(m) * p.n_nblk);
+    const int m = static_cast<int>(ti.tile / n_nblk);
+    ti.nb = static_cast<int>(ti.tile - static_cast<int64_t>(m) * n_nblk);
     int blocks;
     if (MODE != MODE_TN) {
       while (m >= s_mprefix[seg + 1]) ++seg;
@@ -475,8 +481,8 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     ti.kb0 = static_cast<int>(static_cast<int64_t>(blocks) * ti.share / split);
     ti.kb1 = static_cast<int>(static_cast<int64_t>(blocks) * (ti.share + 1) / split);
     if (ti.kb1 < blocks) ti.last_rows = BK;
-    int n_valid = p.n_cols - ti.nb * BN;
-    if (n_valid > BN) n_valid = BN;
+    int n_valid = p.n_cols - ti.nb * bn;
+    if (n_valid > bn) n_valid = bn;
     ti.n_mma = (n_valid + 31) & ~31;  // half of the columns come from each CTA
     return ti;
   };
@@ -489,7 +495,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     for (int64_t t = pair_id; alive && t < total; t += n_pairs) {
       const Tile ti = decode(t, seg);
       const int half = ti.n_mma / 2;
-      const int col0 = ti.nb * BN + static_cast<int>(cta_rank) * half;  // this CTA's B columns
+      const int col0 = ti.nb * bn + static_cast<int>(cta_rank) * half;  // this CTA's B columns
       const int b_boxes = half > 64 ? 2 : 1;
       const uint32_t bytes = kOperandBytes + b_boxes * kBoxBytes;
       const int ragged = MODE == MODE_TN ? ti.last_rows & 15 : 0;
@@ -619,9 +625,9 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         tc_fence_after_sync();
       }
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * BN);
-      const int col0 = ti.nb * BN;
+      const int col0 = ti.nb * bn;
       int n_valid = p.n_cols - col0;
-      if (n_valid > BN) n_valid = BN;
+      if (n_valid > bn) n_valid = bn;
 
       // the rows of the output that this lane stores pieces of (store_transposed): -1 beyond the segment or the gradient
       int64_t dst_row[4];
@@ -681,6 +687,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = 0.f;
           const float* src = parts + (c >> 6) * 1024;
+#pragma unroll 2
           for (int s = 0; s < split; ++s, src += kPairFloats) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] += __ldcg(src + j * 32);
@@ -787,11 +794,40 @@ int launch_train(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const TrainGe
   return cudaLaunchKernelEx(&cfg, train_gemm_kernel<MODE, EPI, ACT, KEEP>, tm_a, tm_b, p) == cudaSuccess ? DICE_OK : DICE_ERR_CUDA;
 }
 
+int64_t col_tiles(int cols, int width) { return (static_cast<int64_t>(cols) + width - 1) / width; }
+
+// scratch of a split: the counters (zeroed here), then every pair's sums
+size_t counter_bytes(int pairs) { return (static_cast<size_t>(pairs) * 2 * kEpilogueWarps * sizeof(unsigned int) + 255) / 256 * 256; }
+size_t split_bytes(int pairs) { return counter_bytes(pairs) + static_cast<size_t>(pairs) * 2 * kEpilogueWarps * kSplitFloats * sizeof(float); }
+int use_scratch(TrainGemm& p, void* scratch, size_t scratch_bytes, int pairs, cudaStream_t s) {
+  if (scratch == nullptr) return DICE_OK;
+  if (scratch_bytes < split_bytes(pairs)) return DICE_ERR_SCRATCH;
+  if (!dice_aligned16(scratch)) return DICE_ERR_ALIGN;
+  if (cudaMemsetAsync(scratch, 0, counter_bytes(pairs), s) != cudaSuccess) return DICE_ERR_CUDA;
+  p.split_count = static_cast<unsigned int*>(scratch);
+  p.split_ws = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + counter_bytes(pairs));
+  return DICE_OK;
+}
+
 }  // namespace
 
+// What a split can use: 0 where it would not be made.  A weight gradient's tiles are known here; an input gradient's
+// depend on the segments, of which at least the rows' own number of tiles exists (a quarter of the pairs at most, so that
+// uneven segments still leave room).  Shares are at least four k-blocks of 64, so the reduction has to have eight.
+size_t dice_internal_split_bytes(int64_t n_rows, int n_dim, int k_dim, int n_slabs, bool weight_gradient) {
+  const int pairs = sm_count_cached() / 2;
+  if (pairs <= 0 || n_rows == 0) return 0;
+  const int64_t cols = col_tiles(k_dim, BN / 2);
+  if (weight_gradient) {
+    const int64_t tiles = static_cast<int64_t>(n_slabs) * ((n_dim + PM - 1) / PM) * cols;
+    return 2 * tiles <= pairs && n_rows >= 2 * kMinSplitBlocks * BK ? split_bytes(pairs) : 0;
+  }
+  return 4 * ((n_rows + PM - 1) / PM) * cols <= pairs && n_dim >= 2 * kMinSplitBlocks * BK ? split_bytes(pairs) : 0;
+}
+
 int dice_internal_tc_dgrad(const void* dy, int64_t n_rows, int n_dim, const void* w, int n_slabs, int k_dim,
-                           const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, void* dx, uint32_t* status,
-                           cudaStream_t s) {
+                           const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, void* dx, void* scratch,
+                           size_t scratch_bytes, uint32_t* status, cudaStream_t s) {
   const int pairs = resident_pairs_train<MODE_NN>();
   if (pairs <= 0) return DICE_ERR_CUDA;
   CUtensorMap tm_a, tm_b;
@@ -806,15 +842,16 @@ int dice_internal_tc_dgrad(const void* dy, int64_t n_rows, int n_dim, const void
   p.n_slabs = n_slabs;
   p.n_rows = static_cast<int>(n_rows);
   p.red_blocks = (n_dim + BK - 1) / BK;
-  p.n_nblk = (k_dim + BN - 1) / BN;
   p.n_cols = k_dim;
   p.out = static_cast<__nv_bfloat16*>(dx);
   p.status = status;
-  return launch_train<MODE_NN>(tm_a, tm_b, p, ((n_rows + PM - 1) / PM + n_seg) * p.n_nblk, pairs, s);
+  if ((rc = use_scratch(p, scratch, scratch_bytes, pairs, s)) != DICE_OK) return rc;
+  return launch_train<MODE_NN>(tm_a, tm_b, p, ((n_rows + PM - 1) / PM + n_seg) * col_tiles(k_dim, BN / 2), pairs, s);
 }
 
 int dice_internal_tc_wgrad(const void* dy, const void* x, int64_t n_rows, int n_dim, int k_dim, const int32_t* seg_offsets,
-                           int n_slabs, int gate_up, void* dw, void* dw_up, uint32_t* status, cudaStream_t s) {
+                           int n_slabs, int gate_up, void* dw, void* dw_up, void* scratch, size_t scratch_bytes, uint32_t* status,
+                           cudaStream_t s) {
   const int pairs = resident_pairs_train<MODE_TN>();
   if (pairs <= 0) return DICE_ERR_CUDA;
   CUtensorMap tm_a, tm_b;
@@ -830,13 +867,13 @@ int dice_internal_tc_wgrad(const void* dy, const void* x, int64_t n_rows, int n_
   p.n_rows = static_cast<int>(n_rows);
   p.n_mblk = (n_dim + PM - 1) / PM;
   p.m_rows = n_dim;
-  p.n_nblk = (k_dim + BN - 1) / BN;
   p.n_cols = k_dim;
   p.gate_up = gate_up;
   p.out = static_cast<__nv_bfloat16*>(dw);
   p.out_up = static_cast<__nv_bfloat16*>(dw_up);
   p.status = status;
-  return launch_train<MODE_TN>(tm_a, tm_b, p, static_cast<int64_t>(n_slabs) * p.n_mblk * p.n_nblk, pairs, s);
+  if ((rc = use_scratch(p, scratch, scratch_bytes, pairs, s)) != DICE_OK) return rc;
+  return launch_train<MODE_TN>(tm_a, tm_b, p, static_cast<int64_t>(n_slabs) * p.n_mblk * col_tiles(k_dim, BN / 2), pairs, s);
 }
 
 namespace {
@@ -845,13 +882,13 @@ template <int ACT, int KEEP>
 int run_keep(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const TrainGemm& p, cudaStream_t s) {
   const int pairs = resident_pairs_train<MODE_NT, EPI_KEEP, ACT, KEEP>();
   if (pairs <= 0) return DICE_ERR_CUDA;
-  return launch_train<MODE_NT, EPI_KEEP, ACT, KEEP>(tm_a, tm_b, p, ((p.n_rows + PM - 1ll) / PM + p.n_seg) * p.n_nblk, pairs, s);
+  return launch_train<MODE_NT, EPI_KEEP, ACT, KEEP>(tm_a, tm_b, p, ((p.n_rows + PM - 1ll) / PM + p.n_seg) * col_tiles(p.n_cols, BN), pairs, s);
 }
 template <int ACT, int KEEP>
 int run_back(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const TrainGemm& p, cudaStream_t s) {
   const int pairs = resident_pairs_train<MODE_NN, EPI_BACK, ACT, KEEP>();
   if (pairs <= 0) return DICE_ERR_CUDA;
-  return launch_train<MODE_NN, EPI_BACK, ACT, KEEP>(tm_a, tm_b, p, ((p.n_rows + PM - 1ll) / PM + p.n_seg) * p.n_nblk, pairs, s);
+  return launch_train<MODE_NN, EPI_BACK, ACT, KEEP>(tm_a, tm_b, p, ((p.n_rows + PM - 1ll) / PM + p.n_seg) * col_tiles(p.n_cols, BN), pairs, s);
 }
 template <int ACT>
 int run_epilogue(bool back, int keep, const CUtensorMap& tm_a, const CUtensorMap& tm_b, const TrainGemm& p, cudaStream_t s) {
@@ -886,7 +923,6 @@ int dice_internal_tc_keep(const void* rows, int64_t n_rows, int hidden, int ffn,
   p.n_slabs = n_slabs;
   p.n_rows = static_cast<int>(n_rows);
   p.red_blocks = (hidden + BK - 1) / BK;
-  p.n_nblk = (p.arg_cols + BN - 1) / BN;
   p.n_cols = p.arg_cols;
   p.out = static_cast<__nv_bfloat16*>(pre);
   p.act_out = static_cast<__nv_bfloat16*>(a);
@@ -912,7 +948,6 @@ int dice_internal_tc_back(const void* d_out, int64_t n_rows, int hidden, int ffn
   p.n_slabs = n_slabs;
   p.n_rows = static_cast<int>(n_rows);
   p.red_blocks = (hidden + BK - 1) / BK;
-  p.n_nblk = (ffn + BN - 1) / BN;
   p.n_cols = ffn;
   p.out = static_cast<__nv_bfloat16*>(d_pre);
   p.act_out = static_cast<__nv_bfloat16*>(a);

@@ -109,11 +109,38 @@ struct SimtParams {
   int red;         // NT / NN: reduction length
   int gate_up;     // TN: 0, or ffn: output rows are packed gate / up blocks
   uint32_t* status;
+  int shares;      // TN: CTAs that share a tile
 };
 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The CTAs of a cluster that share a tile: the first adds the others' 8 x 8 sums to its own, in their order, out of their
+// shared memory (32 pairs a thread, `step` apart from `place`).  Called by all threads; `active` ones hold sums.  True in
+// the first CTA.
+__device__ __forceinline__ bool cluster_total(f32x2 (&acc)[8][4], f32x2* place, int step, unsigned rank, unsigned size, bool active) {
+  if (rank != 0 && active) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) place[i * step] = acc[i >> 2][i & 3];
+  }
+  cluster_sync();
+  if (rank == 0 && active) {
+    const uint32_t here = static_cast<uint32_t>(__cvta_generic_to_shared(place));
+    for (uint32_t other = 1; other < size; ++other) {
+      uint32_t there;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(other));
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        f32x2 y;
+        asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(y) : "r"(there + i * step * 8));
+        acc[i >> 2][i & 3] = add2(acc[i >> 2][i & 3], y);
+      }
+    }
+  }
+  cluster_sync();  // nobody leaves while its sums may be read
+  return rank == 0;
 }
 
 struct Slices {
@@ -209,30 +236,9 @@ __global__ void __launch_bounds__(64 * GROUPS, 2) simt_rows_kernel(const SimtPar
       }
     }
   }
-  if (gridDim.z > 1) {  // the cluster's CTAs: the first adds the others' sums, in their order
-    if (blockIdx.z != 0) {
-      __syncthreads();
-      if (group == 0) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) sums[i * 64 + t] = acc[i >> 2][i & 3];
-      }
-    }
-    cluster_sync();
-    if (blockIdx.z == 0 && group == 0) {
-      const uint32_t here = static_cast<uint32_t>(__cvta_generic_to_shared(sums + t));
-      for (uint32_t other = 1; other < gridDim.z; ++other) {
-        uint32_t there;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(other));
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          f32x2 y;
-          asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(y) : "r"(there + i * 512));
-          acc[i >> 2][i & 3] = add2(acc[i >> 2][i & 3], y);
-        }
-      }
-    }
-    cluster_sync();  // nobody leaves while its sums may be read
-    if (blockIdx.z != 0) return;
+  if (gridDim.z > 1) {
+    if (blockIdx.z != 0) __syncthreads();  // (their last exchange in the same place)
+    if (!cluster_total(acc, sums + t, 64, blockIdx.z, gridDim.z, group == 0)) return;
   }
   if (group != 0) return;
   float* out = static_cast<float*>(p.out) + static_cast<int64_t>(row0) * p.n_cols + col0;
@@ -256,6 +262,7 @@ __device__ __forceinline__ void copy_wide(float (*s)[WM + 4], const float* base,
 struct WideSlices {
   float a[kRing][WK][WM + 4], b[kRing][WK][WN + 4];
 };
+constexpr int kWideSmem = sizeof(WideSlices) > WM * WN * sizeof(float) ? sizeof(WideSlices) : WM * WN * sizeof(float);
 
 __global__ void __launch_bounds__(256, 2) simt_wgrad_kernel(const SimtParams p) {
   extern __shared__ __align__(16) uint8_t smem_wide[];
@@ -268,12 +275,16 @@ __global__ void __launch_bounds__(256, 2) simt_wgrad_kernel(const SimtParams p) 
     if (threadIdx.x == 0 && p.status != nullptr) atomicCAS(p.status, 0u, DICE_STATUS_BAD_SEGMENTS);
     return;
   }
-  const int m0 = static_cast<int>(blockIdx.x) * WM, col0 = blockIdx.y * WN;
+  // the CTAs of a cluster take every shares-th slice of the reduction
+  const int shares = p.shares, share = static_cast<int>(blockIdx.x) % shares, block = static_cast<int>(blockIdx.x) / shares;
+  const int m0 = block * WM, col0 = blockIdx.y * WN;
   const int n_valid = p.n_cols - col0;
   int m_valid = p.m_cols - m0;
   const float* a = static_cast<const float*>(p.a) + static_cast<int64_t>(row0) * p.m_cols + m0;
   const float* b = static_cast<const float*>(p.b) + static_cast<int64_t>(row0) * p.n_cols + col0;
-  int left = end - row0;
+  int left = end - row0 - share * WK;
+  a += static_cast<int64_t>(share) * WK * p.m_cols;
+  b += static_cast<int64_t>(share) * WK * p.n_cols;
 
   const int ra = (threadIdx.x >> 4) * 4, cb = (threadIdx.x & 15) * 4;
   f32x2 acc[8][4] = {};
@@ -281,13 +292,13 @@ __global__ void __launch_bounds__(256, 2) simt_wgrad_kernel(const SimtParams p) 
     if (left > 0) {
       copy_wide(sl.a[buf], a, p.m_cols, m_valid, left);
       copy_wide(sl.b[buf], b, p.n_cols, n_valid, left);
-      a += static_cast<int64_t>(WK) * p.m_cols;
-      b += static_cast<int64_t>(WK) * p.n_cols;
-      left -= WK;
+      a += static_cast<int64_t>(shares) * WK * p.m_cols;
+      b += static_cast<int64_t>(shares) * WK * p.n_cols;
+      left -= shares * WK;
     }
     copies_commit();
   };
-  int todo = (left + WK - 1) / WK;
+  int todo = left > 0 ? (left + shares * WK - 1) / (shares * WK) : 0;
   fetch(0);
   fetch(1);
   for (int buf = 0; todo > 0; --todo) {
@@ -298,13 +309,18 @@ __global__ void __launch_bounds__(256, 2) simt_wgrad_kernel(const SimtParams p) 
     buf = buf == kRing - 1 ? 0 : buf + 1;
   }
 
+  if (shares > 1) {
+    __syncthreads();  // the slices are done with
+    if (!cluster_total(acc, reinterpret_cast<f32x2*>(smem_wide) + threadIdx.x, 256, share, shares, true)) return;
+  }
+
   float* out = static_cast<float*>(p.out);
   if (p.gate_up == 0) {
     out += (static_cast<int64_t>(slab) * p.m_cols + m0) * p.n_cols + col0;
   } else {
     // a tile is one 128-row block of the packed order: even blocks are gate rows, odd ones the matching up rows
-    if (blockIdx.x & 1) out = static_cast<float*>(p.out_up);
-    const int r0 = static_cast<int>(blockIdx.x >> 1) * WM;
+    if (block & 1) out = static_cast<float*>(p.out_up);
+    const int r0 = (block >> 1) * WM;
     out += (static_cast<int64_t>(slab) * p.gate_up + r0) * p.n_cols + col0;
     m_valid = p.gate_up - r0;
   }
@@ -322,6 +338,25 @@ bool allow_smem(K kernel, int bytes, bool (&done)[64]) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
   if (!done[dev]) done[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
   return done[dev];
+}
+
+int launch_cluster(void (*kernel)(SimtParams), dim3 grid, int threads, int smem, dim3 cluster, const SimtParams& p, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster.x;
+  attr[0].val.clusterDim.y = cluster.y;
+  attr[0].val.clusterDim.z = cluster.z;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dice_pdl_enabled() ? 2 : 1;
+  dice_count_launch();
+  return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? DICE_OK : DICE_ERR_CUDA;
 }
 
 // CTAs that share a tile's reduction: as many (a power of two, at most 8) as give every one of the GPU's CTA slots five
@@ -342,22 +377,8 @@ int launch_rows(const SimtParams& p, cudaStream_t s) {
   static bool done[64];
   if (!allow_smem(simt_rows_kernel<MODE>, kRowsSmem, done)) return DICE_ERR_CUDA;
   const unsigned shares = static_cast<unsigned>(shares_of(p, gy));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy), shares);
-  cfg.blockDim = dim3(64 * GROUPS, 1, 1);
-  cfg.dynamicSmemBytes = kRowsSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = shares;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = dice_pdl_enabled() ? 2 : 1;
-  dice_count_launch();
-  return cudaLaunchKernelEx(&cfg, simt_rows_kernel<MODE>, p) == cudaSuccess ? DICE_OK : DICE_ERR_CUDA;
+  return launch_cluster(simt_rows_kernel<MODE>, dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy), shares), 64 * GROUPS,
+                        kRowsSmem, dim3(1, 1, shares), p, s);
 }
 
 }  // namespace
@@ -380,10 +401,15 @@ int dice_internal_simt_wgrad(const void* dy, const void* x, int64_t n_rows, int 
                              const int32_t* seg_offsets, int n_slabs, int gate_up, void* dw, void* dw_up,
                              uint32_t* status, cudaStream_t s) {
   SimtParams p = {dy, x, dw, dw_up, seg_offsets, nullptr, n_slabs, n_slabs, n_rows, n_dim, k_dim, 0, gate_up, status};
-  const int64_t gy = (static_cast<int64_t>(k_dim) + WN - 1) / WN;
+  const int64_t gm = (static_cast<int64_t>(n_dim) + WM - 1) / WM, gy = (static_cast<int64_t>(k_dim) + WN - 1) / WN;
   if (gy > 65535) return DICE_ERR_LIMIT;
-  const dim3 grid(static_cast<unsigned>((n_dim + WM - 1) / WM), static_cast<unsigned>(gy), static_cast<unsigned>(n_slabs));
+  // as many CTAs to a tile (a power of two, at most 8) as fill the GPU's slots once, each with eight slices or more of an
+  // average segment
+  const int64_t tiles = gm * gy * n_slabs, slots = 2ll * dice_umma::sm_count_cached();
+  p.shares = 1;
+  while (p.shares < 8 && 2 * p.shares * tiles <= slots && n_rows >= 16ll * p.shares * WK * n_slabs) p.shares *= 2;
   static bool done[64];
-  if (!allow_smem(simt_wgrad_kernel, static_cast<int>(sizeof(WideSlices)), done)) return DICE_ERR_CUDA;
-  return dice_launch(simt_wgrad_kernel, grid, dim3(256), sizeof(WideSlices), s, p) == cudaSuccess ? DICE_OK : DICE_ERR_CUDA;
+  if (!allow_smem(simt_wgrad_kernel, kWideSmem, done)) return DICE_ERR_CUDA;
+  return launch_cluster(simt_wgrad_kernel, dim3(static_cast<unsigned>(gm * p.shares), static_cast<unsigned>(gy), static_cast<unsigned>(n_slabs)),
+                        256, kWideSmem, dim3(p.shares, 1, 1), p, s);
 }

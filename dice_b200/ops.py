@@ -625,6 +625,14 @@ def _status_ptr(status: Optional[torch.Tensor], index: int) -> int:
 _status_by_index = {}  # device number -> address of its status word, which lives as long as the process
 
 
+def _split_scratch(index: int, n_bytes: int) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
+    """A product's scratch (the tensor, which the caller holds until the launch, its address and its size)."""
+    if n_bytes == 0:
+        return None, None, 0
+    scratch = _new((1, n_bytes), torch.uint8, index)
+    return scratch, scratch.data_ptr(), n_bytes
+
+
 def _check_segments(seg_offsets: torch.Tensor) -> int:
     assert seg_offsets.dtype == torch.int32 and seg_offsets.dim() == 1 and seg_offsets.is_contiguous()
     assert seg_offsets.numel() >= 1, "seg_offsets holds one offset more than there are segments"
@@ -660,9 +668,12 @@ def grouped_dgrad(dy: torch.Tensor, w: torch.Tensor, seg_offsets: torch.Tensor, 
     if out is None:
         out = _new((n_rows, k_dim), dy.dtype, index)
     assert out.is_contiguous() and out.shape == (n_rows, k_dim) and out.dtype == dy.dtype
+    lib = _lib.load()
+    held, scratch, n_bytes = _split_scratch(index, lib.dice_grouped_scratch_bytes(n_rows, n_dim, k_dim, n_slabs, 0, code))
     _lib.check(
-        _lib.load().dice_grouped_dgrad(dy.data_ptr(), n_rows, n_dim, w.data_ptr(), n_slabs, k_dim, seg_offsets.data_ptr(),
-                                       _ptr(seg_slab), n_seg, code, out.data_ptr(), _status_ptr(status, index), _stream_of(index)),
+        lib.dice_grouped_dgrad(dy.data_ptr(), n_rows, n_dim, w.data_ptr(), n_slabs, k_dim, seg_offsets.data_ptr(),
+                               _ptr(seg_slab), n_seg, code, out.data_ptr(), scratch, n_bytes, _status_ptr(status, index),
+                               _stream_of(index)),
         "dice_grouped_dgrad",
     )
     return out
@@ -689,10 +700,12 @@ def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, seg_offsets: torch.Tensor, 
     shape = (n_slabs, gate_up or n_dim, k_dim)
     dw = _new(shape, dy.dtype, index)
     dw_up = _new(shape, dy.dtype, index) if gate_up else None
+    lib = _lib.load()
+    held, scratch, n_bytes = _split_scratch(index, lib.dice_grouped_scratch_bytes(n_rows, n_dim, k_dim, n_slabs, 1, code))
     _lib.check(
-        _lib.load().dice_grouped_wgrad(dy.data_ptr(), x.data_ptr(), n_rows, n_dim, k_dim, seg_offsets.data_ptr(), n_slabs,
-                                       gate_up or 0, code, dw.data_ptr(), _ptr(dw_up), _status_ptr(status, index),
-                                       _stream_of(index)),
+        lib.dice_grouped_wgrad(dy.data_ptr(), x.data_ptr(), n_rows, n_dim, k_dim, seg_offsets.data_ptr(), n_slabs,
+                               gate_up or 0, code, dw.data_ptr(), _ptr(dw_up), scratch, n_bytes, _status_ptr(status, index),
+                               _stream_of(index)),
         "dice_grouped_wgrad",
     )
     return (dw, dw_up) if gate_up else dw
@@ -870,11 +883,17 @@ def grouped_ffn_backward(d_out: torch.Tensor, rows: torch.Tensor, kept: KeptAct,
     d_pre, a, d_rows = _new((n_rows, cols), dt, index), _new((n_rows, ffn), dt, index), _new((n_rows, h), dt, index)
     dw2, dw1 = _new((n_slabs, h, ffn), dt, index), _new((n_slabs, ffn, h), dt, index)
     dw1_up = _new((n_slabs, ffn, h), dt, index) if act == "swiglu" else None
+    lib = _lib.load()
+    held, scratch, n_bytes = _split_scratch(index, max(
+        lib.dice_grouped_scratch_bytes(n_rows, h, ffn, n_slabs, 1, code),
+        lib.dice_grouped_scratch_bytes(n_rows, cols, h, n_slabs, 0, code),
+        lib.dice_grouped_scratch_bytes(n_rows, cols, h, n_slabs, 1, code)))
     _lib.check(
-        _lib.load().dice_grouped_ffn_backward(
+        lib.dice_grouped_ffn_backward(
             d_out.data_ptr(), rows.data_ptr(), codes.data_ptr(), _ptr(scales), n_rows, h, ffn, ACT_CODES[act], keep, code,
             w1.data_ptr(), w2.data_ptr(), n_slabs, seg_offsets.data_ptr(), _ptr(da), d_pre.data_ptr(), a.data_ptr(),
-            d_rows.data_ptr(), dw1.data_ptr(), _ptr(dw1_up), dw2.data_ptr(), _status_ptr(status, index), _stream_of(index),
+            d_rows.data_ptr(), dw1.data_ptr(), _ptr(dw1_up), dw2.data_ptr(), scratch, n_bytes, _status_ptr(status, index),
+            _stream_of(index),
         ),
         "dice_grouped_ffn_backward",
     )

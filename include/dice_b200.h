@@ -330,7 +330,15 @@ DICE_API int dice_grouped_ffn_f32(const void* rows_in, int64_t n_rows, int hidde
  * n_rows, or a slab does not exist: such segments are not computed. */
 DICE_API int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, const void* w, int n_slabs, int k_dim,
                        const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, int dtype, void* dx,
-                       uint32_t* status, void* stream);
+                       void* scratch, size_t scratch_bytes, uint32_t* status, void* stream);
+
+/* Scratch (16-byte aligned, contents irrelevant) with which dice_grouped_dgrad
+ * (weight_gradient == 0) or dice_grouped_wgrad shares a long reduction among
+ * SMs that few output tiles would leave idle; 0 where it would not.  NULL scratch is
+ * always allowed, and slower there.  Calls that overlap on the GPU need
+ * scratch of their own; calls in stream order may share it. */
+DICE_API size_t dice_grouped_scratch_bytes(int64_t n_rows, int n_dim, int k_dim, int n_slabs, int weight_gradient,
+                                  int dtype);
 
 /* Weight gradient of the same product, one segment per slab:
  *   dw[s] = dy[seg s]^T * x[seg s]     (zero for a segment without rows)
@@ -341,7 +349,7 @@ DICE_API int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, const
  * rows (else dw_up is NULL).  n_slabs <= 256. */
 DICE_API int dice_grouped_wgrad(const void* dy, const void* x, int64_t n_rows, int n_dim, int k_dim,
                        const int32_t* seg_offsets, int n_slabs, int gate_up, int dtype, void* dw, void* dw_up,
-                       uint32_t* status, void* stream);
+                       void* scratch, size_t scratch_bytes, uint32_t* status, void* stream);
 
 /* what the forward pass keeps of the activation's argument */
 #define DICE_KEEP_NONE 0 /* the argument itself                                   */
@@ -394,12 +402,14 @@ DICE_API int dice_grouped_ffn_train(const void* rows_in, int64_t n_rows, int hid
  *   d_out [n_rows, hidden] -> d_rows [n_rows, hidden], dw1 (and dw1_up: SWIGLU's
  *   gate and up gradients [n_slabs, ffn, hidden] apart), dw2 [n_slabs, hidden, ffn]
  *   d_pre [n_rows, columns of the first product], a [n_rows, ffn] and, in fp32,
- *   da [n_rows, ffn] are scratch (bf16: da may be NULL). */
+ *   da [n_rows, ffn] are scratch (bf16: da may be NULL); `scratch` as for the
+ *   gradients (the largest of what dice_grouped_scratch_bytes says for
+ *   (hidden, ffn) weight, (columns, hidden) weight and input gradient). */
 DICE_API int dice_grouped_ffn_backward(const void* d_out, const void* rows_in, const void* kept, const float* scales,
                               int64_t n_rows, int hidden, int ffn, int act, int keep, int dtype, const void* w1,
                               const void* w2, int n_slabs, const int32_t* seg_offsets, void* da, void* d_pre,
-                              void* a, void* d_rows, void* dw1, void* dw1_up, void* dw2, uint32_t* status,
-                              void* stream);
+                              void* a, void* d_rows, void* dw1, void* dw1_up, void* dw2, void* scratch,
+                              size_t scratch_bytes, uint32_t* status, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Expert-parallel exchange over NVLink peer memory (one process per GPU, one

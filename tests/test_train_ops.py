@@ -10,7 +10,7 @@ def test_c_abi_refuses_on_the_host():
     lib = _lib.load()
     P = 1 << 20  # a pointer that is aligned and never followed: every call below is refused before a launch
     dgrad = lambda n_rows=4, n=64, k=32, slabs=2, segs=2, dt=0, dy=P, w=P, out=P, seg=P, slab=None: lib.dice_grouped_dgrad(  # noqa: E731
-        dy, n_rows, n, w, slabs, k, seg, slab, segs, dt, out, None, None)
+        dy, n_rows, n, w, slabs, k, seg, slab, segs, dt, out, None, 0, None, None)
     assert dgrad(n=60) == -2 and dgrad(k=36) == -2
     assert dgrad(dt=7) == -3
     assert dgrad(segs=300, slabs=300) == -7 and dgrad(n_rows=1 << 31) == -7
@@ -19,9 +19,12 @@ def test_c_abi_refuses_on_the_host():
     assert dgrad(n_rows=-1) == -1
     assert dgrad(n_rows=0, dy=None, w=None, out=None, seg=None) == 0
     wgrad = lambda n_rows=4, n=256, k=32, slabs=2, gu=0, dt=0, dw=P, up=P: lib.dice_grouped_wgrad(  # noqa: E731
-        P, P, n_rows, n, k, P, slabs, gu, dt, dw, up, None, None)
+        P, P, n_rows, n, k, P, slabs, gu, dt, dw, up, None, 0, None, None)
     assert wgrad(n=60) == -2 and wgrad(gu=200) == -2 and wgrad(gu=100) == -2  # 200 takes 512 packed columns; 100 is no multiple of 8
     assert wgrad(gu=128, up=None) == -1 and wgrad(dw=P + 4) == -4 and wgrad(slabs=257) == -7 and wgrad(gu=-1) == -1
+    # a split needs a GPU whose size is known, a bf16 product, few tiles and a long reduction
+    assert lib.dice_grouped_scratch_bytes(100, 4096, 64, 1, 0, 1) == 0 and lib.dice_grouped_scratch_bytes(0, 4096, 64, 1, 0, 0) == 0
+    assert lib.dice_grouped_scratch_bytes(100, 60, 64, 1, 0, 0) == 0
     keep = lambda ffn=64, act=0, kp=1, dt=0, codes=P, scales=P: lib.dice_act_keep(P, 4, ffn, act, kp, dt, P, codes, scales, None)  # noqa: E731
     assert keep(ffn=60) == -2 and keep(act=5) == -1 and keep(kp=9) == -1 and keep(dt=3) == -3
     assert keep(codes=None) == -1 and keep(scales=None) == -1 and keep(codes=P + 8) == -4
@@ -36,7 +39,7 @@ def test_c_abi_refuses_on_the_host():
     assert train(kp=0) == -1  # no buffer for the first product, which is what would be kept
     assert train(kp=5) == -1
     backward = lambda act=0, up=P, dw2=P, h=64: lib.dice_grouped_ffn_backward(  # noqa: E731
-        P, P, P, P, 4, h, 64, act, 1, 0, P, P, 2, P, P, P, P, P, P, up, dw2, None, None)
+        P, P, P, P, 4, h, 64, act, 1, 0, P, P, 2, P, P, P, P, P, P, up, dw2, None, 0, None, None)
     assert backward(act=9) == -1 and backward(up=None) == -1 and backward(dw2=None) == -1 and backward(h=20) == -2
 
 

@@ -87,6 +87,30 @@ def test_wgrad(cuda_device, counts, n, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("counts,n,k", [
+    ([1], 9216, 64), ([2, 0, 1], 4608, 264), ([300], 2048, 72), ([129, 3], 1160, 520),   # shared by the input gradient
+    ([6000], 72, 64), ([3001, 0, 700], 136, 264), ([1100], 264, 328),                      # and by the weight gradient
+    ([1, 1], 1152, 4608),                                                                   # narrow tiles, nothing shared
+])
+def test_long_reductions_and_few_tiles(cuda_device, counts, n, k, dtype):
+    """Few tiles: the reduction is shared, and added up in a fixed order."""
+    gen = _gen(16)
+    rows, e = sum(counts), len(counts)
+    dy, x, w = _randn(gen, rows, n, dtype=dtype), _randn(gen, rows, k, dtype=dtype), _randn(gen, e, n, k, dtype=dtype, scale=0.02)
+    seg = _seg(counts, cuda_device)
+    dx, dw = ops.grouped_dgrad(dy, w, seg), ops.grouped_wgrad(dy, x, seg)
+    r = 0
+    for s, c in enumerate(counts):
+        a, b, g = dy[r:r + c].to(D), w[s].to(D), x[r:r + c].to(D)
+        _check_product(dx[r:r + c], a @ b, a.abs() @ b.abs(), n, dtype)
+        _check_product(dw[s], a.T @ g, a.abs().T @ g.abs(), c, dtype)
+        r += c
+    for _ in range(5):
+        assert torch.equal(dx, ops.grouped_dgrad(dy, w, seg)) and torch.equal(dw, ops.grouped_wgrad(dy, x, seg))
+    ops.check_status(ops.device_status(cuda_device))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("ffn", [8, 64, 128, 136, 320, 1152])
 def test_wgrad_gate_up(cuda_device, ffn, dtype):
     """The packed rows' gradient written apart is that of the packed form, bit for bit."""
@@ -474,6 +498,16 @@ def test_other_stream_and_two_calls_at_once(cuda_device):
     want = [step(0), step(1)]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    few = [(_randn(gen, 900, 72, dtype=torch.bfloat16), _randn(gen, 900, 64, dtype=torch.bfloat16)) for _ in range(2)]
+    one = _seg([900], cuda_device)  # a shared reduction has scratch, each call its own
+    want_few = [ops.grouped_wgrad(*f, one) for f in few]
+    for _ in range(5):
+        got_few = []
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got_few.append([ops.grouped_wgrad(*few[i], one) for _ in range(4)])
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for gs, w in zip(got_few, want_few) for g in gs)
     for _ in range(5):
         got = []
         for i, st in enumerate(streams):
