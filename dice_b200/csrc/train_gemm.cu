@@ -425,8 +425,8 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     s_mprefix[p.n_seg] = run;
     // shares of the reduction: as many as there are pairs for every tile, if each is long enough
     int split = 1;
-    const int64_t wide_tiles = static_cast<int64_t>(run) * ((p.n_cols + BN - 1) / BN);
-    const int bn = EPI == EPI_PLAIN && 2 * wide_tiles <= n_pairs ? BN / 2 : BN;
+    const int64_t narrow_tiles = static_cast<int64_t>(run) * ((p.n_cols + BN / 2 - 1) / (BN / 2));
+    const int bn = EPI == EPI_PLAIN && narrow_tiles <= n_pairs ? BN / 2 : BN;
     if (EPI == EPI_PLAIN && p.split_ws != nullptr && run > 0) {
       const int64_t per_tile = n_pairs / (static_cast<int64_t>(run) * ((p.n_cols + bn - 1) / bn));
       const int blocks = MODE != MODE_TN ? p.red_blocks : (most + BK - 1) / BK;

@@ -16,7 +16,8 @@
 // reduction, added up in shared memory at the end (1024 rows through 8 experts, 4608 -> 1152: 180 tiles alone would
 // leave most of the GPU's warp slots empty).  Where even that leaves slots empty or a nearly empty last wave, the 2 to 8
 // CTAs of a cluster share a tile's reduction in the same way and the first adds up what the others hold in shared
-// memory.  The order of all these sums is fixed.  TN has many tiles and a short reduction: 128 x 128 tiles, one group.
+// memory.  The order of all these sums is fixed.  A tile with at most 8 rows (single tokens) is bounded by reading the
+// weights: its CTA forgoes the tiling and streams them, every value used for the rows there are.  TN has many tiles and a short reduction: 128 x 128 tiles, one group.
 #include "train.cuh"
 #include "umma.cuh"  // sm_count_cached
 
@@ -147,7 +148,66 @@ struct Slices {
   float a[kRing][TK][TM + 4], b[kRing][TK][TN + 4];
 };
 constexpr int kRowsSmem = GROUPS * sizeof(Slices);
-static_assert(kRowsSmem >= 2 * TM * TN * sizeof(float), "the groups' sums are exchanged in place of the slices");
+static_assert(kRowsSmem >= 2 * TM * TN * sizeof(float) && kRowsSmem >= 16 * 8 * TN * sizeof(float),
+              "sums are exchanged in place of the slices");
+
+// A tile of at most kThinRows rows: every thread sums over its own part of the reduction, straight from memory, and the
+// parts are added in shared memory (`sums`, [ROWS][64] of them at its front at the end).  NN: 16 threads hold a weight
+// row's 64 columns, 16 rows at once.  NT: a warp holds a weight row (one column), its lanes four elements each.
+constexpr int kThinRows = 8;
+template <int MODE, int ROWS>
+__device__ __forceinline__ void thin_tile(const float* a, int64_t lda, const float* w, int64_t ldb, int rows, int n_valid, int red,
+                                          int share, int shares, float* sums) {
+  if (MODE == MODE_NN) {
+    const int c = (threadIdx.x & 15) * 4, n0 = static_cast<int>(threadIdx.x >> 4);
+    float acc[ROWS][4] = {};
+    if (c < n_valid) {
+#pragma unroll 4
+      for (int n = share * 16 + n0; n < red; n += shares * 16) {
+        const float4 x = *reinterpret_cast<const float4*>(w + n * ldb + c);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          const float y = r < rows ? a[r * lda + n] : 0.f;
+          acc[r][0] = fmaf(y, x.x, acc[r][0]);
+          acc[r][1] = fmaf(y, x.y, acc[r][1]);
+          acc[r][2] = fmaf(y, x.z, acc[r][2]);
+          acc[r][3] = fmaf(y, x.w, acc[r][3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) *reinterpret_cast<float4*>(&sums[(n0 * ROWS + r) * TN + c]) = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+    __syncthreads();
+    for (int i = threadIdx.x; i < ROWS * TN; i += 64 * GROUPS) {
+      float t = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) t += sums[k * ROWS * TN + i];
+      sums[i] = t;  // (only this thread reads or writes place i of the 16)
+    }
+  } else {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int c = warp; c < n_valid; c += 2 * GROUPS) {
+      float acc[ROWS] = {};
+#pragma unroll 2
+      for (int k = (share * 32 + lane) * 4; k < red; k += shares * 128) {
+        const float4 x = *reinterpret_cast<const float4*>(w + c * ldb + k);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          if (r < rows) {
+            const float4 y = *reinterpret_cast<const float4*>(a + r * lda + k);
+            acc[r] = fmaf(y.x, x.x, fmaf(y.y, x.y, fmaf(y.z, x.z, fmaf(y.w, x.w, acc[r]))));
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        for (int off = 16; off > 0; off >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], off);
+        if (lane == 0) sums[r * TN + c] = acc[r];
+      }
+    }
+  }
+  __syncthreads();
+}
 
 template <int MODE>
 __global__ void __launch_bounds__(64 * GROUPS, 2) simt_rows_kernel(const SimtParams p) {
@@ -182,7 +242,7 @@ __global__ void __launch_bounds__(64 * GROUPS, 2) simt_rows_kernel(const SimtPar
   __syncthreads();
   if (s_slab < 0) return;
   const int row0 = s_row0, m_valid = s_rows;
-  const int col0 = blockIdx.y * TN, n_valid = p.n_cols - col0;
+  const int col0 = blockIdx.y * TN, n_valid = p.n_cols - col0 < TN ? p.n_cols - col0 : TN;
   const int group = threadIdx.x >> 6, t = threadIdx.x & 63;
   const int ra = (t >> 3) * 4, cb = (t & 7) * 4;
 
@@ -190,6 +250,29 @@ __global__ void __launch_bounds__(64 * GROUPS, 2) simt_rows_kernel(const SimtPar
   const float* a = static_cast<const float*>(p.a) + static_cast<int64_t>(row0) * lda;
   const float* b = static_cast<const float*>(p.b) + (kB ? (static_cast<int64_t>(s_slab) * p.n_cols + col0) * ldb
                                                : static_cast<int64_t>(s_slab) * p.red * ldb + col0);
+  if (m_valid <= kThinRows) {
+    float* sums = reinterpret_cast<float*>(slices);
+    if (m_valid <= 2) thin_tile<MODE, 2>(a, lda, b, ldb, m_valid, n_valid, p.red, blockIdx.z, gridDim.z, sums);
+    else thin_tile<MODE, kThinRows>(a, lda, b, ldb, m_valid, n_valid, p.red, blockIdx.z, gridDim.z, sums);
+    if (gridDim.z > 1) cluster_sync();
+    if (blockIdx.z == 0) {
+      float* out = static_cast<float*>(p.out) + static_cast<int64_t>(row0) * p.n_cols + col0;
+      for (int i = threadIdx.x; i < m_valid * TN; i += 64 * GROUPS) {
+        float t = sums[i];
+        const uint32_t here = static_cast<uint32_t>(__cvta_generic_to_shared(sums + i));
+        for (uint32_t other = 1; other < gridDim.z; ++other) {
+          uint32_t there;
+          float y;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(other));
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(there));
+          t += y;
+        }
+        if (i % TN < n_valid) out[static_cast<int64_t>(i / TN) * p.n_cols + i % TN] = t;
+      }
+    }
+    if (gridDim.z > 1) cluster_sync();
+    return;
+  }
   const int64_t b_slice = kB ? TK : static_cast<int64_t>(TK) * ldb;
   const int sharing = GROUPS * static_cast<int>(gridDim.z), share = static_cast<int>(blockIdx.z) * GROUPS + group;
   a += static_cast<int64_t>(share) * TK;
