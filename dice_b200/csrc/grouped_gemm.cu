@@ -363,6 +363,19 @@ int encode_map3(CUtensorMap* map, const void* base, uint64_t slabs, uint64_t row
   return r == CUDA_SUCCESS ? DICE_OK : DICE_ERR_CUDA;
 }
 
+int encode_store_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int elem_bytes) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (fn == nullptr) return DICE_ERR_CUDA;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * elem_bytes};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(64 / elem_bytes), 32};
+  const cuuint32_t elem_strides[2] = {1, 1};
+  const CUresult r = fn(map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                        const_cast<void*>(base), dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? DICE_OK : DICE_ERR_CUDA;
+}
+
 int sm_count_cached() {
   static int cached[64] = {0};
   int dev = 0;

@@ -43,7 +43,11 @@ enum { MODE_NT = 0, MODE_NN = 1, MODE_TN = 2 };
 enum { EPI_PLAIN = 0, EPI_KEEP = 1, EPI_BACK = 2 };
 
 constexpr int PM = 256;
-constexpr int kStagesT = 6;
+// Operand ring slots and, per epilogue warp, staging buffers of 32 rows x 64 bytes.  The activation's epilogues write (and
+// read) several bytes for every one of a plain product, so they give a ring slot for two more buffers and let the copy
+// unit store them (see Stager).
+constexpr int stages_of(int epi) { return epi == EPI_PLAIN ? 6 : 5; }
+constexpr int buffers_of(int epi) { return epi == EPI_PLAIN ? 1 : 3; }
 constexpr int kStageBytesT = 32768;  // 128 rows (or columns) x 64 of each operand
 constexpr int kOperandBytes = 16384;
 constexpr int kBoxBytes = 8192;      // 64 reduction rows x 128 bytes
@@ -51,7 +55,9 @@ constexpr int kBoxBytes = 8192;      // 64 reduction rows x 128 bytes
 constexpr int threads_of(int mode) { return 32 * (2 + kEpilogueWarps + (mode == MODE_TN ? 1 : 0)); }
 constexpr int kStageStore = 2048;    // per epilogue warp, as in grouped_gemm_pair.cu
 constexpr int kExchangeBytes = 4096;  // EPI_KEEP, SwiGLU: group maxima, [2 tiles][2 halves][gate, up][128 rows]
-constexpr int kSmemT = kStagesT * kStageBytesT + kAuxBytes + kEpilogueWarps * kStageStore + kExchangeBytes + 1024;
+constexpr int smem_of(int epi) {
+  return stages_of(epi) * kStageBytesT + kAuxBytes + kEpilogueWarps * buffers_of(epi) * kStageStore + kExchangeBytes + 1024;
+}
 constexpr int kSplitFloats = 4 * 32 * 32;  // an epilogue warp's part of a tile: 4 chunks of 32 rows x 32 columns
 constexpr int kMinSplitBlocks = 4;         // k-blocks of a share, at least
 constexpr int kMaxSplit = 16;              // the last warp reads the shares one after the other
@@ -78,6 +84,7 @@ struct TrainGemm {
   const float* kept_scales;
   int kept_wide;                // its rows are whole pieces of 32 bytes
   uint8_t* codes;               // EPI_KEEP
+  int codes_tma;                // its rows are whole pieces of 16 bytes
   float* scales;
 };
 
@@ -106,22 +113,57 @@ __device__ __forceinline__ void mbar_complete_tx_cluster(uint32_t cluster_addr, 
 __device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// 32 rows of 64 bytes that a warp holds one row per lane, stored so that an instruction covers whole 64-byte pieces:
-// through shared memory, where lane l then takes piece (l & 3) of rows (l >> 2) + 8 i.  `put(i, piece, v)` stores one.
-template <typename F>
-__device__ __forceinline__ void store_transposed(uint4* buf, int lane, const uint4 (&mine)[4], F put) {
-  const int swz = (lane >> 1) & 3;
+// Stores of 32 rows of 64 bytes that a warp holds one row per lane.  They go through shared memory, laid out as the 64-byte
+// swizzle wants it.  If all 32 rows exist (a segment's last tile may have fewer) and BUFS > 1, the copy unit stores them as
+// one box, clipped to the tensor's columns; a few buffers in turn, of which the one about to be written is no longer read.
+// Else lane l takes piece (l & 3) of rows (l >> 2) + 8 i, so that an instruction covers whole 64-byte pieces:
+// `put(i, piece, v)` stores one.  An SM's memory path handles so many lines a cycle; a chunk's three outputs cost it
+// 48 + 48 + 96 this way and 48 + 0 + 0 by the copy unit, beside the operands' 128 a k-block.
+template <int BUFS>
+struct Stager {
+  uint8_t* buffers;
+  int lane, next, row0;
+  bool whole;
+  template <typename F>
+  __device__ __forceinline__ void store(const uint4 (&mine)[4], const CUtensorMap* map, int c, F put) {
+    const int swz = (lane >> 1) & 3;
+    if (BUFS > 1) {
+      // the copies that may still read: with the copy unit all but the oldest buffer's, else none
+      if (lane == 0) {
+        if (whole && map != nullptr) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(BUFS - 1) : "memory");
+        else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      }
+      __syncwarp();
+    }
+    uint4* buf = reinterpret_cast<uint4*>(buffers + next * kStageStore);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) buf[lane * 4 + (j ^ swz)] = mine[j];
-  __syncwarp();
-  const int piece = lane & 3;
+    for (int j = 0; j < 4; ++j) buf[lane * 4 + (j ^ swz)] = mine[j];
+    if (BUFS > 1 && whole && map != nullptr) {
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                     "r"(c), "r"(row0), "r"(smem_u32(buf))
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+      next = next == BUFS - 1 ? 0 : next + 1;
+      return;
+    }
+    __syncwarp();
+    const int piece = lane & 3;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int rr = i * 8 + (lane >> 2);
-    put(i, piece, buf[rr * 4 + (piece ^ ((rr >> 1) & 3))]);
+    for (int i = 0; i < 4; ++i) {
+      const int rr = i * 8 + (lane >> 2);
+      put(i, piece, buf[rr * 4 + (piece ^ ((rr >> 1) & 3))]);
+    }
+    __syncwarp();
   }
-  __syncwarp();
-}
+  // before the buffers go: everything has been read and written
+  __device__ __forceinline__ void finish() {
+    if (BUFS > 1 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+};
 __device__ __forceinline__ uint4 pack8(const float* v) {
   return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
@@ -129,9 +171,10 @@ __device__ __forceinline__ uint4 pack8(const float* v) {
 // EPI_KEEP: one tile of the first product, by one of the two warps that share 32 rows.  SwiGLU: the tile's columns are
 // 128 gate and 128 up columns of the same 128 activations, a warp takes 64 of them, and the two warps exchange their parts
 // of the groups' maxima; GELU: the tile is two groups, a warp takes one.  Columns behind ffn count as zeros.
-template <int ACT, int KEEP, typename Fetch, typename Store>
+template <int ACT, int KEEP, typename Fetch, typename Store, typename Staging>
 __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, int half, int lane, int row, bool row_ok,
-                                          const int64_t (&dst_row)[4], uint4* stage_buf, float* exchange, uint32_t bar,
+                                          const int64_t (&dst_row)[4], Staging& stager, const CUtensorMap* tm_out,
+                                          const CUtensorMap* tm_act, const CUtensorMap* tm_codes, float* exchange, uint32_t bar,
                                           uint32_t phase, volatile uint32_t* abort_flag, Fetch fetch, Store store_bf16) {
   constexpr bool GLU = ACT == DICE_ACT_SWIGLU;
   // this warp's first activation column, and how many of its 64 (GELU: 128) exist
@@ -194,7 +237,7 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
         const f32x2 x = bf16_pair<f32x2>(w[q][j]);
         ow[j] = to_bf16(GLU ? swiglu2<false>(x, bf16_pair<f32x2>(w[q + 2][j])) : gelu2<false>(x));
       }
-      store_bf16(o, p.act_out, p.ffn, act0 + q * 32, valid - q * 32);
+      store_bf16(o, tm_act, p.act_out, p.ffn, act0 + q * 32, valid - q * 32);
     }
   }
   // what is kept: SwiGLU all 64 gate and 64 up columns (the filling ones are zeros), GELU those that exist
@@ -207,7 +250,7 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
         uint32_t* ow = reinterpret_cast<uint32_t*>(o);
 #pragma unroll
         for (int j = 0; j < 16; ++j) ow[j] = w[q][j];
-        store_bf16(o, p.out, p.arg_cols, GLU ? nb * 256 + (q >> 1) * 128 + half * 64 + (q & 1) * 32 : act0 + q * 32, left);
+        store_bf16(o, tm_out, p.out, p.arg_cols, GLU ? nb * 256 + (q >> 1) * 128 + half * 64 + (q & 1) * 32 : act0 + q * 32, left);
       }
     }
   } else {
@@ -224,7 +267,7 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
           ow[j] = keep_codes4<KEEP>(mul2(bf16_pair<f32x2>(lo), f), mul2(bf16_pair<f32x2>(hi), f));
         }
         const int c = GLU ? nb * 256 + g * 128 + half * 64 : act0 + g * 64;
-        store_transposed(stage_buf, lane, o, [&](int i, int piece, const uint4& v) {
+        stager.store(o, GLU || p.codes_tma ? tm_codes : nullptr, c, [&](int i, int piece, const uint4& v) {
           if (dst_row[i] < 0) return;
           uint8_t* dst = p.codes + dst_row[i] * p.arg_cols + c + piece * 16;
           // a row of GELU codes may start on 8 bytes only, and end in the middle of a piece
@@ -319,7 +362,7 @@ struct BackChunk {
 // packed order's last block (whose filling columns get gradient zero)
 template <int ACT, int KEEP, typename Fetch, typename Store>
 __device__ __forceinline__ void back_tile(const TrainGemm& p, int nb, int half, int row, bool row_ok, BackChunk<ACT, KEEP>& kept,
-                                          Fetch fetch, Store store_bf16) {
+                                          const CUtensorMap* tm_out, const CUtensorMap* tm_act, Fetch fetch, Store store_bf16) {
   constexpr bool GLU = ACT == DICE_ACT_SWIGLU;
   const int end = GLU ? p.arg_cols / 2 : p.ffn;
   for (int h = 0; h < 128; h += 32) {
@@ -346,15 +389,18 @@ __device__ __forceinline__ void back_tile(const TrainGemm& p, int nb, int half, 
     }
     if (h + 32 < 128 && col + 32 < end) kept.load(p, col + 32, row, row_ok);  // on its way while this chunk is stored
     const int at = GLU ? col + col / kKeepGroup * kKeepGroup : col;
-    store_bf16(og, p.out, p.arg_cols, at, GLU ? 32 : left);
-    if (GLU) store_bf16(ou, p.out, p.arg_cols, at + kKeepGroup, 32);
-    if (left > 0) store_bf16(oa, p.act_out, p.ffn, col, left);
+    store_bf16(og, tm_out, p.out, p.arg_cols, at, GLU ? 32 : left);
+    if (GLU) store_bf16(ou, tm_out, p.out, p.arg_cols, at + kKeepGroup, 32);
+    if (left > 0) store_bf16(oa, tm_act, p.act_out, p.ffn, col, left);
   }
 }
 
 template <int MODE, int EPI, int ACT, int KEEP>
 __global__ void __launch_bounds__(threads_of(MODE), 1)
-train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const TrainGemm p) {
+train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                  const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ CUtensorMap tm_act,
+                  const __grid_constant__ CUtensorMap tm_codes, const TrainGemm p) {
+  constexpr int kStagesT = stages_of(EPI);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* aux = smem + kStagesT * kStageBytesT;
@@ -614,6 +660,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     const int half = (warp - 2) >> 2;  // which of the quadrant's warps: its share of the columns
     int acc = 0, seg = 0;
     uint32_t acc_phase = 0, xchg_phase = 0;
+    Stager<buffers_of(EPI)> stager = {aux + kAuxBytes + (warp - 2) * buffers_of(EPI) * kStageStore, lane, 0, 0, false};
     for (int64_t t = pair_id; t < total; t += n_pairs) {
       const Tile ti = decode(t, seg);
       if (ti.zero && ti.share != 0) continue;
@@ -649,10 +696,11 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           }
         }
       }
-      uint4* stage_buf = reinterpret_cast<uint4*>(aux + kAuxBytes + (warp - 2) * kStageStore);
-      // 32 bf16 columns (eight words of eight) from column c of a tensor with ld columns, of which n_left exist
-      auto store_bf16 = [&](const uint4 (&w)[4], __nv_bfloat16* base, int64_t ld, int c, int n_left) {
-        store_transposed(stage_buf, lane, w, [&](int i, int piece, const uint4& v) {
+      stager.row0 = ti.row0 + quad * 32;
+      stager.whole = ti.rows_valid >= quad * 32 + 32;
+      // 32 bf16 columns from column c of a tensor with ld columns, of which n_left exist
+      auto store_bf16 = [&](const uint4 (&w)[4], const CUtensorMap* map, __nv_bfloat16* base, int64_t ld, int c, int n_left) {
+        stager.store(w, map, c, [&](int i, int piece, const uint4& v) {
           if (dst_row[i] >= 0 && piece * 8 < n_left) *reinterpret_cast<uint4*>(base + dst_row[i] * ld + c + piece * 8) = v;
         });
       };
@@ -709,15 +757,17 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           float v[32];
           fetch(c, v);
           const uint4 w[4] = {pack8(v), pack8(v + 8), pack8(v + 16), pack8(v + 24)};
-          store_bf16(w, up_rows ? p.out_up : p.out, p.n_cols, col0 + c, n_valid - c);
+          store_bf16(w, nullptr, up_rows ? p.out_up : p.out, p.n_cols, col0 + c, n_valid - c);
         }
       } else if (EPI == EPI_KEEP) {
         keep_tile<ACT, KEEP>(p, ti.nb, quad, half, lane, ti.row0 + quad * 32 + lane, quad * 32 + lane < ti.rows_valid, dst_row,
-                             stage_buf, reinterpret_cast<float*>(aux + kAuxBytes + kEpilogueWarps * kStageStore),
+                             stager, &tm_out, &tm_act, &tm_codes,
+                             reinterpret_cast<float*>(aux + kAuxBytes + kEpilogueWarps * buffers_of(EPI) * kStageStore),
                              xchg_bar + 8 * quad, xchg_phase, abort_flag, fetch, store_bf16);
         xchg_phase ^= 1u;
       } else {
-        back_tile<ACT, KEEP>(p, ti.nb, half, ti.row0 + quad * 32 + lane, quad * 32 + lane < ti.rows_valid, kept, fetch, store_bf16);
+        back_tile<ACT, KEEP>(p, ti.nb, half, ti.row0 + quad * 32 + lane, quad * 32 + lane < ti.rows_valid, kept, &tm_out, &tm_act,
+                             fetch, store_bf16);
       }
       if (summed) {
         tc_fence_before_sync();
@@ -726,6 +776,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         if (++acc == kAccStages) { acc = 0; acc_phase ^= 1u; }
       }
     }
+    stager.finish();
   }
 
   // ---------------- teardown ----------------
@@ -751,13 +802,13 @@ int resident_pairs_train() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   if (cached[dev] == 0) {
-    if (cudaFuncSetAttribute(train_gemm_kernel<MODE, EPI, ACT, KEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemT) != cudaSuccess) return 0;
+    if (cudaFuncSetAttribute(train_gemm_kernel<MODE, EPI, ACT, KEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of(EPI)) != cudaSuccess) return 0;
     const int sms = sm_count_cached();
     if (sms <= 0) return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(sms & ~1), 1, 1);
     cfg.blockDim = dim3(threads_of(MODE), 1, 1);
-    cfg.dynamicSmemBytes = kSmemT;
+    cfg.dynamicSmemBytes = smem_of(EPI);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
@@ -773,13 +824,13 @@ int resident_pairs_train() {
 }
 
 template <int MODE, int EPI = EPI_PLAIN, int ACT = 0, int KEEP = 0>
-int launch_train(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const TrainGemm& p, int64_t most_tiles, int pairs,
-                 cudaStream_t stream) {
+int launch_train(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const CUtensorMap* stores, const TrainGemm& p,
+                 int64_t most_tiles, int pairs, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   const int64_t use = most_tiles < pairs && p.split_ws == nullptr ? most_tiles : pairs;
   cfg.gridDim = dim3(static_cast<unsigned>(2 * use), 1, 1);
   cfg.blockDim = dim3(threads_of(MODE), 1, 1);
-  cfg.dynamicSmemBytes = kSmemT;
+  cfg.dynamicSmemBytes = smem_of(EPI);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -791,7 +842,7 @@ int launch_train(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const TrainGe
   cfg.attrs = attr;
   cfg.numAttrs = dice_pdl_enabled() ? 2 : 1;
   dice_count_launch();
-  return cudaLaunchKernelEx(&cfg, train_gemm_kernel<MODE, EPI, ACT, KEEP>, tm_a, tm_b, p) == cudaSuccess ? DICE_OK : DICE_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, train_gemm_kernel<MODE, EPI, ACT, KEEP>, tm_a, tm_b, stores[0], stores[1], stores[2], p) == cudaSuccess ? DICE_OK : DICE_ERR_CUDA;
 }
 
 int64_t col_tiles(int cols, int width) { return (static_cast<int64_t>(cols) + width - 1) / width; }
@@ -845,8 +896,9 @@ int dice_internal_tc_dgrad(const void* dy, int64_t n_rows, int n_dim, const void
   p.n_cols = k_dim;
   p.out = static_cast<__nv_bfloat16*>(dx);
   p.status = status;
+  const CUtensorMap no_stores[3] = {tm_a, tm_a, tm_a};  // a plain epilogue stores from registers
   if ((rc = use_scratch(p, scratch, scratch_bytes, pairs, s)) != DICE_OK) return rc;
-  return launch_train<MODE_NN>(tm_a, tm_b, p, ((n_rows + PM - 1) / PM + n_seg) * col_tiles(k_dim, BN / 2), pairs, s);
+  return launch_train<MODE_NN>(tm_a, tm_b, no_stores, p, ((n_rows + PM - 1) / PM + n_seg) * col_tiles(k_dim, BN / 2), pairs, s);
 }
 
 int dice_internal_tc_wgrad(const void* dy, const void* x, int64_t n_rows, int n_dim, int k_dim, const int32_t* seg_offsets,
@@ -872,30 +924,31 @@ int dice_internal_tc_wgrad(const void* dy, const void* x, int64_t n_rows, int n_
   p.out = static_cast<__nv_bfloat16*>(dw);
   p.out_up = static_cast<__nv_bfloat16*>(dw_up);
   p.status = status;
+  const CUtensorMap no_stores[3] = {tm_a, tm_a, tm_a};  // a plain epilogue stores from registers
   if ((rc = use_scratch(p, scratch, scratch_bytes, pairs, s)) != DICE_OK) return rc;
-  return launch_train<MODE_TN>(tm_a, tm_b, p, static_cast<int64_t>(n_slabs) * p.n_mblk * col_tiles(k_dim, BN / 2), pairs, s);
+  return launch_train<MODE_TN>(tm_a, tm_b, no_stores, p, static_cast<int64_t>(n_slabs) * p.n_mblk * col_tiles(k_dim, BN / 2), pairs, s);
 }
 
 namespace {
 
 template <int ACT, int KEEP>
-int run_keep(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const TrainGemm& p, cudaStream_t s) {
+int run_keep(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const CUtensorMap* st, const TrainGemm& p, cudaStream_t s) {
   const int pairs = resident_pairs_train<MODE_NT, EPI_KEEP, ACT, KEEP>();
   if (pairs <= 0) return DICE_ERR_CUDA;
-  return launch_train<MODE_NT, EPI_KEEP, ACT, KEEP>(tm_a, tm_b, p, ((p.n_rows + PM - 1ll) / PM + p.n_seg) * col_tiles(p.n_cols, BN), pairs, s);
+  return launch_train<MODE_NT, EPI_KEEP, ACT, KEEP>(tm_a, tm_b, st, p, ((p.n_rows + PM - 1ll) / PM + p.n_seg) * col_tiles(p.n_cols, BN), pairs, s);
 }
 template <int ACT, int KEEP>
-int run_back(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const TrainGemm& p, cudaStream_t s) {
+int run_back(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const CUtensorMap* st, const TrainGemm& p, cudaStream_t s) {
   const int pairs = resident_pairs_train<MODE_NN, EPI_BACK, ACT, KEEP>();
   if (pairs <= 0) return DICE_ERR_CUDA;
-  return launch_train<MODE_NN, EPI_BACK, ACT, KEEP>(tm_a, tm_b, p, ((p.n_rows + PM - 1ll) / PM + p.n_seg) * col_tiles(p.n_cols, BN), pairs, s);
+  return launch_train<MODE_NN, EPI_BACK, ACT, KEEP>(tm_a, tm_b, st, p, ((p.n_rows + PM - 1ll) / PM + p.n_seg) * col_tiles(p.n_cols, BN), pairs, s);
 }
 template <int ACT>
-int run_epilogue(bool back, int keep, const CUtensorMap& tm_a, const CUtensorMap& tm_b, const TrainGemm& p, cudaStream_t s) {
+int run_epilogue(bool back, int keep, const CUtensorMap& tm_a, const CUtensorMap& tm_b, const CUtensorMap* st, const TrainGemm& p, cudaStream_t s) {
   switch (keep) {
-    case DICE_KEEP_INT8: return back ? run_back<ACT, DICE_KEEP_INT8>(tm_a, tm_b, p, s) : run_keep<ACT, DICE_KEEP_INT8>(tm_a, tm_b, p, s);
-    case DICE_KEEP_E4M3: return back ? run_back<ACT, DICE_KEEP_E4M3>(tm_a, tm_b, p, s) : run_keep<ACT, DICE_KEEP_E4M3>(tm_a, tm_b, p, s);
-    default: return back ? run_back<ACT, DICE_KEEP_NONE>(tm_a, tm_b, p, s) : run_keep<ACT, DICE_KEEP_NONE>(tm_a, tm_b, p, s);
+    case DICE_KEEP_INT8: return back ? run_back<ACT, DICE_KEEP_INT8>(tm_a, tm_b, st, p, s) : run_keep<ACT, DICE_KEEP_INT8>(tm_a, tm_b, st, p, s);
+    case DICE_KEEP_E4M3: return back ? run_back<ACT, DICE_KEEP_E4M3>(tm_a, tm_b, st, p, s) : run_keep<ACT, DICE_KEEP_E4M3>(tm_a, tm_b, st, p, s);
+    default: return back ? run_back<ACT, DICE_KEEP_NONE>(tm_a, tm_b, st, p, s) : run_keep<ACT, DICE_KEEP_NONE>(tm_a, tm_b, st, p, s);
   }
 }
 
@@ -913,10 +966,16 @@ int dice_internal_tc_keep(const void* rows, int64_t n_rows, int hidden, int ffn,
                           uint32_t* status, cudaStream_t s) {
   TrainGemm p = {};
   set_argument(p, ffn, act);
-  CUtensorMap tm_a, tm_b;
+  CUtensorMap tm_a, tm_b, stores[3];
   int rc = encode_map(&tm_a, rows, static_cast<uint64_t>(n_rows), static_cast<uint64_t>(hidden), BM);
   if (rc == DICE_OK)
     rc = encode_map(&tm_b, w1, static_cast<uint64_t>(n_slabs) * static_cast<uint64_t>(p.arg_cols), static_cast<uint64_t>(hidden), BK);
+  // what is stored: pre (if it is kept), the activation, the codes
+  if (rc == DICE_OK) rc = encode_store_map(&stores[1], a, n_rows, ffn, 2);
+  stores[0] = stores[2] = stores[1];
+  p.codes_tma = p.arg_cols % 16 == 0;
+  if (rc == DICE_OK && keep == DICE_KEEP_NONE) rc = encode_store_map(&stores[0], pre, n_rows, p.arg_cols, 2);
+  if (rc == DICE_OK && keep != DICE_KEEP_NONE && p.codes_tma) rc = encode_store_map(&stores[2], codes, n_rows, p.arg_cols, 1);
   if (rc != DICE_OK) return rc;
   p.seg_offsets = seg_offsets;
   p.n_seg = n_seg;
@@ -929,8 +988,8 @@ int dice_internal_tc_keep(const void* rows, int64_t n_rows, int hidden, int ffn,
   p.codes = static_cast<uint8_t*>(codes);
   p.scales = scales;
   p.status = status;
-  return act == DICE_ACT_SWIGLU ? run_epilogue<DICE_ACT_SWIGLU>(false, keep, tm_a, tm_b, p, s)
-                                : run_epilogue<DICE_ACT_GELU_TANH>(false, keep, tm_a, tm_b, p, s);
+  return act == DICE_ACT_SWIGLU ? run_epilogue<DICE_ACT_SWIGLU>(false, keep, tm_a, tm_b, stores, p, s)
+                                : run_epilogue<DICE_ACT_GELU_TANH>(false, keep, tm_a, tm_b, stores, p, s);
 }
 
 int dice_internal_tc_back(const void* d_out, int64_t n_rows, int hidden, int ffn, int act, int keep, const void* w2, int n_slabs,
@@ -938,11 +997,14 @@ int dice_internal_tc_back(const void* d_out, int64_t n_rows, int hidden, int ffn
                           uint32_t* status, cudaStream_t s) {
   TrainGemm p = {};
   set_argument(p, ffn, act);
-  CUtensorMap tm_a, tm_b;
+  CUtensorMap tm_a, tm_b, stores[3];
   int rc = encode_map(&tm_a, d_out, static_cast<uint64_t>(n_rows), static_cast<uint64_t>(hidden), BM);
   if (rc == DICE_OK)
     rc = encode_map3(&tm_b, w2, static_cast<uint64_t>(n_slabs), static_cast<uint64_t>(hidden), static_cast<uint64_t>(ffn), BK);
+  if (rc == DICE_OK) rc = encode_store_map(&stores[0], d_pre, n_rows, p.arg_cols, 2);
+  if (rc == DICE_OK) rc = encode_store_map(&stores[1], a, n_rows, ffn, 2);
   if (rc != DICE_OK) return rc;
+  stores[2] = stores[1];
   p.seg_offsets = seg_offsets;
   p.n_seg = n_slabs;
   p.n_slabs = n_slabs;
@@ -955,6 +1017,6 @@ int dice_internal_tc_back(const void* d_out, int64_t n_rows, int hidden, int ffn
   p.kept_scales = scales;
   p.kept_wide = (reinterpret_cast<uintptr_t>(kept) & 31) == 0 && static_cast<int64_t>(p.arg_cols) * (keep == DICE_KEEP_NONE ? 2 : 1) % 32 == 0;
   p.status = status;
-  return act == DICE_ACT_SWIGLU ? run_epilogue<DICE_ACT_SWIGLU>(true, keep, tm_a, tm_b, p, s)
-                                : run_epilogue<DICE_ACT_GELU_TANH>(true, keep, tm_a, tm_b, p, s);
+  return act == DICE_ACT_SWIGLU ? run_epilogue<DICE_ACT_SWIGLU>(true, keep, tm_a, tm_b, stores, p, s)
+                                : run_epilogue<DICE_ACT_GELU_TANH>(true, keep, tm_a, tm_b, stores, p, s);
 }

@@ -241,6 +241,8 @@ __device__ __forceinline__ void store_row_chunk(__nv_bfloat16* dst, const float 
 int encode_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows);
 // [slabs][rows][cols]; a box never reaches from one slab into the next (zeros are read there)
 int encode_map3(CUtensorMap* map, const void* base, uint64_t slabs, uint64_t rows, uint64_t cols, uint32_t box_rows);
+// a matrix of 1- or 2-byte elements for stores of 32 rows x 64 bytes from shared memory with the 64-byte swizzle
+int encode_store_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int elem_bytes);
 int sm_count_cached();
 
 }  // namespace dice_umma
