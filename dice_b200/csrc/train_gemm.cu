@@ -9,6 +9,12 @@
 // in memory, 64 reduction rows of 64 columns (128 bytes, 128-byte swizzle) per TMA box, and the matrix instruction
 // reads it "MN-major"; nothing is transposed.
 //
+// Bound: the tensor cores; an instruction takes the same time for K-major and MN-major operands (512 cycles a k-block,
+// measured with all operands in shared memory).  Eight segments of 4096 rows: NN 9216 -> 1024 at 1.58 PFLOP/s, TN
+// 9216 x 1024 at 1.50, which is what the 1000 W of the GPU allow.  Where a dimension is not a whole number of tiles (1152 =
+// 4.5 of 256 columns) it is 1.2, and a weight gradient of few rows is bounded by writing it (777 rows, 16 x 1792 x
+// 7168: 111 us = 3.7 TB/s, memset 3.85).
+//
 // A weight gradient's reduction is ragged.  Its last k-block may reach into the next segment (or behind the tensor, or
 // into rows that hold anything): the instructions stop at the last 16 rows that the segment touches, and the up to
 // 15 rows of those that are not the segment's are zeroed in shared memory, in both operands, since a zero in one

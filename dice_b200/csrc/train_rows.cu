@@ -7,6 +7,11 @@
 // All three are bounded by HBM: 16 bytes (bf16) or 32 bytes (fp32) per lane and access, eight columns a lane.  For
 // the activation, 16 lanes own one group of 128 columns, so that the group's maximum is four shuffles; with SwiGLU
 // the same 16 lanes own the group's gate and its up columns, which the packed order puts 128 columns apart.
+//
+// Measured on a B200 whose copy kernel reaches 6.2 TB/s and whose memset 3.85: act_keep (int8, SwiGLU, 32768 x 4608)
+// 204 us = 5.97 TB/s (235 us before one division served four quotients and both groups' maxima shared their shuffles:
+// it issues about 20 instructions an element and was bounded by them); act_backward 228 us = 5.4 TB/s, of which the 906 MB
+// it writes are 235 us at the memset's rate; combine_backward (16384 tokens x 1152) 31.5 us = 6.0 TB/s.
 #include "train.cuh"
 
 namespace {

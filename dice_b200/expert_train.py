@@ -11,9 +11,15 @@ from __future__ import annotations
 from typing import Optional, Sequence
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ops
+
+
+def _first_order_only() -> None:
+    """The kernels' gradients have no graph.  With create_graph=True one would be left out silently, since the saved
+    tensors, not the incoming gradient, carry it."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("train_kernels offers no gradients of gradients (create_graph=True)")
 
 
 def _stack(act: str, ffn: int, dtype: torch.dtype, params: Sequence[torch.Tensor]):
@@ -56,8 +62,8 @@ class RoutedExperts(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _first_order_only()
         x, pos, seg, weights, rows_out, w1, w2, codes, scales = ctx.saved_tensors
         n = x.shape[0]
         d_out, d_weights = ops.combine_backward(dy.contiguous(), rows_out, pos, weights)
@@ -83,8 +89,8 @@ class DenseExpert(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _first_order_only()
         x, seg, w1, w2, codes, scales = ctx.saved_tensors
         dx, dw1, dw2 = ops.grouped_ffn_backward(dy.contiguous(), x, ops.KeptAct(codes, scales), w1, w2, seg, ctx.act, ctx.ffn)
         return (dx, None, None, None, *_param_grads(ctx.act, dw1, dw2, ctx.needs_input_grad[4:], ctx.param_dtypes))

@@ -625,6 +625,18 @@ def _status_ptr(status: Optional[torch.Tensor], index: int) -> int:
 _status_by_index = {}  # device number -> address of its status word, which lives as long as the process
 
 
+def _split_bytes(lib, n_rows: int, n_dim: int, k_dim: int, n_slabs: int, weight_gradient: int, code: int) -> int:
+    """dice_grouped_scratch_bytes; products with more tiles than any GPU has SM pairs for are not asked about."""
+    col_tiles = (k_dim + 127) // 128
+    if weight_gradient:
+        few = 2 * n_slabs * ((n_dim + 255) // 256) * col_tiles <= 128
+    else:
+        few = 4 * ((n_rows + 255) // 256) * col_tiles <= 128
+    if code != DICE_BF16 or not few:
+        return 0
+    return lib.dice_grouped_scratch_bytes(n_rows, n_dim, k_dim, n_slabs, weight_gradient, code)
+
+
 def _split_scratch(index: int, n_bytes: int) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
     """A product's scratch (the tensor, which the caller holds until the launch, its address and its size)."""
     if n_bytes == 0:
@@ -669,7 +681,7 @@ def grouped_dgrad(dy: torch.Tensor, w: torch.Tensor, seg_offsets: torch.Tensor, 
         out = _new((n_rows, k_dim), dy.dtype, index)
     assert out.is_contiguous() and out.shape == (n_rows, k_dim) and out.dtype == dy.dtype
     lib = _lib.load()
-    held, scratch, n_bytes = _split_scratch(index, lib.dice_grouped_scratch_bytes(n_rows, n_dim, k_dim, n_slabs, 0, code))
+    held, scratch, n_bytes = _split_scratch(index, _split_bytes(lib, n_rows, n_dim, k_dim, n_slabs, 0, code))
     _lib.check(
         lib.dice_grouped_dgrad(dy.data_ptr(), n_rows, n_dim, w.data_ptr(), n_slabs, k_dim, seg_offsets.data_ptr(),
                                _ptr(seg_slab), n_seg, code, out.data_ptr(), scratch, n_bytes, _status_ptr(status, index),
@@ -692,6 +704,7 @@ def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, seg_offsets: torch.Tensor, 
     assert dy.dim() == 2 and x.dim() == 2 and x.dtype == dy.dtype
     n_slabs = _check_segments(seg_offsets)
     assert n_slabs >= 1
+    assert gate_up is None or gate_up > 0
     code = _dtype_code(dy)
     dy, x = dy.contiguous(), x.contiguous()
     n_rows, n_dim = dy.shape
@@ -701,7 +714,7 @@ def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, seg_offsets: torch.Tensor, 
     dw = _new(shape, dy.dtype, index)
     dw_up = _new(shape, dy.dtype, index) if gate_up else None
     lib = _lib.load()
-    held, scratch, n_bytes = _split_scratch(index, lib.dice_grouped_scratch_bytes(n_rows, n_dim, k_dim, n_slabs, 1, code))
+    held, scratch, n_bytes = _split_scratch(index, _split_bytes(lib, n_rows, n_dim, k_dim, n_slabs, 1, code))
     _lib.check(
         lib.dice_grouped_wgrad(dy.data_ptr(), x.data_ptr(), n_rows, n_dim, k_dim, seg_offsets.data_ptr(), n_slabs,
                                gate_up or 0, code, dw.data_ptr(), _ptr(dw_up), scratch, n_bytes, _status_ptr(status, index),
@@ -885,9 +898,8 @@ def grouped_ffn_backward(d_out: torch.Tensor, rows: torch.Tensor, kept: KeptAct,
     dw1_up = _new((n_slabs, ffn, h), dt, index) if act == "swiglu" else None
     lib = _lib.load()
     held, scratch, n_bytes = _split_scratch(index, max(
-        lib.dice_grouped_scratch_bytes(n_rows, h, ffn, n_slabs, 1, code),
-        lib.dice_grouped_scratch_bytes(n_rows, cols, h, n_slabs, 0, code),
-        lib.dice_grouped_scratch_bytes(n_rows, cols, h, n_slabs, 1, code)))
+        _split_bytes(lib, n_rows, h, ffn, n_slabs, 1, code), _split_bytes(lib, n_rows, cols, h, n_slabs, 0, code),
+        _split_bytes(lib, n_rows, cols, h, n_slabs, 1, code)))
     _lib.check(
         lib.dice_grouped_ffn_backward(
             d_out.data_ptr(), rows.data_ptr(), codes.data_ptr(), _ptr(scales), n_rows, h, ffn, ACT_CODES[act], keep, code,

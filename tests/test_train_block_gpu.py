@@ -152,3 +152,22 @@ def test_memory_kept_in_8_bits(cuda_device):
     cols = 2 * 8 * 256 // 2  # gate and up columns of a 1024-wide expert
     rows = 2 * 4096
     assert held[None] - held["int8"] >= rows * cols * (2 - 1 - 4 / 128) * 0.99
+
+
+def test_no_tokens_and_retained_graphs(cuda_device):
+    blk = _block(64, 4, 2, cuda_device, train_keep=None)
+    x = torch.zeros(0, 5, 64, device=cuda_device, requires_grad=True)
+    blk.gate.alpha = 0.0  # (the auxiliary loss is a mean over tokens)
+    y = blk(x)
+    assert y.shape == (0, 5, 64)
+    y.sum().backward()
+    assert x.grad.shape == x.shape and bool((blk.experts[0].up_proj.weight.grad == 0).all())
+    x = torch.randn(1, 9, 64, device=cuda_device, requires_grad=True)
+    y = blk(x).sum()
+    first = torch.autograd.grad(y, [x, *blk.experts.parameters()], retain_graph=True)
+    second = torch.autograd.grad(y, [x, *blk.experts.parameters()])
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    with torch.no_grad():
+        assert torch.equal(blk(x), blk(x))
+    with pytest.raises(RuntimeError, match="gradients of gradients"):
+        torch.autograd.grad(blk(x).sum(), x, create_graph=True)

@@ -165,6 +165,15 @@ def test_no_rows_at_all(cuda_device, dtype):
     assert bool((ops.grouped_wgrad(dy, x, seg) == 0).all())
     dy, x = torch.full((5, 64), float("nan"), dtype=dtype, device=cuda_device), torch.ones(5, 72, dtype=dtype, device=cuda_device)
     assert bool((ops.grouped_wgrad(dy, x, seg) == 0).all())  # rows, but none of them any expert's
+    assert ops.grouped_wgrad(dy[:0], x[:0], seg, gate_up=None).shape == (3, 64, 72)
+    with pytest.raises(AssertionError):
+        ops.grouped_wgrad(dy, x, seg, gate_up=-8)
+    with pytest.raises(RuntimeError, match="unsupported shape"):
+        ops.grouped_wgrad(dy, x, seg, gate_up=64)  # 64 gate rows take 256 packed columns
+    with pytest.raises(RuntimeError, match="invalid argument"):
+        ops.grouped_dgrad(dy, w[:2], seg)  # three segments, two slabs, no table
+    with pytest.raises(RuntimeError, match="not 16-byte aligned"):
+        ops.grouped_dgrad(dy, w, seg, out=torch.empty(5 * 72 + 1, dtype=dtype, device=cuda_device)[1:].view(5, 72))
     a, kept = ops.act_keep(dy[:0], "gelu_tanh", 64)
     assert a.shape == (0, 64) and kept.codes.shape == (0, 64)
     d, w2 = ops.combine_backward(dy[:0], dy[:0], torch.empty(0, 2, dtype=torch.int32, device=cuda_device),
@@ -484,6 +493,36 @@ def test_what_is_kept_is_the_operators_own(cuda_device):
         a, kept2 = ops.act_keep(pre, act, ffn, keep="int8")
         assert torch.equal(kept.codes, kept2.codes) and torch.equal(kept.scales, kept2.scales)
         assert torch.equal(out, ops.grouped_gemm(a, w2, seg, ops.EPI_STORE, h, status))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_offsets_past_32_bits(cuda_device, dtype):
+    """Tensors of more than 2^31 elements: the first and the last rows are those of a call on these rows alone."""
+    gen = _gen(17)
+    rows, wide, narrow = 240000, 9216, 64
+    assert rows * wide > 2 ** 31
+    cut = [slice(0, 300), slice(rows - 300, rows)]
+    seg = torch.tensor([0, 300, rows - 300, rows], dtype=torch.int32, device=cuda_device)
+    part = _seg([300], cuda_device)
+    dy, w = _randn(gen, rows, narrow, dtype=dtype), _randn(gen, 3, narrow, wide, dtype=dtype, scale=0.1)
+    dx = ops.grouped_dgrad(dy, w, seg)
+    for c, e in zip(cut, (0, 2)):
+        assert torch.equal(dx[c], ops.grouped_dgrad(dy[c], w[e:e + 1], part))
+    dw = ops.grouped_wgrad(dx, dy, seg)  # its wide operand read back
+    for c, e in zip(cut, (0, 2)):
+        one = ops.grouped_wgrad(dx[c], dy[c], part)[0]
+        # (shares of the reduction may differ between the two calls)
+        far = (dw[e].to(D) - one.to(D)).abs()
+        assert bool((far <= 2 * U[dtype] * one.to(D).abs() + 301 * 2.0 ** -22 * (dx[c].to(D).abs().T @ dy[c].to(D).abs())).all())
+    ffn = wide // 2
+    a, kept = ops.act_keep(dx, "swiglu", ffn, keep="int8")
+    del dx
+    d_pre, a2 = ops.act_backward(a, kept, "swiglu", ffn)
+    for c in cut:
+        a_c, kept_c = ops.act_keep(ops.grouped_dgrad(dy[c], w[0 if c.start == 0 else 2][None], part), "swiglu", ffn, keep="int8")
+        assert torch.equal(a[c], a_c) and torch.equal(kept.codes[c], kept_c.codes) and torch.equal(kept.scales[c], kept_c.scales)
+        d_c, a2_c = ops.act_backward(a_c, kept_c, "swiglu", ffn)
+        assert torch.equal(d_pre[c], d_c) and torch.equal(a2[c], a2_c)
 
 
 def test_other_stream_and_two_calls_at_once(cuda_device):
