@@ -495,6 +495,19 @@ def test_what_is_kept_is_the_operators_own(cuda_device):
         assert torch.equal(out, ops.grouped_gemm(a, w2, seg, ops.EPI_STORE, h, status))
 
 
+def test_wgrad_whose_tiles_go_in_bands(cuda_device):
+    """A segment whose second operand does not stay in L2 takes its tiles in another order; the one beside it does not."""
+    gen = _gen(18)
+    counts, n, k = [4100, 70], 2328, 8264  # 10 row tiles: a band of 8 and one of 2
+    dy, x = _randn(gen, sum(counts), n, dtype=torch.bfloat16), _randn(gen, sum(counts), k, dtype=torch.bfloat16)
+    dw = ops.grouped_wgrad(dy, x, _seg(counts, cuda_device))
+    r = 0
+    for s, c in enumerate(counts):
+        a, b = dy[r:r + c].to(D).T, x[r:r + c].to(D)
+        _check_product(dw[s], a @ b, a.abs() @ b.abs(), c, torch.bfloat16)
+        r += c
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_offsets_past_32_bits(cuda_device, dtype):
     """Tensors of more than 2^31 elements: the first and the last rows are those of a call on these rows alone."""
