@@ -28,6 +28,7 @@ constexpr int WM = 128, WN = 128, WK = 16;           // TN: tile and slice
 constexpr int TM = 64, TN = 64, TK = 8, GROUPS = 4;  // NT, NN: tile, slice, groups that share the reduction
 enum { MODE_NT = 0, MODE_NN = 1 };
 
+static_assert(TK == 8, "sizes are multiples of 8, so a reduction is a whole number of slices");
 constexpr int kRing = 3;  // slices in shared memory: one being multiplied, two on their way
 
 // asynchronous copy of BYTES (4 or 16); zeros where !ok (nothing is read then)
@@ -77,23 +78,22 @@ __device__ __forceinline__ void store_tile_row(float* o, const f32x2 (&acc)[4], 
 }
 
 // One thread's share of a group's 64 x 8 operand slice.  KMAJOR: the reduction index is contiguous in memory
-// ([mn][k]); eight lanes copy a row's eight elements (one 32-byte sector), into eight banks.  Else ([k][mn]).
+// ([mn][k]); eight lanes copy a row's eight elements (one 32-byte sector), into eight banks.  Else ([k][mn]).  Rows and
+// columns that do not exist repeat the last one that does (their sums are not stored); the reduction is a whole number of
+// slices (sizes are multiples of 8), so nothing needs a zero.
 template <bool KMAJOR>
-__device__ __forceinline__ void copy_slice(float (*s)[TM + 4], const float* base, int64_t ld, int mn_valid, int64_t k_valid, int t) {
+__device__ __forceinline__ void copy_slice(float (*s)[TM + 4], const float* base, int ld, int mn_valid, int t) {
   if (KMAJOR) {
     const int k = t & 7, r = t >> 3;
 #pragma unroll
     for (int h = 0; h < 8; ++h) {
-      const bool ok = r + 8 * h < mn_valid && k < k_valid;
-      copy_async<4>(&s[k][r + 8 * h], ok ? base + static_cast<int64_t>(r + 8 * h) * ld + k : base, ok);
+      const int row = r + 8 * h < mn_valid ? r + 8 * h : mn_valid - 1;
+      copy_async<4>(&s[k][r + 8 * h], base + static_cast<uint32_t>(row) * static_cast<uint32_t>(ld) + k, true);
     }
   } else {
-    const int k = t >> 4, c = (t & 15) * 4;
+    const int k = t >> 4, c = (t & 15) * 4, col = c < mn_valid ? c : mn_valid - 4;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const bool ok = c < mn_valid && k + 4 * h < k_valid;
-      copy_async<16>(&s[k + 4 * h][c], ok ? base + static_cast<int64_t>(k + 4 * h) * ld + c : base, ok);
-    }
+    for (int h = 0; h < 2; ++h) copy_async<16>(&s[k + 4 * h][c], base + static_cast<int64_t>(k + 4 * h) * ld + col, true);
   }
 }
 
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(64 * GROUPS, 2) simt_rows_kernel(const SimtPar
   }
   __syncthreads();
   if (s_slab < 0) return;
-  const int row0 = s_row0, m_valid = s_rows;
+  const int row0 = s_row0, m_valid = s_rows < TM ? s_rows : TM;
   const int col0 = blockIdx.y * TN, n_valid = p.n_cols - col0 < TN ? p.n_cols - col0 : TN;
   const int group = threadIdx.x >> 6, t = threadIdx.x & 63;
   const int ra = (t >> 3) * 4, cb = (t & 7) * 4;
@@ -284,8 +284,8 @@ __global__ void __launch_bounds__(64 * GROUPS, 2) simt_rows_kernel(const SimtPar
   Slices& mine = slices[group];
   auto fetch = [&](int buf) {
     if (left > 0) {
-      copy_slice<true>(mine.a[buf], a, lda, m_valid, left, t);
-      copy_slice<kB>(mine.b[buf], b, ldb, n_valid, left, t);
+      copy_slice<true>(mine.a[buf], a, p.red, m_valid, t);
+      copy_slice<kB>(mine.b[buf], b, kB ? p.red : p.n_cols, n_valid, t);
       a += sharing * TK;
       b += sharing * b_slice;
       left -= sharing * TK;
