@@ -87,7 +87,7 @@ SIGNATURES = {
     "dice_grouped_ffn_train": (
         c_int,
         [c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
-         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+         c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p],
     ),
     "dice_grouped_ffn_backward": (
         c_int,

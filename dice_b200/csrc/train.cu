@@ -20,9 +20,12 @@ int check_product(int64_t n_rows, int n_dim, int k_dim, int n_slabs, int n_seg, 
 
 }  // namespace
 
-extern "C" size_t dice_grouped_scratch_bytes(int64_t n_rows, int n_dim, int k_dim, int n_slabs, int weight_gradient, int dtype) {
-  if (dtype != DICE_BF16 || check_product(n_rows, n_dim, k_dim, n_slabs, 0, dtype) != DICE_OK) return 0;
-  return dice_internal_split_bytes(n_rows, n_dim, k_dim, n_slabs, weight_gradient != 0);
+extern "C" size_t dice_grouped_scratch_bytes(int64_t n_rows, int n_dim, int k_dim, int n_slabs, int product, int dtype) {
+  if (product < DICE_PRODUCT_DGRAD || product > DICE_PRODUCT_LINEAR || n_rows <= 0 ||
+      check_product(n_rows, n_dim, k_dim, n_slabs, 0, dtype) != DICE_OK)
+    return 0;
+  if (dtype == DICE_F32) return dice_internal_f32_bytes(product, n_rows, n_dim, k_dim, n_slabs);
+  return product == DICE_PRODUCT_LINEAR ? 0 : dice_internal_split_bytes(n_rows, n_dim, k_dim, n_slabs, product == DICE_PRODUCT_WGRAD);
 }
 
 extern "C" int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, const void* w, int n_slabs, int k_dim,
@@ -37,6 +40,9 @@ extern "C" int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, con
   if (dtype == DICE_BF16)
     return dice_internal_tc_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dx, scratch,
                                   scratch_bytes, status, static_cast<cudaStream_t>(stream));
+  if (scratch != nullptr && dice_internal_f32_bytes(DICE_PRODUCT_DGRAD, n_rows, n_dim, k_dim, n_slabs) > 0)
+    return dice_internal_f32_product(DICE_PRODUCT_DGRAD, dy, w, n_rows, n_dim, k_dim, n_slabs, seg_offsets, seg_slab, n_seg, 0, dx,
+                                     nullptr, scratch, scratch_bytes, status, static_cast<cudaStream_t>(stream));
   return dice_internal_simt_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dx, status,
                                   static_cast<cudaStream_t>(stream));
 }
@@ -53,14 +59,17 @@ extern "C" int dice_grouped_wgrad(const void* dy, const void* x, int64_t n_rows,
   if (dtype == DICE_BF16)
     return dice_internal_tc_wgrad(dy, x, n_rows, n_dim, k_dim, seg_offsets, n_slabs, gate_up, dw, dw_up, scratch,
                                   scratch_bytes, status, static_cast<cudaStream_t>(stream));
+  if (scratch != nullptr && n_rows > 0 && dice_internal_f32_bytes(DICE_PRODUCT_WGRAD, n_rows, n_dim, k_dim, n_slabs) > 0)
+    return dice_internal_f32_product(DICE_PRODUCT_WGRAD, dy, x, n_rows, n_dim, k_dim, n_slabs, seg_offsets, nullptr, n_slabs, gate_up,
+                                     dw, dw_up, scratch, scratch_bytes, status, static_cast<cudaStream_t>(stream));
   return dice_internal_simt_wgrad(dy, x, n_rows, n_dim, k_dim, seg_offsets, n_slabs, gate_up, dw, dw_up, status,
                                   static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int dice_grouped_ffn_train(const void* rows_in, int64_t n_rows, int hidden, int ffn, int act, int keep, int dtype,
                                       const void* w1, const void* w2, int n_slabs, const int32_t* seg_offsets, int n_seg,
-                                      void* pre, void* a, void* codes, float* scales, void* rows_out, uint32_t* status,
-                                      void* stream) {
+                                      void* pre, void* a, void* codes, float* scales, void* rows_out, void* scratch,
+                                      size_t scratch_bytes, uint32_t* status, void* stream) {
   DICE_CHECK_ARG(act == DICE_ACT_SWIGLU || act == DICE_ACT_GELU_TANH, DICE_ERR_ARG);
   DICE_CHECK_ARG(ffn > 0 && n_seg <= n_slabs, DICE_ERR_ARG);
   const int64_t cols = act == DICE_ACT_SWIGLU ? dice_w13_rows(ffn) : ffn;
@@ -86,12 +95,15 @@ extern "C" int dice_grouped_ffn_train(const void* rows_in, int64_t n_rows, int h
     return dice_grouped_gemm(a, n_rows, ffn, w2, n_slabs, hidden, seg_offsets, nullptr, n_seg, DICE_EPI_STORE, rows_out,
                              hidden, hidden, 0, status, stream);
   }
-  rc = dice_internal_simt_linear(rows_in, n_rows, hidden, w1, n_slabs, static_cast<int>(cols), seg_offsets, nullptr, n_seg,
-                                 pre, status, s);
-  if (rc != DICE_OK) return rc;
-  rc = dice_act_keep(pre, n_rows, ffn, act, keep, dtype, a, codes, scales, stream);
-  if (rc != DICE_OK) return rc;
-  return dice_internal_simt_linear(a, n_rows, ffn, w2, n_slabs, hidden, seg_offsets, nullptr, n_seg, rows_out, status, s);
+  auto linear = [&](const void* in, int k_dim, const void* w, int n_dim, void* out) {
+    if (scratch != nullptr && dice_internal_f32_bytes(DICE_PRODUCT_LINEAR, n_rows, n_dim, k_dim, n_slabs) > 0)
+      return dice_internal_f32_product(DICE_PRODUCT_LINEAR, in, w, n_rows, n_dim, k_dim, n_slabs, seg_offsets, nullptr, n_seg, 0,
+                                       out, nullptr, scratch, scratch_bytes, status, s);
+    return dice_internal_simt_linear(in, n_rows, k_dim, w, n_slabs, n_dim, seg_offsets, nullptr, n_seg, out, status, s);
+  };
+  if ((rc = linear(rows_in, hidden, w1, static_cast<int>(cols), pre)) != DICE_OK) return rc;
+  if ((rc = dice_act_keep(pre, n_rows, ffn, act, keep, dtype, a, codes, scales, stream)) != DICE_OK) return rc;
+  return linear(a, ffn, w2, hidden, rows_out);
 }
 
 extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in, const void* kept, const float* scales,
@@ -109,6 +121,12 @@ extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in,
   if (rc != DICE_OK) return rc;
   DICE_CHECK_ARG(seg_offsets && dw1 && dw2 && (!glu || dw1_up), DICE_ERR_ARG);
   DICE_CHECK_ARG(keep == DICE_KEEP_NONE || keep == DICE_KEEP_INT8 || keep == DICE_KEEP_E4M3, DICE_ERR_ARG);
+  // each product takes the scratch only if it can use it
+  auto part = [&](int n_dim, int k_dim, bool weight_gradient) {
+    return dice_grouped_scratch_bytes(n_rows, n_dim, k_dim, n_slabs, weight_gradient ? DICE_PRODUCT_WGRAD : DICE_PRODUCT_DGRAD, dtype) > 0
+               ? scratch
+               : nullptr;
+  };
   if (n_rows > 0) {
     DICE_CHECK_ARG(d_out && rows_in && kept && w1 && w2 && d_pre && a && d_rows && (keep == DICE_KEEP_NONE || scales), DICE_ERR_ARG);
     DICE_CHECK_ARG(da || dtype == DICE_BF16, DICE_ERR_ARG);  // bf16: the activation's gradient stays in the epilogue
@@ -119,14 +137,12 @@ extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in,
                                  static_cast<cudaStream_t>(stream));
       if (rc != DICE_OK) return rc;
     } else {
-      if ((rc = dice_grouped_dgrad(d_out, n_rows, hidden, w2, n_slabs, ffn, seg_offsets, nullptr, n_slabs, dtype, da, nullptr, 0, status, stream)) != DICE_OK) return rc;
+      if ((rc = dice_grouped_dgrad(d_out, n_rows, hidden, w2, n_slabs, ffn, seg_offsets, nullptr, n_slabs, dtype, da,
+                                   part(hidden, ffn, false), scratch_bytes, status, stream)) != DICE_OK)
+        return rc;
       if ((rc = dice_act_backward(da, kept, scales, n_rows, ffn, act, keep, dtype, d_pre, a, stream)) != DICE_OK) return rc;
     }
   }
-  // each product takes the scratch only if it can split
-  auto part = [&](int n_dim, int k_dim, bool weight_gradient) {
-    return dice_grouped_scratch_bytes(n_rows, n_dim, k_dim, n_slabs, weight_gradient, dtype) > 0 ? scratch : nullptr;
-  };
   const int c = static_cast<int>(cols);
   if ((rc = dice_grouped_wgrad(d_out, a, n_rows, hidden, ffn, seg_offsets, n_slabs, 0, dtype, dw2, nullptr,
                                part(hidden, ffn, true), scratch_bytes, status, stream)) != DICE_OK)

@@ -24,6 +24,13 @@ int dice_internal_tc_wgrad(const void* dy, const void* x, int64_t n_rows, int n_
                            int n_slabs, int gate_up, void* dw, void* dw_up, void* scratch, size_t scratch_bytes, uint32_t* status,
                            cudaStream_t s);
 
+// fp32 on the tensor cores, as six products of bf16 planes: scratch that it takes (0: not there), and the product
+constexpr int kF32Rows = 96, kF32WgradRows = 64;  // rows per slab from which it is faster (see dice_internal_f32_bytes)
+size_t dice_internal_f32_bytes(int kind, int64_t n_rows, int n_dim, int k_dim, int n_slabs);
+int dice_internal_f32_product(int kind, const void* a, const void* b, int64_t n_rows, int n_dim, int k_dim, int n_slabs,
+                              const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, int gate_up, void* out,
+                              void* out_up, void* scratch, size_t scratch_bytes, uint32_t* status, cudaStream_t s);
+
 // the forward product with the activation and what is kept in its epilogue, and the second product's input gradient with
 // the activation's backward pass in its epilogue (see train_gemm.cu); pointers as in the public entry points
 int dice_internal_tc_keep(const void* rows, int64_t n_rows, int hidden, int ffn, int act, int keep, const void* w1, int n_slabs,

@@ -31,6 +31,12 @@
 //   NN + EPI_BACK  the second product's input gradient: every column's gradient meets the codes of its argument in fp32
 //                  and leaves as the argument's gradient, beside the activation for the weight gradient behind it.
 //
+// fp32 operands (PLANES 3) come as three bf16 planes each, x = hi + mid + lo exactly (8 bits of the mantissa a plane), and a
+// product is six: hi hi, hi mid, mid hi, mid mid, hi lo, lo hi; what is left out is below 2^-25 of it.  The accumulator
+// in tensor memory is cut, not rounded, after every instruction, so it is emptied after every k-block of 64 into fp32
+// registers that round, and within a block the small products come first.  Six instructions for one leave ~220 TFLOP/s,
+// three times the CUDA cores' 74.  (An infinity in an operand gives NaN: its product with a zero plane.)
+//
 // Few tiles: they are made half as wide if that keeps more pairs busy (one token's two rows, 1152 -> 4608: 36 tiles of
 // 256 columns, 72 of 128).  Fewer still, and a long reduction: the pairs that would idle take a share of the reduction
 // each (split).  Every epilogue
@@ -52,7 +58,7 @@ constexpr int PM = 256;
 // Operand ring slots and, per epilogue warp, staging buffers of 32 rows x 64 bytes.  The activation's epilogues write (and
 // read) several bytes for every one of a plain product, so they give a ring slot for two more buffers and let the copy
 // unit store them (see Stager).
-constexpr int stages_of(int epi) { return epi == EPI_PLAIN ? 6 : 5; }
+constexpr int stages_of(int epi, int planes = 1) { return planes == 3 ? 2 : epi == EPI_PLAIN ? 6 : 5; }
 constexpr int buffers_of(int epi) { return epi == EPI_PLAIN ? 1 : 3; }
 constexpr int kStageBytesT = 32768;  // 128 rows (or columns) x 64 of each operand
 constexpr int kOperandBytes = 16384;
@@ -61,8 +67,8 @@ constexpr int kBoxBytes = 8192;      // 64 reduction rows x 128 bytes
 constexpr int threads_of(int mode) { return 32 * (2 + kEpilogueWarps + (mode == MODE_TN ? 1 : 0)); }
 constexpr int kStageStore = 2048;    // per epilogue warp, as in grouped_gemm_pair.cu
 constexpr int kExchangeBytes = 4096;  // EPI_KEEP, SwiGLU: group maxima, [2 tiles][2 halves][gate, up][128 rows]
-constexpr int smem_of(int epi) {
-  return stages_of(epi) * kStageBytesT + kAuxBytes + kEpilogueWarps * buffers_of(epi) * kStageStore + kExchangeBytes + 1024;
+constexpr int smem_of(int epi, int planes) {
+  return stages_of(epi, planes) * planes * kStageBytesT + kAuxBytes + kEpilogueWarps * buffers_of(epi) * kStageStore + kExchangeBytes + 1024;
 }
 constexpr int kSplitFloats = 4 * 32 * 32;  // an epilogue warp's part of a tile: 4 chunks of 32 rows x 32 columns
 constexpr int kBand = 8;                   // TN: row tiles of a band, and the elements of x from which there are
@@ -79,6 +85,7 @@ struct TrainGemm {
   int n_mblk;       // TN: row tiles of a slab's gradient
   int n_cols;       // output columns
   int m_rows;       // TN: output rows of a slab
+  int a_plane, b_plane;  // PLANES 3: rows (NN: slabs of w) from one plane of an operand to the next
   int gate_up;      // TN: 0, or ffn: the rows are packed gate / up blocks and go to two tensors
   __nv_bfloat16* out;
   __nv_bfloat16* out_up;
@@ -121,6 +128,14 @@ __device__ __forceinline__ void mbar_complete_tx_cluster(uint32_t cluster_addr, 
 __device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
 // Stores of 32 rows of 64 bytes that a warp holds one row per lane.  They go through shared memory, laid out as the 64-byte
 // swizzle wants it.  If all 32 rows exist (a segment's last tile may have fewer) and BUFS > 1, the copy unit stores them as
 // one box, clipped to the tensor's columns; a few buffers in turn, of which the one about to be written is no longer read.
@@ -403,15 +418,15 @@ __device__ __forceinline__ void back_tile(const TrainGemm& p, int nb, int half, 
   }
 }
 
-template <int MODE, int EPI, int ACT, int KEEP>
+template <int MODE, int EPI, int ACT, int KEEP, int PLANES>
 __global__ void __launch_bounds__(threads_of(MODE), 1)
 train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                   const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ CUtensorMap tm_act,
                   const __grid_constant__ CUtensorMap tm_codes, const TrainGemm p) {
-  constexpr int kStagesT = stages_of(EPI);
+  constexpr int kStagesT = stages_of(EPI, PLANES), kSlotBytes = PLANES * kStageBytesT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* aux = smem + kStagesT * kStageBytesT;
+  uint8_t* aux = smem + kStagesT * kSlotBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(aux);
   const uint32_t full_bar = smem_u32(bars);                                 // [kStagesT] used in the leader
   const uint32_t empty_bar = smem_u32(bars + kStagesT);                     // [kStagesT] in both CTAs
@@ -562,35 +577,40 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       const int half = ti.n_mma / 2;
       const int col0 = ti.nb * bn + static_cast<int>(cta_rank) * half;  // this CTA's B columns
       const int b_boxes = half > 64 ? 2 : 1;
-      const uint32_t bytes = kOperandBytes + b_boxes * kBoxBytes;
+      const uint32_t bytes = PLANES * (kOperandBytes + b_boxes * kBoxBytes);
       const int ragged = MODE == MODE_TN ? ti.last_rows & 15 : 0;
       for (int kb = ti.kb0; kb < ti.kb1; ++kb) {
         if (!mbar_wait(empty_bar + 8 * stage, phase ^ 1u, abort_flag, p.status, DICE_STATUS_WAIT_SMEM_EMPTY)) {
           alive = false;
           break;
         }
-        const uint32_t a_dst = tiles_smem + stage * kStageBytesT, b_dst = a_dst + kOperandBytes;
+        const uint32_t slot_smem = tiles_smem + stage * kSlotBytes;
         const uint32_t leader_full = map_to_cta(full_bar + 8 * stage, 0);
         if (elect_one()) {
           if (leader) mbar_expect_tx(full_bar + 8 * stage, 2 * bytes);
-          if (MODE == MODE_NT) {
-            tma_load_2d_pair(a_dst, &tm_a, kb * BK, ti.row0, leader_full);
-            for (int j = 0; j < b_boxes; ++j)
-              tma_load_2d_pair(b_dst + j * kBoxBytes, &tm_b, kb * BK, ti.slab * p.arg_cols + col0 + 64 * j, leader_full);
-          } else if (MODE == MODE_NN) {
-            tma_load_2d_pair(a_dst, &tm_a, kb * BK, ti.row0, leader_full);
-            for (int j = 0; j < b_boxes; ++j)
-              tma_load_3d_pair(b_dst + j * kBoxBytes, &tm_b, col0 + 64 * j, kb * BK, ti.slab, leader_full);
-          } else {
-            const int row = s_seg_off[seg] + kb * BK;
-            uint32_t bar = leader_full;
-            if (ragged != 0 && kb == ti.kb1 - 1) {
-              bar = tail_bar + 8 * stage;
-              mbar_expect_tx(bar, bytes);
-              bar = map_to_cta(bar, cta_rank);
+          uint32_t bar = leader_full;
+          if (MODE == MODE_TN && ragged != 0 && kb == ti.kb1 - 1) {
+            bar = tail_bar + 8 * stage;
+            mbar_expect_tx(bar, bytes);
+            bar = map_to_cta(bar, cta_rank);
+          }
+#pragma unroll
+          for (int pl = 0; pl < PLANES; ++pl) {
+            const uint32_t a_dst = slot_smem + pl * kStageBytesT, b_dst = a_dst + kOperandBytes;
+            const int a_off = pl * p.a_plane, b_off = pl * p.b_plane;
+            if (MODE == MODE_TN) {
+              const int row = s_seg_off[seg] + kb * BK;
+              for (int j = 0; j < 2; ++j) tma_load_2d_pair(a_dst + j * kBoxBytes, &tm_a, ti.row0 + 64 * j, row + a_off, bar);
+              for (int j = 0; j < b_boxes; ++j) tma_load_2d_pair(b_dst + j * kBoxBytes, &tm_b, col0 + 64 * j, row + b_off, bar);
+            } else {
+              tma_load_2d_pair(a_dst, &tm_a, kb * BK, ti.row0 + a_off, bar);
+              for (int j = 0; j < b_boxes; ++j) {
+                if (MODE == MODE_NT)
+                  tma_load_2d_pair(b_dst + j * kBoxBytes, &tm_b, kb * BK, ti.slab * p.arg_cols + col0 + 64 * j + b_off, bar);
+                else
+                  tma_load_3d_pair(b_dst + j * kBoxBytes, &tm_b, col0 + 64 * j, kb * BK, ti.slab + b_off, bar);
+              }
             }
-            for (int j = 0; j < 2; ++j) tma_load_2d_pair(a_dst + j * kBoxBytes, &tm_a, ti.row0 + 64 * j, row, bar);
-            for (int j = 0; j < b_boxes; ++j) tma_load_2d_pair(b_dst + j * kBoxBytes, &tm_b, col0 + 64 * j, row, bar);
           }
         }
         __syncwarp();
@@ -608,10 +628,15 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         if (ti.kb0 == ti.kb1) continue;
         // both operands' majors: A is MN-major in TN, B in NN and TN
         const uint32_t idesc = make_instr_desc(PM, ti.n_mma) | (MODE == MODE_TN ? 1u << 15 : 0u) | (MODE != MODE_NT ? 1u << 16 : 0u);
-        if (!mbar_wait(acc_empty_bar + 8 * acc, acc_phase ^ 1u, abort_flag, p.status, DICE_STATUS_WAIT_ACC_EMPTY)) break;
-        tc_fence_after_sync();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+        if (PLANES == 1) {
+          if (!mbar_wait(acc_empty_bar + 8 * acc, acc_phase ^ 1u, abort_flag, p.status, DICE_STATUS_WAIT_ACC_EMPTY)) break;
+        }
         for (int kb = ti.kb0; kb < ti.kb1; ++kb) {
+          if (PLANES != 1 &&  // every k-block has an accumulator of its own
+              !mbar_wait(acc_empty_bar + 8 * acc, acc_phase ^ 1u, abort_flag, p.status, DICE_STATUS_WAIT_ACC_EMPTY)) {
+            alive = false;
+            break;
+          }
           if (!mbar_wait(full_bar + 8 * stage, phase, abort_flag, p.status, DICE_STATUS_WAIT_SMEM_FULL)) {
             alive = false;
             break;
@@ -622,26 +647,38 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             if (ti.last_rows & 15) fence_cluster();
           }
           tc_fence_after_sync();
-          const uint32_t a_addr = tiles_smem + stage * kStageBytesT;
-          const uint64_t a_desc = MODE != MODE_TN ? make_operand_desc(a_addr) : make_mn_desc(a_addr);
-          const uint64_t b_desc = MODE == MODE_NT ? make_operand_desc(a_addr + kOperandBytes) : make_mn_desc(a_addr + kOperandBytes);
+          const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+          const uint32_t slot_smem = tiles_smem + stage * kSlotBytes;
           // 16 reduction elements further: 32 bytes along a K-major row, 16 rows of 128 bytes in an MN-major box
           constexpr uint64_t kStepA = MODE != MODE_TN ? 2 : 128, kStepB = MODE == MODE_NT ? 2 : 128;
+          constexpr int kProducts = PLANES == 3 ? 6 : 1;
+          constexpr int kPlaneA[6] = {PLANES == 3 ? 2 : 0, 0, 1, 1, 0, 0}, kPlaneB[6] = {0, 2, 1, 0, 1, 0};
           if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < BK / UMMA_K; ++kk)
-              if (kk < steps)
-                umma_bf16_pair(d_tmem, a_desc + kk * kStepA, b_desc + kk * kStepB, idesc,
-                               static_cast<uint32_t>(kb != ti.kb0 || kk != 0));
+            for (int q = 0; q < kProducts; ++q) {
+              const uint32_t a_addr = slot_smem + kPlaneA[q] * kStageBytesT;
+              const uint32_t b_addr = slot_smem + kPlaneB[q] * kStageBytesT + kOperandBytes;
+              const uint64_t a_desc = MODE != MODE_TN ? make_operand_desc(a_addr) : make_mn_desc(a_addr);
+              const uint64_t b_desc = MODE == MODE_NT ? make_operand_desc(b_addr) : make_mn_desc(b_addr);
+#pragma unroll
+              for (int kk = 0; kk < BK / UMMA_K; ++kk)
+                if (kk < steps)
+                  umma_bf16_pair(d_tmem, a_desc + kk * kStepA, b_desc + kk * kStepB, idesc,
+                                 static_cast<uint32_t>((PLANES == 1 && kb != ti.kb0) || q != 0 || kk != 0));
+            }
             umma_commit_pair(empty_bar + 8 * stage);
+            if (PLANES != 1) umma_commit_pair(acc_full_bar + 8 * acc);
           }
           __syncwarp();
           if (++stage == kStagesT) { stage = 0; phase ^= 1u; }
+          if (PLANES != 1 && ++acc == kAccStages) { acc = 0; acc_phase ^= 1u; }
         }
         if (!alive) break;
-        if (elect_one()) umma_commit_pair(acc_full_bar + 8 * acc);
-        __syncwarp();
-        if (++acc == kAccStages) { acc = 0; acc_phase ^= 1u; }
+        if (PLANES == 1) {
+          if (elect_one()) umma_commit_pair(acc_full_bar + 8 * acc);
+          __syncwarp();
+          if (++acc == kAccStages) { acc = 0; acc_phase ^= 1u; }
+        }
       }
     }
   } else if (warp == 2 + kEpilogueWarps) {
@@ -660,15 +697,15 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           tail_phase ^= 1u << stage;
           // rows [valid, next multiple of 16) of the four boxes (a row's 128 bytes are permuted within the row only)
           const int rows = 16 - (valid & 15);
-          uint8_t* base = smem + stage * kStageBytesT + valid * 128;
+          uint8_t* base = smem + stage * kSlotBytes + valid * 128;
           for (int i = lane; i < rows * 8; i += 32)
 #pragma unroll
-            for (int b = 0; b < 4; ++b) *reinterpret_cast<uint4*>(base + b * kBoxBytes + i * 16) = make_uint4(0, 0, 0, 0);
+            for (int b = 0; b < 4 * PLANES; ++b) *reinterpret_cast<uint4*>(base + b * kBoxBytes + i * 16) = make_uint4(0, 0, 0, 0);
           fence_async_smem();
           fence_cluster();
           __syncwarp();
           if (lane == 0)
-            mbar_complete_tx_cluster(map_to_cta(full_bar + 8 * stage, 0), kOperandBytes + (ti.n_mma > 128 ? 2 : 1) * kBoxBytes);
+            mbar_complete_tx_cluster(map_to_cta(full_bar + 8 * stage, 0), PLANES * (kOperandBytes + (ti.n_mma > 128 ? 2 : 1) * kBoxBytes));
         }
         slot = (slot + blocks) % kStagesT;
       }
@@ -686,7 +723,43 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       const bool summed = ti.kb0 != ti.kb1;  // this share has something in tensor memory
       BackChunk<ACT, KEEP> kept;
       if (EPI == EPI_BACK) kept.load_first(p, ti.nb, half, ti.row0 + quad * 32 + lane, quad * 32 + lane < ti.rows_valid);
-      if (summed) {
+      f32x2 sums[PLANES == 3 ? 4 : 1][16];  // PLANES 3: this lane's row of the tile, columns half * 32 + 64 i ..
+      if (PLANES == 3) {
+        bool alive = true;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sums[PLANES == 3 ? i : 0][j] = 0;
+        for (int kb = ti.kb0; kb < ti.kb1; ++kb) {
+          if (!mbar_wait(acc_full_bar + 8 * acc, acc_phase, abort_flag, p.status, DICE_STATUS_WAIT_ACC_FULL)) {
+            alive = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * BN + half * 32);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (half * 32 + 64 * i < ti.n_mma) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint32_t a[16];
+                tmem_ld16(t0 + 64 * i + 16 * h, a);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  f32x2& sum = sums[PLANES == 3 ? i : 0][8 * h + j];
+                  sum = add2(sum, pair<f32x2>(__uint_as_float(a[2 * j]), __uint_as_float(a[2 * j + 1])));
+                }
+              }
+            }
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(map_to_cta(acc_empty_bar + 8 * acc, 0));
+          if (++acc == kAccStages) { acc = 0; acc_phase ^= 1u; }
+        }
+        if (!alive) break;
+      } else if (summed) {
         if (!mbar_wait(acc_full_bar + 8 * acc, acc_phase, abort_flag, p.status, DICE_STATUS_WAIT_ACC_FULL)) break;
         tc_fence_after_sync();
       }
@@ -730,15 +803,27 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       constexpr int64_t kPairFloats = 2ll * kEpilogueWarps * kSplitFloats;
       if (shared_tile) {
         float* mine = p.split_ws + (ti.tile * split + ti.share) * kPairFloats + part + lane;
-        for (int c = half * 32; c < n_valid; c += 64) {
-          uint32_t a[32];
-          if (summed) {
-            tmem_ld32(taddr + c, a);
-            tmem_ld_wait();
-          }
-          float* dst = mine + (c >> 6) * 1024;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) dst[j * 32] = summed ? __uint_as_float(a[j]) : 0.f;
+        for (int i = 0; i < 4; ++i) {
+          const int c = half * 32 + 64 * i;
+          if (c >= n_valid) break;
+          float* dst = mine + i * 1024;
+          if (PLANES == 3) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const two v = halves(sums[PLANES == 3 ? i : 0][j]);
+              dst[2 * j * 32] = v.x;
+              dst[(2 * j + 1) * 32] = v.y;
+            }
+          } else {
+            uint32_t a[32];
+            if (summed) {
+              tmem_ld32(taddr + c, a);
+              tmem_ld_wait();
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) dst[j * 32] = summed ? __uint_as_float(a[j]) : 0.f;
+          }
         }
         __threadfence();
         __syncwarp();
@@ -771,7 +856,38 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         }
       };
 
-      if (EPI == EPI_PLAIN) {
+      if (PLANES == 3) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = half * 32 + 64 * i;
+          if (!store || c >= n_valid) break;
+          float v[32];
+          if (shared_tile) {
+            fetch(c, v);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const two x = halves(sums[PLANES == 3 ? i : 0][j]);
+              v[2 * j] = x.x;
+              v[2 * j + 1] = x.y;
+            }
+          }
+          float* const base = reinterpret_cast<float*>(up_rows ? p.out_up : p.out);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // 16 columns are 64 bytes
+            uint4 w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              w[j] = make_uint4(__float_as_uint(v[16 * h + 4 * j]), __float_as_uint(v[16 * h + 4 * j + 1]),
+                                __float_as_uint(v[16 * h + 4 * j + 2]), __float_as_uint(v[16 * h + 4 * j + 3]));
+            const int at = c + 16 * h, n_left = n_valid - at;
+            stager.store(w, nullptr, 0, [&](int r, int piece, const uint4& x) {
+              if (dst_row[r] >= 0 && piece * 4 < n_left)
+                *reinterpret_cast<uint4*>(base + dst_row[r] * p.n_cols + col0 + at + piece * 4) = x;
+            });
+          }
+        }
+      } else if (EPI == EPI_PLAIN) {
         for (int c = half * 32; store && c < n_valid; c += 64) {
           float v[32];
           fetch(c, v);
@@ -788,7 +904,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         back_tile<ACT, KEEP>(p, ti.nb, half, ti.row0 + quad * 32 + lane, quad * 32 + lane < ti.rows_valid, kept, &tm_out, &tm_act,
                              fetch, store_bf16);
       }
-      if (summed) {
+      if (PLANES == 1 && summed) {
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(map_to_cta(acc_empty_bar + 8 * acc, 0));
@@ -815,19 +931,19 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
 }
 
 // CTA pairs of this kernel that can be resident at once (cached per device); 0 on error
-template <int MODE, int EPI = EPI_PLAIN, int ACT = 0, int KEEP = 0>
+template <int MODE, int EPI = EPI_PLAIN, int ACT = 0, int KEEP = 0, int PLANES = 1>
 int resident_pairs_train() {
   static int cached[64] = {0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   if (cached[dev] == 0) {
-    if (cudaFuncSetAttribute(train_gemm_kernel<MODE, EPI, ACT, KEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of(EPI)) != cudaSuccess) return 0;
+    if (cudaFuncSetAttribute(train_gemm_kernel<MODE, EPI, ACT, KEEP, PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of(EPI, PLANES)) != cudaSuccess) return 0;
     const int sms = sm_count_cached();
     if (sms <= 0) return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(sms & ~1), 1, 1);
     cfg.blockDim = dim3(threads_of(MODE), 1, 1);
-    cfg.dynamicSmemBytes = smem_of(EPI);
+    cfg.dynamicSmemBytes = smem_of(EPI, PLANES);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
@@ -836,20 +952,20 @@ int resident_pairs_train() {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, train_gemm_kernel<MODE, EPI, ACT, KEEP>, &cfg) != cudaSuccess || n <= 0) return 0;
+    if (cudaOccupancyMaxActiveClusters(&n, train_gemm_kernel<MODE, EPI, ACT, KEEP, PLANES>, &cfg) != cudaSuccess || n <= 0) return 0;
     cached[dev] = n < sms / 2 ? n : sms / 2;
   }
   return cached[dev];
 }
 
-template <int MODE, int EPI = EPI_PLAIN, int ACT = 0, int KEEP = 0>
+template <int MODE, int EPI = EPI_PLAIN, int ACT = 0, int KEEP = 0, int PLANES = 1>
 int launch_train(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const CUtensorMap* stores, const TrainGemm& p,
                  int64_t most_tiles, int pairs, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   const int64_t use = most_tiles < pairs && p.split_ws == nullptr ? most_tiles : pairs;
   cfg.gridDim = dim3(static_cast<unsigned>(2 * use), 1, 1);
   cfg.blockDim = dim3(threads_of(MODE), 1, 1);
-  cfg.dynamicSmemBytes = smem_of(EPI);
+  cfg.dynamicSmemBytes = smem_of(EPI, PLANES);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -861,7 +977,7 @@ int launch_train(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const CUtenso
   cfg.attrs = attr;
   cfg.numAttrs = dice_pdl_enabled() ? 2 : 1;
   dice_count_launch();
-  return cudaLaunchKernelEx(&cfg, train_gemm_kernel<MODE, EPI, ACT, KEEP>, tm_a, tm_b, stores[0], stores[1], stores[2], p) == cudaSuccess ? DICE_OK : DICE_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, train_gemm_kernel<MODE, EPI, ACT, KEEP, PLANES>, tm_a, tm_b, stores[0], stores[1], stores[2], p) == cudaSuccess ? DICE_OK : DICE_ERR_CUDA;
 }
 
 int64_t col_tiles(int cols, int width) { return (static_cast<int64_t>(cols) + width - 1) / width; }
@@ -1038,4 +1154,134 @@ int dice_internal_tc_back(const void* d_out, int64_t n_rows, int hidden, int ffn
   p.status = status;
   return act == DICE_ACT_SWIGLU ? run_epilogue<DICE_ACT_SWIGLU>(true, keep, tm_a, tm_b, stores, p, s)
                                 : run_epilogue<DICE_ACT_GELU_TANH>(true, keep, tm_a, tm_b, stores, p, s);
+}
+
+// ---- fp32 operands ------------------------------------------------------------------
+namespace {
+
+// x -> three planes of bf16, each the nearest to what the planes before it leave, so that hi + mid + lo == x.  Two tensors in one launch, eight values a thread.
+struct PlaneJob {
+  const float* x;
+  __nv_bfloat16* planes;
+  int64_t n;  // values (a multiple of 8), also the distance of the planes
+};
+__global__ void __launch_bounds__(256) split_planes_kernel(const PlaneJob first, const PlaneJob second) {
+  pdl_trigger();
+  pdl_wait();
+  int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8;
+  const bool in_first = i < first.n;
+  if (!in_first) i -= first.n;
+  const PlaneJob& job = in_first ? first : second;
+  if (i >= job.n) return;
+  const uint4 lo4 = ldg_stream16(job.x + i), hi4 = ldg_stream16(job.x + i + 4);
+  const uint32_t raw[8] = {lo4.x, lo4.y, lo4.z, lo4.w, hi4.x, hi4.y, hi4.z, hi4.w};
+  uint32_t plane[3][8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = __uint_as_float(raw[j]);
+    // rounded to nearest, which halves what the next plane has to hold twice over; the largest values, which would round
+    // to an infinity, are cut.  A value that is not finite stays as it is, alone (a NaN whose payload is cut away would be
+    // an infinity).
+    uint32_t hi = static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(x))) << 16;
+    const bool finite = (raw[j] & 0x7f800000u) != 0x7f800000u;
+    if (finite && (hi & 0x7f800000u) == 0x7f800000u) hi = raw[j] & 0xffff0000u;
+    const float rest = finite ? x - __uint_as_float(hi) : 0.f;
+    const uint32_t mid = static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(rest))) << 16;
+    plane[0][j] = hi;
+    plane[1][j] = mid;
+    plane[2][j] = static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(rest - __uint_as_float(mid)))) << 16;
+  }
+#pragma unroll
+  for (int q = 0; q < 3; ++q)
+    stg_stream16(job.planes + q * job.n + i, make_uint4((plane[q][0] >> 16) | plane[q][1], (plane[q][2] >> 16) | plane[q][3],
+                                                        (plane[q][4] >> 16) | plane[q][5], (plane[q][6] >> 16) | plane[q][7]));
+}
+
+size_t plane_bytes(int64_t n) { return (static_cast<size_t>(n) * 6 + 255) / 256 * 256; }
+
+}  // namespace
+
+// Scratch of an fp32 product on the tensor cores: both operands' planes, and a split's parts.  0: the CUDA cores are the
+// better place.
+size_t dice_internal_f32_bytes(int kind, int64_t n_rows, int n_dim, int k_dim, int n_slabs) {
+  const int64_t limit = 0x7fffff00LL / 3;
+  if (n_rows >= limit || static_cast<int64_t>(n_slabs) * n_dim >= limit) return 0;
+  const int64_t w = static_cast<int64_t>(n_slabs) * n_dim * k_dim;
+  if (kind == DICE_PRODUCT_WGRAD) {
+    if (n_rows < kF32WgradRows * static_cast<int64_t>(n_slabs)) return 0;
+    return plane_bytes(n_rows * n_dim) + plane_bytes(n_rows * k_dim) + dice_internal_split_bytes(n_rows, n_dim, k_dim, n_slabs, true);
+  }
+  if (n_rows < kF32Rows * static_cast<int64_t>(n_slabs)) return 0;
+  const int a_cols = kind == DICE_PRODUCT_DGRAD ? n_dim : k_dim;
+  const int out_cols = kind == DICE_PRODUCT_DGRAD ? k_dim : n_dim;
+  return plane_bytes(n_rows * a_cols) + plane_bytes(w) + dice_internal_split_bytes(n_rows, a_cols, out_cols, n_slabs, false);
+}
+
+// a, b: what the kind multiplies (forward rows and w, input gradient dy and w, weight gradient dy and x)
+int dice_internal_f32_product(int kind, const void* a, const void* b, int64_t n_rows, int n_dim, int k_dim, int n_slabs,
+                              const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, int gate_up, void* out,
+                              void* out_up, void* scratch, size_t scratch_bytes, uint32_t* status, cudaStream_t s) {
+  if (scratch_bytes < dice_internal_f32_bytes(kind, n_rows, n_dim, k_dim, n_slabs)) return DICE_ERR_SCRATCH;
+  if (!dice_aligned16(scratch)) return DICE_ERR_ALIGN;
+  const bool wgrad = kind == DICE_PRODUCT_WGRAD;
+  const int64_t a_n = n_rows * (kind == DICE_PRODUCT_LINEAR ? k_dim : n_dim);
+  const int64_t b_n = wgrad ? n_rows * k_dim : static_cast<int64_t>(n_slabs) * n_dim * k_dim;
+  uint8_t* at = static_cast<uint8_t*>(scratch);
+  const PlaneJob ja = {static_cast<const float*>(a), reinterpret_cast<__nv_bfloat16*>(at), a_n};
+  at += plane_bytes(a_n);
+  const PlaneJob jb = {static_cast<const float*>(b), reinterpret_cast<__nv_bfloat16*>(at), b_n};
+  at += plane_bytes(b_n);
+  const int64_t blocks = ((a_n + b_n) / 8 + 255) / 256;
+  if (blocks > 0x7fffffffLL) return DICE_ERR_LIMIT;
+  if (dice_launch(split_planes_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, ja, jb) != cudaSuccess) return DICE_ERR_CUDA;
+
+  TrainGemm p = {};
+  p.seg_offsets = seg_offsets;
+  p.seg_slab = seg_slab;
+  p.n_seg = n_seg;
+  p.n_slabs = n_slabs;
+  p.n_rows = static_cast<int>(n_rows);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.out_up = static_cast<__nv_bfloat16*>(out_up);
+  p.status = status;
+  p.a_plane = static_cast<int>(n_rows);
+  CUtensorMap tm_a, tm_b;
+  const uint64_t rows3 = 3 * static_cast<uint64_t>(n_rows), slabs3 = 3 * static_cast<uint64_t>(n_slabs);
+  int rc, pairs;
+  size_t split = 0;
+  if (kind == DICE_PRODUCT_LINEAR) {
+    rc = encode_map(&tm_a, ja.planes, rows3, static_cast<uint64_t>(k_dim), BM);
+    if (rc == DICE_OK) rc = encode_map(&tm_b, jb.planes, slabs3 * static_cast<uint64_t>(n_dim), static_cast<uint64_t>(k_dim), BK);
+    p.b_plane = n_slabs * n_dim;
+    p.arg_cols = p.n_cols = n_dim;
+    p.red_blocks = (k_dim + BK - 1) / BK;
+    pairs = resident_pairs_train<MODE_NT, EPI_PLAIN, 0, 0, 3>();
+    split = dice_internal_split_bytes(n_rows, k_dim, n_dim, n_slabs, false);
+  } else if (kind == DICE_PRODUCT_DGRAD) {
+    rc = encode_map(&tm_a, ja.planes, rows3, static_cast<uint64_t>(n_dim), BM);
+    if (rc == DICE_OK) rc = encode_map3(&tm_b, jb.planes, slabs3, static_cast<uint64_t>(n_dim), static_cast<uint64_t>(k_dim), BK);
+    p.b_plane = n_slabs;
+    p.n_cols = k_dim;
+    p.red_blocks = (n_dim + BK - 1) / BK;
+    pairs = resident_pairs_train<MODE_NN, EPI_PLAIN, 0, 0, 3>();
+    split = dice_internal_split_bytes(n_rows, n_dim, k_dim, n_slabs, false);
+  } else {
+    rc = encode_map(&tm_a, ja.planes, rows3, static_cast<uint64_t>(n_dim), BK);
+    if (rc == DICE_OK) rc = encode_map(&tm_b, jb.planes, rows3, static_cast<uint64_t>(k_dim), BK);
+    p.b_plane = static_cast<int>(n_rows);
+    p.n_mblk = (n_dim + PM - 1) / PM;
+    p.m_rows = n_dim;
+    p.n_cols = k_dim;
+    p.gate_up = gate_up;
+    pairs = resident_pairs_train<MODE_TN, EPI_PLAIN, 0, 0, 3>();
+    split = dice_internal_split_bytes(n_rows, n_dim, k_dim, n_slabs, true);
+  }
+  if (rc != DICE_OK) return rc;
+  if (pairs <= 0) return DICE_ERR_CUDA;
+  if (split > 0 && (rc = use_scratch(p, at, split, pairs, s)) != DICE_OK) return rc;
+  const CUtensorMap no_stores[3] = {tm_a, tm_a, tm_a};
+  const int64_t tiles = (wgrad ? static_cast<int64_t>(n_slabs) * p.n_mblk : (n_rows + PM - 1) / PM + n_seg) * col_tiles(p.n_cols, BN / 2);
+  if (kind == DICE_PRODUCT_LINEAR) return launch_train<MODE_NT, EPI_PLAIN, 0, 0, 3>(tm_a, tm_b, no_stores, p, tiles, pairs, s);
+  if (kind == DICE_PRODUCT_DGRAD) return launch_train<MODE_NN, EPI_PLAIN, 0, 0, 3>(tm_a, tm_b, no_stores, p, tiles, pairs, s);
+  return launch_train<MODE_TN, EPI_PLAIN, 0, 0, 3>(tm_a, tm_b, no_stores, p, tiles, pairs, s);
 }

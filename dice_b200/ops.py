@@ -625,16 +625,20 @@ def _status_ptr(status: Optional[torch.Tensor], index: int) -> int:
 _status_by_index = {}  # device number -> address of its status word, which lives as long as the process
 
 
-def _split_bytes(lib, n_rows: int, n_dim: int, k_dim: int, n_slabs: int, weight_gradient: int, code: int) -> int:
-    """dice_grouped_scratch_bytes; products with more tiles than any GPU has SM pairs for are not asked about."""
-    col_tiles = (k_dim + 127) // 128
-    if weight_gradient:
-        few = 2 * n_slabs * ((n_dim + 255) // 256) * col_tiles <= 128
-    else:
-        few = 4 * ((n_rows + 255) // 256) * col_tiles <= 128
-    if code != DICE_BF16 or not few:
-        return 0
-    return lib.dice_grouped_scratch_bytes(n_rows, n_dim, k_dim, n_slabs, weight_gradient, code)
+PRODUCT_DGRAD, PRODUCT_WGRAD, PRODUCT_LINEAR = 0, 1, 2
+
+
+def _split_bytes(lib, n_rows: int, n_dim: int, k_dim: int, n_slabs: int, product: int, code: int) -> int:
+    """dice_grouped_scratch_bytes; bf16 products with more tiles than any GPU has SM pairs for are not asked about."""
+    if code == DICE_BF16:
+        col_tiles = (k_dim + 127) // 128
+        if product == PRODUCT_WGRAD:
+            few = 2 * n_slabs * ((n_dim + 255) // 256) * col_tiles <= 128
+        else:
+            few = product == PRODUCT_DGRAD and 4 * ((n_rows + 255) // 256) * col_tiles <= 128
+        if not few:
+            return 0
+    return lib.dice_grouped_scratch_bytes(n_rows, n_dim, k_dim, n_slabs, product, code)
 
 
 def _split_scratch(index: int, n_bytes: int) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
@@ -681,7 +685,7 @@ def grouped_dgrad(dy: torch.Tensor, w: torch.Tensor, seg_offsets: torch.Tensor, 
         out = _new((n_rows, k_dim), dy.dtype, index)
     assert out.is_contiguous() and out.shape == (n_rows, k_dim) and out.dtype == dy.dtype
     lib = _lib.load()
-    held, scratch, n_bytes = _split_scratch(index, _split_bytes(lib, n_rows, n_dim, k_dim, n_slabs, 0, code))
+    held, scratch, n_bytes = _split_scratch(index, _split_bytes(lib, n_rows, n_dim, k_dim, n_slabs, PRODUCT_DGRAD, code))
     _lib.check(
         lib.dice_grouped_dgrad(dy.data_ptr(), n_rows, n_dim, w.data_ptr(), n_slabs, k_dim, seg_offsets.data_ptr(),
                                _ptr(seg_slab), n_seg, code, out.data_ptr(), scratch, n_bytes, _status_ptr(status, index),
@@ -714,7 +718,7 @@ def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, seg_offsets: torch.Tensor, 
     dw = _new(shape, dy.dtype, index)
     dw_up = _new(shape, dy.dtype, index) if gate_up else None
     lib = _lib.load()
-    held, scratch, n_bytes = _split_scratch(index, _split_bytes(lib, n_rows, n_dim, k_dim, n_slabs, 1, code))
+    held, scratch, n_bytes = _split_scratch(index, _split_bytes(lib, n_rows, n_dim, k_dim, n_slabs, PRODUCT_WGRAD, code))
     _lib.check(
         lib.dice_grouped_wgrad(dy.data_ptr(), x.data_ptr(), n_rows, n_dim, k_dim, seg_offsets.data_ptr(), n_slabs,
                                gate_up or 0, code, dw.data_ptr(), _ptr(dw_up), scratch, n_bytes, _status_ptr(status, index),
@@ -865,11 +869,14 @@ def grouped_ffn_train(rows: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, se
         kept = KeptAct(pre, None)
     else:
         kept = KeptAct(_new((n_rows, cols), KEEP_DTYPES[keep], index), _new((n_rows, _groups(cols)), torch.float32, index))
+    lib = _lib.load()
+    held, scratch, n_bytes = _split_scratch(index, 0 if code == DICE_BF16 else max(
+        _split_bytes(lib, n_rows, n, k, n_slabs, PRODUCT_LINEAR, code) for n, k in ((cols, h), (h, ffn))))
     _lib.check(
-        _lib.load().dice_grouped_ffn_train(
+        lib.dice_grouped_ffn_train(
             rows.data_ptr(), n_rows, h, ffn, ACT_CODES[act], KEEP_CODES[keep], code, w1.data_ptr(), w2.data_ptr(), n_slabs,
             seg_offsets.data_ptr(), n_slabs, _ptr(pre), a.data_ptr(), None if keep is None else kept.codes.data_ptr(),
-            _ptr(kept.scales), rows_out.data_ptr(), _status_ptr(status, index), _stream_of(index),
+            _ptr(kept.scales), rows_out.data_ptr(), scratch, n_bytes, _status_ptr(status, index), _stream_of(index),
         ),
         "dice_grouped_ffn_train",
     )
@@ -898,8 +905,8 @@ def grouped_ffn_backward(d_out: torch.Tensor, rows: torch.Tensor, kept: KeptAct,
     dw1_up = _new((n_slabs, ffn, h), dt, index) if act == "swiglu" else None
     lib = _lib.load()
     held, scratch, n_bytes = _split_scratch(index, max(
-        _split_bytes(lib, n_rows, h, ffn, n_slabs, 1, code), _split_bytes(lib, n_rows, cols, h, n_slabs, 0, code),
-        _split_bytes(lib, n_rows, cols, h, n_slabs, 1, code)))
+        _split_bytes(lib, n_rows, n, k, n_slabs, product, code)
+        for n, k in ((h, ffn), (cols, h)) for product in (PRODUCT_DGRAD, PRODUCT_WGRAD)))
     _lib.check(
         lib.dice_grouped_ffn_backward(
             d_out.data_ptr(), rows.data_ptr(), codes.data_ptr(), _ptr(scales), n_rows, h, ffn, ACT_CODES[act], keep, code,

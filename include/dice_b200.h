@@ -332,12 +332,18 @@ DICE_API int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, const
                        const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, int dtype, void* dx,
                        void* scratch, size_t scratch_bytes, uint32_t* status, void* stream);
 
-/* Scratch (16-byte aligned, contents irrelevant) with which dice_grouped_dgrad
- * (weight_gradient == 0) or dice_grouped_wgrad shares a long reduction among
- * SMs that few output tiles would leave idle; 0 where it would not.  NULL scratch is
- * always allowed, and slower there.  Calls that overlap on the GPU need
- * scratch of their own; calls in stream order may share it. */
-DICE_API size_t dice_grouped_scratch_bytes(int64_t n_rows, int n_dim, int k_dim, int n_slabs, int weight_gradient,
+/* Scratch (16-byte aligned, contents irrelevant) that makes a product faster:
+ * bf16, a long reduction shared among SMs that few output tiles would leave
+ * idle; fp32, the operands as three bf16 planes each for the tensor cores
+ * (24 bits; without it, and where few rows meet a weight, the CUDA cores).
+ * 0 where it would not.  `product`: which one, with n_dim and k_dim as the
+ * entry point names them (forward product: w [n_slabs, n_dim, k_dim]).  NULL
+ * scratch is always allowed.  Calls that overlap on the GPU need scratch of
+ * their own; calls in stream order may share it. */
+#define DICE_PRODUCT_DGRAD 0
+#define DICE_PRODUCT_WGRAD 1
+#define DICE_PRODUCT_LINEAR 2 /* the forward product of dice_grouped_ffn_train, fp32 */
+DICE_API size_t dice_grouped_scratch_bytes(int64_t n_rows, int n_dim, int k_dim, int n_slabs, int product,
                                   int dtype);
 
 /* Weight gradient of the same product, one segment per slab:
@@ -392,19 +398,21 @@ DICE_API int dice_combine_backward(const void* dout, const void* rows_out, const
  * what is kept of its argument, the second product.
  *   pre   [n_rows, columns of the first product]: what is kept with keep ==
  *         NONE, else scratch in fp32 and not used in bf16 (may be NULL)
- *   a     [n_rows, ffn] scratch */
+ *   a     [n_rows, ffn] scratch
+ *   scratch  the larger of what dice_grouped_scratch_bytes says for the forward
+ *         products (columns, hidden) and (hidden, ffn) */
 DICE_API int dice_grouped_ffn_train(const void* rows_in, int64_t n_rows, int hidden, int ffn, int act, int keep, int dtype,
                            const void* w1, const void* w2, int n_slabs, const int32_t* seg_offsets, int n_seg,
-                           void* pre, void* a, void* codes, float* scales, void* rows_out, uint32_t* status,
-                           void* stream);
+                           void* pre, void* a, void* codes, float* scales, void* rows_out, void* scratch,
+                           size_t scratch_bytes, uint32_t* status, void* stream);
 
 /* and its backward pass from what was kept:
  *   d_out [n_rows, hidden] -> d_rows [n_rows, hidden], dw1 (and dw1_up: SWIGLU's
  *   gate and up gradients [n_slabs, ffn, hidden] apart), dw2 [n_slabs, hidden, ffn]
  *   d_pre [n_rows, columns of the first product], a [n_rows, ffn] and, in fp32,
  *   da [n_rows, ffn] are scratch (bf16: da may be NULL); `scratch` as for the
- *   gradients (the largest of what dice_grouped_scratch_bytes says for
- *   (hidden, ffn) weight, (columns, hidden) weight and input gradient). */
+ *   gradients (the largest of what dice_grouped_scratch_bytes says for the
+ *   weight and the input gradients of (hidden, ffn) and (columns, hidden)). */
 DICE_API int dice_grouped_ffn_backward(const void* d_out, const void* rows_in, const void* kept, const float* scales,
                               int64_t n_rows, int hidden, int ffn, int act, int keep, int dtype, const void* w1,
                               const void* w2, int n_slabs, const int32_t* seg_offsets, void* da, void* d_pre,

@@ -22,9 +22,12 @@ def test_c_abi_refuses_on_the_host():
         P, P, n_rows, n, k, P, slabs, gu, dt, dw, up, None, 0, None, None)
     assert wgrad(n=60) == -2 and wgrad(gu=200) == -2 and wgrad(gu=100) == -2  # 200 takes 512 packed columns; 100 is no multiple of 8
     assert wgrad(gu=128, up=None) == -1 and wgrad(dw=P + 4) == -4 and wgrad(slabs=257) == -7 and wgrad(gu=-1) == -1
-    # a split needs a GPU whose size is known, a bf16 product, few tiles and a long reduction
-    assert lib.dice_grouped_scratch_bytes(100, 4096, 64, 1, 0, 1) == 0 and lib.dice_grouped_scratch_bytes(0, 4096, 64, 1, 0, 0) == 0
-    assert lib.dice_grouped_scratch_bytes(100, 60, 64, 1, 0, 0) == 0
+    # no scratch without rows, for sizes that are refused, for an unknown product; fp32 planes take 6 bytes a value
+    assert lib.dice_grouped_scratch_bytes(0, 4096, 64, 1, 0, 0) == 0 and lib.dice_grouped_scratch_bytes(0, 4096, 64, 1, 1, 1) == 0
+    assert lib.dice_grouped_scratch_bytes(100, 60, 64, 1, 0, 0) == 0 and lib.dice_grouped_scratch_bytes(5000, 64, 64, 1, 3, 1) == 0
+    assert lib.dice_grouped_scratch_bytes(4, 4096, 64, 1, 0, 1) == 0  # few rows: the CUDA cores
+    assert lib.dice_grouped_scratch_bytes(5120, 512, 256, 2, 1, 1) >= 6 * 5120 * (512 + 256)
+    assert lib.dice_grouped_scratch_bytes(5120, 512, 256, 2, 2, 1) >= 6 * (5120 * 256 + 2 * 512 * 256)
     keep = lambda ffn=64, act=0, kp=1, dt=0, codes=P, scales=P: lib.dice_act_keep(P, 4, ffn, act, kp, dt, P, codes, scales, None)  # noqa: E731
     assert keep(ffn=60) == -2 and keep(act=5) == -1 and keep(kp=9) == -1 and keep(dt=3) == -3
     assert keep(codes=None) == -1 and keep(scales=None) == -1 and keep(codes=P + 8) == -4
@@ -34,7 +37,7 @@ def test_c_abi_refuses_on_the_host():
     assert comb(h=60) == -2 and comb(dt=9) == -3 and comb(pos=None) == -1 and comb(pos=P + 4) == -4 and comb(dw=P + 4) == -4
     assert comb(tokens=0, pos=None) == 0
     train = lambda act=0, h=64, ffn=64, segs=2, kp=1: lib.dice_grouped_ffn_train(  # noqa: E731
-        P, 4, h, ffn, act, kp, 0, P, P, 2, P, segs, None, P, P, P, P, None, None)
+        P, 4, h, ffn, act, kp, 0, P, P, 2, P, segs, None, P, P, P, P, None, 0, None, None)
     assert train(act=7) == -1 and train(h=60) == -2 and train(ffn=12) == -2 and train(segs=3) == -1
     assert train(kp=0) == -1  # no buffer for the first product, which is what would be kept
     assert train(kp=5) == -1
