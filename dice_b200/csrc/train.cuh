@@ -25,7 +25,6 @@ int dice_internal_tc_wgrad(const void* dy, const void* x, int64_t n_rows, int n_
                            cudaStream_t s);
 
 // fp32 on the tensor cores, as six products of bf16 planes: scratch that it takes (0: not there), and the product
-constexpr int kF32Rows = 96, kF32WgradRows = 64;  // rows per slab from which it is faster (see dice_internal_f32_bytes)
 size_t dice_internal_f32_bytes(int kind, int64_t n_rows, int n_dim, int k_dim, int n_slabs);
 int dice_internal_f32_product(int kind, const void* a, const void* b, int64_t n_rows, int n_dim, int k_dim, int n_slabs,
                               const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, int gate_up, void* out,

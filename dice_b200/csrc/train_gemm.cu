@@ -38,7 +38,7 @@
 // three times the CUDA cores' 74.  (An infinity in an operand gives NaN: its product with a zero plane.)
 //
 // Few tiles: they are made half as wide if that keeps more pairs busy (one token's two rows, 1152 -> 4608: 36 tiles of
-// 256 columns, 72 of 128).  Fewer still, and a long reduction: the pairs that would idle take a share of the reduction
+// 256 columns, 72 of 128; 80 tiles on 74 pairs are two rounds, and so are 144 of half the width).  Fewer still, and a long reduction: the pairs that would idle take a share of the reduction
 // each (split).  Every epilogue
 // warp files its part of the sum in fp32; the last one to arrive at a part adds them up in the order of the shares, so
 // the result does not depend on who was last.
@@ -494,8 +494,10 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     s_mprefix[p.n_seg] = run;
     // shares of the reduction: as many as there are pairs for every tile, if each is long enough
     int split = 1;
-    const int64_t narrow_tiles = static_cast<int64_t>(run) * ((p.n_cols + BN / 2 - 1) / (BN / 2));
-    const int bn = EPI == EPI_PLAIN && narrow_tiles <= n_pairs ? BN / 2 : BN;
+    // narrow tiles take about 0.65 of a wide one's time each
+    const int64_t wide_waves = (static_cast<int64_t>(run) * ((p.n_cols + BN - 1) / BN) + n_pairs - 1) / n_pairs;
+    const int64_t narrow_waves = (static_cast<int64_t>(run) * ((p.n_cols + BN / 2 - 1) / (BN / 2)) + n_pairs - 1) / n_pairs;
+    const int bn = EPI == EPI_PLAIN && 13 * narrow_waves < 20 * wide_waves ? BN / 2 : BN;
     if (EPI == EPI_PLAIN && p.split_ws != nullptr && run > 0) {
       const int64_t per_tile = n_pairs / (static_cast<int64_t>(run) * ((p.n_cols + bn - 1) / bn));
       const int blocks = MODE != MODE_TN ? p.red_blocks : (most + BK - 1) / BK;
@@ -1202,7 +1204,13 @@ size_t plane_bytes(int64_t n) { return (static_cast<size_t>(n) * 6 + 255) / 256 
 }  // namespace
 
 // Scratch of an fp32 product on the tensor cores: both operands' planes, and a split's parts.  0: the CUDA cores are the
-// better place.
+// better place.  Where a weight takes part, making its planes has to be paid by enough rows of a slab, and three launches'
+// worth of latency by enough work; a weight gradient's operands are the rows themselves.  Measured, CUDA cores / tensor
+// cores, 8 slabs of 4608 x 1152: input gradient 64 rows a slab 155 / 183 us, 128 rows 287 / 185; weight gradient 32 rows
+// 71 / 77, 64 rows 111 / 83.  One slab, 1000 rows, 512 x 256 (2^27 multiplications): 16 / 28; 4 slabs of 2000 rows, 256 x
+// 512 (2^30): 69 / 27.
+constexpr int kF32Rows = 96, kF32WgradRows = 48;
+constexpr int64_t kF32Work = 1ll << 28;
 size_t dice_internal_f32_bytes(int kind, int64_t n_rows, int n_dim, int k_dim, int n_slabs) {
   const int64_t limit = 0x7fffff00LL / 3;
   if (n_rows >= limit || static_cast<int64_t>(n_slabs) * n_dim >= limit) return 0;
@@ -1211,7 +1219,7 @@ size_t dice_internal_f32_bytes(int kind, int64_t n_rows, int n_dim, int k_dim, i
     if (n_rows < kF32WgradRows * static_cast<int64_t>(n_slabs)) return 0;
     return plane_bytes(n_rows * n_dim) + plane_bytes(n_rows * k_dim) + dice_internal_split_bytes(n_rows, n_dim, k_dim, n_slabs, true);
   }
-  if (n_rows < kF32Rows * static_cast<int64_t>(n_slabs)) return 0;
+  if (n_rows < kF32Rows * static_cast<int64_t>(n_slabs) || n_rows < kF32Work / (static_cast<int64_t>(n_dim) * k_dim)) return 0;
   const int a_cols = kind == DICE_PRODUCT_DGRAD ? n_dim : k_dim;
   const int out_cols = kind == DICE_PRODUCT_DGRAD ? k_dim : n_dim;
   return plane_bytes(n_rows * a_cols) + plane_bytes(w) + dice_internal_split_bytes(n_rows, a_cols, out_cols, n_slabs, false);

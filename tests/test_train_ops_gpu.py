@@ -1,8 +1,9 @@
 """The training operators against plain implementations in 64 bits.
 
 Bounds.  u(t) = half a step of type t (bf16 2^-8, fp32 2^-24).  A sum of K products in fp32 is off by at most
-K 2^-23 sum|a b| (twice the usual bound K 2^-24: the tensor cores may cut where the CUDA cores round), and rounding it
-to type t adds u(t) of the value.  The sigmoid of z is off by at most delta = (8 + 4 |z|) 2^-23 of its value: expf's
+K 2^-23 sum|a b| (twice the usual bound K 2^-24: the tensor cores may cut where the CUDA cores round; fp32 operands in
+three bf16 planes leave out less than 2^-25 of a product, and K counts from 1, so K + 1 covers it), and rounding it to
+type t adds u(t) of the value.  The sigmoid of z is off by at most delta = (8 + 4 |z|) 2^-23 of its value: expf's
 and the division's few units plus the argument's own rounding, which exp multiplies by |z|.
 """
 import math
@@ -495,6 +496,43 @@ def test_what_is_kept_is_the_operators_own(cuda_device):
         assert torch.equal(out, ops.grouped_gemm(a, w2, seg, ops.EPI_STORE, h, status))
 
 
+@pytest.mark.parametrize("counts,n,k", [([700, 1, 0, 300], 1032, 1160), ([97, 95, 96], 1152, 4608), ([2000, 30], 264, 520)])
+def test_fp32_on_the_tensor_cores(cuda_device, counts, n, k):
+    """Sizes that take the six products of bf16 planes: as near to 64 bits as fp32 sums are, element by element, over
+    magnitudes from 2^-40 to 2^40 in one operand's rows, and with the largest values."""
+    gen = _gen(19)
+    rows, e = sum(counts), len(counts)
+    dy, x = _randn(gen, rows, n, dtype=torch.float32), _randn(gen, rows, k, dtype=torch.float32)
+    w = _randn(gen, e, n, k, dtype=torch.float32)
+    dy *= torch.exp2(torch.randint(-40, 41, (rows, 1), generator=gen, device=cuda_device).float())
+    dy[5, 7], x[5, :] = torch.finfo(torch.float32).max, 0.25  # would round to an infinity in 16 bits
+    seg = _seg(counts, cuda_device)
+    for product in (ops.PRODUCT_DGRAD, ops.PRODUCT_WGRAD):
+        assert ops._split_bytes(ops._lib.load(), rows, n, k, e, product, ops.DICE_F32) >= 6 * rows * n
+    w[0, 7, :] = 0.125
+    dx, dw = ops.grouped_dgrad(dy, w, seg), ops.grouped_wgrad(dy, x, seg)
+    r = 0
+    for s, c in enumerate(counts):
+        a, b, g = dy[r:r + c].to(D), w[s].to(D), x[r:r + c].to(D)
+        _check_product(dx[r:r + c], a @ b, a.abs() @ b.abs(), n, torch.float32)
+        _check_product(dw[s], a.T @ g, a.abs().T @ g.abs(), c, torch.float32)
+        r += c
+    # without scratch the CUDA cores do it: another order of sums, the same bounds
+    lib, out = ops._lib.load(), torch.empty_like(dx)
+    ops._lib.check(lib.dice_grouped_dgrad(dy.data_ptr(), rows, n, w.data_ptr(), e, k, seg.data_ptr(), None, e, ops.DICE_F32,
+                                          out.data_ptr(), None, 0, None, torch.cuda.current_stream().cuda_stream), "dgrad")
+    r = 0
+    for s, c in enumerate(counts):
+        a, b = dy[r:r + c].to(D), w[s].to(D)
+        _check_product(out[r:r + c], a @ b, a.abs() @ b.abs(), n, torch.float32)
+        r += c
+    # a scratch that is too small is refused
+    small = torch.empty(1024, dtype=torch.uint8, device=cuda_device)
+    with pytest.raises(RuntimeError, match="scratch"):
+        ops._lib.check(lib.dice_grouped_dgrad(dy.data_ptr(), rows, n, w.data_ptr(), e, k, seg.data_ptr(), None, e, ops.DICE_F32,
+                                              out.data_ptr(), small.data_ptr(), 1024, None, torch.cuda.current_stream().cuda_stream), "dgrad")
+
+
 def test_wgrad_whose_tiles_go_in_bands(cuda_device):
     """A segment whose second operand does not stay in L2 takes its tiles in another order; the one beside it does not."""
     gen = _gen(18)
@@ -510,29 +548,29 @@ def test_wgrad_whose_tiles_go_in_bands(cuda_device):
 
 @pytest.mark.parametrize("dtype", TYPES)
 def test_offsets_past_32_bits(cuda_device, dtype):
-    """Tensors of more than 2^31 elements: the first and the last rows are those of a call on these rows alone."""
+    """Tensors of more than 2^31 elements: the first and the last rows against 64 bits (products) and against calls on these
+    rows alone (the row-wise operators, which go row by row whatever their number)."""
     gen = _gen(17)
     rows, wide, narrow = 240000, 9216, 64
     assert rows * wide > 2 ** 31
     cut = [slice(0, 300), slice(rows - 300, rows)]
     seg = torch.tensor([0, 300, rows - 300, rows], dtype=torch.int32, device=cuda_device)
-    part = _seg([300], cuda_device)
     dy, w = _randn(gen, rows, narrow, dtype=dtype), _randn(gen, 3, narrow, wide, dtype=dtype, scale=0.1)
     dx = ops.grouped_dgrad(dy, w, seg)
     for c, e in zip(cut, (0, 2)):
-        assert torch.equal(dx[c], ops.grouped_dgrad(dy[c], w[e:e + 1], part))
+        a, b = dy[c].to(D), w[e].to(D)
+        _check_product(dx[c], a @ b, a.abs() @ b.abs(), narrow, dtype)
     dw = ops.grouped_wgrad(dx, dy, seg)  # its wide operand read back
     for c, e in zip(cut, (0, 2)):
-        one = ops.grouped_wgrad(dx[c], dy[c], part)[0]
-        # (shares of the reduction may differ between the two calls)
-        far = (dw[e].to(D) - one.to(D)).abs()
-        assert bool((far <= 2 * U[dtype] * one.to(D).abs() + 301 * 2.0 ** -22 * (dx[c].to(D).abs().T @ dy[c].to(D).abs())).all())
+        a, b = dx[c].to(D).T, dy[c].to(D)
+        _check_product(dw[e], a @ b, a.abs() @ b.abs(), 300, dtype)
     ffn = wide // 2
     a, kept = ops.act_keep(dx, "swiglu", ffn, keep="int8")
+    parts = [dx[c].clone() for c in cut]
     del dx
     d_pre, a2 = ops.act_backward(a, kept, "swiglu", ffn)
-    for c in cut:
-        a_c, kept_c = ops.act_keep(ops.grouped_dgrad(dy[c], w[0 if c.start == 0 else 2][None], part), "swiglu", ffn, keep="int8")
+    for c, part in zip(cut, parts):
+        a_c, kept_c = ops.act_keep(part, "swiglu", ffn, keep="int8")
         assert torch.equal(a[c], a_c) and torch.equal(kept.codes[c], kept_c.codes) and torch.equal(kept.scales[c], kept_c.scales)
         d_c, a2_c = ops.act_backward(a_c, kept_c, "swiglu", ffn)
         assert torch.equal(d_pre[c], d_c) and torch.equal(a2[c], a2_c)
