@@ -4,7 +4,7 @@
 
 #include "common.cuh"
 
-// fp32 on the CUDA cores (train_simt.cu)
+// fp32 on the CUDA cores (train_simt.cu): few rows, or no scratch
 int dice_internal_simt_linear(const void* a, int64_t n_rows, int k_dim, const void* w, int n_slabs, int n_dim,
                               const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, void* out,
                               uint32_t* status, cudaStream_t s);

@@ -1,5 +1,5 @@
-// Products grouped by expert on the CUDA cores, for the training step's fp32 form (the tensor cores would round
-// fp32 operands to tf32) in its three directions:
+// Products grouped by expert on the CUDA cores, for the training step's fp32 form where few rows meet a weight (from 96
+// rows a slab on, train_gemm.cu makes six tensor-core products of it), in its three directions:
 //
 //   NT  out[r, n] = sum_k a[r, k] w[seg(r)][n, k]        the forward product (nn.Linear weights)
 //   NN  dx[r, k]  = sum_n dy[r, n] w[seg(r)][n, k]       its input gradient
@@ -17,7 +17,7 @@
 // reduction, added up in shared memory at the end (1024 rows through 8 experts, 4608 -> 1152: 180 tiles alone would
 // leave most of the GPU's warp slots empty).  Where even that leaves slots empty or a nearly empty last wave, the 2 to 8
 // CTAs of a cluster share a tile's reduction in the same way and the first adds up what the others hold in shared
-// memory.  The order of all these sums is fixed.  A tile with at most 8 rows (single tokens) is bounded by reading the
+// memory.  The order of all these sums is fixed.  A tile with at most 12 rows (single tokens) is bounded by reading the
 // weights: its CTA forgoes the tiling and streams them, every value used for the rows there are.  TN has many tiles and a short reduction: 128 x 128 tiles, one group.
 #include "train.cuh"
 #include "umma.cuh"  // sm_count_cached
@@ -45,8 +45,8 @@ __device__ __forceinline__ void store4(float* p, const float* v) {
 }
 
 
-// 8 x 8 sums of one slice: rows ra .. ra+3 and ra+STEP .. of A, columns likewise of B
-template <int DEPTH, int WIDTH, int STEP>
+// 8 x 8 sums of one slice: rows ra .. ra+3 and ra+STEP .. of A (HALF: the first four only), columns likewise of B
+template <int DEPTH, int WIDTH, int STEP, bool HALF = false>
 __device__ __forceinline__ void multiply(const float (*As)[WIDTH + 4], const float (*Bs)[WIDTH + 4], int ra, int cb,
                                          f32x2 (&acc)[8][4]) {
 #pragma unroll
@@ -54,11 +54,11 @@ __device__ __forceinline__ void multiply(const float (*As)[WIDTH + 4], const flo
     float ar[8];
     f32x2 br[4];
     *reinterpret_cast<float4*>(ar) = *reinterpret_cast<const float4*>(&As[k][ra]);
-    *reinterpret_cast<float4*>(ar + 4) = *reinterpret_cast<const float4*>(&As[k][ra + STEP]);
+    if (!HALF) *reinterpret_cast<float4*>(ar + 4) = *reinterpret_cast<const float4*>(&As[k][ra + STEP]);
     *reinterpret_cast<ulonglong2*>(br) = *reinterpret_cast<const ulonglong2*>(&Bs[k][cb]);
     *reinterpret_cast<ulonglong2*>(br + 2) = *reinterpret_cast<const ulonglong2*>(&Bs[k][cb + STEP]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < (HALF ? 4 : 8); ++i) {
       const f32x2 a2 = both<f32x2>(ar[i]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = fma2(a2, br[j], acc[i][j]);
@@ -149,65 +149,92 @@ struct Slices {
   float a[kRing][TK][TM + 4], b[kRing][TK][TN + 4];
 };
 constexpr int kRowsSmem = GROUPS * sizeof(Slices);
-static_assert(kRowsSmem >= 2 * TM * TN * sizeof(float) && kRowsSmem >= 16 * 8 * TN * sizeof(float),
+static_assert(kRowsSmem >= 2 * TM * TN * sizeof(float) && kRowsSmem >= (12 + 16 * 8) * TN * sizeof(float),
               "sums are exchanged in place of the slices");
 
 // A tile of at most kThinRows rows: every thread sums over its own part of the reduction, straight from memory, and the
 // parts are added in shared memory (`sums`, [ROWS][64] of them at its front at the end).  NN: 16 threads hold a weight
-// row's 64 columns, 16 rows at once.  NT: a warp holds a weight row (one column), its lanes four elements each.
-constexpr int kThinRows = 8;
+// row's 64 columns, 16 times four rows at once.  NT: a warp holds four weight rows (columns of the output), its lanes four
+// elements of each.  Either way a value of the few rows is used for four of the weight's.
+constexpr int kThinRows = 12;  // (8 slabs of 4608 x 1152: 4 rows 65 us, 12 rows 106, 16 rows 145; half a tile takes 129)
 template <int MODE, int ROWS>
 __device__ __forceinline__ void thin_tile(const float* a, int64_t lda, const float* w, int64_t ldb, int rows, int n_valid, int red,
                                           int share, int shares, float* sums) {
+  float acc[ROWS][4] = {};
   if (MODE == MODE_NN) {
     const int c = (threadIdx.x & 15) * 4, n0 = static_cast<int>(threadIdx.x >> 4);
-    float acc[ROWS][4] = {};
     if (c < n_valid) {
-#pragma unroll 4
-      for (int n = share * 16 + n0; n < red; n += shares * 16) {
-        const float4 x = *reinterpret_cast<const float4*>(w + n * ldb + c);
+      for (int n = (share * 16 + n0) * 4; n < red; n += shares * 64) {  // (red is a multiple of 8)
+        float4 x[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] = *reinterpret_cast<const float4*>(w + (n + q) * ldb + c);
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-          const float y = r < rows ? a[r * lda + n] : 0.f;
-          acc[r][0] = fmaf(y, x.x, acc[r][0]);
-          acc[r][1] = fmaf(y, x.y, acc[r][1]);
-          acc[r][2] = fmaf(y, x.z, acc[r][2]);
-          acc[r][3] = fmaf(y, x.w, acc[r][3]);
+          if (r < rows) {
+            const float4 y = *reinterpret_cast<const float4*>(a + r * lda + n);
+            const float ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              acc[r][0] = fmaf(ys[q], x[q].x, acc[r][0]);
+              acc[r][1] = fmaf(ys[q], x[q].y, acc[r][1]);
+              acc[r][2] = fmaf(ys[q], x[q].z, acc[r][2]);
+              acc[r][3] = fmaf(ys[q], x[q].w, acc[r][3]);
+            }
+          }
         }
       }
     }
+    // the 16 parts, a few rows at a time (all of 12 would not fit)
+    constexpr int kRows = ROWS % 8 == 0 ? 8 : ROWS % 4 == 0 ? 4 : ROWS;
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) *reinterpret_cast<float4*>(&sums[(n0 * ROWS + r) * TN + c]) = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
-    __syncthreads();
-    for (int i = threadIdx.x; i < ROWS * TN; i += 64 * GROUPS) {
-      float t = 0.f;
+    for (int r0 = 0; r0 < ROWS; r0 += kRows) {
+      float* part = sums + ROWS * TN;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) t += sums[k * ROWS * TN + i];
-      sums[i] = t;  // (only this thread reads or writes place i of the 16)
+      for (int r = 0; r < kRows; ++r)
+        *reinterpret_cast<float4*>(&part[(n0 * kRows + r) * TN + c]) = make_float4(acc[r0 + r][0], acc[r0 + r][1], acc[r0 + r][2], acc[r0 + r][3]);
+      __syncthreads();
+      for (int i = threadIdx.x; i < kRows * TN; i += 64 * GROUPS) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) t += part[k * kRows * TN + i];
+        sums[r0 * TN + i] = t;
+      }
+      __syncthreads();
     }
   } else {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int c = warp; c < n_valid; c += 2 * GROUPS) {
-      float acc[ROWS] = {};
-#pragma unroll 2
+    for (int c = warp * 4; c < n_valid; c += 8 * GROUPS) {  // (n_valid is a multiple of 8)
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[r][q] = 0.f;
       for (int k = (share * 32 + lane) * 4; k < red; k += shares * 128) {
-        const float4 x = *reinterpret_cast<const float4*>(w + c * ldb + k);
+        float4 x[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] = *reinterpret_cast<const float4*>(w + (c + q) * ldb + k);
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
           if (r < rows) {
             const float4 y = *reinterpret_cast<const float4*>(a + r * lda + k);
-            acc[r] = fmaf(y.x, x.x, fmaf(y.y, x.y, fmaf(y.z, x.z, fmaf(y.w, x.w, acc[r]))));
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              acc[r][q] = fmaf(y.x, x[q].x, fmaf(y.y, x[q].y, fmaf(y.z, x[q].z, fmaf(y.w, x[q].w, acc[r][q]))));
           }
         }
       }
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
-        for (int off = 16; off > 0; off >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], off);
-        if (lane == 0) sums[r * TN + c] = acc[r];
+        if (r < rows) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            for (int off = 16; off > 0; off >>= 1) acc[r][q] += __shfl_xor_sync(0xffffffffu, acc[r][q], off);
+          }
+          if (lane == 0) *reinterpret_cast<float4*>(&sums[r * TN + c]) = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+        }
       }
     }
+    __syncthreads();
   }
-  __syncthreads();
 }
 
 template <int MODE>
@@ -254,6 +281,7 @@ __global__ void __launch_bounds__(64 * GROUPS, 2) simt_rows_kernel(const SimtPar
   if (m_valid <= kThinRows) {
     float* sums = reinterpret_cast<float*>(slices);
     if (m_valid <= 2) thin_tile<MODE, 2>(a, lda, b, ldb, m_valid, n_valid, p.red, blockIdx.z, gridDim.z, sums);
+    else if (m_valid <= 8) thin_tile<MODE, 8>(a, lda, b, ldb, m_valid, n_valid, p.red, blockIdx.z, gridDim.z, sums);
     else thin_tile<MODE, kThinRows>(a, lda, b, ldb, m_valid, n_valid, p.red, blockIdx.z, gridDim.z, sums);
     if (gridDim.z > 1) cluster_sync();
     if (blockIdx.z == 0) {
@@ -299,7 +327,8 @@ __global__ void __launch_bounds__(64 * GROUPS, 2) simt_rows_kernel(const SimtPar
     copies_wait();
     asm volatile("bar.sync %0, 64;" ::"r"(group + 1) : "memory");  // the slice is there, the one before it is done with
     fetch(buf == 0 ? kRing - 1 : buf - 1);
-    multiply<TK, TM, 32>(mine.a[buf], mine.b[buf], ra, cb, acc);
+    if (m_valid > TM / 2) multiply<TK, TM, 32>(mine.a[buf], mine.b[buf], ra, cb, acc);
+    else multiply<TK, TM, 32, true>(mine.a[buf], mine.b[buf], ra, cb, acc);  // (32 rows a slab: 152 -> 129 us)
     buf = buf == kRing - 1 ? 0 : buf + 1;
   }
 

@@ -92,7 +92,7 @@ def test_wgrad(cuda_device, counts, n, k, dtype):
     ([1], 9216, 64), ([2, 0, 1], 4608, 264), ([300], 2048, 72), ([129, 3], 1160, 520),   # shared by the input gradient
     ([6000], 72, 64), ([3001, 0, 700], 136, 264), ([1100], 264, 328),                      # and by the weight gradient
     ([1, 1], 1152, 4608),                                                                   # narrow tiles, nothing shared
-    ([8, 5, 1, 9], 328, 1160), ([2] * 16, 1032, 264),                                       # fp32: tiles of few rows
+    ([8, 5, 1, 9], 328, 1160), ([2] * 16, 1032, 264), ([12, 13, 32, 33, 76], 520, 264),     # fp32: tiles of few rows
 ])
 def test_long_reductions_and_few_tiles(cuda_device, counts, n, k, dtype):
     """Few tiles: the reduction is shared, and added up in a fixed order."""
@@ -440,7 +440,7 @@ def _ffn_inputs(gen, counts, h, ffn, act, dtype, dev):
 @pytest.mark.parametrize("act", ["swiglu", "gelu_tanh"])
 @pytest.mark.parametrize("keep", ["int8", "e4m3", None])
 @pytest.mark.parametrize("counts,h,ffn", [([1], 64, 64), ([0, 33, 300, 0, 7], 200, 264), ([128, 0, 256], 384, 512),
-                                          ([5, 1, 8, 2, 70], 136, 1032), ([1, 3], 1792, 7168)])
+                                          ([5, 1, 8, 2, 70, 12, 9], 136, 1032), ([1, 3], 1792, 7168)])
 def test_ffn_forward_and_backward(cuda_device, dtype, act, keep, counts, h, ffn):
     """The whole pass against 64 bits, fed with the kernel's own kept argument.  Norm bounds: every rounding to the type
     on the way moves its tensor by at most u of each value, and a product carries relative errors of its factors on; five
