@@ -37,6 +37,9 @@ extern "C" int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, con
   if (n_rows == 0 || n_seg == 0) return DICE_OK;
   DICE_CHECK_ARG(dy && w && seg_offsets && dx, DICE_ERR_ARG);
   DICE_CHECK_ARG(dice_aligned16(dy) && dice_aligned16(w) && dice_aligned16(dx), DICE_ERR_ALIGN);
+  if (dtype == DICE_BF16 && n_rows <= kThinTotal)
+    return dice_internal_thin_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dx, status,
+                                    static_cast<cudaStream_t>(stream));
   if (dtype == DICE_BF16)
     return dice_internal_tc_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dx, scratch,
                                   scratch_bytes, status, static_cast<cudaStream_t>(stream));

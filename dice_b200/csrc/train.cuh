@@ -15,6 +15,12 @@ int dice_internal_simt_wgrad(const void* dy, const void* x, int64_t n_rows, int 
                              const int32_t* seg_offsets, int n_slabs, int gate_up, void* dw, void* dw_up,
                              uint32_t* status, cudaStream_t s);
 
+// bf16 input gradient of at most kThinTotal rows, on the CUDA cores (train_thin.cu)
+constexpr int kThinTotal = 4;
+int dice_internal_thin_dgrad(const void* dy, int64_t n_rows, int n_dim, const void* w, int n_slabs, int k_dim,
+                             const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, void* dx, uint32_t* status,
+                             cudaStream_t s);
+
 // bf16 on the tensor cores (train_gemm.cu)
 size_t dice_internal_split_bytes(int64_t n_rows, int n_dim, int k_dim, int n_slabs, bool weight_gradient);
 int dice_internal_tc_dgrad(const void* dy, int64_t n_rows, int n_dim, const void* w, int n_slabs, int k_dim,

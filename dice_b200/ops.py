@@ -578,8 +578,8 @@ class KeptAct(NamedTuple):
 
 
 # The small calls of a training step are bounded by the host: one token's gradients cost the GPU a few microseconds, and
-# every torch.empty with keyword arguments two, every look-up of a device half of one.  Hence one comparison per tensor
-# (_one_device), allocations through torch's own short path where it exists, and widths computed here.
+# every torch.empty with keyword arguments two, every look-up of a device half of one.  Hence one comparison per tensor,
+# written out, allocations through torch's own short path where it exists, and widths computed here.
 _empty_cuda = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 
 
@@ -601,9 +601,8 @@ def _one_device(*tensors: Optional[torch.Tensor]) -> int:
     return index
 
 
-def _away(index: int):
-    """Launches go to the current device's current stream: the context for tensors of another device, None for its own."""
-    return None if index == torch.cuda.current_device() else torch.cuda.device(index)
+# Launches go to the current device's current stream, so a call on another device's tensors makes that device current.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _stream_of(index: int) -> int:
@@ -669,9 +668,8 @@ def grouped_dgrad(dy: torch.Tensor, w: torch.Tensor, seg_offsets: torch.Tensor, 
     """Input gradient of :func:`grouped_gemm`: ``dx[r] = dy[r] @ w[slab(seg(r))]`` with ``dy [R, N]``,
     ``w [S, N, K]`` (bf16 or fp32).  Rows of no segment are left as they are in ``out`` (uninitialised without it)."""
     index = _one_device(dy, w, seg_offsets, status, seg_slab, out)
-    away = _away(index)
-    if away is not None:
-        with away:
+    if index != _current_device():
+        with torch.cuda.device(index):
             return grouped_dgrad(dy, w, seg_offsets, status, seg_slab, out)
     assert dy.dim() == 2 and w.dim() == 3 and w.dtype == dy.dtype
     n_seg = _check_segments(seg_offsets)
@@ -701,9 +699,8 @@ def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, seg_offsets: torch.Tensor, 
     for a segment without rows.  ``gate_up=ffn``: ``dy`` has the packed gate / up columns of :func:`pack_w13`, and the
     result is the pair of gradients ``[S, ffn, K]`` of the gate and the up projections."""
     index = _one_device(dy, x, seg_offsets, status)
-    away = _away(index)
-    if away is not None:
-        with away:
+    if index != _current_device():
+        with torch.cuda.device(index):
             return grouped_wgrad(dy, x, seg_offsets, status, gate_up)
     assert dy.dim() == 2 and x.dim() == 2 and x.dtype == dy.dtype
     n_slabs = _check_segments(seg_offsets)
@@ -757,9 +754,8 @@ def act_keep(pre: torch.Tensor, act: str, ffn: int, keep: Optional[str] = "int8"
     scale.  ``keep=None`` keeps ``pre`` itself."""
     _check_keep(keep)
     index = _one_device(pre)
-    away = _away(index)
-    if away is not None:
-        with away:
+    if index != _current_device():
+        with torch.cuda.device(index):
             return act_keep(pre, act, ffn, keep)
     cols = act_columns(act, ffn)
     assert pre.dim() == 2
@@ -787,9 +783,8 @@ def act_backward(da: torch.Tensor, kept: KeptAct, act: str, ffn: int, want_act: 
     gradient needs."""
     codes, scales = kept
     index = _one_device(da, codes, scales)
-    away = _away(index)
-    if away is not None:
-        with away:
+    if index != _current_device():
+        with torch.cuda.device(index):
             return act_backward(da, kept, act, ffn, want_act)
     cols = act_columns(act, ffn)
     assert da.dim() == 2
@@ -813,26 +808,27 @@ def combine_backward(dout: torch.Tensor, rows_out: torch.Tensor, pos: torch.Tens
     ``d_rows[pos[t, s]] = weights[t, s] * dout[t]`` and ``d_weights [N, 2]`` fp32 ``= <dout[t], rows_out[pos[t, s]]>``.
     ``pos`` int32 ``[N, 2]`` names no row twice (a plan's); rows that it does not name are left uninitialised, a
     position outside ``rows_out`` has gradient 0."""
-    index = _one_device(dout, rows_out, pos, weights)
-    away = _away(index)
-    if away is not None:
-        with away:
+    index = dout.get_device()
+    if index < 0 or rows_out.get_device() != index or pos.get_device() != index or weights.get_device() != index:
+        _one_device(dout, rows_out, pos, weights)
+    if index != _current_device():
+        with torch.cuda.device(index):
             return combine_backward(dout, rows_out, pos, weights)
-    assert dout.dim() == 2 and rows_out.dim() == 2 and rows_out.dtype == dout.dtype
+    assert dout.dim() == 2 and rows_out.dim() == 2
     n_tokens, h = dout.shape
     n_rows, row_cols = rows_out.shape
-    assert row_cols == h
+    dtype = dout.dtype
+    assert row_cols == h and rows_out.dtype == dtype
     assert pos.dtype == torch.int32 and pos.shape == (n_tokens, 2)
     assert weights.dtype == torch.float32 and weights.shape == (n_tokens, 2)
     code = _dtype_code(dout)
     dout, rows_out, pos, weights = dout.contiguous(), rows_out.contiguous(), pos.contiguous(), weights.contiguous()
-    d_rows = _new((n_rows, h), dout.dtype, index)
+    d_rows = _new((n_rows, h), dtype, index)
     d_weights = _new((n_tokens, 2), torch.float32, index)
-    _lib.check(
-        _lib.load().dice_combine_backward(dout.data_ptr(), rows_out.data_ptr(), pos.data_ptr(), weights.data_ptr(), n_tokens,
-                                          n_rows, h, code, d_rows.data_ptr(), d_weights.data_ptr(), _stream_of(index)),
-        "dice_combine_backward",
-    )
+    rc = _lib.load().dice_combine_backward(dout.data_ptr(), rows_out.data_ptr(), pos.data_ptr(), weights.data_ptr(), n_tokens,
+                                           n_rows, h, code, d_rows.data_ptr(), d_weights.data_ptr(), _stream_of(index))
+    if rc:
+        _lib.check(rc, "dice_combine_backward")
     return d_rows, d_weights
 
 
@@ -854,9 +850,8 @@ def grouped_ffn_train(rows: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, se
     cores, or the CUDA cores where few rows meet a weight)."""
     _check_keep(keep)
     index = _one_device(rows, w1, w2, seg_offsets, status)
-    away = _away(index)
-    if away is not None:
-        with away:
+    if index != _current_device():
+        with torch.cuda.device(index):
             return grouped_ffn_train(rows, w1, w2, seg_offsets, act, ffn, status, keep)
     code = _dtype_code(rows)
     n_slabs, h, cols = _check_ffn(rows, w1, w2, seg_offsets, act, ffn)
@@ -890,9 +885,8 @@ def grouped_ffn_backward(d_out: torch.Tensor, rows: torch.Tensor, kept: KeptAct,
     pair of the gate and the up projections' gradients ``[S, ffn, h]``."""
     codes, scales = kept
     index = _one_device(d_out, rows, codes, scales, w1, w2, seg_offsets, status)
-    away = _away(index)
-    if away is not None:
-        with away:
+    if index != _current_device():
+        with torch.cuda.device(index):
             return grouped_ffn_backward(d_out, rows, kept, w1, w2, seg_offsets, act, ffn, status)
     code = _dtype_code(rows)
     n_slabs, h, cols = _check_ffn(rows, w1, w2, seg_offsets, act, ffn)

@@ -158,6 +158,36 @@ def test_rows_outside_the_segments(cuda_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k", [(8, 8), (1160, 136), (4608, 2056)])
+def test_dgrad_of_single_tokens(cuda_device, dtype, n, k):
+    """One to four rows: together, apart, beside rows of no expert that hold NaN, through a table of slabs."""
+    gen = _gen(20)
+    w = _randn(gen, 3, n, k, dtype=dtype, scale=0.1)
+    for offsets, slab in [([0, 1], [2]), ([0, 0, 2, 2], None), ([0, 1, 1, 2], None), ([0, 4], [1]), ([0, 3, 4, 4], None),
+                          ([1, 2, 2, 3], [0, -1, 2]), ([0, 1, 2, 4], [1, -1, 1])]:
+        rows = 4 if offsets[0] else offsets[-1]
+        dy = _randn(gen, rows, n, dtype=dtype)
+        fine = torch.zeros(rows, dtype=torch.bool, device=cuda_device)
+        seg = torch.tensor(offsets, dtype=torch.int32, device=cuda_device)
+        table = None if slab is None else torch.tensor(slab, dtype=torch.int32, device=cuda_device)
+        slabs = slab if slab is not None else range(3)
+        for s, beg, end in zip(slabs, offsets, offsets[1:]):
+            fine[beg:end] = s >= 0
+        dy[~fine] = float("nan")
+        out = torch.full((rows, k), -7.0, dtype=dtype, device=cuda_device)
+        ops.grouped_dgrad(dy, w if slab is not None or len(offsets) == 4 else w[:len(offsets) - 1], seg, seg_slab=table, out=out)
+        assert bool((out[~fine] == -7).all())
+        for s, beg, end in zip(slabs, offsets, offsets[1:]):
+            if s >= 0 and end > beg:
+                a, b = dy[beg:end].to(D), w[s].to(D)
+                _check_product(out[beg:end], a @ b, a.abs() @ b.abs(), n, dtype)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    ops.grouped_dgrad(dy, w, torch.tensor([0, 2, 1, 4], dtype=torch.int32, device=cuda_device), status=status)
+    with pytest.raises(RuntimeError, match="segment offsets"):
+        ops.check_status(status)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_no_rows_at_all(cuda_device, dtype):
     seg = torch.zeros(4, dtype=torch.int32, device=cuda_device)
     dy, x = torch.empty(0, 64, dtype=dtype, device=cuda_device), torch.empty(0, 72, dtype=dtype, device=cuda_device)
