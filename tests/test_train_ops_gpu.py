@@ -470,7 +470,7 @@ def _ffn_inputs(gen, counts, h, ffn, act, dtype, dev):
 @pytest.mark.parametrize("act", ["swiglu", "gelu_tanh"])
 @pytest.mark.parametrize("keep", ["int8", "e4m3", None])
 @pytest.mark.parametrize("counts,h,ffn", [([1], 64, 64), ([0, 33, 300, 0, 7], 200, 264), ([128, 0, 256], 384, 512),
-                                          ([5, 1, 8, 2, 70, 12, 9], 136, 1032), ([1, 3], 1792, 7168)])
+                                          ([5, 1, 8, 2, 70, 12, 9], 136, 1032), ([1, 3], 1792, 7168), ([200, 100, 0, 250], 264, 2056)])
 def test_ffn_forward_and_backward(cuda_device, dtype, act, keep, counts, h, ffn):
     """The whole pass against 64 bits, fed with the kernel's own kept argument.  Norm bounds: every rounding to the type
     on the way moves its tensor by at most u of each value, and a product carries relative errors of its factors on; five
@@ -561,6 +561,30 @@ def test_fp32_on_the_tensor_cores(cuda_device, counts, n, k):
     with pytest.raises(RuntimeError, match="scratch"):
         ops._lib.check(lib.dice_grouped_dgrad(dy.data_ptr(), rows, n, w.data_ptr(), e, k, seg.data_ptr(), None, e, ops.DICE_F32,
                                               out.data_ptr(), small.data_ptr(), 1024, None, torch.cuda.current_stream().cuda_stream), "dgrad")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_masked_rows_on_the_tensor_cores(cuda_device, dtype):
+    """As test_rows_outside_the_segments, at sizes where fp32 is on the tensor cores too: NaN and infinities around the
+    segments, in a neighbour and in unused weights change no other bit."""
+    gen = _gen(21)
+    counts, n, k = [301, 0, 205, 90], 1032, 1160
+    seg = _seg(counts, cuda_device, start=5)
+    rows = int(seg[-1]) + 9
+    dy, x, w = (_randn(gen, *sh, dtype=dtype) for sh in ((rows, n), (rows, k), (4, n, k)))
+    want_dx, want_dw = ops.grouped_dgrad(dy, w, seg), ops.grouped_wgrad(dy, x, seg)
+    for bad in (float("nan"), float("inf")):
+        dy2, x2, w2 = dy.clone(), x.clone(), w.clone()
+        for t in (dy2, x2):
+            t[:5] = t[int(seg[-1]):] = t[int(seg[2]):int(seg[3])] = bad
+        w2[1] = bad
+        out = torch.full((rows, k), -7.0, dtype=dtype, device=cuda_device)
+        dx, dw = ops.grouped_dgrad(dy2, w2, seg, out=out), ops.grouped_wgrad(dy2, x2, seg)
+        for s in (0, 3):
+            assert torch.equal(dx[int(seg[s]):int(seg[s + 1])], want_dx[int(seg[s]):int(seg[s + 1])])
+        assert bool((dx[:5] == -7).all()) and bool((dx[int(seg[-1]):] == -7).all())
+        assert not bool(torch.isfinite(dx[int(seg[2]):int(seg[3])]).any())
+        assert torch.equal(dw[[0, 1, 3]], want_dw[[0, 1, 3]]) and not bool(torch.isfinite(dw[2]).any())
 
 
 def test_wgrad_whose_tiles_go_in_bands(cuda_device):
