@@ -654,6 +654,15 @@ def _check_segments(seg_offsets: torch.Tensor) -> int:
     return seg_offsets.numel() - 1
 
 
+def _check_out(out: torch.Tensor, *operands: torch.Tensor) -> None:
+    """The kernels write ``out`` while they still read their (contiguous) operands."""
+    begin = out.data_ptr()
+    end = begin + out.numel() * out.element_size()
+    for t in operands:
+        if t.data_ptr() < end and begin < t.data_ptr() + t.numel() * t.element_size():
+            raise ValueError("out shares memory with an operand")
+
+
 def act_columns(act: str, ffn: int) -> int:
     """Columns of an activation's argument: ``ffn``, or the packed gate / up width of SwiGLU (``w13_rows(ffn)``)."""
     if act == "swiglu":
@@ -666,7 +675,8 @@ def act_columns(act: str, ffn: int) -> int:
 def grouped_dgrad(dy: torch.Tensor, w: torch.Tensor, seg_offsets: torch.Tensor, status: Optional[torch.Tensor] = None,
                   seg_slab: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Input gradient of :func:`grouped_gemm`: ``dx[r] = dy[r] @ w[slab(seg(r))]`` with ``dy [R, N]``,
-    ``w [S, N, K]`` (bf16 or fp32).  Rows of no segment are left as they are in ``out`` (uninitialised without it)."""
+    ``w [S, N, K]`` (bf16 or fp32).  Rows of no segment are left as they are in ``out`` (uninitialised without it), which
+    shares no memory with the operands.  fp32: an infinity in a row or a weight may come out as NaN."""
     index = _one_device(dy, w, seg_offsets, status, seg_slab, out)
     if index != _current_device():
         with torch.cuda.device(index):
@@ -681,6 +691,8 @@ def grouped_dgrad(dy: torch.Tensor, w: torch.Tensor, seg_offsets: torch.Tensor, 
     assert w_rows == n_dim
     if out is None:
         out = _new((n_rows, k_dim), dy.dtype, index)
+    else:
+        _check_out(out, dy, w)
     assert out.is_contiguous() and out.shape == (n_rows, k_dim) and out.dtype == dy.dtype
     lib = _lib.load()
     held, scratch, n_bytes = _split_scratch(index, _split_bytes(lib, n_rows, n_dim, k_dim, n_slabs, PRODUCT_DGRAD, code))
@@ -696,7 +708,7 @@ def grouped_dgrad(dy: torch.Tensor, w: torch.Tensor, seg_offsets: torch.Tensor, 
 def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, seg_offsets: torch.Tensor, status: Optional[torch.Tensor] = None,
                   gate_up: Optional[int] = None):
     """Weight gradient of :func:`grouped_gemm`: ``dw[s] = dy[seg s].T @ x[seg s]`` ``[S, N, K]`` in the rows' type, zero
-    for a segment without rows.  ``gate_up=ffn``: ``dy`` has the packed gate / up columns of :func:`pack_w13`, and the
+    for a segment without rows (fp32: an infinity may come out as NaN).  ``gate_up=ffn``: ``dy`` has the packed gate / up columns of :func:`pack_w13`, and the
     result is the pair of gradients ``[S, ffn, K]`` of the gate and the up projections."""
     index = _one_device(dy, x, seg_offsets, status)
     if index != _current_device():

@@ -83,3 +83,11 @@ def test_a_block_without_train_kernels_trains_as_before():
     x = torch.randn(2, 5, 32, requires_grad=True)
     blk(x).sum().backward()
     assert x.grad is not None and blk.gate.weight.grad is not None and not blk.train_kernels
+
+
+def test_result_that_shares_memory_with_an_operand():
+    z = torch.zeros(10, 64)
+    ops._check_out(z[:5], z[5:], torch.zeros(4))
+    for out, operand in ((z, z), (z[:5], z[4:]), (z[2:4], z), (z, z.view(-1)[64:72])):
+        with pytest.raises(ValueError, match="shares memory"):
+            ops._check_out(out, torch.zeros(4), operand)
