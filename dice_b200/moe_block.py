@@ -74,6 +74,11 @@ def _compute_dtype(x: torch.Tensor) -> torch.dtype:
     return torch.bfloat16
 
 
+def _check_train_kernels(para_mode, num_experts_per_tok: int) -> None:
+    if para_mode.ep or num_experts_per_tok != 2:
+        raise ValueError("train_kernels takes two experts per token and no expert parallelism")
+
+
 def layer_is_async(para_mode, layer_idx, total_layers) -> bool:
     """Which layers use the asynchronous exchange under each selective-sync
     mode (models.py:328-340)."""
@@ -406,8 +411,8 @@ class SparseMoeBlock(nn.Module):
         assert expert_act in ("swiglu", "gelu_tanh")
         if train_keep not in ops.KEEP_CODES:
             raise ValueError(f"train_keep is None, 'int8' or 'e4m3', got {train_keep!r}")
-        if train_kernels and (para_mode.ep or num_experts_per_tok != 2):
-            raise ValueError("train_kernels takes two experts per token and no expert parallelism")
+        if train_kernels:
+            _check_train_kernels(para_mode, num_experts_per_tok)
         self.train_kernels, self.train_keep = train_kernels, train_keep
         self.num_experts_per_tok = num_experts_per_tok
         self.expert_act = expert_act
@@ -625,6 +630,8 @@ class SparseMoeBlock(nn.Module):
         """The experts' part of the training forward on the kernels."""
         from .expert_train import DenseExpert, RoutedExperts
 
+        # the switch may have been set on a block that was built without it
+        _check_train_kernels(self.para_mode, topk_idx.shape[-1])
         if not hidden_states.is_cuda:
             raise RuntimeError("a SparseMoeBlock with train_kernels trains on CUDA tensors only (no CPU fallback)")
         if not self.layer_idx:

@@ -1,0 +1,28 @@
+"""What the training path asks of a block and of its callers, as far as no GPU is needed."""
+import pytest
+import torch
+
+from dice_b200.moe_block import ParaMode, SparseMoeBlock
+
+
+def _block(k=2, **kw):
+    return SparseMoeBlock(32, 2, 4, k, 1, 0, 1, ParaMode(), **kw).train()
+
+
+@pytest.mark.parametrize("k", [1, 4])
+def test_kernels_switched_on_after_construction(k):
+    """The kernels gather rows two to a token: with four, they would read behind the tokens."""
+    blk = _block(k)
+    blk.train_kernels = True
+    with pytest.raises(ValueError, match="two experts per token"):
+        blk(torch.zeros(1, 3, 32))
+    blk = _block()
+    blk.train_kernels = True
+    blk.gate.top_k = k
+    with pytest.raises(ValueError, match="two experts per token"):
+        blk(torch.zeros(1, 3, 32))
+    blk = _block()
+    blk.train_kernels = True
+    blk.para_mode = ParaMode(ep=True)
+    with pytest.raises(ValueError, match="expert parallelism"):
+        blk(torch.zeros(1, 3, 32))
