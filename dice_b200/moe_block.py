@@ -403,6 +403,10 @@ class SparseMoeBlock(nn.Module):
     argument for the backward pass: "int8" or "e4m3" (8 bits, one scale per
     128 values) or None (all of it)."""
 
+    # for blocks that were pickled before these attributes existed
+    train_kernels = False
+    train_keep: Optional[str] = None
+
     def __init__(self, embed_dim, mlp_ratio=4, num_experts=16, num_experts_per_tok=2, pretraining_tp=2,
                  layer_idx=None, total_layers=None, para_mode: ParaMode = None, *, expert_act="swiglu",
                  shared_expert=True, train_kernels=False, train_keep: Optional[str] = "int8"):

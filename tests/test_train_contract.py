@@ -26,3 +26,12 @@ def test_kernels_switched_on_after_construction(k):
     blk.para_mode = ParaMode(ep=True)
     with pytest.raises(ValueError, match="expert parallelism"):
         blk(torch.zeros(1, 3, 32))
+
+
+def test_block_without_the_attributes():
+    """A block restored from a pickle of before train_kernels existed has neither attribute; it trains as it did."""
+    blk = _block()
+    del blk.__dict__["train_kernels"], blk.__dict__["train_keep"]
+    x = torch.randn(1, 3, 32, requires_grad=True)
+    blk(x).sum().backward()
+    assert x.grad is not None
