@@ -399,7 +399,7 @@ class SparseMoeBlock(nn.Module):
     (the reference's switch, models.py:170).  ``train_kernels=True`` trains
     the experts on the kernels (CUDA tensors, one device, two experts per
     token; the gate stays with torch), in bf16 wherever the eval path would
-    compute in bf16; ``train_keep`` says what they keep of the activation's
+    compute in bf16 (float64 is refused); ``train_keep`` says what they keep of the activation's
     argument for the backward pass: "int8" or "e4m3" (8 bits, one scale per
     128 values) or None (all of it)."""
 
@@ -636,6 +636,10 @@ class SparseMoeBlock(nn.Module):
 
         # the switch may have been set on a block that was built without it
         _check_train_kernels(self.para_mode, topk_idx.shape[-1])
+        params = [p for e in self.experts for p in ExpertPack._params(e)[1]]
+        shared = ExpertPack._params(self.shared_experts)[1] if self.n_shared_experts is not None else ()
+        if any(t.dtype == torch.float64 for t in (hidden_states, *params, *shared)):
+            raise TypeError("train_kernels computes in bf16 or fp32: float64 trains without it")
         if not hidden_states.is_cuda:
             raise RuntimeError("a SparseMoeBlock with train_kernels trains on CUDA tensors only (no CPU fallback)")
         if not self.layer_idx:
@@ -643,13 +647,11 @@ class SparseMoeBlock(nn.Module):
         h = hidden_states.shape[-1]
         x = hidden_states.reshape(-1, h).to(_compute_dtype(hidden_states))
         act, ffn = self.expert_act, self.experts[0].intermediate_size
-        params = [p for e in self.experts for p in ExpertPack._params(e)[1]]
         y = RoutedExperts.apply(x, topk_idx, topk_weight.float(), act, ffn, self.train_keep, *params)
         y = y.view(hidden_states.shape).to(hidden_states.dtype)
         if aux_loss is not None:
             y = AddAuxiliaryLoss.apply(y, aux_loss)
         if self.n_shared_experts is not None:
-            shared = self.shared_experts
-            s = DenseExpert.apply(x, act, shared.intermediate_size, self.train_keep, *ExpertPack._params(shared)[1])
+            s = DenseExpert.apply(x, act, self.shared_experts.intermediate_size, self.train_keep, *shared)
             y = y + s.view(hidden_states.shape).to(hidden_states.dtype)
         return y

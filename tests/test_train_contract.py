@@ -35,3 +35,18 @@ def test_block_without_the_attributes():
     x = torch.randn(1, 3, 32, requires_grad=True)
     blk(x).sum().backward()
     assert x.grad is not None
+
+
+def test_float64_is_refused():
+    """The default loop computes in 64 bits; the kernels have 32 at most and do not pretend otherwise."""
+    with pytest.raises(TypeError, match="float64"):
+        _block(train_kernels=True).double()(torch.zeros(1, 3, 32, dtype=torch.float64))
+    blk = _block(train_kernels=True)
+    blk.experts[1].double()
+    with pytest.raises(TypeError, match="float64"):
+        blk(torch.zeros(1, 3, 32))
+    blk = _block(train_kernels=True)
+    blk.shared_experts.double()
+    with pytest.raises(TypeError, match="float64"):
+        blk(torch.zeros(1, 3, 32))
+    assert _block().double()(torch.zeros(1, 3, 32, dtype=torch.float64)).dtype == torch.float64
