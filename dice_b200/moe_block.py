@@ -400,8 +400,9 @@ class SparseMoeBlock(nn.Module):
     the experts on the kernels (CUDA tensors, one device, two experts per
     token; the gate stays with torch), in bf16 wherever the eval path would
     compute in bf16 (float64 is refused); ``train_keep`` says what they keep of the activation's
-    argument for the backward pass: "int8" or "e4m3" (8 bits, one scale per
-    128 values) or None (all of it)."""
+    argument for the backward pass: None (all of it), or "int8" or "e4m3"
+    (8 bits, one scale per 128 values: half the bytes, and gradients off by
+    what 8 bits cost)."""
 
     # for blocks that were pickled before these attributes existed
     train_kernels = False
@@ -409,7 +410,7 @@ class SparseMoeBlock(nn.Module):
 
     def __init__(self, embed_dim, mlp_ratio=4, num_experts=16, num_experts_per_tok=2, pretraining_tp=2,
                  layer_idx=None, total_layers=None, para_mode: ParaMode = None, *, expert_act="swiglu",
-                 shared_expert=True, train_kernels=False, train_keep: Optional[str] = "int8"):
+                 shared_expert=True, train_kernels=False, train_keep: Optional[str] = None):
         super().__init__()
         assert para_mode is not None
         assert expert_act in ("swiglu", "gelu_tanh")

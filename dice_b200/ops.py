@@ -855,9 +855,9 @@ def _check_ffn(rows, w1, w2, seg_offsets, act, ffn):
 
 
 def grouped_ffn_train(rows: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, seg_offsets: torch.Tensor, act: str, ffn: int,
-                      status: Optional[torch.Tensor] = None, keep: Optional[str] = "int8"):
-    """:func:`grouped_ffn` for training: ``(rows_out, kept)``, where ``kept`` is the activation's argument in 8 bits
-    (``keep`` "int8" or "e4m3") or as it is (None), for :func:`grouped_ffn_backward`.  The first product is rounded to
+                      status: Optional[torch.Tensor] = None, keep: Optional[str] = None):
+    """:func:`grouped_ffn` for training: ``(rows_out, kept)``, where ``kept`` is the activation's argument as it is
+    (``keep`` None) or in 8 bits ("int8" or "e4m3"), for :func:`grouped_ffn_backward`.  The first product is rounded to
     the rows' type before the activation, and the activation before the second product.  bf16, or fp32 with fp32's
     precision (three bf16 planes an operand on the tensor cores, or the CUDA cores where few rows meet a weight)."""
     _check_keep(keep)

@@ -1,7 +1,10 @@
 """What the training path asks of a block and of its callers, as far as no GPU is needed."""
+import inspect
+
 import pytest
 import torch
 
+from dice_b200 import ops
 from dice_b200.moe_block import ParaMode, SparseMoeBlock
 
 
@@ -50,3 +53,8 @@ def test_float64_is_refused():
     with pytest.raises(TypeError, match="float64"):
         blk(torch.zeros(1, 3, 32))
     assert _block().double()(torch.zeros(1, 3, 32, dtype=torch.float64)).dtype == torch.float64
+
+
+def test_nothing_is_quantised_unasked():
+    assert _block(train_kernels=True).train_keep is None
+    assert inspect.signature(ops.grouped_ffn_train).parameters["keep"].default is None
