@@ -122,7 +122,7 @@ extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in,
   int rc = check_product(n_rows, hidden, ffn, n_slabs, n_slabs, dtype);
   if (rc == DICE_OK) rc = check_product(n_rows, static_cast<int>(cols), hidden, n_slabs, n_slabs, dtype);
   if (rc != DICE_OK) return rc;
-  DICE_CHECK_ARG(seg_offsets && dw1 && dw2 && (!glu || dw1_up), DICE_ERR_ARG);
+  DICE_CHECK_ARG(seg_offsets && (!dw1 || (dw2 && (!glu || dw1_up))), DICE_ERR_ARG);
   DICE_CHECK_ARG(keep == DICE_KEEP_NONE || keep == DICE_KEEP_INT8 || keep == DICE_KEEP_E4M3, DICE_ERR_ARG);
   // each product takes the scratch only if it can use it
   auto part = [&](int n_dim, int k_dim, bool weight_gradient) {
@@ -130,8 +130,9 @@ extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in,
                ? scratch
                : nullptr;
   };
-  if (n_rows > 0) {
-    DICE_CHECK_ARG(d_out && rows_in && kept && w1 && w2 && d_pre && a && d_rows && (keep == DICE_KEEP_NONE || scales), DICE_ERR_ARG);
+  // a gradient whose pointer is NULL is not made, and without any there is nothing to do
+  if (n_rows > 0 && (d_rows || dw2)) {
+    DICE_CHECK_ARG(d_out && rows_in && kept && w1 && w2 && d_pre && a && (keep == DICE_KEEP_NONE || scales), DICE_ERR_ARG);
     DICE_CHECK_ARG(da || dtype == DICE_BF16, DICE_ERR_ARG);  // bf16: the activation's gradient stays in the epilogue
     DICE_CHECK_ARG(dice_aligned16(d_out) && dice_aligned16(kept) && dice_aligned16(w2) && dice_aligned16(d_pre) && dice_aligned16(a),
                    DICE_ERR_ALIGN);
@@ -147,12 +148,15 @@ extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in,
     }
   }
   const int c = static_cast<int>(cols);
-  if ((rc = dice_grouped_wgrad(d_out, a, n_rows, hidden, ffn, seg_offsets, n_slabs, 0, dtype, dw2, nullptr,
+  if (dw2 &&
+      (rc = dice_grouped_wgrad(d_out, a, n_rows, hidden, ffn, seg_offsets, n_slabs, 0, dtype, dw2, nullptr,
                                part(hidden, ffn, true), scratch_bytes, status, stream)) != DICE_OK)
     return rc;
-  if ((rc = dice_grouped_dgrad(d_pre, n_rows, c, w1, n_slabs, hidden, seg_offsets, nullptr, n_slabs, dtype, d_rows,
+  if (d_rows &&
+      (rc = dice_grouped_dgrad(d_pre, n_rows, c, w1, n_slabs, hidden, seg_offsets, nullptr, n_slabs, dtype, d_rows,
                                part(c, hidden, false), scratch_bytes, status, stream)) != DICE_OK)
     return rc;
+  if (!dw1) return DICE_OK;
   return dice_grouped_wgrad(d_pre, rows_in, n_rows, c, hidden, seg_offsets, n_slabs, glu ? ffn : 0, dtype, dw1, dw1_up,
                             part(c, hidden, true), scratch_bytes, status, stream);
 }

@@ -34,11 +34,17 @@ def _stack(act: str, ffn: int, dtype: torch.dtype, params: Sequence[torch.Tensor
     return torch.stack([p.to(dtype) for p in fc1]), torch.stack([p.to(dtype) for p in fc2])
 
 
-def _param_grads(act: str, dw1, dw2: torch.Tensor, needs: Sequence[bool], params_dtype):
-    """Stacked gradients back to one per parameter, in the parameters' order."""
-    stacks = (*dw1, dw2) if act == "swiglu" else (dw1, dw2)
-    grads = [g for per_expert in zip(*(s.unbind(0) for s in stacks)) for g in per_expert]
-    return [g.to(dt) if need else None for g, need, dt in zip(grads, needs, params_dtype)]
+def _ffn_grads(ctx, d_out, rows, kept, w1, w2, seg, want_rows: bool, needs: Sequence[bool]):
+    """The rows' gradient (None unless wanted) and the parameters', one each in their order; no product is made for
+    gradients that nobody needs (frozen experts)."""
+    n_firsts = 2 if ctx.act == "swiglu" else 1  # matrices of the first product
+    per = n_firsts + 1
+    want_w1, want_w2 = any(n for i, n in enumerate(needs) if i % per != n_firsts), any(needs[n_firsts::per])
+    d_rows, dw1, dw2 = ops.grouped_ffn_backward(d_out, rows, kept, w1, w2, seg, ctx.act, ctx.ffn, want_rows=want_rows,
+                                                want_w1=want_w1, want_w2=want_w2)
+    stacks = [*(dw1 if ctx.act == "swiglu" and want_w1 else [dw1] * n_firsts), dw2]
+    grads = [stacks[i % per][i // per].to(dt) if need else None for i, (need, dt) in enumerate(zip(needs, ctx.param_dtypes))]
+    return d_rows, grads
 
 
 class RoutedExperts(torch.autograd.Function):
@@ -67,10 +73,12 @@ class RoutedExperts(torch.autograd.Function):
         x, pos, seg, weights, rows_out, w1, w2, codes, scales = ctx.saved_tensors
         n = x.shape[0]
         d_out, d_weights = ops.combine_backward(dy.contiguous(), rows_out, pos, weights)
+        want_x, needs = ctx.needs_input_grad[0], ctx.needs_input_grad[6:]
+        if not (want_x or any(needs)):
+            return (None, None, d_weights, None, None, None, *[None] * len(needs))
         rows = ops.permute_rows(x, pos.view(-1), 2)
-        d_rows, dw1, dw2 = ops.grouped_ffn_backward(d_out, rows, ops.KeptAct(codes, scales), w1, w2, seg, ctx.act, ctx.ffn)
-        dx = ops.unpermute_combine(d_rows, pos[:, 0], d_rows, pos[:, 1], None, None, n)
-        grads = _param_grads(ctx.act, dw1, dw2, ctx.needs_input_grad[6:], ctx.param_dtypes)
+        d_rows, grads = _ffn_grads(ctx, d_out, rows, ops.KeptAct(codes, scales), w1, w2, seg, want_x, needs)
+        dx = ops.unpermute_combine(d_rows, pos[:, 0], d_rows, pos[:, 1], None, None, n) if want_x else None
         return (dx, None, d_weights, None, None, None, *grads)
 
 
@@ -92,5 +100,6 @@ class DenseExpert(torch.autograd.Function):
     def backward(ctx, dy):
         _first_order_only()
         x, seg, w1, w2, codes, scales = ctx.saved_tensors
-        dx, dw1, dw2 = ops.grouped_ffn_backward(dy.contiguous(), x, ops.KeptAct(codes, scales), w1, w2, seg, ctx.act, ctx.ffn)
-        return (dx, None, None, None, *_param_grads(ctx.act, dw1, dw2, ctx.needs_input_grad[4:], ctx.param_dtypes))
+        dx, grads = _ffn_grads(ctx, dy.contiguous(), x, ops.KeptAct(codes, scales), w1, w2, seg, ctx.needs_input_grad[0],
+                               ctx.needs_input_grad[4:])
+        return (dx, None, None, None, *grads)

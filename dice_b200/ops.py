@@ -892,33 +892,41 @@ def grouped_ffn_train(rows: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, se
 
 
 def grouped_ffn_backward(d_out: torch.Tensor, rows: torch.Tensor, kept: KeptAct, w1: torch.Tensor, w2: torch.Tensor,
-                         seg_offsets: torch.Tensor, act: str, ffn: int, status: Optional[torch.Tensor] = None):
+                         seg_offsets: torch.Tensor, act: str, ffn: int, status: Optional[torch.Tensor] = None,
+                         want_rows: bool = True, want_w1: bool = True, want_w2: bool = True):
     """Backward pass of :func:`grouped_ffn_train` from what it kept: ``(d_rows, dw1, dw2)``; for SwiGLU ``dw1`` is the
-    pair of the gate and the up projections' gradients ``[S, ffn, h]``."""
+    pair of the gate and the up projections' gradients ``[S, ffn, h]``.  A gradient that is not wanted is not made, and
+    None in its place (dw2 comes along where dw1 is wanted)."""
     codes, scales = kept
     index = _one_device(d_out, rows, codes, scales, w1, w2, seg_offsets, status)
     if index != _current_device():
         with torch.cuda.device(index):
-            return grouped_ffn_backward(d_out, rows, kept, w1, w2, seg_offsets, act, ffn, status)
+            return grouped_ffn_backward(d_out, rows, kept, w1, w2, seg_offsets, act, ffn, status, want_rows, want_w1, want_w2)
     code = _dtype_code(rows)
     n_slabs, h, cols = _check_ffn(rows, w1, w2, seg_offsets, act, ffn)
     n_rows, dt = rows.shape[0], rows.dtype
     assert d_out.shape == rows.shape and d_out.dtype == dt
     keep = _check_kept(codes, scales, n_rows, cols, dt)
     d_out, rows = d_out.contiguous(), rows.contiguous()
+    want_w2 = want_w2 or want_w1
+    if not (want_rows or want_w2):
+        return None, None, None
     da = _new((n_rows, ffn), dt, index) if code == DICE_F32 else None  # bf16: stays in the product's epilogue
-    d_pre, a, d_rows = _new((n_rows, cols), dt, index), _new((n_rows, ffn), dt, index), _new((n_rows, h), dt, index)
-    dw2, dw1 = _new((n_slabs, h, ffn), dt, index), _new((n_slabs, ffn, h), dt, index)
-    dw1_up = _new((n_slabs, ffn, h), dt, index) if act == "swiglu" else None
+    d_pre, a = _new((n_rows, cols), dt, index), _new((n_rows, ffn), dt, index)
+    d_rows = _new((n_rows, h), dt, index) if want_rows else None
+    dw2 = _new((n_slabs, h, ffn), dt, index) if want_w2 else None
+    dw1 = _new((n_slabs, ffn, h), dt, index) if want_w1 else None
+    dw1_up = _new((n_slabs, ffn, h), dt, index) if want_w1 and act == "swiglu" else None
     lib = _lib.load()
     held, scratch, n_bytes = _split_scratch(index, max(
-        _split_bytes(lib, n_rows, n, k, n_slabs, product, code)
-        for n, k in ((h, ffn), (cols, h)) for product in (PRODUCT_DGRAD, PRODUCT_WGRAD)))
+        _split_bytes(lib, n_rows, n, k, n_slabs, product, code) if made else 0
+        for n, k, product, made in ((h, ffn, PRODUCT_DGRAD, code == DICE_F32), (h, ffn, PRODUCT_WGRAD, want_w2),
+                                    (cols, h, PRODUCT_DGRAD, want_rows), (cols, h, PRODUCT_WGRAD, want_w1))))
     _lib.check(
         lib.dice_grouped_ffn_backward(
             d_out.data_ptr(), rows.data_ptr(), codes.data_ptr(), _ptr(scales), n_rows, h, ffn, ACT_CODES[act], keep, code,
             w1.data_ptr(), w2.data_ptr(), n_slabs, seg_offsets.data_ptr(), _ptr(da), d_pre.data_ptr(), a.data_ptr(),
-            d_rows.data_ptr(), dw1.data_ptr(), _ptr(dw1_up), dw2.data_ptr(), scratch, n_bytes, _status_ptr(status, index),
+            _ptr(d_rows), _ptr(dw1), _ptr(dw1_up), _ptr(dw2), scratch, n_bytes, _status_ptr(status, index),
             _stream_of(index),
         ),
         "dice_grouped_ffn_backward",

@@ -414,7 +414,9 @@ DICE_API int dice_grouped_ffn_train(const void* rows_in, int64_t n_rows, int hid
  *   d_pre [n_rows, columns of the first product], a [n_rows, ffn] and, in fp32,
  *   da [n_rows, ffn] are scratch (bf16: da may be NULL); `scratch` as for the
  *   gradients (the largest of what dice_grouped_scratch_bytes says for the
- *   weight and the input gradients of (hidden, ffn) and (columns, hidden)). */
+ *   weight and the input gradients of (hidden, ffn) and (columns, hidden)).
+ *   A gradient whose pointer is NULL is not made (frozen weights, inputs without
+ *   a gradient): d_rows, dw1, or dw1 and dw2. */
 DICE_API int dice_grouped_ffn_backward(const void* d_out, const void* rows_in, const void* kept, const float* scales,
                               int64_t n_rows, int hidden, int ffn, int act, int keep, int dtype, const void* w1,
                               const void* w2, int n_slabs, const int32_t* seg_offsets, void* da, void* d_pre,

@@ -1,0 +1,82 @@
+"""The training operators where a gradient is not wanted, an argument is at its limit or a value at the end of its range.
+
+Bounds are those of test_train_ops_gpu: half a step of the type for a rounding, K 2^-23 of the products' magnitudes for a
+sum of K in fp32.
+"""
+import pytest
+import torch
+
+from dice_b200 import _lib, ops
+from dice_b200.moe_block import ParaMode, SparseMoeBlock
+
+pytestmark = pytest.mark.gpu
+D = torch.float64
+
+
+def _block(dev, act, dtype, **kw):
+    torch.manual_seed(0)
+    blk = SparseMoeBlock(64, 2, 4, 2, 1, 0, 1, ParaMode(), expert_act=act, train_kernels=True, **kw)
+    return blk.to(dev, dtype).train()
+
+
+def _launches(fn):
+    before = _lib.load().dice_kernel_launches()
+    out = fn()
+    return out, _lib.load().dice_kernel_launches() - before
+
+
+# ---- gradients that nobody needs -----------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("act", ["swiglu", "gelu_tanh"])
+def test_frozen_weights_cost_no_products(cuda_device, act, dtype):
+    """With every expert frozen the backward pass makes the rows' gradients alone: two weight gradients fewer for the
+    routed and two for the shared experts.  With inputs that need none, the rows' own."""
+    x = torch.randn(1, 200, 64, device=cuda_device, dtype=dtype)
+    dy = torch.randn_like(x)
+    blk = _block(cuda_device, act, dtype)
+    firsts = [n for n, _ in blk.named_parameters() if "expert" in n and ("gate_proj" in n or "up_proj" in n or "fc1" in n)]
+    seconds = [n for n, _ in blk.named_parameters() if "expert" in n and n not in firsts]
+
+    def step(frozen, want_x):
+        params = dict(blk.named_parameters())
+        for n, p in params.items():
+            p.requires_grad_(n not in frozen)
+            p.grad = None
+        xx = x.clone().requires_grad_(want_x)
+        y = blk(xx)
+        _, n_launches = _launches(lambda: y.backward(dy))
+        return n_launches, xx.grad, {n: p.grad for n, p in params.items()}
+
+    full, dx, grads = step([], True)
+    for frozen, want_x, fewer in [(firsts + seconds, True, 4), (firsts, True, 2), (seconds, True, 0), ([], False, 3),
+                                  (firsts, False, 5)]:
+        n_launches, dx2, grads2 = step(frozen, want_x)
+        if dtype == torch.bfloat16:  # (fp32 has further launches for its operands)
+            assert n_launches == full - fewer, (frozen, want_x)
+        else:
+            assert n_launches <= full - fewer
+        assert torch.equal(dx, dx2) if want_x else dx2 is None
+        for n, g in grads2.items():
+            assert g is None if n in frozen else torch.equal(g, grads[n]), n
+    # the gate alone: its weights' gradient needs the combine's, and no product
+    n_launches, _, grads2 = step(firsts + seconds, False)
+    assert n_launches == 1 and torch.equal(grads2["gate.weight"], grads["gate.weight"])
+
+
+def test_ffn_backward_of_what_is_wanted(cuda_device):
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=cuda_device).to(torch.bfloat16)  # noqa: E731
+    rows, d_out, w1, w2 = rand(90, 64), rand(90, 64), rand(2, 256, 64), rand(2, 64, 128)
+    seg = torch.tensor([0, 50, 90], dtype=torch.int32, device=cuda_device)
+    _, kept = ops.grouped_ffn_train(rows, w1, w2, seg, "swiglu", 128)
+    back = lambda **kw: ops.grouped_ffn_backward(d_out, rows, kept, w1, w2, seg, "swiglu", 128, **kw)  # noqa: E731
+    d_rows, (gate, up), dw2 = back()
+    assert back(want_rows=False, want_w1=False, want_w2=False) == (None, None, None)
+    a = back(want_w1=False, want_w2=False)
+    assert torch.equal(a[0], d_rows) and a[1] is None and a[2] is None
+    a = back(want_rows=False, want_w1=False)
+    assert a[0] is None and a[1] is None and torch.equal(a[2], dw2)
+    a = back(want_rows=False, want_w2=False)  # dw2 comes along
+    assert a[0] is None and torch.equal(a[1][0], gate) and torch.equal(a[1][1], up) and torch.equal(a[2], dw2)
