@@ -87,8 +87,8 @@ extern "C" int dice_grouped_ffn_train(const void* rows_in, int64_t n_rows, int h
   DICE_CHECK_ARG(dice_aligned16(rows_in) && dice_aligned16(w1) && dice_aligned16(w2) && dice_aligned16(pre) &&
                      dice_aligned16(a) && dice_aligned16(rows_out),
                  DICE_ERR_ALIGN);
-  DICE_CHECK_ARG(keep == DICE_KEEP_NONE || keep == DICE_KEEP_INT8 || keep == DICE_KEEP_E4M3, DICE_ERR_ARG);
-  DICE_CHECK_ARG(keep == DICE_KEEP_NONE || (codes && scales), DICE_ERR_ARG);
+  DICE_CHECK_ARG(keep == DICE_KEEP_NONE || keep == DICE_KEEP_INT8 || keep == DICE_KEEP_E4M3 || keep == DICE_KEEP_NOTHING, DICE_ERR_ARG);
+  DICE_CHECK_ARG(keep == DICE_KEEP_NONE || keep == DICE_KEEP_NOTHING || (codes && scales), DICE_ERR_ARG);
   DICE_CHECK_ARG(dice_aligned16(codes), DICE_ERR_ALIGN);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == DICE_BF16) {
@@ -105,7 +105,7 @@ extern "C" int dice_grouped_ffn_train(const void* rows_in, int64_t n_rows, int h
     return dice_internal_simt_linear(in, n_rows, k_dim, w, n_slabs, n_dim, seg_offsets, nullptr, n_seg, out, status, s);
   };
   if ((rc = linear(rows_in, hidden, w1, static_cast<int>(cols), pre)) != DICE_OK) return rc;
-  if ((rc = dice_act_keep(pre, n_rows, ffn, act, keep, dtype, a, codes, scales, stream)) != DICE_OK) return rc;
+  if ((rc = dice_act_keep(pre, n_rows, ffn, act, keep == DICE_KEEP_NOTHING ? DICE_KEEP_NONE : keep, dtype, a, codes, scales, stream)) != DICE_OK) return rc;
   return linear(a, ffn, w2, hidden, rows_out);
 }
 

@@ -202,7 +202,7 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
                                           const int64_t (&dst_row)[4], Staging& stager, const CUtensorMap* tm_out,
                                           const CUtensorMap* tm_act, const CUtensorMap* tm_codes, float* exchange, uint32_t bar,
                                           uint32_t phase, volatile uint32_t* abort_flag, Fetch fetch, Store store_bf16) {
-  constexpr bool GLU = ACT == DICE_ACT_SWIGLU;
+  constexpr bool GLU = ACT == DICE_ACT_SWIGLU, CODES = KEEP == DICE_KEEP_INT8 || KEEP == DICE_KEEP_E4M3;
   // this warp's first activation column, and how many of its 64 (GELU: 128) exist
   const int act0 = GLU ? nb * 128 + half * 64 : nb * 256 + half * 128;
   int valid = p.ffn - act0;
@@ -219,7 +219,7 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         w[q][j] = 2 * j < left ? pack_bf16x2(v[2 * j], v[2 * j + 1]) : 0u;  // (valid is a multiple of 8)
-        if (KEEP != DICE_KEEP_NONE) {
+        if (CODES) {
           uint32_t& m = most2[GLU ? q >> 1 : 0];
           asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[q][j] & 0x7fff7fffu));
         }
@@ -230,7 +230,7 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
     }
   }
   float scale[2], factor[2];
-  if (KEEP != DICE_KEEP_NONE) {
+  if (CODES) {
     float most[2];
 #pragma unroll
     for (int g = 0; g < 2; ++g) most[g] = max_nan(bf16lo_to_f32(most2[g]), bf16hi_to_f32(most2[g]));
@@ -279,7 +279,7 @@ __device__ __forceinline__ void keep_tile(const TrainGemm& p, int nb, int quad, 
         store_bf16(o, tm_out, p.out, p.arg_cols, GLU ? nb * 256 + (q >> 1) * 128 + half * 64 + (q & 1) * 32 : act0 + q * 32, left);
       }
     }
-  } else {
+  } else if (CODES) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {  // 64 codes each
       const int left = GLU ? 64 : valid - g * 64;
@@ -1087,6 +1087,7 @@ template <int ACT>
 int run_epilogue(bool back, int keep, const CUtensorMap& tm_a, const CUtensorMap& tm_b, const CUtensorMap* st, const TrainGemm& p, cudaStream_t s) {
   switch (keep) {
     case DICE_KEEP_INT8: return back ? run_back<ACT, DICE_KEEP_INT8>(tm_a, tm_b, st, p, s) : run_keep<ACT, DICE_KEEP_INT8>(tm_a, tm_b, st, p, s);
+    case DICE_KEEP_NOTHING: return run_keep<ACT, DICE_KEEP_NOTHING>(tm_a, tm_b, st, p, s);  // (a backward pass has something)
     case DICE_KEEP_E4M3: return back ? run_back<ACT, DICE_KEEP_E4M3>(tm_a, tm_b, st, p, s) : run_keep<ACT, DICE_KEEP_E4M3>(tm_a, tm_b, st, p, s);
     default: return back ? run_back<ACT, DICE_KEEP_NONE>(tm_a, tm_b, st, p, s) : run_keep<ACT, DICE_KEEP_NONE>(tm_a, tm_b, st, p, s);
   }
@@ -1115,7 +1116,7 @@ int dice_internal_tc_keep(const void* rows, int64_t n_rows, int hidden, int ffn,
   stores[0] = stores[2] = stores[1];
   p.codes_tma = p.arg_cols % 16 == 0;
   if (rc == DICE_OK && keep == DICE_KEEP_NONE) rc = encode_store_map(&stores[0], pre, n_rows, p.arg_cols, 2);
-  if (rc == DICE_OK && keep != DICE_KEEP_NONE && p.codes_tma) rc = encode_store_map(&stores[2], codes, n_rows, p.arg_cols, 1);
+  if (rc == DICE_OK && (keep == DICE_KEEP_INT8 || keep == DICE_KEEP_E4M3) && p.codes_tma) rc = encode_store_map(&stores[2], codes, n_rows, p.arg_cols, 1);
   if (rc != DICE_OK) return rc;
   p.seg_offsets = seg_offsets;
   p.n_seg = n_seg;

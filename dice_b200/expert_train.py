@@ -47,6 +47,11 @@ def _ffn_grads(ctx, d_out, rows, kept, w1, w2, seg, want_rows: bool, needs: Sequ
     return d_rows, grads
 
 
+def without_grad(*tensors: torch.Tensor):
+    """Under torch.no_grad() autograd functions still see which inputs require gradients; without that, nothing is kept."""
+    return tensors if torch.is_grad_enabled() else tuple(t.detach() for t in tensors)
+
+
 class RoutedExperts(torch.autograd.Function):
     """``y[t] = sum_s weights[t, s] * expert[idx[t, s]](x[t])`` with gradients for ``x``, ``weights`` and every expert
     parameter.  ``x [N, h]`` bf16 or fp32, ``idx`` int64 ``[N, 2]``, ``weights`` fp32 ``[N, 2]``."""
@@ -60,10 +65,12 @@ class RoutedExperts(torch.autograd.Function):
         w1, w2 = _stack(act, ffn, x.dtype, params)
         pos, seg, _ = ops.permute_plan(idx.reshape(-1), n_experts)
         rows = ops.permute_rows(x, pos, 2)
-        rows_out, kept = ops.grouped_ffn_train(rows, w1, w2, seg, act, ffn, keep=keep)
+        trains = any(ctx.needs_input_grad)
+        rows_out, kept = ops.grouped_ffn_train(rows, w1, w2, seg, act, ffn, keep=keep, want_kept=trains)
         pos = pos.view(n, 2)
         y = ops.unpermute_combine(rows_out, pos[:, 0], rows_out, pos[:, 1], weights[:, 0], weights[:, 1], n)
-        ctx.save_for_backward(x, pos, seg, weights, rows_out, w1, w2, *kept)
+        if trains:
+            ctx.save_for_backward(x, pos, seg, weights, rows_out, w1, w2, *kept)
         ctx.act, ctx.ffn, ctx.param_dtypes = act, ffn, [p.dtype for p in params]
         return y
 
@@ -91,8 +98,10 @@ class DenseExpert(torch.autograd.Function):
         w1, w2 = _stack(act, ffn, x.dtype, params)
         seg = torch.zeros(2, dtype=torch.int32, device=x.device)
         seg[1:].fill_(x.shape[0])
-        y, kept = ops.grouped_ffn_train(x, w1, w2, seg, act, ffn, keep=keep)
-        ctx.save_for_backward(x, seg, w1, w2, *kept)
+        trains = any(ctx.needs_input_grad)
+        y, kept = ops.grouped_ffn_train(x, w1, w2, seg, act, ffn, keep=keep, want_kept=trains)
+        if trains:
+            ctx.save_for_backward(x, seg, w1, w2, *kept)
         ctx.act, ctx.ffn, ctx.param_dtypes = act, ffn, [p.dtype for p in params]
         return y
 

@@ -633,7 +633,7 @@ class SparseMoeBlock(nn.Module):
 
     def _experts_train(self, hidden_states, topk_idx, topk_weight, aux_loss):
         """The experts' part of the training forward on the kernels."""
-        from .expert_train import DenseExpert, RoutedExperts
+        from .expert_train import DenseExpert, RoutedExperts, without_grad
 
         # the switch may have been set on a block that was built without it
         _check_train_kernels(self.para_mode, topk_idx.shape[-1])
@@ -648,11 +648,12 @@ class SparseMoeBlock(nn.Module):
         h = hidden_states.shape[-1]
         x = hidden_states.reshape(-1, h).to(_compute_dtype(hidden_states))
         act, ffn = self.expert_act, self.experts[0].intermediate_size
-        y = RoutedExperts.apply(x, topk_idx, topk_weight.float(), act, ffn, self.train_keep, *params)
+        x, weights = without_grad(x, topk_weight.float())
+        y = RoutedExperts.apply(x, topk_idx, weights, act, ffn, self.train_keep, *without_grad(*params))
         y = y.view(hidden_states.shape).to(hidden_states.dtype)
         if aux_loss is not None:
             y = AddAuxiliaryLoss.apply(y, aux_loss)
         if self.n_shared_experts is not None:
-            s = DenseExpert.apply(x, act, self.shared_experts.intermediate_size, self.train_keep, *shared)
+            s = DenseExpert.apply(x, act, self.shared_experts.intermediate_size, self.train_keep, *without_grad(*shared))
             y = y + s.view(hidden_states.shape).to(hidden_states.dtype)
         return y

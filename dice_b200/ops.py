@@ -561,6 +561,7 @@ def shared_expert_can_ride() -> bool:
 # --------------------------------------------------------------------------- #
 
 KEEP_CODES = {None: 0, "int8": 1, "e4m3": 2}
+KEEP_NOTHING = 3  # no backward pass will follow
 KEEP_DTYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
 KEEP_GROUP = 128  # columns that share a scale
 
@@ -855,36 +856,41 @@ def _check_ffn(rows, w1, w2, seg_offsets, act, ffn):
 
 
 def grouped_ffn_train(rows: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, seg_offsets: torch.Tensor, act: str, ffn: int,
-                      status: Optional[torch.Tensor] = None, keep: Optional[str] = None):
+                      status: Optional[torch.Tensor] = None, keep: Optional[str] = None, want_kept: bool = True):
     """:func:`grouped_ffn` for training: ``(rows_out, kept)``, where ``kept`` is the activation's argument as it is
-    (``keep`` None) or in 8 bits ("int8" or "e4m3"), for :func:`grouped_ffn_backward`.  The first product is rounded to
+    (``keep`` None) or in 8 bits ("int8" or "e4m3"), for :func:`grouped_ffn_backward`; None without ``want_kept``, when no
+    backward pass will follow.  The first product is rounded to
     the rows' type before the activation, and the activation before the second product.  bf16, or fp32 with fp32's
     precision (three bf16 planes an operand on the tensor cores, or the CUDA cores where few rows meet a weight)."""
     _check_keep(keep)
     index = _one_device(rows, w1, w2, seg_offsets, status)
     if index != _current_device():
         with torch.cuda.device(index):
-            return grouped_ffn_train(rows, w1, w2, seg_offsets, act, ffn, status, keep)
+            return grouped_ffn_train(rows, w1, w2, seg_offsets, act, ffn, status, keep, want_kept)
     code = _dtype_code(rows)
     n_slabs, h, cols = _check_ffn(rows, w1, w2, seg_offsets, act, ffn)
     rows = rows.contiguous()
     n_rows, dt = rows.shape[0], rows.dtype
     # bf16 makes the activation and the 8-bit codes in the first product's epilogue
-    pre = _new((n_rows, cols), dt, index) if keep is None or code == DICE_F32 else None
+    pre = _new((n_rows, cols), dt, index) if (keep is None and want_kept) or code == DICE_F32 else None
     a = _new((n_rows, ffn), dt, index)
     rows_out = _new((n_rows, h), dt, index)
-    if keep is None:
-        kept = KeptAct(pre, None)
+    codes = scales = kept = None
+    if not want_kept:
+        keep_code = KEEP_NOTHING
+    elif keep is None:
+        keep_code, kept = KEEP_CODES[None], KeptAct(pre, None)
     else:
-        kept = KeptAct(_new((n_rows, cols), KEEP_DTYPES[keep], index), _new((n_rows, _groups(cols)), torch.float32, index))
+        keep_code = KEEP_CODES[keep]
+        codes, scales = kept = KeptAct(_new((n_rows, cols), KEEP_DTYPES[keep], index),
+                                       _new((n_rows, _groups(cols)), torch.float32, index))
     lib = _lib.load()
     held, scratch, n_bytes = _split_scratch(index, 0 if code == DICE_BF16 else max(
         _split_bytes(lib, n_rows, n, k, n_slabs, PRODUCT_LINEAR, code) for n, k in ((cols, h), (h, ffn))))
     _lib.check(
         lib.dice_grouped_ffn_train(
-            rows.data_ptr(), n_rows, h, ffn, ACT_CODES[act], KEEP_CODES[keep], code, w1.data_ptr(), w2.data_ptr(), n_slabs,
-            seg_offsets.data_ptr(), n_slabs, _ptr(pre), a.data_ptr(), None if keep is None else kept.codes.data_ptr(),
-            _ptr(kept.scales), rows_out.data_ptr(), scratch, n_bytes, _status_ptr(status, index), _stream_of(index),
+            rows.data_ptr(), n_rows, h, ffn, ACT_CODES[act], keep_code, code, w1.data_ptr(), w2.data_ptr(), n_slabs,
+            seg_offsets.data_ptr(), n_slabs, _ptr(pre), a.data_ptr(), _ptr(codes), _ptr(scales), rows_out.data_ptr(), scratch, n_bytes, _status_ptr(status, index), _stream_of(index),
         ),
         "dice_grouped_ffn_train",
     )

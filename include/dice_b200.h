@@ -363,6 +363,7 @@ DICE_API int dice_grouped_wgrad(const void* dy, const void* x, int64_t n_rows, i
 #define DICE_KEEP_NONE 0 /* the argument itself                                   */
 #define DICE_KEEP_INT8 1 /* 8-bit integers, one fp32 scale per row and 128 columns */
 #define DICE_KEEP_E4M3 2 /* 8-bit floats (e4m3), the same scales                  */
+#define DICE_KEEP_NOTHING 3 /* dice_grouped_ffn_train alone: no backward pass follows */
 
 /* The activation, and its argument in 8 bits:
  *   SWIGLU     pre [n_rows, dice_w13_rows(ffn)] in the packed order (gate and up
@@ -400,6 +401,7 @@ DICE_API int dice_combine_backward(const void* dout, const void* rows_out, const
  * what is kept of its argument, the second product.
  *   pre   [n_rows, columns of the first product]: what is kept with keep ==
  *         NONE, else scratch in fp32 and not used in bf16 (may be NULL)
+ *   codes, scales: with keep == NONE or NOTHING not used (may be NULL)
  *   a     [n_rows, ffn] scratch
  *   scratch  the larger of what dice_grouped_scratch_bytes says for the forward
  *         products (columns, hidden) and (hidden, ffn) */

@@ -80,3 +80,39 @@ def test_ffn_backward_of_what_is_wanted(cuda_device):
     assert a[0] is None and a[1] is None and torch.equal(a[2], dw2)
     a = back(want_rows=False, want_w2=False)  # dw2 comes along
     assert a[0] is None and torch.equal(a[1][0], gate) and torch.equal(a[1][1], up) and torch.equal(a[2], dw2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("act", ["swiglu", "gelu_tanh"])
+@pytest.mark.parametrize("ffn", [64, 200, 392])
+def test_nothing_kept_where_nothing_follows(cuda_device, act, dtype, ffn):
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=cuda_device).to(dtype)  # noqa: E731
+    cols = ops.act_columns(act, ffn)
+    rows, w1, w2 = rand(333, 72), rand(3, cols, 72), rand(3, 72, ffn)
+    seg = torch.tensor([0, 300, 300, 333], dtype=torch.int32, device=cuda_device)
+    for keep in (None, "int8", "e4m3"):
+        out, kept = ops.grouped_ffn_train(rows, w1, w2, seg, act, ffn, keep=keep)
+        out2, nothing = ops.grouped_ffn_train(rows, w1, w2, seg, act, ffn, keep=keep, want_kept=False)
+        assert kept is not None and nothing is None and torch.equal(out, out2)
+    ops.check_status(ops.device_status(cuda_device))
+
+
+@pytest.mark.parametrize("keep", [None, "int8"])
+def test_no_grad_in_training_mode_keeps_nothing(cuda_device, keep, monkeypatch):
+    """The same bits as with gradients, and no kept argument."""
+    blk = _block(cuda_device, "swiglu", torch.bfloat16, train_keep=keep)
+    x = torch.randn(1, 100, 64, device=cuda_device, dtype=torch.bfloat16)
+    want, real = blk(x).detach(), ops.grouped_ffn_train
+    wanted = []
+
+    def spy(*args, **kw):
+        wanted.append(kw["want_kept"])
+        return real(*args, **kw)
+
+    monkeypatch.setattr(ops, "grouped_ffn_train", spy)
+    with torch.no_grad():
+        assert torch.equal(blk(x), want)
+    assert wanted == [False, False]
+    blk(x).sum().backward()
+    assert wanted[2:] == [True, True]
