@@ -25,7 +25,8 @@ extern "C" size_t dice_grouped_scratch_bytes(int64_t n_rows, int n_dim, int k_di
       check_product(n_rows, n_dim, k_dim, n_slabs, 0, dtype) != DICE_OK)
     return 0;
   if (dtype == DICE_F32) return dice_internal_f32_bytes(product, n_rows, n_dim, k_dim, n_slabs);
-  return product == DICE_PRODUCT_LINEAR ? 0 : dice_internal_split_bytes(n_rows, n_dim, k_dim, n_slabs, product == DICE_PRODUCT_WGRAD);
+  if (product == DICE_PRODUCT_LINEAR || (product == DICE_PRODUCT_DGRAD && n_rows <= kThinTotal)) return 0;
+  return dice_internal_split_bytes(n_rows, n_dim, k_dim, n_slabs, product == DICE_PRODUCT_WGRAD);
 }
 
 extern "C" int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, const void* w, int n_slabs, int k_dim,
@@ -40,10 +41,12 @@ extern "C" int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, con
   if (dtype == DICE_BF16 && n_rows <= kThinTotal)
     return dice_internal_thin_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dx, status,
                                     static_cast<cudaStream_t>(stream));
+  // a product that has no use for scratch takes whatever it is given, and leaves it alone
+  if (dice_grouped_scratch_bytes(n_rows, n_dim, k_dim, n_slabs, DICE_PRODUCT_DGRAD, dtype) == 0) scratch = nullptr;
   if (dtype == DICE_BF16)
     return dice_internal_tc_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dx, scratch,
                                   scratch_bytes, status, static_cast<cudaStream_t>(stream));
-  if (scratch != nullptr && dice_internal_f32_bytes(DICE_PRODUCT_DGRAD, n_rows, n_dim, k_dim, n_slabs) > 0)
+  if (scratch != nullptr)
     return dice_internal_f32_product(DICE_PRODUCT_DGRAD, dy, w, n_rows, n_dim, k_dim, n_slabs, seg_offsets, seg_slab, n_seg, 0, dx,
                                      nullptr, scratch, scratch_bytes, status, static_cast<cudaStream_t>(stream));
   return dice_internal_simt_dgrad(dy, n_rows, n_dim, w, n_slabs, k_dim, seg_offsets, seg_slab, n_seg, dx, status,
@@ -59,10 +62,11 @@ extern "C" int dice_grouped_wgrad(const void* dy, const void* x, int64_t n_rows,
   DICE_CHECK_ARG(gate_up == 0 || (gate_up % 8 == 0 && static_cast<int64_t>(n_dim) == dice_w13_rows(gate_up)), DICE_ERR_SHAPE);
   DICE_CHECK_ARG(seg_offsets && dw && (gate_up == 0 || dw_up) && (n_rows == 0 || (dy && x)), DICE_ERR_ARG);
   DICE_CHECK_ARG(dice_aligned16(dy) && dice_aligned16(x) && dice_aligned16(dw) && dice_aligned16(dw_up), DICE_ERR_ALIGN);
+  if (dice_grouped_scratch_bytes(n_rows, n_dim, k_dim, n_slabs, DICE_PRODUCT_WGRAD, dtype) == 0) scratch = nullptr;
   if (dtype == DICE_BF16)
     return dice_internal_tc_wgrad(dy, x, n_rows, n_dim, k_dim, seg_offsets, n_slabs, gate_up, dw, dw_up, scratch,
                                   scratch_bytes, status, static_cast<cudaStream_t>(stream));
-  if (scratch != nullptr && n_rows > 0 && dice_internal_f32_bytes(DICE_PRODUCT_WGRAD, n_rows, n_dim, k_dim, n_slabs) > 0)
+  if (scratch != nullptr)
     return dice_internal_f32_product(DICE_PRODUCT_WGRAD, dy, x, n_rows, n_dim, k_dim, n_slabs, seg_offsets, nullptr, n_slabs, gate_up,
                                      dw, dw_up, scratch, scratch_bytes, status, static_cast<cudaStream_t>(stream));
   return dice_internal_simt_wgrad(dy, x, n_rows, n_dim, k_dim, seg_offsets, n_slabs, gate_up, dw, dw_up, status,
@@ -124,12 +128,6 @@ extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in,
   if (rc != DICE_OK) return rc;
   DICE_CHECK_ARG(seg_offsets && (!dw1 || (dw2 && (!glu || dw1_up))), DICE_ERR_ARG);
   DICE_CHECK_ARG(keep == DICE_KEEP_NONE || keep == DICE_KEEP_INT8 || keep == DICE_KEEP_E4M3, DICE_ERR_ARG);
-  // each product takes the scratch only if it can use it
-  auto part = [&](int n_dim, int k_dim, bool weight_gradient) {
-    return dice_grouped_scratch_bytes(n_rows, n_dim, k_dim, n_slabs, weight_gradient ? DICE_PRODUCT_WGRAD : DICE_PRODUCT_DGRAD, dtype) > 0
-               ? scratch
-               : nullptr;
-  };
   // a gradient whose pointer is NULL is not made, and without any there is nothing to do
   if (n_rows > 0 && (d_rows || dw2)) {
     DICE_CHECK_ARG(d_out && rows_in && kept && w1 && w2 && d_pre && a && (keep == DICE_KEEP_NONE || scales), DICE_ERR_ARG);
@@ -142,7 +140,7 @@ extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in,
       if (rc != DICE_OK) return rc;
     } else {
       if ((rc = dice_grouped_dgrad(d_out, n_rows, hidden, w2, n_slabs, ffn, seg_offsets, nullptr, n_slabs, dtype, da,
-                                   part(hidden, ffn, false), scratch_bytes, status, stream)) != DICE_OK)
+                                   scratch, scratch_bytes, status, stream)) != DICE_OK)
         return rc;
       if ((rc = dice_act_backward(da, kept, scales, n_rows, ffn, act, keep, dtype, d_pre, a, stream)) != DICE_OK) return rc;
     }
@@ -150,13 +148,13 @@ extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in,
   const int c = static_cast<int>(cols);
   if (dw2 &&
       (rc = dice_grouped_wgrad(d_out, a, n_rows, hidden, ffn, seg_offsets, n_slabs, 0, dtype, dw2, nullptr,
-                               part(hidden, ffn, true), scratch_bytes, status, stream)) != DICE_OK)
+                               scratch, scratch_bytes, status, stream)) != DICE_OK)
     return rc;
   if (d_rows &&
       (rc = dice_grouped_dgrad(d_pre, n_rows, c, w1, n_slabs, hidden, seg_offsets, nullptr, n_slabs, dtype, d_rows,
-                               part(c, hidden, false), scratch_bytes, status, stream)) != DICE_OK)
+                               scratch, scratch_bytes, status, stream)) != DICE_OK)
     return rc;
   if (!dw1) return DICE_OK;
   return dice_grouped_wgrad(d_pre, rows_in, n_rows, c, hidden, seg_offsets, n_slabs, glu ? ffn : 0, dtype, dw1, dw1_up,
-                            part(c, hidden, true), scratch_bytes, status, stream);
+                            scratch, scratch_bytes, status, stream);
 }

@@ -626,16 +626,18 @@ _status_by_index = {}  # device number -> address of its status word, which live
 
 
 PRODUCT_DGRAD, PRODUCT_WGRAD, PRODUCT_LINEAR = 0, 1, 2
+THIN_ROWS = 4  # as kThinTotal of csrc/train.cuh
 
 
 def _split_bytes(lib, n_rows: int, n_dim: int, k_dim: int, n_slabs: int, product: int, code: int) -> int:
-    """dice_grouped_scratch_bytes; bf16 products with more tiles than any GPU has SM pairs for are not asked about."""
+    """dice_grouped_scratch_bytes; bf16 products with more tiles than any GPU has SM pairs for are not asked about, nor
+    the input gradients of few rows, which have a kernel of their own."""
     if code == DICE_BF16:
         col_tiles = (k_dim + 127) // 128
         if product == PRODUCT_WGRAD:
             few = 2 * n_slabs * ((n_dim + 255) // 256) * col_tiles <= 128
         else:
-            few = product == PRODUCT_DGRAD and 4 * ((n_rows + 255) // 256) * col_tiles <= 128
+            few = product == PRODUCT_DGRAD and n_rows > THIN_ROWS and 4 * ((n_rows + 255) // 256) * col_tiles <= 128
         if not few:
             return 0
     return lib.dice_grouped_scratch_bytes(n_rows, n_dim, k_dim, n_slabs, product, code)

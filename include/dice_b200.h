@@ -338,7 +338,8 @@ DICE_API int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, const
  * idle; fp32, the operands as three bf16 planes each for the tensor cores
  * (24 bits; without it, and where few rows meet a weight, the CUDA cores;
  * by planes, an infinity times a number with an empty plane is NaN).
- * 0 where it would not.  `product`: which one, with n_dim and k_dim as the
+ * 0 where it would not (a scratch given to such a call is left alone, whatever
+ * its size).  `product`: which one, with n_dim and k_dim as the
  * entry point names them (forward product: w [n_slabs, n_dim, k_dim]).  NULL
  * scratch is always allowed.  Calls that overlap on the GPU need scratch of
  * their own; calls in stream order may share it. */

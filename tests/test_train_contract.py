@@ -58,3 +58,18 @@ def test_float64_is_refused():
 def test_nothing_is_quantised_unasked():
     assert _block(train_kernels=True).train_keep is None
     assert inspect.signature(ops.grouped_ffn_train).parameters["keep"].default is None
+
+
+def test_single_tokens_ask_for_no_scratch():
+    class Lib:
+        asked = 0
+
+        def dice_grouped_scratch_bytes(self, *args):
+            self.asked += 1
+            return 1 << 20
+
+    lib = Lib()
+    for rows in range(1, 5):
+        assert ops._split_bytes(lib, rows, 9216, 1152, 8, ops.PRODUCT_DGRAD, ops.DICE_BF16) == 0
+    assert lib.asked == 0
+    assert ops._split_bytes(lib, 5, 9216, 1152, 8, ops.PRODUCT_DGRAD, ops.DICE_BF16) == 1 << 20

@@ -116,3 +116,41 @@ def test_no_grad_in_training_mode_keeps_nothing(cuda_device, keep, monkeypatch):
     assert wanted == [False, False]
     blk(x).sum().backward()
     assert wanted[2:] == [True, True]
+
+
+# ---- scratch ------------------------------------------------------------------------------
+
+
+def test_scratch_that_is_not_needed(cuda_device):
+    """A product for which the size query says 0 leaves any scratch alone, whatever its size; one that has a use for
+    scratch refuses too little."""
+    lib = _lib.load()
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=cuda_device).to(torch.bfloat16)  # noqa: E731
+    stream = torch.cuda.current_stream().cuda_stream
+    n, k = 9216, 64
+    for rows, needs in [(1, False), (4, False), (5, True), (300, True), (20000, False)]:
+        assert (lib.dice_grouped_scratch_bytes(rows, n, k, 1, ops.PRODUCT_DGRAD, ops.DICE_BF16) > 0) == needs, rows
+    small = torch.full((1024,), 7, dtype=torch.uint8, device=cuda_device)
+
+    def dgrad(rows, scratch, n_bytes):
+        dy, seg, out = rand(rows, n), torch.tensor([0, rows], dtype=torch.int32, device=cuda_device), None
+        w = rand(1, n, k)
+        out = torch.empty(rows, k, dtype=torch.bfloat16, device=cuda_device)
+        rc = lib.dice_grouped_dgrad(dy.data_ptr(), rows, n, w.data_ptr(), 1, k, seg.data_ptr(), None, 1, ops.DICE_BF16,
+                                    out.data_ptr(), scratch.data_ptr(), n_bytes, None, stream)
+        return rc, out, ops.grouped_dgrad(dy, w, seg)
+
+    for rows in (1, 4, 20000):
+        rc, out, want = dgrad(rows, small, 1024)
+        assert rc == 0 and torch.equal(out, want)
+    assert dgrad(300, small, 1024)[0] < 0
+    # a weight gradient with as many tiles as SM pairs, or a short reduction
+    for rows, nn, kk in [(3000, 2048, 2056), (100, 64, 64)]:
+        assert lib.dice_grouped_scratch_bytes(rows, nn, kk, 1, ops.PRODUCT_WGRAD, ops.DICE_BF16) == 0
+        dy, x, seg = rand(rows, nn), rand(rows, kk), torch.tensor([0, rows], dtype=torch.int32, device=cuda_device)
+        dw = torch.empty(1, nn, kk, dtype=torch.bfloat16, device=cuda_device)
+        rc = lib.dice_grouped_wgrad(dy.data_ptr(), x.data_ptr(), rows, nn, kk, seg.data_ptr(), 1, 0, ops.DICE_BF16,
+                                    dw.data_ptr(), None, small.data_ptr(), 1024, None, stream)
+        assert rc == 0 and torch.equal(dw, ops.grouped_wgrad(dy, x, seg))
+    assert bool((small == 7).all())
