@@ -132,7 +132,7 @@ extern "C" int dice_grouped_ffn_backward(const void* d_out, const void* rows_in,
   if (n_rows > 0 && (d_rows || dw2)) {
     DICE_CHECK_ARG(d_out && rows_in && kept && w1 && w2 && d_pre && a && (keep == DICE_KEEP_NONE || scales), DICE_ERR_ARG);
     DICE_CHECK_ARG(da || dtype == DICE_BF16, DICE_ERR_ARG);  // bf16: the activation's gradient stays in the epilogue
-    DICE_CHECK_ARG(dice_aligned16(d_out) && dice_aligned16(kept) && dice_aligned16(w2) && dice_aligned16(d_pre) && dice_aligned16(a),
+    DICE_CHECK_ARG(dice_aligned16(d_out) && kept_aligned(kept, keep) && dice_aligned16(w2) && dice_aligned16(d_pre) && dice_aligned16(a),
                    DICE_ERR_ALIGN);
     if (dtype == DICE_BF16) {
       rc = dice_internal_tc_back(d_out, n_rows, hidden, ffn, act, keep, w2, n_slabs, seg_offsets, kept, scales, d_pre, a, status,

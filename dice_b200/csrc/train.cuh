@@ -48,6 +48,11 @@ int dice_internal_tc_back(const void* d_out, int64_t n_rows, int hidden, int ffn
 constexpr int kKeepGroup = 128;               // columns of a kept argument that share a scale
 constexpr float kKeepFloor = 7.888609e-31f;   // 2^-100: the smallest group maximum a scale is made from
 
+// where what was kept may start: codes are read eight at a time, an argument in its own type 16 bytes at a time
+inline bool kept_aligned(const void* kept, int keep) {
+  return (reinterpret_cast<uintptr_t>(kept) & (keep == DICE_KEEP_NONE ? 15u : 7u)) == 0;
+}
+
 // ---- two fp32 values --------------------------------------------------------------
 // The functions below work on two values at a time, in one of two forms that round alike: `f32x2` is a register pair for
 // Blackwell's two-wide multiplies and adds, half the instructions where those are what bounds a kernel (the products'

@@ -356,7 +356,7 @@ extern "C" int dice_act_backward(const void* da, const void* kept, const float* 
   if (rc != DICE_OK) return rc;
   if (n_rows == 0) return DICE_OK;
   DICE_CHECK_ARG(da && kept && d_pre && (keep == DICE_KEEP_NONE || scales), DICE_ERR_ARG);
-  DICE_CHECK_ARG(dice_aligned16(da) && dice_aligned16(kept) && dice_aligned16(d_pre) && dice_aligned16(a), DICE_ERR_ALIGN);
+  DICE_CHECK_ARG(dice_aligned16(da) && kept_aligned(kept, keep) && dice_aligned16(d_pre) && dice_aligned16(a), DICE_ERR_ALIGN);
   ActParams p = {};
   p.in = da;
   p.kept = kept;

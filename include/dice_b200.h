@@ -381,6 +381,7 @@ DICE_API int dice_act_keep(const void* pre, int64_t n_rows, int ffn, int act, in
                   float* scales, void* stream);
 
 /* Its backward pass.  p = codes * scale (keep == NONE: `kept` is pre itself):
+ *   (codes may start at any multiple of 8 bytes: some rows of a larger tensor)
  *   d_pre = da * act'(p)  [n_rows, columns of pre] (filling columns: zero)
  *   a     = act(p)        [n_rows, ffn], what the second product's weight
  *           gradient is made from (NULL to skip) */

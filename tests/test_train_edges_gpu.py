@@ -154,3 +154,28 @@ def test_scratch_that_is_not_needed(cuda_device):
                                     dw.data_ptr(), None, small.data_ptr(), 1024, None, stream)
         assert rc == 0 and torch.equal(dw, ops.grouped_wgrad(dy, x, seg))
     assert bool((small == 7).all())
+
+
+# ---- kept codes that are a part of a tensor ----------------------------------------------------
+
+
+@pytest.mark.parametrize("keep", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("ffn", [72, 136, 328])
+def test_kept_codes_that_start_on_8_bytes(cuda_device, keep, dtype, ffn):
+    """Rows of GELU codes are a multiple of 8 bytes long, and so is the start of a slice of them."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=cuda_device).to(dtype)  # noqa: E731
+    rows, d_out, da, w1, w2 = rand(67, 64), rand(66, 64), rand(66, ffn), rand(2, ffn, 64), rand(2, 64, ffn)
+    _, kept = ops.act_keep(rand(67, ffn), "gelu_tanh", ffn, keep=keep)
+    part = ops.KeptAct(kept.codes[1:], kept.scales[1:])
+    assert part.codes.data_ptr() % 16 == 8 and part.codes.is_contiguous()
+    whole = ops.KeptAct(*(t.clone() for t in part))
+    for a, b in zip(ops.act_backward(da, part, "gelu_tanh", ffn), ops.act_backward(da, whole, "gelu_tanh", ffn)):
+        assert torch.equal(a, b)
+    seg = torch.tensor([0, 40, 66], dtype=torch.int32, device=cuda_device)
+    back = lambda k: ops.grouped_ffn_backward(d_out, rows[1:], k, w1, w2, seg, "gelu_tanh", ffn)  # noqa: E731
+    assert all(torch.equal(a, b) for a, b in zip(back(part), back(whole)))
+    out = ops.KeptAct(torch.empty(66 * ffn + 4, dtype=part.codes.dtype, device=cuda_device)[4:].view(66, ffn), part.scales)
+    with pytest.raises(RuntimeError, match="aligned"):
+        ops.act_backward(da, out, "gelu_tanh", ffn)
