@@ -581,12 +581,17 @@ class KeptAct(NamedTuple):
 # The small calls of a training step are bounded by the host: one token's gradients cost the GPU a few microseconds, and
 # every torch.empty with keyword arguments two, every look-up of a device half of one.  Hence one comparison per tensor,
 # written out, allocations through torch's own short path where it exists, and widths computed here.
+# That path goes past dispatch modes and past the filling of uninitialised memory that deterministic algorithms may ask
+# for, so it is not taken where either is on.
 _empty_cuda = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+_dispatch_modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
+if _dispatch_modes is None:
+    _empty_cuda = None
 
 
 def _new(shape: Tuple[int, ...], dtype: torch.dtype, index: int) -> torch.Tensor:
     """An uninitialised contiguous tensor on the current device, which is number ``index``."""
-    if _empty_cuda is not None:
+    if _empty_cuda is not None and not torch.are_deterministic_algorithms_enabled() and not _dispatch_modes():
         stride = (shape[1], 1) if len(shape) == 2 else (shape[1] * shape[2], shape[2], 1)
         return _empty_cuda(shape, stride, dtype)
     return torch.empty(shape, dtype=dtype, device=torch.device("cuda", index))

@@ -179,3 +179,37 @@ def test_kept_codes_that_start_on_8_bytes(cuda_device, keep, dtype, ffn):
     out = ops.KeptAct(torch.empty(66 * ffn + 4, dtype=part.codes.dtype, device=cuda_device)[4:].view(66, ffn), part.scales)
     with pytest.raises(RuntimeError, match="aligned"):
         ops.act_backward(da, out, "gelu_tanh", ffn)
+
+
+# ---- memory of the results ---------------------------------------------------------------------
+
+
+def test_uninitialised_memory_is_filled_if_asked(cuda_device):
+    """Deterministic algorithms fill what is left uninitialised with NaN (torch's own rule for torch.empty)."""
+    dy, w = torch.ones(9, 64, device=cuda_device), torch.ones(1, 64, 72, device=cuda_device)
+    seg = torch.tensor([2, 7], dtype=torch.int32, device=cuda_device)
+    ops.grouped_dgrad(dy, w, seg)  # (its memory goes back to the cache, with 64 in it)
+    torch.use_deterministic_algorithms(True)
+    try:
+        dx = ops.grouped_dgrad(dy, w, seg)
+    finally:
+        torch.use_deterministic_algorithms(False)
+    assert bool(torch.isnan(dx[:2]).all()) and bool(torch.isnan(dx[7:]).all()) and bool((dx[2:7] == 64).all())
+
+
+def test_dispatch_modes_see_the_allocations(cuda_device):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    x = torch.ones(9, 64, device=cuda_device)
+    with Seen() as seen:
+        ops.act_keep(x, "gelu_tanh", 64)
+    assert sum("empty" in n for n in seen.names) == 3
