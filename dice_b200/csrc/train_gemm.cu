@@ -34,10 +34,14 @@
 // operands are bf16 (a second plane of 8 more bits would double that product).  A result of the second product is then
 // off by the roundings of the activation and its own, 2.4e-3 of its norm against 1.7e-3 for its own alone.
 //
-// fp32 operands (PLANES 3) come as three bf16 planes each, x = hi + mid + lo exactly (8 bits of the mantissa a plane), and a
-// product is six: hi hi, hi mid, mid hi, mid mid, hi lo, lo hi; what is left out is below 2^-25 of it.  The accumulator
-// in tensor memory is cut, not rounded, after every instruction, so it is emptied after every k-block of 64 into fp32
-// registers that round, and within a block the small products come first.  Six instructions for one leave ~220 TFLOP/s,
+// fp32 operands (PLANES 3) come as three bf16 planes each, x = hi + 2^-8 mid + 2^-16 lo exactly (8 bits of the mantissa a
+// plane), and a product is six: hi hi, hi mid, mid hi, mid mid, hi lo, lo hi; what is left out is below 2^-25 of it.  The
+// accumulator in tensor memory is cut, not rounded, after every instruction, so it is emptied after every k-block of 64 into
+// fp32 registers that round, and within a block the small products come first: those of 2^-16, then, the sum scaled by 2^-8
+// as the first of them is added, those of 2^-8, then, scaled again, hi hi.  The planes hold their bits at hi's own
+// magnitude, since bf16 ends where fp32 does: unscaled, mid and lo of values below 2^-110 would have lost their last bits
+// there, which a large factor on the other side makes visible (fp32's own subnormals, below 2^-126, have their bits in mid
+// and lo: their products are good to 2^-8).  Six instructions for one leave ~220 TFLOP/s,
 // three times the CUDA cores' 74.  (An infinity in an operand gives NaN: its product with a zero plane.)
 //
 // Few tiles: they are made half as wide if that keeps more pairs busy (one token's two rows, 1152 -> 4608: 36 tiles of
@@ -116,6 +120,15 @@ __device__ __forceinline__ uint64_t make_mn_desc(uint32_t smem_addr) {
   d |= static_cast<uint64_t>(1) << 46;
   d |= static_cast<uint64_t>(2) << 61;
   return d;
+}
+// D = A B + 2^-8 D
+__device__ __forceinline__ void umma_bf16_pair_scaled(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.eq.b32 p, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p, 8;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc)
+      : "memory");
 }
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
   asm volatile(
@@ -657,6 +670,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           // 16 reduction elements further: 32 bytes along a K-major row, 16 rows of 128 bytes in an MN-major box
           constexpr uint64_t kStepA = MODE != MODE_TN ? 2 : 128, kStepB = MODE == MODE_NT ? 2 : 128;
           constexpr int kProducts = PLANES == 3 ? 6 : 1;
+          // (planes scaled by 2^16 together, by 2^8, by 1: the sum is brought to the next one's scale on the way)
           constexpr int kPlaneA[6] = {PLANES == 3 ? 2 : 0, 0, 1, 1, 0, 0}, kPlaneB[6] = {0, 2, 1, 0, 1, 0};
           if (elect_one()) {
 #pragma unroll
@@ -667,9 +681,13 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
               const uint64_t b_desc = MODE == MODE_NT ? make_operand_desc(b_addr) : make_mn_desc(b_addr);
 #pragma unroll
               for (int kk = 0; kk < BK / UMMA_K; ++kk)
-                if (kk < steps)
-                  umma_bf16_pair(d_tmem, a_desc + kk * kStepA, b_desc + kk * kStepB, idesc,
-                                 static_cast<uint32_t>((PLANES == 1 && kb != ti.kb0) || q != 0 || kk != 0));
+                if (kk < steps) {
+                  if (PLANES == 3 && kk == 0 && (q == 3 || q == 5))
+                    umma_bf16_pair_scaled(d_tmem, a_desc, b_desc, idesc);
+                  else
+                    umma_bf16_pair(d_tmem, a_desc + kk * kStepA, b_desc + kk * kStepB, idesc,
+                                   static_cast<uint32_t>((PLANES == 1 && kb != ti.kb0) || q != 0 || kk != 0));
+                }
             }
             umma_commit_pair(empty_bar + 8 * stage);
             if (PLANES != 1) umma_commit_pair(acc_full_bar + 8 * acc);
@@ -1165,7 +1183,14 @@ int dice_internal_tc_back(const void* d_out, int64_t n_rows, int hidden, int ffn
 // ---- fp32 operands ------------------------------------------------------------------
 namespace {
 
-// x -> three planes of bf16, each the nearest to what the planes before it leave, so that hi + mid + lo == x.  Two tensors in one launch, eight values a thread.
+// x -> three planes of bf16, x == hi + 2^-8 mid + 2^-16 lo for every finite x, the smallest included.  A plane is the
+// nearest to what the planes before it leave, times 2^8 for each of them.  Two tensors in one launch, eight values a thread.
+// Rounded to nearest, which halves what the next plane has to hold twice over; the largest values, which would round to an
+// infinity, are cut (what a cut leaves is below 2^-7 of the value: times 2^8 it is still finite).
+__device__ __forceinline__ uint32_t nearest_plane(float x) {
+  const uint32_t near = static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(x))) << 16;
+  return (near & 0x7f800000u) == 0x7f800000u ? __float_as_uint(x) & 0xffff0000u : near;
+}
 struct PlaneJob {
   const float* x;
   __nv_bfloat16* planes;
@@ -1185,17 +1210,12 @@ __global__ void __launch_bounds__(256) split_planes_kernel(const PlaneJob first,
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float x = __uint_as_float(raw[j]);
-    // rounded to nearest, which halves what the next plane has to hold twice over; the largest values, which would round
-    // to an infinity, are cut.  A value that is not finite stays as it is, alone (a NaN whose payload is cut away would be
-    // an infinity).
-    uint32_t hi = static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(x))) << 16;
+    // a value that is not finite stays as it is, alone (a NaN whose payload is cut away would be an infinity)
     const bool finite = (raw[j] & 0x7f800000u) != 0x7f800000u;
-    if (finite && (hi & 0x7f800000u) == 0x7f800000u) hi = raw[j] & 0xffff0000u;
-    const float rest = finite ? x - __uint_as_float(hi) : 0.f;
-    const uint32_t mid = static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(rest))) << 16;
-    plane[0][j] = hi;
-    plane[1][j] = mid;
-    plane[2][j] = static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(rest - __uint_as_float(mid)))) << 16;
+    plane[0][j] = finite ? nearest_plane(x) : static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(x))) << 16;
+    const float rest = finite ? (x - __uint_as_float(plane[0][j])) * 256.0f : 0.f;
+    plane[1][j] = nearest_plane(rest);
+    plane[2][j] = nearest_plane((rest - __uint_as_float(plane[1][j])) * 256.0f);
   }
 #pragma unroll
   for (int q = 0; q < 3; ++q)

@@ -213,3 +213,64 @@ def test_dispatch_modes_see_the_allocations(cuda_device):
     with Seen() as seen:
         ops.act_keep(x, "gelu_tanh", 64)
     assert sum("empty" in n for n in seen.names) == 3
+
+
+# ---- fp32 over all of its range -------------------------------------------------------------------
+
+
+def _check_f32(got, a, b, of_mass=0.0):
+    """a, b in 64 bits; K 2^-23 of the magnitudes and half a step of the result, as test_train_ops_gpu derives it, and
+    ``of_mass`` of the magnitudes"""
+    ref, mass = a @ b, a.abs() @ b.abs()
+    err, bound = (got.to(D) - ref).abs(), 2.0 ** -24 * ref.abs() + ((a.shape[1] + 1) * 2.0 ** -23 + of_mass) * mass
+    assert bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("low,high", [(-126, 120), (-112, 100), (-100, 100), (100, -112), (120, -126)])
+def test_fp32_planes_at_the_end_of_the_range(cuda_device, low, high):
+    """Values whose last bits lie below what bf16 can hold, met by factors that bring them back into sight."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    rows, n, k = 440, 1032, 712
+    seg = torch.tensor([0, 200, 200, 440], dtype=torch.int32, device=cuda_device)
+    rand = lambda *s, e: (torch.randn(*s, generator=gen, device=cuda_device, dtype=D) * 2.0 ** e).float()  # noqa: E731
+    dy, x, w = rand(rows, n, e=low), rand(rows, k, e=high), rand(3, n, k, e=high)
+    for product in (ops.PRODUCT_DGRAD, ops.PRODUCT_WGRAD):
+        assert ops._split_bytes(_lib.load(), rows, n, k, 3, product, ops.DICE_F32) >= 6 * rows * n
+    dx, dw = ops.grouped_dgrad(dy, w, seg), ops.grouped_wgrad(dy, x, seg)
+    w1 = w.transpose(1, 2).contiguous()
+    _, kept = ops.grouped_ffn_train(dy, w1, torch.zeros_like(w), seg, "gelu_tanh", k)
+    for s, (beg, end) in enumerate([(0, 200), (200, 200), (200, 440)]):
+        a, b, g = dy[beg:end].to(D), w[s].to(D), x[beg:end].to(D)
+        _check_f32(dx[beg:end], a, b)
+        _check_f32(dw[s], a.T, g)
+        _check_f32(kept.codes[beg:end], a, b)
+
+
+def test_fp32_subnormals(cuda_device):
+    """Subnormals have their bits in the second and the third plane, whose products with the other operand's second and
+    third (at most 2^-9 and 2^-17 of it, what rounding to 8 and to 16 bits leaves) are left out: 2^-8 covers both.  The
+    first plane alone, and any flush to zero, would be off by all of it."""
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    rows, n, k = 440, 1032, 712
+    seg = torch.tensor([0, 440], dtype=torch.int32, device=cuda_device)
+    rand = lambda *s, e: (torch.randn(*s, generator=gen, device=cuda_device, dtype=D) * 2.0 ** e).float()  # noqa: E731
+    dy, x, w = rand(rows, n, e=-141), rand(rows, k, e=120), rand(1, n, k, e=120)
+    _check_f32(ops.grouped_dgrad(dy, w, seg), dy.to(D), w[0].to(D), of_mass=2.0 ** -8)
+    _check_f32(ops.grouped_wgrad(dy, x, seg)[0], dy.to(D).T, x.to(D), of_mass=2.0 ** -8)
+    # a call without scratch is on the CUDA cores, and exact
+    out = torch.empty(rows, k, device=cuda_device)
+    rc = _lib.load().dice_grouped_dgrad(dy.data_ptr(), rows, n, w.data_ptr(), 1, k, seg.data_ptr(), None, 1, ops.DICE_F32,
+                                        out.data_ptr(), None, 0, None, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    _check_f32(out, dy.to(D), w[0].to(D))
+
+
+def test_one_small_value_among_ordinary_ones(cuda_device):
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    dy = torch.randn(300, 1032, generator=gen, device=cuda_device)
+    dy[:, 7] = (dy[:, 7].double() * 2.0 ** -122).float()
+    w = torch.zeros(1, 1032, 1160, device=cuda_device)
+    w[0, 7] = (torch.randn(1160, generator=gen, device=cuda_device, dtype=D) * 2.0 ** 118).float()
+    seg = torch.tensor([0, 300], dtype=torch.int32, device=cuda_device)
+    assert ops._split_bytes(_lib.load(), 300, 1032, 1160, 1, ops.PRODUCT_DGRAD, ops.DICE_F32) > 0
+    _check_f32(ops.grouped_dgrad(dy, w, seg), dy.to(D), w[0].to(D))
