@@ -15,6 +15,11 @@ int dice_internal_simt_wgrad(const void* dy, const void* x, int64_t n_rows, int 
                              const int32_t* seg_offsets, int n_slabs, int gate_up, void* dw, void* dw_up,
                              uint32_t* status, cudaStream_t s);
 
+// the values of an fp32 product (kind: DICE_PRODUCT_*) that are not finite, made again if `non_finite` says that there are any
+int dice_internal_f32_repair(int kind, const void* a, const void* b, int64_t n_rows, int n_dim, int k_dim, int n_slabs,
+                             const int32_t* seg_offsets, const int32_t* seg_slab, int n_seg, int gate_up, void* out,
+                             void* out_up, const unsigned int* non_finite, cudaStream_t s);
+
 // bf16 input gradient of at most kThinTotal rows, on the CUDA cores (train_thin.cu)
 constexpr int kThinTotal = 4;
 int dice_internal_thin_dgrad(const void* dy, int64_t n_rows, int n_dim, const void* w, int n_slabs, int k_dim,

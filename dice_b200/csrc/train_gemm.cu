@@ -42,7 +42,9 @@
 // magnitude, since bf16 ends where fp32 does: unscaled, mid and lo of values below 2^-110 would have lost their last bits
 // there, which a large factor on the other side makes visible (fp32's own subnormals, below 2^-126, have their bits in mid
 // and lo: their products are good to 2^-8).  Six instructions for one leave ~220 TFLOP/s,
-// three times the CUDA cores' 74.  (An infinity in an operand gives NaN: its product with a zero plane.)
+// three times the CUDA cores' 74.  An infinity in an operand (times a zero plane), or planes' products that overflow to
+// infinities of both signs, leave a NaN where the sum may be an infinity or a number: an epilogue that sees a value that is
+// not finite says so, and the CUDA cores make those values again (dice_internal_f32_repair).
 //
 // Few tiles: they are made half as wide if that keeps more pairs busy (one token's two rows, 1152 -> 4608: 36 tiles of
 // 256 columns, 72 of 128; 80 tiles on 74 pairs are two rounds, and so are 144 of half the width).  Fewer still, and a long reduction: the pairs that would idle take a share of the reduction
@@ -105,6 +107,7 @@ struct TrainGemm {
   const void* kept;             // EPI_BACK: codes or pre
   const float* kept_scales;
   int kept_wide;                // its rows are whole pieces of 32 bytes
+  unsigned int* non_finite;     // PLANES 3: set where a result is (see dice_internal_f32_repair)
   uint8_t* codes;               // EPI_KEEP
   int codes_tma;                // its rows are whole pieces of 16 bytes
   float* scales;
@@ -895,6 +898,10 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
               v[2 * j + 1] = x.y;
             }
           }
+          float zero = 0.f;  // NaN if one of the values is not finite
+#pragma unroll
+          for (int j = 0; j < 32; ++j) zero = fmaf(v[j], 0.f, zero);
+          if (zero != 0.f && quad * 32 + lane < ti.rows_valid) *static_cast<volatile unsigned int*>(p.non_finite) = 1u;
           float* const base = reinterpret_cast<float*>(up_rows ? p.out_up : p.out);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {  // 16 columns are 64 bytes
@@ -1196,9 +1203,10 @@ struct PlaneJob {
   __nv_bfloat16* planes;
   int64_t n;  // values (a multiple of 8), also the distance of the planes
 };
-__global__ void __launch_bounds__(256) split_planes_kernel(const PlaneJob first, const PlaneJob second) {
+__global__ void __launch_bounds__(256) split_planes_kernel(const PlaneJob first, const PlaneJob second, unsigned int* non_finite) {
   pdl_trigger();
   pdl_wait();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *non_finite = 0u;
   int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8;
   const bool in_first = i < first.n;
   if (!in_first) i -= first.n;
@@ -1223,6 +1231,7 @@ __global__ void __launch_bounds__(256) split_planes_kernel(const PlaneJob first,
                                                         (plane[q][4] >> 16) | plane[q][5], (plane[q][6] >> 16) | plane[q][7]));
 }
 
+constexpr size_t kFlagBytes = 256;  // at the scratch's end: whether a result is not finite
 size_t plane_bytes(int64_t n) { return (static_cast<size_t>(n) * 6 + 255) / 256 * 256; }
 
 }  // namespace
@@ -1241,12 +1250,13 @@ size_t dice_internal_f32_bytes(int kind, int64_t n_rows, int n_dim, int k_dim, i
   const int64_t w = static_cast<int64_t>(n_slabs) * n_dim * k_dim;
   if (kind == DICE_PRODUCT_WGRAD) {
     if (n_rows < kF32WgradRows * static_cast<int64_t>(n_slabs)) return 0;
-    return plane_bytes(n_rows * n_dim) + plane_bytes(n_rows * k_dim) + dice_internal_split_bytes(n_rows, n_dim, k_dim, n_slabs, true);
+    return plane_bytes(n_rows * n_dim) + plane_bytes(n_rows * k_dim) +
+           dice_internal_split_bytes(n_rows, n_dim, k_dim, n_slabs, true) + kFlagBytes;
   }
   if (n_rows < kF32Rows * static_cast<int64_t>(n_slabs) || n_rows < kF32Work / (static_cast<int64_t>(n_dim) * k_dim)) return 0;
   const int a_cols = kind == DICE_PRODUCT_DGRAD ? n_dim : k_dim;
   const int out_cols = kind == DICE_PRODUCT_DGRAD ? k_dim : n_dim;
-  return plane_bytes(n_rows * a_cols) + plane_bytes(w) + dice_internal_split_bytes(n_rows, a_cols, out_cols, n_slabs, false);
+  return plane_bytes(n_rows * a_cols) + plane_bytes(w) + dice_internal_split_bytes(n_rows, a_cols, out_cols, n_slabs, false) + kFlagBytes;
 }
 
 // a, b: what the kind multiplies (forward rows and w, input gradient dy and w, weight gradient dy and x)
@@ -1265,7 +1275,6 @@ int dice_internal_f32_product(int kind, const void* a, const void* b, int64_t n_
   at += plane_bytes(b_n);
   const int64_t blocks = ((a_n + b_n) / 8 + 255) / 256;
   if (blocks > 0x7fffffffLL) return DICE_ERR_LIMIT;
-  if (dice_launch(split_planes_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, ja, jb) != cudaSuccess) return DICE_ERR_CUDA;
 
   TrainGemm p = {};
   p.seg_offsets = seg_offsets;
@@ -1311,9 +1320,15 @@ int dice_internal_f32_product(int kind, const void* a, const void* b, int64_t n_
   if (rc != DICE_OK) return rc;
   if (pairs <= 0) return DICE_ERR_CUDA;
   if (split > 0 && (rc = use_scratch(p, at, split, pairs, s)) != DICE_OK) return rc;
+  p.non_finite = reinterpret_cast<unsigned int*>(at + split);
+  if (dice_launch(split_planes_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, ja, jb, p.non_finite) != cudaSuccess)
+    return DICE_ERR_CUDA;
   const CUtensorMap no_stores[3] = {tm_a, tm_a, tm_a};
   const int64_t tiles = (wgrad ? static_cast<int64_t>(n_slabs) * p.n_mblk : (n_rows + PM - 1) / PM + n_seg) * col_tiles(p.n_cols, BN / 2);
-  if (kind == DICE_PRODUCT_LINEAR) return launch_train<MODE_NT, EPI_PLAIN, 0, 0, 3>(tm_a, tm_b, no_stores, p, tiles, pairs, s);
-  if (kind == DICE_PRODUCT_DGRAD) return launch_train<MODE_NN, EPI_PLAIN, 0, 0, 3>(tm_a, tm_b, no_stores, p, tiles, pairs, s);
-  return launch_train<MODE_TN, EPI_PLAIN, 0, 0, 3>(tm_a, tm_b, no_stores, p, tiles, pairs, s);
+  if (kind == DICE_PRODUCT_LINEAR) rc = launch_train<MODE_NT, EPI_PLAIN, 0, 0, 3>(tm_a, tm_b, no_stores, p, tiles, pairs, s);
+  else if (kind == DICE_PRODUCT_DGRAD) rc = launch_train<MODE_NN, EPI_PLAIN, 0, 0, 3>(tm_a, tm_b, no_stores, p, tiles, pairs, s);
+  else rc = launch_train<MODE_TN, EPI_PLAIN, 0, 0, 3>(tm_a, tm_b, no_stores, p, tiles, pairs, s);
+  if (rc != DICE_OK) return rc;
+  return dice_internal_f32_repair(kind, a, b, n_rows, n_dim, k_dim, n_slabs, seg_offsets, seg_slab, n_seg, gate_up, out, out_up,
+                                  p.non_finite, s);
 }

@@ -684,7 +684,7 @@ def grouped_dgrad(dy: torch.Tensor, w: torch.Tensor, seg_offsets: torch.Tensor, 
                   seg_slab: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Input gradient of :func:`grouped_gemm`: ``dx[r] = dy[r] @ w[slab(seg(r))]`` with ``dy [R, N]``,
     ``w [S, N, K]`` (bf16 or fp32).  Rows of no segment are left as they are in ``out`` (uninitialised without it), which
-    shares no memory with the operands.  fp32: an infinity in a row or a weight may come out as NaN."""
+    shares no memory with the operands."""
     index = _one_device(dy, w, seg_offsets, status, seg_slab, out)
     if index != _current_device():
         with torch.cuda.device(index):
@@ -716,7 +716,7 @@ def grouped_dgrad(dy: torch.Tensor, w: torch.Tensor, seg_offsets: torch.Tensor, 
 def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, seg_offsets: torch.Tensor, status: Optional[torch.Tensor] = None,
                   gate_up: Optional[int] = None):
     """Weight gradient of :func:`grouped_gemm`: ``dw[s] = dy[seg s].T @ x[seg s]`` ``[S, N, K]`` in the rows' type, zero
-    for a segment without rows (fp32: an infinity may come out as NaN).  ``gate_up=ffn``: ``dy`` has the packed gate / up columns of :func:`pack_w13`, and the
+    for a segment without rows.  ``gate_up=ffn``: ``dy`` has the packed gate / up columns of :func:`pack_w13`, and the
     result is the pair of gradients ``[S, ffn, K]`` of the gate and the up projections."""
     index = _one_device(dy, x, seg_offsets, status)
     if index != _current_device():

@@ -318,8 +318,7 @@ DICE_API int dice_grouped_ffn_f32(const void* rows_in, int64_t n_rows, int hidde
  * The training step of the expert FFN (the reference trains through autograd
  * over a Python loop of experts, models.py:313-320).  Rows are expert-sorted as
  * above; both element types are taken everywhere: bf16, and fp32 to fp32's
- * precision (an infinity in an operand may come out as NaN: see
- * dice_grouped_scratch_bytes).  Sums are fp32; outputs are rounded once.
+ * precision.  Sums are fp32; outputs are rounded once.
  *
  * Input gradient of a product grouped by expert (out = a * w^T):
  *   dx[r, :] = dy[r, :] * w[slab(seg(r))]
@@ -336,8 +335,7 @@ DICE_API int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, const
 /* Scratch (16-byte aligned, contents irrelevant) that makes a product faster:
  * bf16, a long reduction shared among SMs that few output tiles would leave
  * idle; fp32, the operands as three bf16 planes each for the tensor cores
- * (24 bits; without it, and where few rows meet a weight, the CUDA cores;
- * by planes, an infinity times a number with an empty plane is NaN).
+ * (24 bits; without it, and where few rows meet a weight, the CUDA cores).
  * 0 where it would not (a scratch given to such a call is left alone, whatever
  * its size).  `product`: which one, with n_dim and k_dim as the
  * entry point names them (forward product: w [n_slabs, n_dim, k_dim]).  NULL

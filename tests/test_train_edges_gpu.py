@@ -274,3 +274,105 @@ def test_one_small_value_among_ordinary_ones(cuda_device):
     seg = torch.tensor([0, 300], dtype=torch.int32, device=cuda_device)
     assert ops._split_bytes(_lib.load(), 300, 1032, 1160, 1, ops.PRODUCT_DGRAD, ops.DICE_F32) > 0
     _check_f32(ops.grouped_dgrad(dy, w, seg), dy.to(D), w[0].to(D))
+
+
+def _products(dy, x, w, seg):
+    """dx, dw and the forward product (rows dy) of one call each"""
+    w1 = w.transpose(1, 2).contiguous()
+    _, kept = ops.grouped_ffn_train(dy, w1, torch.zeros_like(w), seg, "gelu_tanh", w.shape[2])
+    return ops.grouped_dgrad(dy, w, seg), ops.grouped_wgrad(dy, x, seg), kept.codes
+
+
+@pytest.mark.parametrize("rows,n,k", [(40, 1032, 712), (440, 1032, 712), (513, 2048, 72), (3000, 264, 328)])
+def test_fp32_infinities_stay_infinities(cuda_device, rows, n, k):
+    """Whether few rows or many (CUDA cores, or planes on the tensor cores): an infinity meets factors that are not zero and
+    stays one, of the right sign; with its like of the other sign, or a zero, it is NaN; nothing else changes a bit."""
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    cut = rows * 3 // 5
+    seg = torch.tensor([0, cut, cut, rows - 1], dtype=torch.int32, device=cuda_device)  # the last row is nobody's
+    dy, x, w = (torch.randn(*s, generator=gen, device=cuda_device) for s in ((rows, n), (rows, k), (3, n, k)))
+    want = _products(dy, x, w, seg)
+    inf = float("inf")
+    dy2, x2, w2 = dy.clone(), x.clone(), w.clone()
+    dy2[1, 3], dy2[cut, 4], dy2[cut, 5], dy2[rows - 1] = inf, inf, inf, inf
+    w2[0, 3, 9], w2[0, 6, 11], x2[2, 13], x2[rows - 1] = 0.0, -inf, -inf, float("nan")
+    w2[1] = float("nan")  # an expert without rows
+    got = _products(dy2, x2, w2, seg)
+    ref64 = []
+    for a, b in (((dy2, w2),) * 2):
+        ref64.append(torch.cat([dy2[:cut].double() @ w2[0].double(), dy2[cut:rows - 1].double() @ w2[2].double()]))
+    dw64 = torch.stack([dy2[:cut].double().T @ x2[:cut].double(), torch.zeros(n, k, device=cuda_device, dtype=D),
+                        dy2[cut:rows - 1].double().T @ x2[cut:rows - 1].double()])
+    for g, ref, clean in ((got[0][:rows - 1], ref64[0], want[0][:rows - 1]), (got[1], dw64, want[1]),
+                          (got[2][:rows - 1], ref64[1], want[2][:rows - 1])):
+        odd = ~torch.isfinite(ref)
+        assert 0 < int(odd.sum()) < odd.numel()
+        assert torch.equal(torch.isnan(g), torch.isnan(ref)) and torch.equal(g[odd].nan_to_num(7.0), ref[odd].float().nan_to_num(7.0))
+        same = ~odd
+        if g.shape == got[0][:rows - 1].shape and g is not got[1]:
+            same[:, 9] = False  # (the weight that was set to zero)
+            same[:cut, 9] = False
+        assert torch.equal(g[same], clean[same])
+    # and without the infinities again: the clean bits (nothing stays of the call before)
+    assert all(torch.equal(a[:rows - 1], b[:rows - 1]) for a, b in zip(_products(dy, x, w, seg), want))
+    ops.check_status(ops.device_status(cuda_device))
+
+
+@pytest.mark.parametrize("rows", [40, 600])
+def test_fp32_products_that_overflow(cuda_device, rows):
+    """Finite values whose products overflow in one direction: an infinity, as fp32 sums give it, not NaN; a neighbour
+    whose values fit keeps every bit."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    n, k = 1032, 712
+    seg = torch.tensor([0, rows], dtype=torch.int32, device=cuda_device)
+    dy, x, w = (torch.rand(*s, generator=gen, device=cuda_device) + 0.5 for s in ((rows, n), (rows, k), (1, n, k)))
+    want = _products(dy, x, w, seg)
+    dy2, x2, w2 = dy.clone(), x.clone(), w.clone()
+    dy2[5] *= 2.0 ** 90
+    w2[0, :, 7] *= -2.0 ** 90
+    x2[:, 11] *= -2.0 ** 127  # times dy[5]: beyond the range whatever the rest
+    x2[:, 11] = x2[:, 11].clamp(min=-3e38)
+    dx, dw, fwd = _products(dy2, x2, w2, seg)
+    for g, clean in ((dx, want[0]), (fwd, want[2])):
+        assert bool((g[5, 7] == -float("inf")).all()) and bool(torch.isfinite(g[5, :7]).all()) and bool(torch.isfinite(g[:5, 7]).all())
+        others = torch.ones_like(g, dtype=torch.bool)
+        others[5], others[:, 7] = False, False
+        assert torch.equal(g[others], clean[others])
+    assert bool((dw[0, :, 11] == -float("inf")).all()) and bool(torch.isfinite(dw[0, :, :11]).all())
+
+
+@pytest.mark.parametrize("ffn", [200, 328])
+def test_fp32_infinities_with_gate_and_up_apart(cuda_device, ffn):
+    gen = torch.Generator(device="cuda").manual_seed(10)
+    cols, k = ops.w13_rows(ffn), 328
+    seg = torch.tensor([0, 300, 500], dtype=torch.int32, device=cuda_device)
+    dy, x = (torch.randn(500, c, generator=gen, device=cuda_device) for c in (cols, k))
+    dy[7, 130], dy[400, 3], x[310, 17] = float("inf"), -float("inf"), float("inf")
+    packed = ops.grouped_wgrad(dy, x, seg).unflatten(1, (-1, 2, 128))
+    gate, up = ops.grouped_wgrad(dy, x, seg, gate_up=ffn)
+    for got, part in ((gate, 0), (up, 1)):
+        want = packed[:, :, part].flatten(1, 2)[:, :ffn]
+        assert torch.equal(got.nan_to_num(7.0, 8.0, 9.0), want.nan_to_num(7.0, 8.0, 9.0))
+    ref = torch.stack([dy[:300].double().T @ x[:300].double(), dy[300:].double().T @ x[300:].double()]).unflatten(1, (-1, 2, 128))
+    assert torch.equal(torch.isnan(packed), torch.isnan(ref)) and torch.equal(torch.isinf(packed), torch.isinf(ref))
+
+
+def test_fp32_infinities_in_a_graph(cuda_device):
+    """Captured without an infinity, replayed with one and without again."""
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    dy, w = torch.randn(300, 1032, generator=gen, device=cuda_device), torch.randn(1, 1032, 1160, generator=gen, device=cuda_device)
+    seg = torch.tensor([0, 300], dtype=torch.int32, device=cuda_device)
+    clean = ops.grouped_dgrad(dy, w, seg)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dx = ops.grouped_dgrad(dy, w, seg)
+    for value in (float("inf"), 1.0, float("inf"), 1.0):
+        before = dy[3, 3].clone()
+        dy[3, 3] *= value
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool(torch.isinf(dx[3]).all()) == (value != 1.0) and not bool(torch.isnan(dx).any())
+        dx2 = dx.clone()
+        dx2[3] = clean[3]
+        assert torch.equal(dx2, clean)
+        dy[3, 3] = before
