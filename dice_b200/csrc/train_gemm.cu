@@ -143,6 +143,29 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
 __device__ __forceinline__ void mbar_complete_tx_cluster(uint32_t cluster_addr, uint32_t bytes) {
   asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cluster.b64 [%0], %1;" ::"r"(cluster_addr), "r"(bytes) : "memory");
 }
+// Wait for a ragged end.  Any number of tiles without one may lie between it and the last, so the limit is on a standstill:
+// it starts anew whenever the loader has filled another slot (its own waits are bounded one by one).
+__device__ __noinline__ bool mbar_wait_behind(uint32_t bar, uint32_t parity, volatile uint32_t* filled, volatile uint32_t* abort_flag,
+                                              uint32_t* status) {
+  uint64_t t0 = global_timer_ns();
+  uint32_t seen = *filled, spins = 0;
+  while (!mbar_try_wait(bar, parity)) {
+    if ((++spins & 127u) != 0) continue;
+    if (*abort_flag != 0) return false;
+    const uint32_t now = *filled;
+    const uint64_t t = global_timer_ns();
+    if (now != seen) {
+      seen = now;
+      t0 = t;
+    } else if (t - t0 > kWaitLimitNs) {
+      if (status != nullptr) atomicCAS(status, 0u, DICE_STATUS_WAIT_SMEM_FULL);
+      *abort_flag = 1;
+      __threadfence_block();
+      return false;
+    }
+  }
+  return true;
+}
 // orders the zeroing before that (release), and after it in the issuing warp (acquire)
 __device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -456,7 +479,8 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * kStagesT + 2 * kAccStages + 4);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   int* s_split = reinterpret_cast<int*>(tmem_slot + 2);  // shares of the reduction; columns of a tile
-  int* s_seg_off = reinterpret_cast<int*>(tmem_slot + 4);
+  volatile uint32_t* filled = tmem_slot + 4;             // TN: slots that the loader has filled so far
+  int* s_seg_off = reinterpret_cast<int*>(tmem_slot + 5);
   int* s_mprefix = s_seg_off + (kMaxSeg + 1);  // NT, NN: first row tile of every segment
   const uint32_t tiles_smem = smem_u32(smem);
 
@@ -479,6 +503,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     }
     for (int q = 0; q < 4; ++q) mbar_init(xchg_bar + 8 * q, 2);
     *abort_flag = 0;
+    *filled = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc_pair(smem_u32(tmem_slot), kTmemCols);
@@ -591,7 +616,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   if (warp == 0) {
     // ---------------- loader (both CTAs) ----------------
     int stage = 0, seg = 0;
-    uint32_t phase = 0;
+    uint32_t phase = 0, n_filled = 0;
     bool alive = true;
     for (int64_t t = pair_id; alive && t < total; t += n_pairs) {
       const Tile ti = decode(t, seg);
@@ -607,7 +632,9 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         }
         const uint32_t slot_smem = tiles_smem + stage * kSlotBytes;
         const uint32_t leader_full = map_to_cta(full_bar + 8 * stage, 0);
+        ++n_filled;
         if (elect_one()) {
+          if (MODE == MODE_TN) *filled = n_filled;
           if (leader) mbar_expect_tx(full_bar + 8 * stage, 2 * bytes);
           uint32_t bar = leader_full;
           if (MODE == MODE_TN && ragged != 0 && kb == ti.kb1 - 1) {
@@ -719,7 +746,7 @@ train_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         const int valid = ti.last_rows;
         if (blocks > 0 && (valid & 15) != 0) {
           const int stage = (slot + blocks - 1) % kStagesT;
-          if (!mbar_wait(tail_bar + 8 * stage, (tail_phase >> stage) & 1u, abort_flag, p.status, DICE_STATUS_WAIT_SMEM_FULL)) break;
+          if (!mbar_wait_behind(tail_bar + 8 * stage, (tail_phase >> stage) & 1u, filled, abort_flag, p.status)) break;
           tail_phase ^= 1u << stage;
           // rows [valid, next multiple of 16) of the four boxes (a row's 128 bytes are permuted within the row only)
           const int rows = 16 - (valid & 15);

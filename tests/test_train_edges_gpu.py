@@ -376,3 +376,29 @@ def test_fp32_infinities_in_a_graph(cuda_device):
         dx2[3] = clean[3]
         assert torch.equal(dx2, clean)
         dy[3, 3] = before
+
+
+# ---- long calls ---------------------------------------------------------------------------------------
+
+
+def test_ragged_end_behind_a_second_of_work(cuda_device):
+    """The first segment's reduction is whole, the second one's is not: the warp that zeroes ragged ends has nothing to do
+    for over a second (2.8e14 multiply-adds' operations at some 220 TFLOP/s), which is no reason to give up."""
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("takes 80 GB")
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    rows, n = 32768, 65536
+    dy, x = (torch.randn(rows + 5, n, generator=gen, device=cuda_device) for _ in range(2))
+    seg = torch.tensor([0, rows, rows + 5], dtype=torch.int32, device=cuda_device)
+    start, stop = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    dw = ops.grouped_wgrad(dy, x, seg)
+    stop.record()
+    ops.check_status(ops.device_status(cuda_device))
+    assert start.elapsed_time(stop) > 1000
+    at = torch.arange(0, n, 4099, device=cuda_device)
+    for s, (beg, end) in enumerate([(0, rows), (rows, rows + 5)]):
+        _check_f32(dw[s][at][:, at], dy[beg:end, at].to(D).T.contiguous(), x[beg:end, at].to(D))
+    del dw, dy, x
+    torch.cuda.empty_cache()
