@@ -402,3 +402,64 @@ def test_ragged_end_behind_a_second_of_work(cuda_device):
         _check_f32(dw[s][at][:, at], dy[beg:end, at].to(D).T.contiguous(), x[beg:end, at].to(D))
     del dw, dy, x
     torch.cuda.empty_cache()
+
+
+def _sums_of_one_sign(dev, rows, n, k):
+    """Values of one sign with all their 8 bits: a sum that is cut after every few products falls behind.  The second
+    operand's columns have factors of their own, so that the results' roundings differ from column to column."""
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    rand = lambda *s: torch.rand(*s, generator=gen, device=dev) + 1  # noqa: E731
+    return rand(rows, n).to(torch.bfloat16), (rand(rows, k) * rand(1, k)).to(torch.bfloat16)
+
+
+def _check_sums_of_one_sign(got, ref):
+    """Half a step of the result (2^-8 of the value), 2^-12 of it for the accumulator's cuts over at most 32768 of the
+    reduction (2048 instructions of up to 2^-23 each), and roundings to nearest of 2^-24 for every chain of 32768 and every
+    share (fewer than 128): 2^-17.  In the mean the first averages out: roundings spread over +-2^-8 have a deviation of
+    2^-8 / sqrt(3), of which four, over the square root of the number of columns, are allowed."""
+    err = (got.to(D) - ref) / ref
+    assert bool((err.abs() <= 2.0 ** -8 + 2.0 ** -12 + 2.0 ** -17).all()), float(err.abs().max())
+    assert abs(float(err.mean())) <= 2.0 ** -12 + 2.0 ** -17 + 4 * 2.0 ** -8 / (3 * ref.shape[1]) ** 0.5, float(err.mean())
+
+
+@pytest.mark.parametrize("counts,n,k", [([1 << 21], 264, 136), ([700001, 0, 13, 1 << 20], 136, 264), ([32768, 32769], 264, 328)])
+@pytest.mark.parametrize("scratch", [True, False])
+def test_long_sums_of_one_sign(cuda_device, counts, n, k, scratch):
+    """A bf16 weight gradient over many rows: the error does not grow with them."""
+    rows = sum(counts)
+    dy, x = _sums_of_one_sign(cuda_device, rows, n, k)
+    seg = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], dtype=torch.int32, device=cuda_device)
+    if scratch:
+        dw = ops.grouped_wgrad(dy, x, seg)
+    else:
+        dw = torch.empty(len(counts), n, k, dtype=torch.bfloat16, device=cuda_device)
+        rc = _lib.load().dice_grouped_wgrad(dy.data_ptr(), x.data_ptr(), rows, n, k, seg.data_ptr(), len(counts), 0, ops.DICE_BF16,
+                                            dw.data_ptr(), None, None, 0, None, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+    beg = 0
+    for s, c in enumerate(counts):
+        ref = torch.zeros(n, k, dtype=D, device=cuda_device)
+        for at in range(beg, beg + c, 1 << 18):
+            end = min(at + (1 << 18), beg + c)
+            ref += dy[at:end].to(D).T @ x[at:end].to(D)
+        if c:
+            _check_sums_of_one_sign(dw[s], ref)
+        else:
+            assert bool((dw[s] == 0).all())
+        beg += c
+    ops.check_status(ops.device_status(cuda_device))
+
+
+def test_long_input_gradient_of_one_sign(cuda_device):
+    dy, w = _sums_of_one_sign(cuda_device, 300, 1 << 19, 8)[0], _sums_of_one_sign(cuda_device, 1 << 19, 136, 8)[0]
+    seg = torch.tensor([0, 300], dtype=torch.int32, device=cuda_device)
+    ref = dy.to(D) @ w.to(D)
+    for scratch in (True, False):
+        dx = torch.empty(300, 136, dtype=torch.bfloat16, device=cuda_device)
+        if scratch:
+            ops.grouped_dgrad(dy, w.unsqueeze(0), seg, out=dx)
+        else:
+            rc = _lib.load().dice_grouped_dgrad(dy.data_ptr(), 300, 1 << 19, w.data_ptr(), 1, 136, seg.data_ptr(), None, 1,
+                                                ops.DICE_BF16, dx.data_ptr(), None, 0, None, torch.cuda.current_stream().cuda_stream)
+            assert rc == 0
+        _check_sums_of_one_sign(dx, ref)
