@@ -104,6 +104,11 @@ __device__ __forceinline__ two mul2(two a, two b) { return {__fmul_rn(a.x, b.x),
 __device__ __forceinline__ two add2(two a, two b) { return {__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)}; }
 __device__ __forceinline__ two fma2(two a, two b, two c) { return {__fmaf_rn(a.x, b.x, c.x), __fmaf_rn(a.y, b.y, c.y)}; }
 template <typename V>
+__device__ __forceinline__ V most2(V v, float most) {
+  const two f = halves(v);
+  return pair<V>(fminf(f.x, most), fminf(f.y, most));
+}
+template <typename V>
 __device__ __forceinline__ V bf16_pair(uint32_t w) { return pair<V>(bf16lo_to_f32(w), bf16hi_to_f32(w)); }
 template <typename V>
 __device__ __forceinline__ uint32_t to_bf16(V v) {
@@ -147,7 +152,8 @@ template <bool EXACT, typename V>
 __device__ __forceinline__ V gelu_grad2(V p, V& a) {
   const V s = gelu_sigmoid2<EXACT>(p), one = both<V>(1.0f);
   a = mul2(p, s);
-  const V inner = mul2(both<V>(kGeluTwoC), fma2(mul2(both<V>(3.0f * 0.044715f), p), p, one));
+  // (the square may be beyond the range; 1 - s, which it meets, is 0 or a is long before)
+  const V inner = mul2(both<V>(kGeluTwoC), add2(most2(mul2(mul2(both<V>(3.0f * 0.044715f), p), p), 1e30f), one));
   return fma2(mul2(a, fma2(s, both<V>(-1.0f), one)), inner, s);
 }
 template <bool EXACT, typename V>

@@ -463,3 +463,48 @@ def test_long_input_gradient_of_one_sign(cuda_device):
                                                 ops.DICE_BF16, dx.data_ptr(), None, 0, None, torch.cuda.current_stream().cuda_stream)
             assert rc == 0
         _check_sums_of_one_sign(dx, ref)
+
+
+# ---- activation at the end of the range -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("act", ["swiglu", "gelu_tanh"])
+@pytest.mark.parametrize("keep", ["int8", "e4m3", None])
+def test_slopes_of_large_arguments(cuda_device, dtype, act, keep):
+    """Far out an activation is the identity or zero: slope 1 or 0, not infinity times zero."""
+    magnitudes = torch.tensor([2.0 ** e for e in (5, 8, 20, 60, 64, 65, 66, 90, 127)], dtype=D)
+    for big in magnitudes.tolist():
+        pre = torch.zeros(2, ops.act_columns(act, 128), dtype=dtype, device=cuda_device)
+        pre[0, :128], pre[1, :128] = big, -big
+        if act == "swiglu":
+            pre[:, 128:] = 0.5
+        a, kept = ops.act_keep(pre, act, 128, keep=keep)
+        d_pre, a2 = ops.act_backward(torch.ones(2, 128, dtype=dtype, device=cuda_device), kept, act, 128)
+        unit = 0.5 if act == "swiglu" else 1.0
+        # the 8-bit codes' scale and factor are rounded to fp32: 2^-22, and half a step of the type
+        for got, want in ((a[0], unit * big), (a2[0], unit * big), (d_pre[0, :128], unit)):
+            assert bool(((got.to(D) - want).abs() <= (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -21) * want).all()), big
+        # below zero: e^-32 of 2^5 at most
+        for got in (a[1], a2[1], d_pre[1, :128]):
+            assert bool((got.to(D).abs() <= 2.0 ** 5 * 2.0 ** -46).all()), big
+
+
+@pytest.mark.parametrize("big", [2.0 ** 65, 2.0 ** 100])
+def test_slopes_of_large_arguments_in_the_product(cuda_device, big):
+    """The same in the second product's epilogue: one column of each expert's argument is large."""
+    gen = torch.Generator(device="cuda").manual_seed(14)
+    h, ffn, n = 64, 264, 70
+    rows = torch.zeros(n, h, device=cuda_device, dtype=torch.bfloat16)
+    rows[:, 0] = 1
+    w1 = torch.zeros(1, ffn, h, device=cuda_device, dtype=torch.bfloat16)
+    w1[0, 5, 0], w1[0, 200, 0] = big, -big
+    w2 = torch.randn(1, h, ffn, generator=gen, device=cuda_device).to(torch.bfloat16)
+    d_out = torch.randn(n, h, generator=gen, device=cuda_device).to(torch.bfloat16)
+    seg = torch.tensor([0, n], dtype=torch.int32, device=cuda_device)
+    _, kept = ops.grouped_ffn_train(rows, w1, w2, seg, "gelu_tanh", ffn)
+    d_rows, dw1, dw2 = ops.grouped_ffn_backward(d_out, rows, kept, w1, w2, seg, "gelu_tanh", ffn)
+    want = (d_out.to(D) @ w2[0].to(D))[:, 5].sum()  # slope 1; column 200: slope 0
+    mass = (d_out.to(D).abs() @ w2[0].to(D).abs())[:, 5].sum()
+    assert abs(float(dw1[0, 5, 0].to(D) - want)) <= 2.0 ** -8 * float(want.abs()) + (2.0 ** -8 + 200 * 2.0 ** -23) * float(mass)
+    assert float(dw1[0, 200, 0]) == 0.0 and bool(torch.isfinite(dw1).all()) and bool(torch.isfinite(d_rows).all())
