@@ -399,7 +399,11 @@ class SparseMoeBlock(nn.Module):
     (the reference's switch, models.py:170).  ``train_kernels=True`` trains
     the experts on the kernels (CUDA tensors, one device, two experts per
     token; the gate stays with torch), in bf16 wherever the eval path would
-    compute in bf16 (float64 is refused); ``train_keep`` says what they keep of the activation's
+    compute in bf16 (float64 is refused).  In bf16 the first product, the
+    activation, the argument's gradient and the results are rounded to bf16
+    (the torch loop in bf16 rounds there too); ``train_dtype=
+    torch.float32`` computes in fp32 whatever the inputs, rounding the
+    results alone, for about four times the time.  ``train_keep`` says what they keep of the activation's
     argument for the backward pass: None (all of it), or "int8" or "e4m3"
     (8 bits, one scale per 128 values: half the bytes, and gradients off by
     what 8 bits cost)."""
@@ -407,18 +411,22 @@ class SparseMoeBlock(nn.Module):
     # for blocks that were pickled before these attributes existed
     train_kernels = False
     train_keep: Optional[str] = None
+    train_dtype: Optional[torch.dtype] = None
 
     def __init__(self, embed_dim, mlp_ratio=4, num_experts=16, num_experts_per_tok=2, pretraining_tp=2,
                  layer_idx=None, total_layers=None, para_mode: ParaMode = None, *, expert_act="swiglu",
-                 shared_expert=True, train_kernels=False, train_keep: Optional[str] = None):
+                 shared_expert=True, train_kernels=False, train_keep: Optional[str] = None,
+                 train_dtype: Optional[torch.dtype] = None):
         super().__init__()
         assert para_mode is not None
         assert expert_act in ("swiglu", "gelu_tanh")
         if train_keep not in ops.KEEP_CODES:
             raise ValueError(f"train_keep is None, 'int8' or 'e4m3', got {train_keep!r}")
+        if train_dtype not in (None, torch.bfloat16, torch.float32):
+            raise ValueError(f"train_dtype is None, torch.bfloat16 or torch.float32, got {train_dtype!r}")
         if train_kernels:
             _check_train_kernels(para_mode, num_experts_per_tok)
-        self.train_kernels, self.train_keep = train_kernels, train_keep
+        self.train_kernels, self.train_keep, self.train_dtype = train_kernels, train_keep, train_dtype
         self.num_experts_per_tok = num_experts_per_tok
         self.expert_act = expert_act
         inter = mlp_ratio * embed_dim
@@ -646,7 +654,7 @@ class SparseMoeBlock(nn.Module):
         if not self.layer_idx:
             ops.poll_status(hidden_states.device)
         h = hidden_states.shape[-1]
-        x = hidden_states.reshape(-1, h).to(_compute_dtype(hidden_states))
+        x = hidden_states.reshape(-1, h).to(self.train_dtype or _compute_dtype(hidden_states))
         act, ffn = self.expert_act, self.experts[0].intermediate_size
         x, weights = without_grad(x, topk_weight.float())
         y = RoutedExperts.apply(x, topk_idx, weights, act, ffn, self.train_keep, *without_grad(*params))

@@ -867,8 +867,9 @@ def grouped_ffn_train(rows: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, se
     """:func:`grouped_ffn` for training: ``(rows_out, kept)``, where ``kept`` is the activation's argument as it is
     (``keep`` None) or in 8 bits ("int8" or "e4m3"), for :func:`grouped_ffn_backward`; None without ``want_kept``, when no
     backward pass will follow.  The first product is rounded to
-    the rows' type before the activation, and the activation before the second product.  bf16, or fp32 with fp32's
-    precision (three bf16 planes an operand on the tensor cores, or the CUDA cores where few rows meet a weight)."""
+    the rows' type before the activation, and the activation before the second product (and the argument's gradient in the
+    backward pass): in bf16 a result is 2.4e-3 of its norm from 64 bits, where its own rounding alone is 1.7e-3; who wants
+    that much less hands over rows and weights in fp32, which has fp32's precision throughout (three bf16 planes an operand on the tensor cores, or the CUDA cores where few rows meet a weight)."""
     _check_keep(keep)
     index = _one_device(rows, w1, w2, seg_offsets, status)
     if index != _current_device():

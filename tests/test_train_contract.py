@@ -73,3 +73,12 @@ def test_single_tokens_ask_for_no_scratch():
         assert ops._split_bytes(lib, rows, 9216, 1152, 8, ops.PRODUCT_DGRAD, ops.DICE_BF16) == 0
     assert lib.asked == 0
     assert ops._split_bytes(lib, 5, 9216, 1152, 8, ops.PRODUCT_DGRAD, ops.DICE_BF16) == 1 << 20
+
+
+def test_train_dtype():
+    assert _block().train_dtype is None
+    with pytest.raises(ValueError, match="train_dtype"):
+        _block(train_kernels=True, train_dtype=torch.float16)
+    blk = _block()
+    del blk.__dict__["train_dtype"]  # as a block pickled before it existed
+    assert blk.train_dtype is None
