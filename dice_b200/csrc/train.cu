@@ -1,6 +1,7 @@
 // Entry points of the expert FFN's training step: the gradients of the products grouped by expert, and the whole
-// forward and backward pass over expert-sorted rows (arguments are checked here, the kernels are in train_simt.cu
-// and train_rows.cu; the forward products are those of the eval path).
+// forward and backward pass over expert-sorted rows.  Arguments are checked here, and the kernel is chosen: train_gemm.cu
+// (tensor cores, bf16 and fp32), train_simt.cu (fp32 of few rows), train_thin.cu (bf16 input gradients of single tokens),
+// train_rows.cu (row-wise operators); the second forward product in bf16 is the eval path's.
 #include "train.cuh"
 
 namespace {

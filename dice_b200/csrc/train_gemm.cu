@@ -9,11 +9,12 @@
 // in memory, 64 reduction rows of 64 columns (128 bytes, 128-byte swizzle) per TMA box, and the matrix instruction
 // reads it "MN-major"; nothing is transposed.
 //
-// Bound: the tensor cores; an instruction takes the same time for K-major and MN-major operands (512 cycles a k-block,
-// measured with all operands in shared memory).  Eight segments of 4096 rows: NN 9216 -> 1024 at 1.58 PFLOP/s, TN
-// 9216 x 1024 at 1.50, which is what the 1000 W of the GPU allow.  Where a dimension is not a whole number of tiles (1152 =
-// 4.5 of 256 columns) it is 1.2, and a weight gradient of few rows is bounded by writing it (777 rows, 16 x 1792 x
-// 7168: 111 us = 3.7 TB/s, memset 3.85).
+// Bound: the tensor cores, and in calls that follow each other the GPU's power; an instruction takes the same time for
+// K-major and MN-major operands (512 cycles a k-block, measured with all operands in shared memory).  Eight segments of 4096
+// rows, 9216 x 1024 and 9216 x 1152 (4.5 tiles of columns), PFLOP/s of one call after a pause / of calls for a second, at SM
+// clocks of 1.1-1.24 of 1.97 GHz under the power cap: NN 1.48 / 1.24 and 1.38 / 1.17, TN 1.47 / 1.24 and 1.43 / 1.19, cuBLAS
+// (all rows, one weight) 1.50 / 1.25 and 1.47 / 1.21.  So the half tile costs 3 to 7 %, the power 16 %.  A weight gradient
+// of few rows is bounded by writing it (777 rows, 16 x 1792 x 7168: 411 MB in 111 us = 3.7 TB/s, memset 3.8).
 //
 // A weight gradient's reduction is ragged.  Its last k-block may reach into the next segment (or behind the tensor, or
 // into rows that hold anything): the instructions stop at the last 16 rows that the segment touches, and the up to

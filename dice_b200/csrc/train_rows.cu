@@ -8,10 +8,11 @@
 // the activation, 16 lanes own one group of 128 columns, so that the group's maximum is four shuffles; with SwiGLU
 // the same 16 lanes own the group's gate and its up columns, which the packed order puts 128 columns apart.
 //
-// Measured on a B200 whose copy kernel reaches 6.2 TB/s and whose memset 3.85: act_keep (int8, SwiGLU, 32768 x 4608)
-// 204 us = 5.97 TB/s (235 us before one division served four quotients and both groups' maxima shared their shuffles:
-// it issues about 20 instructions an element and was bounded by them); act_backward 228 us = 5.4 TB/s, of which the 906 MB
-// it writes are 235 us at the memset's rate; combine_backward (16384 tokens x 1152) 31.5 us = 6.0 TB/s.
+// Measured on a B200 whose copies reach 6.55 TB/s, two sets of inputs in turn: act_keep (int8, SwiGLU, 32768 x 4608) moves
+// 1217 MB in 203 us = 6.0 TB/s (235 us before one division served four quotients and both groups' maxima shared their
+// shuffles: it issues about 20 instructions an element and was bounded by them); act_backward 1519 MB in 228 us = 6.7 TB/s
+// (906 MB of them written; a memset, which only writes, takes 244 us for as many); combine_backward (16384 tokens x 1152)
+// 189 MB in 31.5 us = 6.0 TB/s.
 #include "train.cuh"
 
 namespace {

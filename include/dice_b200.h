@@ -335,7 +335,8 @@ DICE_API int dice_grouped_dgrad(const void* dy, int64_t n_rows, int n_dim, const
 /* Scratch (16-byte aligned, contents irrelevant) that makes a product faster:
  * bf16, a long reduction shared among SMs that few output tiles would leave
  * idle; fp32, the operands as three bf16 planes each for the tensor cores
- * (24 bits; without it, and where few rows meet a weight, the CUDA cores).
+ * (6 bytes for each value of both; without it, and where few rows meet a weight,
+ * the CUDA cores).
  * 0 where it would not (a scratch given to such a call is left alone, whatever
  * its size).  `product`: which one, with n_dim and k_dim as the
  * entry point names them (forward product: w [n_slabs, n_dim, k_dim]).  NULL
