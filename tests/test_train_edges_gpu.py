@@ -508,3 +508,130 @@ def test_slopes_of_large_arguments_in_the_product(cuda_device, big):
     mass = (d_out.to(D).abs() @ w2[0].to(D).abs())[:, 5].sum()
     assert abs(float(dw1[0, 5, 0].to(D) - want)) <= 2.0 ** -8 * float(want.abs()) + (2.0 ** -8 + 200 * 2.0 ** -23) * float(mass)
     assert float(dw1[0, 200, 0]) == 0.0 and bool(torch.isfinite(dw1).all()) and bool(torch.isfinite(d_rows).all())
+
+
+# ---- calls at the limits of what is documented ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("per_expert", [1, 3, 100])
+def test_as_many_experts_as_there_may_be(cuda_device, dtype, per_expert):
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    e, h, ffn = 256, 64, 72
+    rows = e * per_expert
+    rand = lambda *s: torch.randn(*s, generator=gen, device=cuda_device).to(dtype)  # noqa: E731
+    x, d_out, w1, w2 = rand(rows, h), rand(rows, h), rand(e, ffn, h), rand(e, h, ffn)
+    seg = torch.arange(0, rows + 1, per_expert, dtype=torch.int32, device=cuda_device)
+    half = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}[dtype]
+    dx, dw = ops.grouped_dgrad(x, w2, seg), ops.grouped_wgrad(d_out, x, seg)
+    a, b, g = (t.to(D).view(e, -1, t.shape[-1]) for t in (x, w2, d_out))
+    for got, p, q, n in ((dx.view(e, -1, ffn), a, b, h), (dw, g.transpose(1, 2), a, per_expert)):
+        ref, mass = p @ q, p.abs() @ q.abs()
+        assert bool(((got.to(D) - ref).abs() <= half * ref.abs() + (n + 1) * 2.0 ** -23 * mass).all())
+    out, kept = ops.grouped_ffn_train(x, w1, w2, seg, "gelu_tanh", ffn)
+    grads = ops.grouped_ffn_backward(d_out, x, kept, w1, w2, seg, "gelu_tanh", ffn)
+    p = kept.codes.to(D).view(e, -1, ffn)
+    act = torch.nn.functional.gelu(p, approximate="tanh")
+    for got, ref in ((out, (act @ w2.to(D).transpose(1, 2)).flatten(0, 1)), (grads[2], g.transpose(1, 2) @ act)):
+        assert float((got.to(D) - ref).norm() / ref.norm()) <= (6 if dtype == torch.bfloat16 else 64) * half  # (as test_train_ops_gpu and test_train_block_gpu)
+    with pytest.raises(RuntimeError, match="documented maximum"):
+        ops.grouped_wgrad(d_out[:1], x[:1], torch.zeros(258, dtype=torch.int32, device=cuda_device))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("act", ["swiglu", "gelu_tanh"])
+@pytest.mark.parametrize("keep", [None, "int8"])
+def test_the_smallest_ffn(cuda_device, dtype, act, keep):
+    """Eight columns everywhere, one row in the last of three experts."""
+    gen = torch.Generator(device="cuda").manual_seed(16)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=cuda_device).to(dtype)  # noqa: E731
+    x, d_out, w1, w2 = rand(1, 8), rand(1, 8), rand(3, ops.act_columns(act, 8), 8), rand(3, 8, 8)
+    seg = torch.tensor([0, 0, 0, 1], dtype=torch.int32, device=cuda_device)
+    out, kept = ops.grouped_ffn_train(x, w1, w2, seg, act, 8, keep=keep)
+    d_rows, dw1, dw2 = ops.grouped_ffn_backward(d_out, x, kept, w1, w2, seg, act, 8)
+    a = w1[2].to(D).requires_grad_()
+    b, xx = w2[2].to(D).requires_grad_(), x.to(D).requires_grad_()
+    pre = (xx @ a.T)
+    if act == "swiglu":
+        mid = torch.nn.functional.silu(pre[:, :8]) * pre[:, 128:136]
+    else:
+        mid = torch.nn.functional.gelu(pre, approximate="tanh")
+    want = mid @ b.T
+    want.backward(d_out.to(D))
+    # five roundings on the way at most, and int8's half step of the largest of the group: 1/254 of it, for 8 values of
+    # which the others may be smaller by any factor, so against the largest result
+    tol = {torch.bfloat16: 8 * 2.0 ** -8, torch.float32: 64 * 2.0 ** -24}[dtype] + (0.05 if keep else 0)
+    gate_up = [a.grad[:8], a.grad[128:136]] if act == "swiglu" else [a.grad]
+    for got, ref in [(out, want), (d_rows, xx.grad), (dw2[2], b.grad), *zip(dw1 if act == "swiglu" else [dw1], gate_up)]:
+        got = got[2] if got.dim() == 3 else got
+        assert float((got.to(D) - ref.detach()).abs().max()) <= tol * float(ref.detach().abs().max()) + 1e-30
+    assert bool((dw2[:2] == 0).all()) and all(bool((t[:2] == 0).all()) for t in (dw1 if act == "swiglu" else [dw1]))
+
+
+def test_fp32_slab_table_on_the_tensor_cores(cuda_device):
+    """Segments that share a slab, one without an expert (its rows hold NaN), an infinity in a shared slab."""
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    counts, slab, n, k = [150, 60, 40, 250], [1, 0, -1, 1], 1032, 712
+    seg = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], dtype=torch.int32, device=cuda_device)
+    dy, w = torch.randn(500, n, generator=gen, device=cuda_device), torch.randn(2, n, k, generator=gen, device=cuda_device)
+    assert ops._split_bytes(_lib.load(), 500, n, k, 2, ops.PRODUCT_DGRAD, ops.DICE_F32) > 0
+    dy[210:250] = float("nan")
+    table = torch.tensor(slab, dtype=torch.int32, device=cuda_device)
+    out = torch.full((500, k), -7.0, device=cuda_device)
+    clean = ops.grouped_dgrad(dy, w, seg, seg_slab=table, out=out).clone()
+    w2 = w.clone()
+    w2[1, 100, 200] = float("inf")
+    got = ops.grouped_dgrad(dy, w2, seg, seg_slab=table)
+    at = 0
+    for c, s in zip(counts, slab):
+        cut = slice(at, at + c)
+        at += c
+        if s < 0:
+            assert bool((clean[cut] == -7).all())
+            continue
+        _check_f32(clean[cut], dy[cut].to(D), w[s].to(D))
+        others = torch.arange(k, device=cuda_device) != 200
+        assert torch.equal(got[cut][:, others], clean[cut][:, others])
+        if s == 1:
+            assert torch.equal(got[cut][:, 200], torch.sign(dy[cut][:, 100]) * float("inf"))
+        else:
+            assert torch.equal(got[cut], clean[cut])
+
+
+@pytest.mark.parametrize("rows", [33000, 70001])
+def test_long_weight_gradient_with_gate_and_up_apart(cuda_device, rows):
+    """More than 32768 rows take the form that empties its accumulator: the same bits packed and apart, and 64 bits'."""
+    gen = torch.Generator(device="cuda").manual_seed(18)
+    ffn, k = 136, 72
+    cols = ops.w13_rows(ffn)
+    dy, x = (torch.randn(rows, c, generator=gen, device=cuda_device).to(torch.bfloat16) for c in (cols, k))
+    seg = torch.tensor([0, 32800, 32800, rows], dtype=torch.int32, device=cuda_device)
+    packed = ops.grouped_wgrad(dy, x, seg)
+    gate, up = ops.grouped_wgrad(dy, x, seg, gate_up=ffn)
+    parts = packed.unflatten(1, (-1, 2, 128))
+    assert torch.equal(gate, parts[:, :, 0].flatten(1, 2)[:, :ffn]) and torch.equal(up, parts[:, :, 1].flatten(1, 2)[:, :ffn])
+    for s, (beg, end) in enumerate([(0, 32800), (32800, 32800), (32800, rows)]):
+        a, b = dy[beg:end].to(D).T, x[beg:end].to(D)
+        ref, mass = a @ b, a.abs() @ b.abs()
+        assert bool(((packed[s].to(D) - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -12 * mass).all())
+
+
+def test_two_fp32_calls_at_once(cuda_device):
+    """Planes, the word for values that are not finite and shared reductions are each call's own."""
+    gen = torch.Generator(device="cuda").manual_seed(19)
+    seg = torch.tensor([0, 700], dtype=torch.int32, device=cuda_device)
+    ins = [[torch.randn(*s, generator=gen, device=cuda_device) for s in ((700, 1032), (700, 72), (1, 1032, 712))] for _ in range(2)]
+    ins[1][0][3, 3] = float("inf")
+    call = lambda i: (ops.grouped_dgrad(ins[i][0], ins[i][2], seg), ops.grouped_wgrad(ins[i][0], ins[i][1], seg))  # noqa: E731
+    want = [call(0), call(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for pair in got[i]:
+            assert all(torch.equal(a.nan_to_num(7.0, 8.0, 9.0), b.nan_to_num(7.0, 8.0, 9.0)) for a, b in zip(pair, want[i]))
