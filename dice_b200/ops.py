@@ -585,13 +585,14 @@ class KeptAct(NamedTuple):
 # for, so it is not taken where either is on.
 _empty_cuda = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 _dispatch_modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
+_deterministic = getattr(torch._C, "_get_deterministic_algorithms", torch.are_deterministic_algorithms_enabled)
 if _dispatch_modes is None:
     _empty_cuda = None
 
 
 def _new(shape: Tuple[int, ...], dtype: torch.dtype, index: int) -> torch.Tensor:
     """An uninitialised contiguous tensor on the current device, which is number ``index``."""
-    if _empty_cuda is not None and not torch.are_deterministic_algorithms_enabled() and not _dispatch_modes():
+    if _empty_cuda is not None and not _deterministic() and not _dispatch_modes():
         stride = (shape[1], 1) if len(shape) == 2 else (shape[1] * shape[2], shape[2], 1)
         return _empty_cuda(shape, stride, dtype)
     return torch.empty(shape, dtype=dtype, device=torch.device("cuda", index))
