@@ -42,24 +42,25 @@
 // as the first of them is added, those of 2^-8, then, scaled again, hi hi.  The planes hold their bits at hi's own
 // magnitude, since bf16 ends where fp32 does: unscaled, mid and lo of values below 2^-110 would have lost their last bits
 // there, which a large factor on the other side makes visible (fp32's own subnormals, below 2^-126, have their bits in mid
-// and lo: their products are good to 2^-8).  Six instructions for one leave ~220 TFLOP/s,
-// three times the CUDA cores' 74.  An infinity in an operand (times a zero plane), or planes' products that overflow to
-// infinities of both signs, leave a NaN where the sum may be an infinity or a number: an epilogue that sees a value that is
-// not finite says so, and the CUDA cores make those values again (dice_internal_f32_repair).
+// and lo: their products are good to 2^-8).  Six instructions for one leave ~220 TFLOP/s, three times the CUDA cores' 74.
+// An infinity in an operand (times a zero plane), or planes' products that overflow to infinities of both signs, leave a NaN
+// where the sum may be an infinity or a number: an epilogue that sees a value that is not finite says so, and the CUDA cores
+// make those values again (dice_internal_f32_repair).
 //
 // A bf16 product's accumulator is cut after every 16 of the reduction too, always towards zero, by up to 2^-23 of the sum so
 // far.  Over 32768 of the reduction (512 k-blocks) that is at most 2^-12 of a sum whose terms have one sign, an eighth of
 // half a step of the bf16 result, but it grows with the length: 2^21 rows would lose 2^-6.  Products that may be longer
 // (LONG: weight gradients of more than 32768 rows, input gradients of more than 32768 columns of dy) empty the accumulator
 // every 512 k-blocks into fp32 registers that round, as planes do every one (65536 rows, 8 x 9216 x 1152: 973 -> 1000 us;
-// 2304 x 1152: 356 -> 333; 131072 rows, 4608 x 1152: 1610 -> 1760; the same without a cut, so not the emptying).  The products with the activation in their
-// epilogue, which reduce over the hidden dimension, are not cut up: 32768 is beyond any hidden dimension known.
+// 2304 x 1152: 356 -> 333; 131072 rows, 4608 x 1152: 1610 -> 1760; the same without a cut, so not the emptying).  The
+// products with the activation in their epilogue, which reduce over the hidden dimension, are not cut up: 32768 is beyond
+// any hidden dimension known.
 //
 // Few tiles: they are made half as wide if that keeps more pairs busy (one token's two rows, 1152 -> 4608: 36 tiles of
-// 256 columns, 72 of 128; 80 tiles on 74 pairs are two rounds, and so are 144 of half the width).  Fewer still, and a long reduction: the pairs that would idle take a share of the reduction
-// each (split).  Every epilogue
-// warp files its part of the sum in fp32; the last one to arrive at a part adds them up in the order of the shares, so
-// the result does not depend on who was last.
+// 256 columns, 72 of 128; 80 tiles on 74 pairs are two rounds, and so are 144 of half the width).  Fewer still, and a long
+// reduction: the pairs that would idle take a share of the reduction each (split).  Every epilogue warp files its part of
+// the sum in fp32; the last one to arrive at a part adds them up in the order of the shares, so the result does not depend
+// on who was last.
 #include <cuda.h>
 
 #include "train.cuh"

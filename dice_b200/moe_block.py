@@ -403,8 +403,8 @@ class SparseMoeBlock(nn.Module):
     activation, the argument's gradient and the results are rounded to bf16
     (the torch loop in bf16 rounds there too); ``train_dtype=
     torch.float32`` computes in fp32 whatever the inputs, rounding the
-    results alone, for five to six times the time.  ``train_keep`` says what they keep of the activation's
-    argument for the backward pass: None (all of it), or "int8" or "e4m3"
+    results alone, for five to six times the time.  ``train_keep`` says what
+    they keep of the activation's argument for the backward pass: None (all of it), or "int8" or "e4m3"
     (8 bits, one scale per 128 values: half the bytes, and gradients off by
     what 8 bits cost)."""
 

@@ -867,10 +867,10 @@ def grouped_ffn_train(rows: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, se
                       status: Optional[torch.Tensor] = None, keep: Optional[str] = None, want_kept: bool = True):
     """:func:`grouped_ffn` for training: ``(rows_out, kept)``, where ``kept`` is the activation's argument as it is
     (``keep`` None) or in 8 bits ("int8" or "e4m3"), for :func:`grouped_ffn_backward`; None without ``want_kept``, when no
-    backward pass will follow.  The first product is rounded to
-    the rows' type before the activation, and the activation before the second product (and the argument's gradient in the
-    backward pass): in bf16 a result is 2.4e-3 of its norm from 64 bits, where its own rounding alone is 1.7e-3; who wants
-    that much less hands over rows and weights in fp32, which has fp32's precision throughout (three bf16 planes an operand on the tensor cores, or the CUDA cores where few rows meet a weight)."""
+    backward pass will follow.  The first product is rounded to the rows' type before the activation, and the activation
+    before the second product (and the argument's gradient in the backward pass): in bf16 a result is 2.4e-3 of its norm
+    from 64 bits, where its own rounding alone is 1.7e-3.  fp32 rows and weights have fp32's precision throughout (three
+    bf16 planes an operand on the tensor cores, or the CUDA cores where few rows meet a weight)."""
     _check_keep(keep)
     index = _one_device(rows, w1, w2, seg_offsets, status)
     if index != _current_device():
@@ -899,7 +899,8 @@ def grouped_ffn_train(rows: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, se
     _lib.check(
         lib.dice_grouped_ffn_train(
             rows.data_ptr(), n_rows, h, ffn, ACT_CODES[act], keep_code, code, w1.data_ptr(), w2.data_ptr(), n_slabs,
-            seg_offsets.data_ptr(), n_slabs, _ptr(pre), a.data_ptr(), _ptr(codes), _ptr(scales), rows_out.data_ptr(), scratch, n_bytes, _status_ptr(status, index), _stream_of(index),
+            seg_offsets.data_ptr(), n_slabs, _ptr(pre), a.data_ptr(), _ptr(codes), _ptr(scales), rows_out.data_ptr(), scratch,
+            n_bytes, _status_ptr(status, index), _stream_of(index),
         ),
         "dice_grouped_ffn_train",
     )
